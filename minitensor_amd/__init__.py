@@ -130,7 +130,7 @@ def lib() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build it with `python -m minitensor_amd.build` "
                 "(there is no CPU fallback)")
         h = ctypes.CDLL(str(LIB_PATH))
-        for name, (res, args) in _SIGS.items():
+        for name, (res, args) in {**_SIGS, **_LOWBIT_SIGS}.items():
             fn = getattr(h, name)
             fn.restype = res
             fn.argtypes = args
@@ -487,3 +487,9 @@ def forced_config(family: int, cfg: int, splits: int = 1):
 def tolerance(K: int, amax: float, bmax: float) -> float:
     """The parity bound: 1e-5·√K·max|A|·max|B| (fp32 accumulation order differs)."""
     return 1e-5 * (max(K, 1) ** 0.5) * amax * bmax
+
+
+from .lowbit import (Q4Weight, Q8Rows, RmsNorm, dequantize_q4, dequantize_q8,  # noqa: E402, F401
+                     linear_backward_q8, linear_q4, quantize_q4, quantize_q8, rms_norm,
+                     rms_norm_backward)
+from .lowbit import SIGS as _LOWBIT_SIGS  # noqa: E402

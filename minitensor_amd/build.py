@@ -49,6 +49,7 @@ def _units():
     units.append((CSRC / "gemm_ksw_instances.hip", OBJDIR / "gemm_ksw.o", []))
     units.append((CSRC / "gemm_skinny_instances.hip", OBJDIR / "gemm_skinny.o", []))
     units.append((CSRC / "mtgemm_api.hip", OBJDIR / "mtgemm_api.o", []))
+    units.append((CSRC / "lowbit_api.hip", OBJDIR / "lowbit_api.o", []))
     return units
 
 

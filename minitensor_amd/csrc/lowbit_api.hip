@@ -1,0 +1,471 @@
+// lowbit_api.hip -- the C ABI of include/mtlowbit.h: argument checking, the
+// choice of kernel and split, launches.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "lowbit_back_kernel.hpp"
+#include "lowbit_q4_kernel.hpp"
+#include "lowbit_rows_kernel.hpp"
+#include "mtlowbit.h"
+
+using namespace mtk;
+
+namespace {
+
+constexpr int64_t kMaxDim = (int64_t)1 << 31;   // extents are 32-bit inside the kernels
+constexpr int64_t kMaxOut = (int64_t)1 << 26;   // rows of a 4-bit weight (32 threads each in a grid)
+constexpr int kCus = 256;                       // what plans fill (MI355X)
+
+int launched() {
+    // (as mt_gemm_f32: a launch recorded by a stream capture reports this)
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess || e == hipErrorStreamCaptureUnsupported ? MT_OK : MT_ERR_HIP;
+}
+
+// A 2-D fp32 view; written: no two elements on one address.
+bool valid(const mt_mat_f32* X, bool written) {
+    if (!X || X->batch != 1 || X->rows < 0 || X->cols < 0 || X->row_stride < 0 ||
+        X->col_stride < 0 || X->offset < 0 || X->rows >= kMaxDim || X->cols >= kMaxDim)
+        return false;
+    if (X->rows == 0 || X->cols == 0) return true;
+    if (!X->base) return false;
+    return !written || ((X->rows <= 1 || X->row_stride > 0) && (X->cols <= 1 || X->col_stride > 0));
+}
+bool same_shape(const mt_mat_f32* A, const mt_mat_f32* B) {
+    return A->rows == B->rows && A->cols == B->cols;
+}
+bool valid(const mt_rows_q8* Q) {
+    if (!Q || Q->rows < 0 || Q->cols < 0 || Q->rows >= kMaxDim || Q->cols >= kMaxDim ||
+        Q->row_stride < 0 || (Q->rows > 1 && Q->row_stride < Q->cols))
+        return false;
+    return Q->rows == 0 || (Q->scale && (Q->cols == 0 || Q->q));
+}
+bool valid(const mt_weight_q4* W) {
+    if (!W || W->n < 0 || W->k < 0 || W->n >= kMaxOut || W->k >= kMaxDim - 128 ||
+        (W->group != 32 && W->group != 64 && W->group != 128) || W->row_stride < 0 ||
+        W->scale_stride < 0)
+        return false;
+    if (W->n == 0 || W->k == 0) return true;
+    if (!W->packed || !W->scale || ((uintptr_t)W->packed & 15) || (W->row_stride & 15)) return false;
+    return W->n == 1 || (W->row_stride >= (W->k + 31) / 32 * 16 &&
+                         W->scale_stride >= (W->k + W->group - 1) / W->group);
+}
+
+RowView view(const mt_mat_f32* X) {
+    if (!X) return {nullptr, 0, 0};
+    return {const_cast<float*>(X->base) + X->offset, X->row_stride, X->col_stride};
+}
+// Rows whose elements are neighbours (or absent).
+bool unit(const RowView& v) { return !v.p || v.cs == 1; }
+// 16-byte aligned ones.
+bool aligned_rows(const RowView& v, int64_t rows) {
+    return v.cs == 1 && ((uintptr_t)v.p & 15) == 0 && (rows <= 1 || (v.rs & 3) == 0);
+}
+
+// Threads of a row: 16 values each (lowbit_rows_kernel.hpp).
+int row_threads(int64_t cols) { return cols <= 1024 ? 64 : cols <= 4096 ? 256 : 1024; }
+bool row_resident(int64_t cols) { return cols <= 16384; }
+// (workgroups beyond these take a second row: a grid's threads are a 32-bit number)
+unsigned row_blocks(int64_t rows, int nt) {
+    return (unsigned)std::min<int64_t>(nt == 64 ? (rows + 3) / 4 : rows, 1 << 20);
+}
+
+// Calls go(NT, MODE, RES) as constants: see lowbit_rows_kernel.hpp.
+template <class Go>
+void row_kernel(int64_t cols, bool units, Go go) {
+    using std::integral_constant;
+    using Res = std::true_type;
+    using Again = std::false_type;
+    if (!units) return go(integral_constant<int, 1024>{}, integral_constant<int, R_STRIDED>{}, Again{});
+    auto pick = [&](auto mode) {
+        if (!row_resident(cols)) go(integral_constant<int, 1024>{}, mode, Again{});
+        else if (row_threads(cols) == 64) go(integral_constant<int, 64>{}, mode, Res{});
+        else if (row_threads(cols) == 256) go(integral_constant<int, 256>{}, mode, Res{});
+        else go(integral_constant<int, 1024>{}, mode, Res{});
+    };
+    if (cols & 3) pick(integral_constant<int, R_TAIL>{});
+    else pick(integral_constant<int, R_VEC>{});
+}
+
+template <bool NORM>
+void launch_rows(const RowParams& p, bool units, hipStream_t s) {
+    row_kernel(p.cols, units, [&](auto nt, auto mode, auto res) {
+        hipLaunchKernelGGL((rows_forward<nt(), mode(), res(), NORM>), dim3(row_blocks(p.rows, nt())),
+                           dim3(std::max<int>(nt(), 256)), 0, s, p);
+    });
+}
+
+// Row groups of the backward kernel, each of which keeps a part of dweight: a
+// multiple of four, whether a workgroup holds four groups or one.
+int64_t row_groups(int64_t rows, int64_t cols) {
+    const int nt = row_threads(cols);
+    const int64_t most = nt == 64 ? 2048 : nt == 256 ? 1024 : 512;
+    return (std::min(rows, most) + 3) / 4 * 4;
+}
+
+struct Q4Plan {
+    bool few;
+    int bm, splits, kps;
+    size_t ws;
+};
+Q4Plan q4_plan(int64_t M, int64_t N, int64_t K, bool q8) {
+    Q4Plan p{};
+    const int64_t parts = q8 ? 1 : 3;
+    if (M * parts <= 48) {
+        p.few = true;
+        return p;
+    }
+    p.bm = M <= 64 ? 64 : 128;
+    const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + 127) / 128);
+    // splits of whole blocks of 128 inputs, at least four of them
+    const int64_t blocks = (K + 127) / 128;
+    int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * kCus / std::max<int64_t>(tiles, 1), blocks / 4));
+    const int64_t per = (blocks + s - 1) / s;
+    s = std::max<int64_t>(1, (blocks + per - 1) / std::max<int64_t>(per, 1));
+    p.splits = (int)s;
+    p.kps = (int)(per * 128);
+    p.ws = s > 1 ? (size_t)(s * M * N) * 4 : 0;
+    return p;
+}
+
+template <bool Q8, int G>
+void launch_few(const Q4Params& p, hipStream_t s) {
+    const unsigned grid = (unsigned)((p.N + 15) / 16);
+    const int rows = p.M * (Q8 ? 1 : 3);
+    if (rows <= 16)
+        hipLaunchKernelGGL((q4_few<1, G, Q8, 8>), dim3(grid), dim3(512), 0, s, p);
+    else if (rows <= 32)
+        hipLaunchKernelGGL((q4_few<2, G, Q8, 8>), dim3(grid), dim3(512), 0, s, p);
+    else
+        hipLaunchKernelGGL((q4_few<3, G, Q8, 8>), dim3(grid), dim3(512), 0, s, p);
+}
+template <bool Q8, int G>
+void launch_gemm(const Q4Params& p, int bm, hipStream_t s) {
+    const int64_t tiles = (int64_t)((p.M + bm - 1) / bm) * ((p.N + 127) / 128) * p.splits;
+    if (bm == 64)
+        hipLaunchKernelGGL((q4_gemm<64, 128, 32, 64, G, Q8>), dim3((unsigned)tiles), dim3(256), 0, s,
+                           p);
+    else
+        hipLaunchKernelGGL((q4_gemm<128, 128, 64, 64, G, Q8>), dim3((unsigned)tiles), dim3(256), 0,
+                           s, p);
+}
+
+template <bool Q8>
+int run_q4(Q4Params p, int64_t M, const mt_weight_q4* W, const float* bias, int64_t bias_stride,
+           const mt_mat_f32* Y, void* workspace, size_t ws_bytes, hipStream_t s) {
+    if (M == 0 || W->n == 0) return MT_OK;
+    const RowView y = view(Y);
+    p.w = W->packed;
+    p.w_n = W->row_stride;
+    p.s = W->scale;
+    p.s_n = W->scale_stride;
+    p.bias = bias;
+    p.bias_stride = bias_stride;
+    p.y = y.p;
+    p.y_m = y.rs;
+    p.y_n = y.cs;
+    p.M = (int)M;
+    p.N = (int)W->n;
+    p.K = (int)W->k;
+    const Q4Plan plan = q4_plan(M, W->n, W->k, Q8);
+    if (W->k == 0) {                                  // no inputs: the bias alone
+        const unsigned blocks = (unsigned)std::min<int64_t>((M * W->n + 255) / 256, 4096);
+        hipLaunchKernelGGL(lb_sum, dim3(blocks), dim3(256), 0, s, nullptr, 0, p.M, p.N, bias,
+                           bias_stride, p.y, p.y_m, p.y_n, 0.f);
+        return launched();
+    }
+    if (plan.ws > 0 && (!workspace || ws_bytes < plan.ws)) return MT_ERR_WORKSPACE;
+    p.splits = plan.few ? 1 : plan.splits;
+    p.k_per_split = plan.kps;
+    p.part = static_cast<float*>(workspace);
+    auto go = [&](auto g) {
+        constexpr int G = decltype(g)::value;
+        if (plan.few) launch_few<Q8, G>(p, s);
+        else launch_gemm<Q8, G>(p, plan.bm, s);
+    };
+    if (W->group == 32) go(std::integral_constant<int, 32>{});
+    else if (W->group == 64) go(std::integral_constant<int, 64>{});
+    else go(std::integral_constant<int, 128>{});
+    if (p.splits > 1) {
+        const unsigned blocks = (unsigned)std::min<int64_t>((M * W->n + 255) / 256, 8192);
+        hipLaunchKernelGGL(lb_sum, dim3(blocks), dim3(256), 0, s, p.part, p.splits, p.M, p.N, bias,
+                           bias_stride, p.y, p.y_m, p.y_n, 0.f);
+    }
+    return launched();
+}
+
+struct BackPlan {
+    int bm, bn, splits, rps;
+    size_t ws;
+};
+BackPlan back_plan(int64_t R, int64_t O, int64_t C) {
+    BackPlan p{};
+    const bool small = ((O + 127) / 128) * ((C + 127) / 128) < kCus;
+    p.bm = p.bn = small ? 64 : 128;
+    const int64_t tiles = ((O + p.bm - 1) / p.bm) * ((C + p.bn - 1) / p.bn);
+    const int64_t blocks = (R + 127) / 128;
+    int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * kCus / std::max<int64_t>(tiles, 1), blocks / 4));
+    const int64_t per = std::max<int64_t>(1, (blocks + s - 1) / s);
+    s = std::max<int64_t>(1, (blocks + per - 1) / per);
+    p.splits = (int)s;
+    p.rps = (int)(per * 128);
+    p.ws = s > 1 ? (size_t)(s * O * C) * 4 : 0;
+    return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mt_rms_norm_f32(const mt_mat_f32* X, const mt_mat_f32* R, const float* weight,
+                    int64_t weight_stride, float eps, const mt_mat_f32* H, const mt_mat_f32* Y,
+                    const mt_rows_q8* Q, float* rstd, void* stream) {
+    if (!valid(X, false) || (R && (!valid(R, false) || !same_shape(X, R))) ||
+        (H && (!valid(H, true) || !same_shape(X, H))) ||
+        (Y && (!valid(Y, true) || !same_shape(X, Y))) ||
+        (Q && (!valid(Q) || Q->rows != X->rows || Q->cols != X->cols)) || weight_stride < 0 ||
+        !(eps >= 0.f))
+        return MT_ERR_INVALID;
+    if (X->rows == 0 || X->cols == 0) return MT_OK;
+    RowParams p{};
+    p.x = view(X);
+    p.r = view(R);
+    p.h = view(H);
+    p.y = view(Y);
+    p.w = weight;
+    p.ws = weight_stride;
+    if (Q) {
+        p.q = Q->q;
+        p.qs = Q->row_stride;
+        p.scale = Q->scale;
+    }
+    p.rstd = rstd;
+    p.eps = eps;
+    p.rows = X->rows;
+    p.cols = (int)X->cols;
+    const bool units = unit(p.x) && unit(p.r) && unit(p.h) && unit(p.y) &&
+                       (!weight || weight_stride == 1);
+    launch_rows<true>(p, units, static_cast<hipStream_t>(stream));
+    return launched();
+}
+
+size_t mt_rms_norm_backward_workspace_f32(int64_t rows, int64_t cols) {
+    if (rows <= 0 || cols <= 0 || rows >= kMaxDim || cols >= kMaxDim) return 0;
+    return (size_t)(row_groups(rows, cols) * cols) * 4;
+}
+
+int mt_rms_norm_backward_f32(const mt_mat_f32* dY, const mt_mat_f32* H, const float* weight,
+                             int64_t weight_stride, const float* rstd, const mt_mat_f32* dH0,
+                             const mt_mat_f32* dH, float* dweight, int64_t dweight_stride,
+                             float beta, void* workspace, size_t ws_bytes, void* stream) {
+    if (!valid(dY, false) || !valid(H, false) || !same_shape(dY, H) ||
+        (dH0 && (!valid(dH0, false) || !same_shape(dY, dH0))) ||
+        (dH && (!valid(dH, true) || !same_shape(dY, dH))) || weight_stride < 0 ||
+        (dweight && (dweight_stride < 0 || (dY->cols > 1 && dweight_stride == 0))) ||
+        (dY->rows > 0 && !rstd))
+        return MT_ERR_INVALID;
+    if (dY->cols == 0 || (!dH && !dweight)) return MT_OK;
+    const size_t need = dweight ? mt_rms_norm_backward_workspace_f32(dY->rows, dY->cols) : 0;
+    if (need > 0 && (!workspace || ws_bytes < need)) return MT_ERR_WORKSPACE;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    RowBwdParams p{};
+    p.dy = view(dY);
+    p.h = view(H);
+    p.dh0 = view(dH0);
+    p.dh = view(dH);
+    p.w = weight;
+    p.ws = weight_stride;
+    p.rstd = rstd;
+    p.part = dweight ? static_cast<float*>(workspace) : nullptr;
+    p.rows = dY->rows;
+    p.cols = (int)dY->cols;
+    const int64_t groups = row_groups(p.rows, p.cols);
+    if (p.rows > 0) {
+        p.row_step = (int)groups;
+        const bool units = unit(p.dy) && unit(p.h) && unit(p.dh0) && unit(p.dh) &&
+                           (!weight || weight_stride == 1);
+        row_kernel(p.cols, units, [&](auto nt, auto mode, auto res) {
+            hipLaunchKernelGGL((rms_backward<nt(), mode(), res()>),
+                               dim3((unsigned)(nt() == 64 ? groups / 4 : groups)),
+                               dim3(std::max<int>(nt(), 256)), 0, s, p);
+        });
+    }
+    if (dweight)
+        hipLaunchKernelGGL(rms_dweight_sum, dim3((unsigned)((p.cols + 63) / 64)), dim3(1024), 0, s,
+                           p.part, p.rows > 0 ? (int)groups : 0, p.cols, dweight, dweight_stride,
+                           beta);
+    return launched();
+}
+
+int mt_quantize_q8_f32(const mt_mat_f32* X, const mt_rows_q8* Q, void* stream) {
+    if (!valid(X, false) || !valid(Q) || Q->rows != X->rows || Q->cols != X->cols)
+        return MT_ERR_INVALID;
+    if (X->rows == 0 || X->cols == 0) return MT_OK;
+    RowParams p{};
+    p.x = view(X);
+    p.q = Q->q;
+    p.qs = Q->row_stride;
+    p.scale = Q->scale;
+    p.rows = X->rows;
+    p.cols = (int)X->cols;
+    launch_rows<false>(p, unit(p.x), static_cast<hipStream_t>(stream));
+    return launched();
+}
+
+int mt_dequantize_q8_f32(const mt_rows_q8* Q, const mt_mat_f32* Y, void* stream) {
+    if (!valid(Q) || !valid(Y, true) || Q->rows != Y->rows || Q->cols != Y->cols)
+        return MT_ERR_INVALID;
+    if (Y->rows == 0 || Y->cols == 0) return MT_OK;
+    const RowView y = view(Y);
+    const int v = y.cs != 1 ? 1 : (Y->cols & 15) == 0 ? 16 : (Y->cols & 3) == 0 ? 4 : 1;
+    const int64_t n = Y->rows * (Y->cols / v);
+    const unsigned blocks = (unsigned)std::min<int64_t>((n + 255) / 256, 1 << 16);
+    auto go = [&](auto w) {
+        hipLaunchKernelGGL(dequantize_q8<w()>, dim3(blocks), dim3(256), 0,
+                           static_cast<hipStream_t>(stream), Q->q, Q->row_stride, Q->scale, y,
+                           Y->rows, (int)Y->cols);
+    };
+    if (v == 16) go(std::integral_constant<int, 16>{});
+    else if (v == 4) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 1>{});
+    return launched();
+}
+
+size_t mt_linear_backward_q8_workspace_f32(int64_t rows, int64_t in_f, int64_t out_f) {
+    if (rows < 0 || in_f < 0 || out_f < 0 || rows >= kMaxDim || in_f >= kMaxDim || out_f >= kMaxDim)
+        return 0;
+    return std::max(mt_linear_workspace_f32(rows, in_f, out_f), back_plan(rows, out_f, in_f).ws);
+}
+
+int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const mt_mat_f32* W,
+                              const mt_mat_f32* dX, const mt_mat_f32* dW, float beta_w, float* db,
+                              int64_t db_stride, float beta_b, void* workspace, size_t ws_bytes,
+                              void* stream) {
+    if (!valid(dY, false) || !valid(X) || dY->rows != X->rows) return MT_ERR_INVALID;
+    if (dX && (!W || !valid(W, false) || W->rows != dY->cols || W->cols != X->cols ||
+               !valid(dX, true) || dX->rows != X->rows || dX->cols != X->cols))
+        return MT_ERR_INVALID;
+    if (dW && (!valid(dW, true) || dW->rows != dY->cols || dW->cols != X->cols))
+        return MT_ERR_INVALID;
+    if (db && (db_stride < 0 || (dY->cols > 1 && db_stride == 0))) return MT_ERR_INVALID;
+    const BackPlan plan = back_plan(X->rows, dY->cols, X->cols);
+    if (dW && plan.ws > 0 && (!workspace || ws_bytes < plan.ws)) return MT_ERR_WORKSPACE;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dX) {
+        const int rc = mt_gemm_f32(dY, W, dX, nullptr, workspace, ws_bytes, stream);
+        if (rc != MT_OK) return rc;
+    }
+    if (dW && dW->rows > 0 && dW->cols > 0) {
+        BackParams p{};
+        const RowView dy = view(dY), dw = view(dW);
+        p.dy = dy.p;
+        p.dy_r = dy.rs;
+        p.dy_o = dy.cs;
+        p.q = X->q;
+        p.q_r = X->row_stride;
+        p.scale = X->scale;
+        p.dw = dw.p;
+        p.dw_o = dw.rs;
+        p.dw_c = dw.cs;
+        p.beta = beta_w;
+        p.part = static_cast<float*>(workspace);
+        p.R = (int)X->rows;
+        p.O = (int)dY->cols;
+        p.C = (int)X->cols;
+        p.splits = plan.splits;
+        p.r_per_split = plan.rps;
+        p.q_vec = ((uintptr_t)X->q & 3) == 0 && (X->rows <= 1 || (X->row_stride & 3) == 0);
+        const unsigned sum_blocks = (unsigned)std::min<int64_t>(((int64_t)p.O * p.C + 255) / 256, 8192);
+        if (p.R == 0) {                               // no rows: beta_w·dW
+            hipLaunchKernelGGL(lb_sum, dim3(sum_blocks), dim3(256), 0, s, nullptr, 0, p.O, p.C,
+                               nullptr, 0, p.dw, p.dw_o, p.dw_c, beta_w);
+        } else {
+            const int64_t tiles = (int64_t)((p.O + plan.bm - 1) / plan.bm) *
+                                  ((p.C + plan.bn - 1) / plan.bn) * p.splits;
+            if (plan.bm == 64)
+                hipLaunchKernelGGL((back_dw<64, 64, 32, 32>), dim3((unsigned)tiles), dim3(256), 0, s,
+                                   p);
+            else
+                hipLaunchKernelGGL((back_dw<128, 128, 64, 64>), dim3((unsigned)tiles), dim3(256), 0,
+                                   s, p);
+            if (p.splits > 1)
+                hipLaunchKernelGGL(lb_sum, dim3(sum_blocks), dim3(256), 0, s, p.part, p.splits, p.O,
+                                   p.C, nullptr, 0, p.dw, p.dw_o, p.dw_c, beta_w);
+        }
+        if (launched() != MT_OK) return MT_ERR_HIP;
+    }
+    if (db) return mt_colsum_f32(dY, db, db_stride, beta_b, stream);
+    return MT_OK;
+}
+
+int mt_quantize_q4_f32(const mt_mat_f32* W, const mt_weight_q4* Q, void* stream) {
+    if (!valid(W, false) || !valid(Q) || W->rows != Q->n || W->cols != Q->k) return MT_ERR_INVALID;
+    if (Q->n == 0 || Q->k == 0) return MT_OK;
+    const RowView w = view(W);
+    const int64_t groups = (Q->k + Q->group - 1) / Q->group;
+    const int64_t n = Q->n * groups * (Q->group / 8);
+    const unsigned blocks = (unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    auto go = [&](auto g) {
+        hipLaunchKernelGGL(quantize_q4<g()>, dim3(blocks), dim3(256), 0, s, w.p, w.rs, w.cs, Q->packed, Q->row_stride, Q->scale,
+                           Q->scale_stride, (int)Q->n, (int)Q->k);
+    };
+    if (Q->group == 32) go(std::integral_constant<int, 32>{});
+    else if (Q->group == 64) go(std::integral_constant<int, 64>{});
+    else go(std::integral_constant<int, 128>{});
+    return launched();
+}
+
+int mt_dequantize_q4_f32(const mt_weight_q4* Q, const mt_mat_f32* W, void* stream) {
+    if (!valid(Q) || !valid(W, true) || W->rows != Q->n || W->cols != Q->k) return MT_ERR_INVALID;
+    if (Q->n == 0 || Q->k == 0) return MT_OK;
+    const RowView w = view(W);
+    const int64_t n = Q->n * ((Q->k + 7) / 8);
+    const unsigned blocks = (unsigned)std::min<int64_t>((n + 255) / 256, 1 << 16);
+    hipLaunchKernelGGL(dequantize_q4, dim3(blocks), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       Q->packed, Q->row_stride, Q->scale, Q->scale_stride, (int)Q->group, w.p, w.rs,
+                       w.cs, (int)Q->n, (int)Q->k);
+    return launched();
+}
+
+size_t mt_linear_q4_workspace(int64_t rows, int64_t in_f, int64_t out_f) {
+    if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxDim - 128 ||
+        out_f >= kMaxDim)
+        return 0;
+    return std::max(q4_plan(rows, out_f, in_f, false).ws, q4_plan(rows, out_f, in_f, true).ws);
+}
+
+int mt_linear_q4_f32(const mt_mat_f32* X, const mt_weight_q4* W, const float* bias,
+                     int64_t bias_stride, const mt_mat_f32* Y, void* workspace, size_t ws_bytes,
+                     void* stream) {
+    if (!valid(X, false) || !valid(W) || !valid(Y, true) || X->cols != W->k || Y->rows != X->rows ||
+        Y->cols != W->n || (bias && bias_stride < 0))
+        return MT_ERR_INVALID;
+    Q4Params p{};
+    const RowView x = view(X);
+    p.x = x.p;
+    p.x_m = x.rs;
+    p.x_k = x.cs;
+    p.x_vec = aligned_rows(x, X->rows);
+    return run_q4<false>(p, X->rows, W, bias, bias_stride, Y, workspace, ws_bytes,
+                         static_cast<hipStream_t>(stream));
+}
+
+int mt_linear_q4_q8(const mt_rows_q8* X, const mt_weight_q4* W, const float* bias,
+                    int64_t bias_stride, const mt_mat_f32* Y, void* workspace, size_t ws_bytes,
+                    void* stream) {
+    if (!valid(X) || !valid(W) || !valid(Y, true) || X->cols != W->k || Y->rows != X->rows ||
+        Y->cols != W->n || (bias && bias_stride < 0))
+        return MT_ERR_INVALID;
+    Q4Params p{};
+    p.q = X->q;
+    p.q_m = X->row_stride;
+    p.q_scale = X->scale;
+    p.x_vec = ((uintptr_t)X->q & 7) == 0 && (X->rows <= 1 || (X->row_stride & 7) == 0);
+    return run_q4<true>(p, X->rows, W, bias, bias_stride, Y, workspace, ws_bytes,
+                        static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include "mtgemm.h"
+#include "mtlowbit.h"
 
 namespace py = pybind11;
 
@@ -268,6 +269,226 @@ py::object conv2d_backward(py::handle px, py::handle pw, py::handle pdy, int64_t
     return py::make_tuple(tensor(dx), rdw, tensor(db));
 }
 
+// ---- include/mtlowbit.h ------------------------------------------------------
+
+// A plain tensor of another type, of `dim` dimensions with neighbouring elements
+// in its rows.
+at::Tensor rows_arg(py::handle h, at::ScalarType type, int64_t dim, bool* ok) {
+    if (!THPVariable_Check(h.ptr())) {
+        *ok = false;
+        return {};
+    }
+    at::Tensor t = THPVariable_Unpack(h.ptr());
+    if (!t.defined() || !t.is_cuda() || t.scalar_type() != type || t.layout() != at::kStrided ||
+        !t.has_storage() || t.is_neg() || t.unsafeGetTensorImpl()->is_python_dispatch() ||
+        t.dim() != dim || (t.size(dim - 1) > 1 && t.stride(dim - 1) != 1))
+        *ok = false;
+    return t;
+}
+
+at::Tensor empty_as(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) {
+    return at::empty(shape, at::TensorOptions().dtype(type).device(like.device()));
+}
+
+float* out_ptr(const at::Tensor& t) { return const_cast<float*>(ptr(t)); }
+
+// A vector of n floats, or nothing.
+bool vec_of(const at::Tensor& t, int64_t n) {
+    return !t.defined() || (t.dim() == 1 && t.size(0) == n);
+}
+int64_t step(const at::Tensor& t) { return t.defined() && t.size(0) > 1 ? t.stride(0) : 1; }
+bool shaped(const at::Tensor& t, int64_t r, int64_t c) {
+    return !t.defined() || (t.dim() == 2 && t.size(0) == r && t.size(1) == c);
+}
+
+mt_rows_q8 rows_q8(const at::Tensor& q, const at::Tensor& scale) {
+    return {static_cast<int8_t*>(q.data_ptr()), out_ptr(scale), q.size(0), q.size(1),
+            q.size(0) > 1 ? q.stride(0) : q.size(1)};
+}
+
+py::object rms_norm(py::handle px, py::handle pw, py::handle pres, float eps, bool want_y,
+                    bool want_q8, py::handle ph, py::handle stream) {
+    bool ok = true;
+    const at::Tensor x = arg(px, &ok), w = arg(pw, &ok), res = arg(pres, &ok);
+    at::Tensor h = arg(ph, &ok);
+    if (!ok || !x.defined() || x.dim() != 2) return py::none();
+    const int64_t n = x.size(0), c = x.size(1);
+    if (!vec_of(w, c) || !shaped(res, n, c) || !shaped(h, n, c)) return py::none();
+    void* const s = stream_of(stream);
+    at::Tensor y, rstd, q, scale;
+    {
+        const py::gil_scoped_release nogil;
+        if (!h.defined() && res.defined()) h = empty({n, c}, x);
+        rstd = empty({n}, x);
+        if (want_y) y = empty({n, c}, x);
+        mt_rows_q8 dq{};
+        if (want_q8) {
+            q = empty_as({n, c}, at::kChar, x);
+            scale = empty({n}, x);
+            dq = rows_q8(q, scale);
+        }
+        const mt_mat_f32 mx = mat(x);
+        mt_mat_f32 mr{}, mh{}, my{};
+        if (res.defined()) mr = mat(res);
+        if (h.defined()) mh = mat(h);
+        if (want_y) my = mat(y);
+        check(mt_rms_norm_f32(&mx, res.defined() ? &mr : nullptr, ptr(w), step(w), eps,
+                              h.defined() ? &mh : nullptr, want_y ? &my : nullptr,
+                              want_q8 ? &dq : nullptr, out_ptr(rstd), s),
+              "mt_rms_norm_f32");
+    }
+    const py::object rh = !ph.is_none() ? py::reinterpret_borrow<py::object>(ph)
+                          : h.defined() ? tensor(h)
+                                        : py::reinterpret_borrow<py::object>(px);
+    return py::make_tuple(tensor(y), rh, tensor(rstd), tensor(q), tensor(scale));
+}
+
+py::object rms_norm_backward(py::handle pdy, py::handle ph, py::handle pw, py::handle prstd,
+                             py::handle pdh, bool need_dh, bool need_dw, py::handle pout,
+                             py::handle pdw, float beta, py::handle pws, py::handle stream) {
+    bool ok = true;
+    const at::Tensor gws = given_ws(pws, &ok);
+    const at::Tensor dy = arg(pdy, &ok), h = arg(ph, &ok), w = arg(pw, &ok), rstd = arg(prstd, &ok),
+                     dh = arg(pdh, &ok);
+    at::Tensor out = arg(pout, &ok), dw = arg(pdw, &ok);
+    if (!ok || !dy.defined() || !h.defined() || !rstd.defined() || dy.dim() != 2) return py::none();
+    const int64_t n = dy.size(0), c = dy.size(1);
+    if (!shaped(h, n, c) || !vec_of(w, c) || !vec_of(rstd, n) || step(rstd) != 1 ||
+        !shaped(dh, n, c) || !shaped(out, n, c) || !vec_of(dw, c) ||
+        (need_dw && !dw.defined() && beta != 0.f))
+        return py::none();
+    void* const s = stream_of(stream);
+    {
+        const py::gil_scoped_release nogil;
+        if (need_dh && !out.defined()) out = empty({n, c}, dy);
+        if (need_dw && !dw.defined()) dw = empty({c}, dy);
+        const mt_mat_f32 mdy = mat(dy), mh = mat(h);
+        mt_mat_f32 m0{}, mo{};
+        if (dh.defined()) m0 = mat(dh);
+        if (need_dh) mo = mat(out);
+        const Workspace ws(gws, dy, [&]() -> size_t {
+            return need_dw ? mt_rms_norm_backward_workspace_f32(n, c) : 0;
+        });
+        check(mt_rms_norm_backward_f32(&mdy, &mh, ptr(w), step(w), ptr(rstd),
+                                       dh.defined() ? &m0 : nullptr, need_dh ? &mo : nullptr,
+                                       need_dw ? out_ptr(dw) : nullptr, step(dw), beta, ws.p, ws.n,
+                                       s),
+              "mt_rms_norm_backward_f32");
+    }
+    const auto back = [](bool need, py::handle given, const at::Tensor& t) {
+        return !need             ? py::object(py::none())
+               : given.is_none() ? tensor(t)
+                                 : py::reinterpret_borrow<py::object>(given);
+    };
+    return py::make_tuple(back(need_dh, pout, out), back(need_dw, pdw, dw));
+}
+
+py::object quantize_q8(py::handle px, py::handle stream) {
+    bool ok = true;
+    const at::Tensor x = arg(px, &ok);
+    if (!ok || !x.defined() || x.dim() != 2) return py::none();
+    void* const s = stream_of(stream);
+    at::Tensor q, scale;
+    {
+        const py::gil_scoped_release nogil;
+        q = empty_as(x.sizes(), at::kChar, x);
+        scale = empty({x.size(0)}, x);
+        const mt_mat_f32 mx = mat(x);
+        const mt_rows_q8 dq = rows_q8(q, scale);
+        check(mt_quantize_q8_f32(&mx, &dq, s), "mt_quantize_q8_f32");
+    }
+    return py::make_tuple(tensor(q), tensor(scale));
+}
+
+py::object linear_backward_q8(py::handle pdy, py::handle pq, py::handle pscale, py::handle pw,
+                              bool need_dw, bool need_db, py::handle pdx, py::handle pdw,
+                              py::handle pdb, float beta_w, float beta_b, py::handle pws,
+                              py::handle stream) {
+    bool ok = true;
+    const at::Tensor gws = given_ws(pws, &ok);
+    const at::Tensor dy = arg(pdy, &ok), w = arg(pw, &ok);
+    const at::Tensor q = rows_arg(pq, at::kChar, 2, &ok);
+    const at::Tensor scale = rows_arg(pscale, at::kFloat, 1, &ok);
+    at::Tensor dx = arg(pdx, &ok), dw = arg(pdw, &ok), db = arg(pdb, &ok);
+    if (!ok || !dy.defined() || dy.dim() != 2) return py::none();
+    const int64_t n = q.size(0), fin = q.size(1), fout = dy.size(1);
+    const bool need_dx = w.defined();
+    if (dy.size(0) != n || scale.size(0) != n || !shaped(w, fout, fin) || !shaped(dx, n, fin) ||
+        !shaped(dw, fout, fin) || !vec_of(db, fout) ||
+        (need_dw && !dw.defined() && beta_w != 0.f) || (need_db && !db.defined() && beta_b != 0.f))
+        return py::none();
+    void* const s = stream_of(stream);
+    {
+        const py::gil_scoped_release nogil;
+        if (need_dx && !dx.defined()) dx = empty({n, fin}, dy);
+        if (need_dw && !dw.defined()) dw = empty({fout, fin}, dy);
+        if (need_db && !db.defined()) db = empty({fout}, dy);
+        const mt_mat_f32 mdy = mat(dy);
+        const mt_rows_q8 mq = rows_q8(q, scale);
+        mt_mat_f32 mw{}, mdx{}, mdw{};
+        if (need_dx) {
+            mw = mat(w);
+            mdx = mat(dx);
+        }
+        if (need_dw) mdw = mat(dw);
+        const Workspace ws(gws, dy,
+                           [&] { return mt_linear_backward_q8_workspace_f32(n, fin, fout); });
+        check(mt_linear_backward_q8_f32(&mdy, &mq, need_dx ? &mw : nullptr,
+                                        need_dx ? &mdx : nullptr, need_dw ? &mdw : nullptr, beta_w,
+                                        need_db ? out_ptr(db) : nullptr, step(db), beta_b, ws.p,
+                                        ws.n, s),
+              "mt_linear_backward_q8_f32");
+    }
+    const auto back = [](bool need, py::handle given, const at::Tensor& t) {
+        return !need             ? py::object(py::none())
+               : given.is_none() ? tensor(t)
+                                 : py::reinterpret_borrow<py::object>(given);
+    };
+    return py::make_tuple(back(need_dx, pdx, dx), back(need_dw, pdw, dw), back(need_db, pdb, db));
+}
+
+// x: fp32 rows (pxscale None) or 8-bit ones.
+py::object linear_q4(py::handle px, py::handle pxscale, py::handle ppacked, py::handle pscale,
+                     int64_t k, int64_t group, py::handle pb, py::handle pout, py::handle pws,
+                     py::handle stream) {
+    bool ok = true;
+    const bool q8 = !pxscale.is_none();
+    const at::Tensor gws = given_ws(pws, &ok);
+    const at::Tensor x = q8 ? rows_arg(px, at::kChar, 2, &ok) : arg(px, &ok);
+    at::Tensor xscale;
+    if (q8) xscale = rows_arg(pxscale, at::kFloat, 1, &ok);
+    const at::Tensor packed = rows_arg(ppacked, at::kByte, 2, &ok);
+    const at::Tensor scale = rows_arg(pscale, at::kFloat, 2, &ok), b = arg(pb, &ok);
+    at::Tensor out = arg(pout, &ok);
+    if (!ok || !x.defined() || x.dim() != 2 || k < 0 || (group != 32 && group != 64 && group != 128))
+        return py::none();
+    const int64_t rows = x.size(0), n = packed.size(0);
+    const int64_t prs = n > 1 ? packed.stride(0) : packed.size(1);
+    if (x.size(1) != k || (q8 && xscale.size(0) != rows) || scale.size(0) != n ||
+        packed.size(1) != (k + 31) / 32 * 16 || scale.size(1) != (k + group - 1) / group ||
+        (packed.numel() > 0 && ((uintptr_t)packed.data_ptr() % 16 != 0 || prs % 16 != 0)) ||
+        !vec_of(b, n) || !shaped(out, rows, n))
+        return py::none();
+    void* const s = stream_of(stream);
+    {
+        const py::gil_scoped_release nogil;
+        if (!out.defined()) out = empty({rows, n}, packed);
+        const mt_weight_q4 w{static_cast<uint8_t*>(packed.data_ptr()), out_ptr(scale), n, k, prs,
+                             n > 1 ? scale.stride(0) : scale.size(1), (int32_t)group};
+        const mt_mat_f32 my = mat(out);
+        const Workspace ws(gws, packed, [&] { return mt_linear_q4_workspace(rows, k, n); });
+        if (q8) {
+            const mt_rows_q8 mx = rows_q8(x, xscale);
+            check(mt_linear_q4_q8(&mx, &w, ptr(b), step(b), &my, ws.p, ws.n, s), "mt_linear_q4_q8");
+        } else {
+            const mt_mat_f32 mx = mat(x);
+            check(mt_linear_q4_f32(&mx, &w, ptr(b), step(b), &my, ws.p, ws.n, s),
+                  "mt_linear_q4_f32");
+        }
+    }
+    return pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -276,4 +497,9 @@ PYBIND11_MODULE(_native, m) {
     m.def("linear_backward", &linear_backward);
     m.def("conv2d", &conv2d);
     m.def("conv2d_backward", &conv2d_backward);
+    m.def("rms_norm", &rms_norm);
+    m.def("rms_norm_backward", &rms_norm_backward);
+    m.def("quantize_q8", &quantize_q8);
+    m.def("linear_backward_q8", &linear_backward_q8);
+    m.def("linear_q4", &linear_q4);
 }
