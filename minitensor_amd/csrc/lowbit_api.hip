@@ -59,10 +59,6 @@ RowView view(const mt_mat_f32* X) {
 }
 // Rows whose elements are neighbours (or absent).
 bool unit(const RowView& v) { return !v.p || v.cs == 1; }
-// 16-byte aligned ones.
-bool aligned_rows(const RowView& v, int64_t rows) {
-    return v.cs == 1 && ((uintptr_t)v.p & 15) == 0 && (rows <= 1 || (v.rs & 3) == 0);
-}
 
 // Threads of a row: 16 values each (lowbit_rows_kernel.hpp).
 int row_threads(int64_t cols) { return cols <= 1024 ? 64 : cols <= 4096 ? 256 : 1024; }
@@ -117,8 +113,8 @@ Q4Plan q4_plan(int64_t M, int64_t N, int64_t K, bool q8) {
         p.few = true;
         return p;
     }
-    p.bm = M <= 64 ? 64 : 128;
-    const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + 127) / 128);
+    p.bm = ((M + 127) / 128) * ((N + 255) / 256) < kCus / 2 ? 64 : 128;
+    const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + 2 * p.bm - 1) / (2 * p.bm));
     // splits of whole blocks of 128 inputs, at least four of them
     const int64_t blocks = (K + 127) / 128;
     int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * kCus / std::max<int64_t>(tiles, 1), blocks / 4));
@@ -143,12 +139,12 @@ void launch_few(const Q4Params& p, hipStream_t s) {
 }
 template <bool Q8, int G>
 void launch_gemm(const Q4Params& p, int bm, hipStream_t s) {
-    const int64_t tiles = (int64_t)((p.M + bm - 1) / bm) * ((p.N + 127) / 128) * p.splits;
+    const int64_t tiles = (int64_t)((p.M + bm - 1) / bm) * ((p.N + 2 * bm - 1) / (2 * bm)) * p.splits;
     if (bm == 64)
         hipLaunchKernelGGL((q4_gemm<64, 128, 32, 64, G, Q8>), dim3((unsigned)tiles), dim3(256), 0, s,
                            p);
     else
-        hipLaunchKernelGGL((q4_gemm<128, 128, 64, 64, G, Q8>), dim3((unsigned)tiles), dim3(256), 0,
+        hipLaunchKernelGGL((q4_gemm<128, 256, 32, 128, G, Q8>), dim3((unsigned)tiles), dim3(512), 0,
                            s, p);
 }
 
@@ -202,8 +198,9 @@ struct BackPlan {
 };
 BackPlan back_plan(int64_t R, int64_t O, int64_t C) {
     BackPlan p{};
-    const bool small = ((O + 127) / 128) * ((C + 127) / 128) < kCus;
-    p.bm = p.bn = small ? 64 : 128;
+    const bool small = ((O + 127) / 128) * ((C + 255) / 256) < kCus / 2;
+    p.bm = small ? 64 : 128;
+    p.bn = 2 * p.bm;
     const int64_t tiles = ((O + p.bm - 1) / p.bm) * ((C + p.bn - 1) / p.bn);
     const int64_t blocks = (R + 127) / 128;
     int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * kCus / std::max<int64_t>(tiles, 1), blocks / 4));
@@ -376,7 +373,6 @@ int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const m
         p.C = (int)X->cols;
         p.splits = plan.splits;
         p.r_per_split = plan.rps;
-        p.q_vec = ((uintptr_t)X->q & 3) == 0 && (X->rows <= 1 || (X->row_stride & 3) == 0);
         const unsigned sum_blocks = (unsigned)std::min<int64_t>(((int64_t)p.O * p.C + 255) / 256, 8192);
         if (p.R == 0) {                               // no rows: beta_w·dW
             hipLaunchKernelGGL(lb_sum, dim3(sum_blocks), dim3(256), 0, s, nullptr, 0, p.O, p.C,
@@ -385,10 +381,10 @@ int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const m
             const int64_t tiles = (int64_t)((p.O + plan.bm - 1) / plan.bm) *
                                   ((p.C + plan.bn - 1) / plan.bn) * p.splits;
             if (plan.bm == 64)
-                hipLaunchKernelGGL((back_dw<64, 64, 32, 32>), dim3((unsigned)tiles), dim3(256), 0, s,
+                hipLaunchKernelGGL((back_dw<64, 128, 32, 64>), dim3((unsigned)tiles), dim3(256), 0, s,
                                    p);
             else
-                hipLaunchKernelGGL((back_dw<128, 128, 64, 64>), dim3((unsigned)tiles), dim3(256), 0,
+                hipLaunchKernelGGL((back_dw<128, 256, 32, 128>), dim3((unsigned)tiles), dim3(512), 0,
                                    s, p);
             if (p.splits > 1)
                 hipLaunchKernelGGL(lb_sum, dim3(sum_blocks), dim3(256), 0, s, p.part, p.splits, p.O,
@@ -448,7 +444,6 @@ int mt_linear_q4_f32(const mt_mat_f32* X, const mt_weight_q4* W, const float* bi
     p.x = x.p;
     p.x_m = x.rs;
     p.x_k = x.cs;
-    p.x_vec = aligned_rows(x, X->rows);
     return run_q4<false>(p, X->rows, W, bias, bias_stride, Y, workspace, ws_bytes,
                          static_cast<hipStream_t>(stream));
 }
@@ -463,7 +458,6 @@ int mt_linear_q4_q8(const mt_rows_q8* X, const mt_weight_q4* W, const float* bia
     p.q = X->q;
     p.q_m = X->row_stride;
     p.q_scale = X->scale;
-    p.x_vec = ((uintptr_t)X->q & 7) == 0 && (X->rows <= 1 || (X->row_stride & 7) == 0);
     return run_q4<true>(p, X->rows, W, bias, bias_stride, Y, workspace, ws_bytes,
                         static_cast<hipStream_t>(stream));
 }

@@ -2,13 +2,11 @@
 // in 8 bits: dW[o][c] = sum_r (dY[r][o]·scale[r]) q[r][c].
 //
 // The row's scale goes to dY (one fp32 rounding), and q is exact in bf16: three
-// bf16 products on the matrix units in fp32's precision, as lowbit_q4_kernel.hpp,
-// where a product of two fp32 operands takes six.  The sums of 128 rows are
-// taken on the matrix unit from zero and added up in fp32: the unit does not
-// round to nearest, and over 10^5 rows that would show.
+// bf16 products in fp32's precision (lowbit_gemm.hpp), where a product of two fp32
+// operands takes six.
 #pragma once
 
-#include "lowbit_q4_kernel.hpp"
+#include "lowbit_gemm.hpp"
 
 namespace mtk {
 
@@ -24,28 +22,134 @@ struct BackParams {
     float* part;                      // [splits][O][C] where splits > 1
     int R, O, C;
     int splits, r_per_split;          // a multiple of 128
-    int q_vec;                        // q's rows are 4-byte aligned
 };
 
-// Tiles of BM outputs x BN inputs.  Both operands lie across k (= r): a thread
-// takes eight rows of one output (loads of consecutive outputs on consecutive
-// lanes), and four rows of four inputs, which change places in registers.  The
-// entries of four neighbouring inputs lie in four runs, so that consecutive
-// lanes write consecutive entries; the runs start 32 bytes apart modulo 128, so
-// that a fragment's rows fall on different banks.
-template <int BN>
-constexpr int back_run() { return BN / 4 + 2; }
-template <int BN>
-constexpr int back_group() { return 4 * back_run<BN>() * 16; }
+// Both operands lie across k (= r).  dY: a thread takes eight rows of one output,
+// consecutive outputs on consecutive lanes.
+template <int BM, int NT>
+struct BackDy {
+    static constexpr int N = BM * 4 / NT, kGroup = lb_group<BM>(), kBytes = lb_plane<BM>();
+    static_assert(N * NT == BM * 4 && BM % 64 == 0, "whole items, rows the same across a wave");
+    struct Raw {
+        float a[N][8], s[N][8];
+    };
+    const float* src[N];              // output of the item, row 0
+    const float* scale;
+    int64_t ld;
+    int R, t, g[N];
+    __device__ __forceinline__ static int entry(int row) { return row; }
+    __device__ __forceinline__ BackDy(const BackParams& p, int m0, int t_) : scale(p.scale), ld(p.dy_r), R(p.R), t(t_) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            g[i] = __builtin_amdgcn_readfirstlane((i * NT + t) / BM);
+            src[i] = p.dy + (int64_t)min(m0 + (i * NT + t) % BM, p.O - 1) * p.dy_o;
+        }
+    }
+    __device__ __forceinline__ void load(Raw& x, int k0) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = k0 + 8 * g[i];
+            if (k0 + 32 <= R) {
+                const float* const q = src[i] + r * ld;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x.a[i][e] = q[e * ld];
+                    x.s[i][e] = scale[r + e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x.a[i][e] = r + e < R ? src[i][(r + e) * ld] : 0.f;
+                    x.s[i][e] = r + e < R ? scale[r + e] : 0.f;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void store(const Raw& x, char* buf) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float a[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a[e] = x.a[i][e] * x.s[i][e];
+            u32x4 h, m, l;
+            cut8(a, h, m, l);
+            char* const d = buf + g[i] * kGroup + (i * NT + t) % BM * 16;
+            *reinterpret_cast<u32x4*>(d) = h;
+            *reinterpret_cast<u32x4*>(d + kBytes) = m;
+            *reinterpret_cast<u32x4*>(d + 2 * kBytes) = l;
+        }
+    }
+};
+
+// q: a thread takes four rows of four inputs (a dword each, at any byte's address),
+// which change places in registers.  The entries of four neighbouring inputs lie
+// in four runs, so that consecutive lanes write consecutive entries; the runs start 32
+// bytes apart modulo 128, so that a fragment's rows fall on different banks.
+template <int BN, int NT>
+struct BackQ {
+    static constexpr int N = BN * 2 / NT, kRun = BN / 4 + 2, kGroup = 4 * kRun * 16,
+                         kBytes = 4 * kGroup;
+    static_assert(N * NT == BN * 2, "whole items");
+    struct Raw {
+        uint32_t q[N][4];
+    };
+    const int8_t* src[N];             // the item's inputs, row 0
+    int64_t ld;
+    int R, t, left[N];                // inputs from the item's first on
+    __device__ __forceinline__ static int entry(int c) { return (c & 3) * kRun + (c >> 2); }
+    __device__ __forceinline__ BackQ(const BackParams& p, int n0, int t_) : ld(p.q_r), R(p.R), t(t_) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = n0 + (i * NT + t) % (BN / 4) * 4;
+            src[i] = p.q + c;
+            left[i] = p.C - c;
+        }
+    }
+    __device__ __forceinline__ void load(Raw& x, int k0) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = k0 + 4 * ((i * NT + t) / (BN / 4));
+            if (k0 + 32 <= R && left[i] >= 4) {
+                const int8_t* const q = src[i] + r * ld;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x.q[i][e] = *reinterpret_cast<const row_codes*>(q + e * ld);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t v = 0;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        if (r + e < R && b < left[i])
+                            v |= (uint32_t)(uint8_t)src[i][(r + e) * ld + b] << (8 * b);
+                    x.q[i][e] = v;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void store(const Raw& x, char* buf) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int v = i * NT + t, c4 = v % (BN / 4), kq = v / (BN / 4);
+            char* const d = buf + (kq >> 1) * kGroup + c4 * 16 + (kq & 1) * 8;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                float f[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(x.q[i][e] >> (8 * b));
+                *reinterpret_cast<u32x2*>(d + b * kRun * 16) =
+                    u32x2{bf16_exact(f[0], f[1]), bf16_exact(f[2], f[3])};
+            }
+        }
+    }
+};
 
 template <int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) back_dw(BackParams p) {
     constexpr int WAVES_N = BN / WN, NT = BM / WM * WAVES_N * 64;
     constexpr int MB = WM / 32, NB = WN / 32;
-    constexpr int NA = BM * 4 / NT, NQ = (BN * 2 + NT - 1) / NT;
-    static_assert(NA * NT == BM * 4, "whole items per thread");
-    constexpr int APL = lb_plane<BM>(), BUF = 3 * APL + 4 * back_group<BN>();
-    __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+    using LA = BackDy<BM, NT>;
+    using LB = BackQ<BN, NT>;
+    __shared__ __attribute__((aligned(16))) char smem[2 * (3 * LA::kBytes + LB::kBytes)];
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int ra = wave / WAVES_N * WM, rb = wave % WAVES_N * WN;
@@ -55,136 +159,30 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) back_dw(BackParam
     lb_tile(blockIdx.x - split * tiles_m * tiles_n, tiles_m, tiles_n, im, in);
     const int m0 = im * BM, n0 = in * BN;
     const int rbeg = split * p.r_per_split, rend = min(p.R, rbeg + p.r_per_split);
-    const int nk = (rend - rbeg + 31) >> 5;
-
-    struct Items {
-        float a[NA][8];
-        uint32_t q[NQ][4];            // four inputs of each of four rows
-    };
-    auto load = [&](Items& x, int r0) {
-#pragma unroll
-        for (int i = 0; i < NA; ++i) {
-            const int v = i * NT + t, o = min(m0 + v % BM, p.O - 1);
-            const int r = r0 + 8 * __builtin_amdgcn_readfirstlane(v / BM);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)                    // (r is the same in a wave)
-                x.a[i][e] = r + e < p.R ? p.dy[(int64_t)(r + e) * p.dy_r + (int64_t)o * p.dy_o] *
-                                              p.scale[r + e]
-                                        : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            const int v = i * NT + t, c = n0 + v % (BN / 4) * 4, r = r0 + 4 * (v / (BN / 4));
-            if (NQ * NT > BN * 2 && v >= BN * 2) continue;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x.q[i][e] = 0;
-                if (r + e >= p.R) continue;
-                const int8_t* const src = p.q + (int64_t)(r + e) * p.q_r + c;
-                if (p.q_vec && c + 4 <= p.C) {
-                    x.q[i][e] = *reinterpret_cast<const uint32_t*>(src);
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 4; ++b)
-                        if (c + b < p.C) x.q[i][e] |= (uint32_t)(uint8_t)src[b] << (8 * b);
-                }
-            }
-        }
-    };
-    auto store = [&](const Items& x, char* buf) {
-#pragma unroll
-        for (int i = 0; i < NA; ++i) {
-            const int v = i * NT + t;
-            const float* const a = x.a[i];
-            u32x4 h, m, l;
-            cut8(rowf4{a[0], a[1], a[2], a[3]}, rowf4{a[4], a[5], a[6], a[7]}, h, m, l);
-            char* const d = buf + v / BM * lb_group<BM>() + v % BM * 16;
-            *reinterpret_cast<u32x4*>(d) = h;
-            *reinterpret_cast<u32x4*>(d + APL) = m;
-            *reinterpret_cast<u32x4*>(d + 2 * APL) = l;
-        }
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            const int v = i * NT + t, c4 = v % (BN / 4), kq = v / (BN / 4);
-            if (NQ * NT > BN * 2 && v >= BN * 2) continue;
-            char* const d = buf + 3 * APL + (kq >> 1) * back_group<BN>() + c4 * 16 + (kq & 1) * 8;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                float f[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(x.q[i][e] >> (8 * b));
-                u32x2 w;
-                w[0] = __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302);
-                w[1] = __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302);
-                *reinterpret_cast<u32x2*>(d + b * back_run<BN>() * 16) = w;
-            }
-        }
-    };
-
+    LA la(p, m0, t);
+    LB lb(p, n0, t);
     f32x16 sum[MB][NB], acc[MB][NB];
     zero_blocks<MB, NB>(sum);
-    zero_blocks<MB, NB>(acc);
-    const int half = lane >> 5, row = lane & 31;
-    auto multiply = [&](const char* buf) {
+    lb_product<3, 4, MB, NB>(la, lb, smem, rbeg, rend, ra, rb, lane, acc, [&](int) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            u32x4 a[3][MB], b[NB];
+        for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int jn = 0; jn < NB; ++jn) {
-                const int c = rb + 32 * jn + row;
-                b[jn] = *reinterpret_cast<const u32x4*>(buf + 3 * APL + (2 * s + half) * back_group<BN>() +
-                                                        ((c & 3) * back_run<BN>() + (c >> 2)) * 16);
-            }
+            for (int j = 0; j < NB; ++j)
 #pragma unroll
-            for (int q = 0; q < 3; ++q)
-#pragma unroll
-                for (int i = 0; i < MB; ++i)
-                    a[q][i] = *reinterpret_cast<const u32x4*>(
-                        buf + q * APL + (2 * s + half) * lb_group<BM>() + (ra + 32 * i + row) * 16);
-#pragma unroll
-            for (int q = 2; q >= 0; --q)
-#pragma unroll
-                for (int i = 0; i < MB; ++i)
-#pragma unroll
-                    for (int jn = 0; jn < NB; ++jn)
-                        acc[i][jn] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            __builtin_bit_cast(bf16x8, a[q][i]), __builtin_bit_cast(bf16x8, b[jn]),
-                            acc[i][jn], 0, 0, 0);
-        }
-    };
-    Items x;
-    load(x, rbeg);
-    store(x, smem);
-    for (int c = 0; c < nk; ++c) {
-        __syncthreads();
-        const bool more = c + 1 < nk;
-        if (more) load(x, rbeg + 32 * (c + 1));
-        multiply(smem + (c & 1) * BUF);
-        if (more) store(x, smem + ((c + 1) & 1) * BUF);
-        if ((c & 3) == 3 || !more) {
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int jn = 0; jn < NB; ++jn)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        sum[i][jn][r] += acc[i][jn][r];
-                        acc[i][jn][r] = 0.f;
-                    }
-        }
-    }
+                for (int r = 0; r < 16; ++r) sum[i][j][r] += acc[i][j][r];
+    });
     const bool part = p.splits > 1;
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int jn = 0; jn < NB; ++jn) {
-            const int n = n0 + rb + 32 * jn + (lane & 31);
+        for (int j = 0; j < NB; ++j) {
+            const int n = n0 + rb + 32 * j + (lane & 31);
             if (n >= p.C) continue;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int m = m0 + ra + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                const int m = m0 + ra + 32 * i + lb_row(lane, r);
                 if (m >= p.O) continue;
-                const float v = sum[i][jn][r];
+                const float v = sum[i][j][r];
                 if (part) {
                     p.part[((int64_t)split * p.O + m) * p.C + n] = v;
                 } else {

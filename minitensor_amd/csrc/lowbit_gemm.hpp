@@ -1,0 +1,185 @@
+// lowbit_gemm.hpp -- the product that the operators of include/mtlowbit.h share: an
+// operand A in fp32, cut into three bf16 values, or in 8 bits (exact in bf16), times
+// an operand B in 8 or 4 bits, on the bf16 matrix units.
+//
+// Tiles of BM x BN over chunks of 32 k, in two LDS buffers: while chunk c is multiplied,
+// chunk c+1, loaded into registers a chunk before, is converted to bf16 and written to
+// the other buffer, and chunk c+2 is on its way from memory.  One barrier per chunk; it
+// waits for LDS alone, so that the loads stay in flight across it.
+//
+// Each wave multiplies WM x WN in blocks of 32x32.  A's parts make a row three times
+// as dear as a column in LDS reads (three fragments, one for B) and four to five times
+// as dear in conversions, so tiles and waves are wider than high: 128x256 in waves of 32x128
+// reads 7 fragments per 12 MFMAs, 64x64 ones 8.
+//
+// The sums of a group of k are taken on the matrix unit from zero and then added to
+// the result in fp32, by the group's scale where there is one: the unit does not
+// round to nearest, and over 10^5 terms that would show.
+#pragma once
+
+#include "gemm_split.hpp"
+#include "lowbit_rows_kernel.hpp"
+
+namespace mtk {
+
+// The parts of eight values.  What is left of an infinity or a NaN (a NaN) is
+// made zero, so that its products are those of fp32: the middle of (r, r, 0)
+// is r, and 0 where r is a NaN.
+__device__ __forceinline__ void cut8(const float (&x)[8], u32x4& h, u32x4& m, u32x4& l) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
+        float r0 = x[2 * i] - bf16_lo(h[i]), r1 = x[2 * i + 1] - bf16_hi(h[i]);
+        r0 = __builtin_amdgcn_fmed3f(r0, r0, 0.f);
+        r1 = __builtin_amdgcn_fmed3f(r1, r1, 0.f);
+        m[i] = bf16_pair(r0, r1);
+        l[i] = bf16_pair(r0 - bf16_lo(m[i]), r1 - bf16_hi(m[i]));
+    }
+}
+
+// Two floats that are exact in bf16.
+__device__ __forceinline__ uint32_t bf16_exact(float a, float b) {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+}
+
+// Eight int8 values as bf16.
+__device__ __forceinline__ u32x4 q8_bf16(const u32x2& q) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = q[i >> 1] >> (16 * (i & 1));
+        r[i] = bf16_exact((float)(int8_t)w, (float)(int8_t)(w >> 8));
+    }
+    return r;
+}
+
+// A barrier that orders LDS alone.
+__device__ __forceinline__ void lb_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// LDS of a chunk: per part four groups of eight k, each a column of 16-byte entries, one
+// per row, and two entries more, so that the groups of a row start 32 bytes apart modulo
+// the banks' 128.
+template <int ROWS>
+constexpr int lb_group() { return (ROWS + 2) * 16; }
+template <int ROWS>
+constexpr int lb_plane() { return 4 * lb_group<ROWS>(); }
+
+// The tile of a workgroup: eight XCDs take consecutive workgroups in turn; each
+// gets a run of tiles, walked down eight rows of tiles at a time, so that the
+// tiles in flight on one L2 share their operands.
+__device__ __forceinline__ void lb_tile(int b, int tm, int tn, int& im, int& in) {
+    const int n = tm * tn;
+    const int xcd = b & 7, q = n >> 3, rem = n & 7;
+    b = xcd * q + min(xcd, rem) + (b >> 3);
+    const int band = 8 * tn, first = b / band * 8, h = min(8, tm - first);
+    const int w = b % band;
+    im = first + w % h;
+    in = w / h;
+}
+
+// The loop.  LA, LB: loaders with
+//   Raw                          what a thread holds of a chunk
+//   load(Raw&, int k0)           chunk of 32 k from k0 on, zero past the end
+//   store(const Raw&, char*)     converted, to its part of the buffer
+//   kBytes, entry(row)           LDS size of a part, and the entry of a row in a group
+// P: parts of A.  GC: chunks (1, 2 or 4) whose sums are taken on the matrix unit;
+// flush(k) adds those that end before k to the result and is called in order.
+template <int P, int GC, int MB, int NB, class LA, class LB, class Flush>
+__device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_begin, int k_end, int ra,
+                                           int rb, int lane, f32x16 (&acc)[MB][NB], Flush flush) {
+    constexpr int BUF = P * LA::kBytes + LB::kBytes;
+    const int nk = (k_end - k_begin + 31) >> 5;
+    const int half = lane >> 5, row = lane & 31;
+    typename LA::Raw xa, ya;
+    typename LB::Raw xb, yb;
+    auto fetch = [&](typename LA::Raw& a, typename LB::Raw& b, int c) {
+        if (c >= nk) return;
+        la.load(a, k_begin + 32 * c);
+        lb.load(b, k_begin + 32 * c);
+    };
+    auto put = [&](const typename LA::Raw& a, const typename LB::Raw& b, int buf) {
+        la.store(a, smem + buf * BUF);
+        lb.store(b, smem + buf * BUF + P * LA::kBytes);
+    };
+    auto multiply = [&](const char* buf, bool first) {
+        const char* const pb = buf + P * LA::kBytes;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            u32x4 a[P][MB], b[NB];
+            const int g = 2 * s + half;
+#pragma unroll
+            for (int q = P - 1; q >= 0; --q)
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+                    a[q][i] = *reinterpret_cast<const u32x4*>(buf + q * LA::kBytes + g * LA::kGroup +
+                                                              LA::entry(ra + 32 * i + row) * 16);
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                b[j] = *reinterpret_cast<const u32x4*>(pb + g * LB::kGroup +
+                                                       LB::entry(rb + 32 * j + row) * 16);
+#pragma unroll
+            for (int q = P - 1; q >= 0; --q)
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) {
+                        f32x16 c = acc[i][j];
+                        if (first && s == 0 && q == P - 1)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) c[r] = 0.f;
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            __builtin_bit_cast(bf16x8, a[q][i]), __builtin_bit_cast(bf16x8, b[j]), c,
+                            0, 0, 0);
+                    }
+        }
+    };
+    // Chunk c out of LDS; a, b hold chunk c+1 and take chunk c+3, na, nb hold c+2.
+    auto step = [&](int c, int s, typename LA::Raw& a, typename LB::Raw& b, typename LA::Raw& na,
+                    typename LB::Raw& nb) {
+        lb_barrier();
+        fetch(na, nb, c + 2);
+        multiply(smem + (s & 1) * BUF, s % GC == 0);
+        if (c + 1 < nk) put(a, b, (s + 1) & 1);
+        if (s % GC == GC - 1 || c + 1 == nk) flush(k_begin + 32 * (c + 1));
+    };
+    if (nk <= 0) return;
+    fetch(xa, xb, 0);
+    fetch(ya, yb, 1);
+    put(xa, xb, 0);
+    for (int c = 0; c < nk; c += 4) {
+        step(c, 0, ya, yb, xa, xb);
+        if (c + 1 >= nk) break;
+        step(c + 1, 1, xa, xb, ya, yb);
+        if (c + 2 >= nk) break;
+        step(c + 2, 2, ya, yb, xa, xb);
+        if (c + 3 >= nk) break;
+        step(c + 3, 3, xa, xb, ya, yb);
+    }
+}
+
+// Block element r of a lane: row 8*(r/4) + 4*(lane/32) + r%4, column lane%32.
+__device__ __forceinline__ int lb_row(int lane, int r) {
+    return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+}
+
+// y[m][n] = beta*y + bias[n] + the splits' partials [splits][M][N] in order (no
+// splits: part is not read).
+__global__ void __launch_bounds__(256)
+lb_sum(const float* part, int splits, int M, int N, const float* bias, int64_t bias_stride, float* y,
+       int64_t y_m, int64_t y_n, float beta) {
+    const int64_t n = (int64_t)M * N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int m = (int)(i / N), c = (int)(i - (int64_t)m * N);
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += part[s * n + i];
+        if (bias) v += bias[(int64_t)c * bias_stride];
+        float* const d = y + (int64_t)m * y_m + (int64_t)c * y_n;
+        *d = beta != 0.f ? beta * *d + v : v;
+    }
+}
+
+}  // namespace mtk

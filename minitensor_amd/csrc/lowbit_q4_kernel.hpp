@@ -12,8 +12,7 @@
 // q4_few: few rows of x, bound by the weight's bytes.  q4_gemm: the rest.
 #pragma once
 
-#include "gemm_split.hpp"
-#include "lowbit_rows_kernel.hpp"
+#include "lowbit_gemm.hpp"
 
 namespace mtk {
 
@@ -34,7 +33,6 @@ struct Q4Params {
     float* part;                      // [splits][M][N] partial sums, where splits > 1
     int M, N, K;
     int splits, k_per_split;          // a multiple of 128
-    int x_vec;                        // rows of x are 16-byte aligned (8-bit ones 8-byte) runs
 };
 
 // The eight codes of a dword, over 16, as bf16 (exact): v_cvt_off_f32_i4 gives
@@ -51,63 +49,30 @@ __device__ __forceinline__ u32x4 q4_unpack(uint32_t w) {
 }
 constexpr float kQ4Unit = 16.f;
 
-// The parts of eight values.  What is left of an infinity or a NaN (a NaN) is
-// made zero, so that its products are those of fp32: the middle of (r, r, 0)
-// is r, and 0 where r is a NaN.
-__device__ __forceinline__ void cut8(const rowf4& a, const rowf4& b, u32x4& h, u32x4& m, u32x4& l) {
-    const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        h[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
-        float r0 = x[2 * i] - bf16_lo(h[i]), r1 = x[2 * i + 1] - bf16_hi(h[i]);
-        r0 = __builtin_amdgcn_fmed3f(r0, r0, 0.f);
-        r1 = __builtin_amdgcn_fmed3f(r1, r1, 0.f);
-        m[i] = bf16_pair(r0, r1);
-        l[i] = bf16_pair(r0 - bf16_lo(m[i]), r1 - bf16_hi(m[i]));
-    }
-}
-
-// Eight int8 values as bf16.
-__device__ __forceinline__ u32x4 q8_bf16(uint32_t lo, uint32_t hi) {
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t w = i < 2 ? lo : hi;
-        const float a = (float)(int8_t)(w >> (16 * (i & 1)));
-        const float b = (float)(int8_t)(w >> (16 * (i & 1) + 8));
-        r[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
-    }
-    return r;
-}
+typedef u32x2 u32x2_u __attribute__((aligned(1)));
 
 // Eight consecutive inputs k..k+7 of row m, zero from K on.
-__device__ __forceinline__ void q4_x8(const Q4Params& p, int m, int k, rowf4& a, rowf4& b) {
-    const float* const src = p.x + (int64_t)m * p.x_m + (int64_t)k * p.x_k;
-    if (p.x_vec && k + 8 <= p.K) {
-        a = *reinterpret_cast<const rowf4*>(src);
-        b = *reinterpret_cast<const rowf4*>(src + 4);
-        return;
-    }
+__device__ __forceinline__ void q4_x8(const Q4Params& p, const float* row, int k, float (&x)[8]) {
+    if (p.x_k == 1 && k + 8 <= p.K) {
+        const rowf4 a = *reinterpret_cast<const rowf4_u*>(row + k);
+        const rowf4 b = *reinterpret_cast<const rowf4_u*>(row + k + 4);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        a[e] = k + e < p.K ? src[e * p.x_k] : 0.f;
-        b[e] = k + 4 + e < p.K ? src[(4 + e) * p.x_k] : 0.f;
+        for (int e = 0; e < 4; ++e) {
+            x[e] = a[e];
+            x[4 + e] = b[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = k + e < p.K ? row[(k + e) * p.x_k] : 0.f;
     }
 }
-__device__ __forceinline__ void q4_q8(const Q4Params& p, int m, int k, uint32_t& lo, uint32_t& hi) {
-    const int8_t* const src = p.q + (int64_t)m * p.q_m + k;
-    if (p.x_vec && k + 8 <= p.K) {
-        const uint2 v = *reinterpret_cast<const uint2*>(src);
-        lo = v.x;
-        hi = v.y;
-        return;
-    }
-    lo = hi = 0;
+__device__ __forceinline__ u32x2 q4_x8(const Q4Params& p, const int8_t* row, int k) {
+    if (k + 8 <= p.K) return *reinterpret_cast<const u32x2_u*>(row + k);
+    u32x2 r = {0u, 0u};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        lo |= (k + e < p.K ? (uint32_t)(uint8_t)src[e] : 0u) << (8 * e);
-        hi |= (k + 4 + e < p.K ? (uint32_t)(uint8_t)src[4 + e] : 0u) << (8 * e);
-    }
+    for (int e = 0; e < 8; ++e)
+        if (k + e < p.K) r[e >> 2] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e & 3));
+    return r;
 }
 
 __device__ __forceinline__ f32x4 mfma_16(const u32x4& a, const u32x4& b, const f32x4& c) {
@@ -180,14 +145,13 @@ __global__ void __launch_bounds__(64 * W) q4_few(Q4Params p) {
             const int m = e >> 4, piece = e & 15;
             char* const d = xs + P * m * RS + piece * 16;
             if constexpr (Q8) {
-                uint32_t lo, hi;
-                q4_q8(p, m, k0 + 8 * piece, lo, hi);
-                *reinterpret_cast<u32x4*>(d) = q8_bf16(lo, hi);
+                *reinterpret_cast<u32x4*>(d) =
+                    q8_bf16(q4_x8(p, p.q + (int64_t)m * p.q_m, k0 + 8 * piece));
             } else {
-                rowf4 a, b;
+                float x[8];
                 u32x4 h, mm, l;
-                q4_x8(p, m, k0 + 8 * piece, a, b);
-                cut8(a, b, h, mm, l);
+                q4_x8(p, p.x + (int64_t)m * p.x_m, k0 + 8 * piece, x);
+                cut8(x, h, mm, l);
                 *reinterpret_cast<u32x4*>(d) = h;
                 *reinterpret_cast<u32x4*>(d + RS) = mm;
                 *reinterpret_cast<u32x4*>(d + 2 * RS) = l;
@@ -242,70 +206,90 @@ __global__ void __launch_bounds__(64 * W) q4_few(Q4Params p) {
     }
 }
 
-// LDS of a chunk of 32 k: per part four groups of eight k, each a column of
-// 16-byte entries, one per row, and two entries more (the groups of a row then
-// start 32 bytes apart modulo the banks' 128).
-template <int ROWS>
-constexpr int lb_group() { return (ROWS + 2) * 16; }
-template <int ROWS>
-constexpr int lb_plane() { return 4 * lb_group<ROWS>(); }
-
-// One chunk of 32 k for a wave's MB x NB blocks of 32x32: P parts of A times B,
-// the small parts first.
-template <int P, int MB, int NB, int BM, int BN>
-__device__ __forceinline__ void lb_multiply(const char* lds, int ra, int rb, int lane,
-                                            f32x16 (&acc)[MB][NB]) {
-    const int half = lane >> 5, row = lane & 31;
-    const char* const lb = lds + P * lb_plane<BM>();
+// Many rows: x as A, in fp32 or in 8 bits; a thread takes eight inputs of a row.
+template <bool Q8, int BM, int NT>
+struct Q4X {
+    static constexpr int N = BM * 4 / NT, kGroup = lb_group<BM>(), kBytes = lb_plane<BM>();
+    static_assert(N * NT == BM * 4, "whole items");
+    struct Raw {
+        float a[Q8 ? 1 : N][8];
+        u32x2 q[Q8 ? N : 1];
+    };
+    const Q4Params& p;
+    const float* x[N];
+    const int8_t* q[N];
+    int t;
+    __device__ __forceinline__ static int entry(int row) { return row; }
+    __device__ __forceinline__ Q4X(const Q4Params& p_, int m0, int t_) : p(p_), t(t_) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        u32x4 a[P][MB], b[NB];
-#pragma unroll
-        for (int jn = 0; jn < NB; ++jn)
-            b[jn] = *reinterpret_cast<const u32x4*>(lb + (2 * s + half) * lb_group<BN>() +
-                                                    (rb + 32 * jn + row) * 16);
-#pragma unroll
-        for (int q = 0; q < P; ++q)
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-                a[q][i] = *reinterpret_cast<const u32x4*>(lds + q * lb_plane<BM>() +
-                                                          (2 * s + half) * lb_group<BM>() +
-                                                          (ra + 32 * i + row) * 16);
-#pragma unroll
-        for (int q = P - 1; q >= 0; --q)
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int jn = 0; jn < NB; ++jn)
-                    acc[i][jn] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                        __builtin_bit_cast(bf16x8, a[q][i]), __builtin_bit_cast(bf16x8, b[jn]),
-                        acc[i][jn], 0, 0, 0);
+        for (int i = 0; i < N; ++i) {                      // (rows past M: the last, not stored)
+            const int64_t m = min(m0 + ((i * NT + t) >> 2), p.M - 1);
+            if constexpr (Q8) q[i] = p.q + m * p.q_m;
+            else x[i] = p.x + m * p.x_m;
+        }
     }
-}
+    __device__ __forceinline__ void load(Raw& r, int k0) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int k = k0 + 8 * (t & 3);
+            if constexpr (Q8) r.q[i] = q4_x8(p, q[i], k);
+            else q4_x8(p, x[i], k, r.a[i]);
+        }
+    }
+    __device__ __forceinline__ void store(const Raw& r, char* buf) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            char* const d = buf + (t & 3) * kGroup + ((i * NT + t) >> 2) * 16;
+            if constexpr (Q8) {
+                *reinterpret_cast<u32x4*>(d) = q8_bf16(r.q[i]);
+            } else {
+                u32x4 h, m, l;
+                cut8(r.a[i], h, m, l);
+                *reinterpret_cast<u32x4*>(d) = h;
+                *reinterpret_cast<u32x4*>(d + kBytes) = m;
+                *reinterpret_cast<u32x4*>(d + 2 * kBytes) = l;
+            }
+        }
+    }
+};
 
-// The tile of a workgroup: eight XCDs take consecutive workgroups in turn; each
-// gets a run of tiles, walked down eight rows of tiles at a time, so that the
-// tiles in flight on one L2 share their operands.
-__device__ __forceinline__ void lb_tile(int b, int tm, int tn, int& im, int& in) {
-    const int n = tm * tn;
-    const int xcd = b & 7, q = n >> 3, rem = n & 7;
-    b = xcd * q + min(xcd, rem) + (b >> 3);
-    const int band = 8 * tn, first = b / band * 8, h = min(8, tm - first);
-    const int w = b % band;
-    im = first + w % h;
-    in = w / h;
-}
+// The weight as B: a thread takes eight inputs (a dword of codes) of a column.
+template <int BN, int NT>
+struct Q4W {
+    static constexpr int N = BN * 4 / NT, kGroup = lb_group<BN>(), kBytes = lb_plane<BN>();
+    static_assert(N * NT == BN * 4, "whole items");
+    struct Raw {
+        uint32_t w[N];
+    };
+    const uint8_t* w[N];
+    int kp, t;
+    __device__ __forceinline__ static int entry(int c) { return c; }
+    __device__ __forceinline__ Q4W(const Q4Params& p, int n0, int t_) : kp((p.K + 31) & ~31), t(t_) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)                        // (columns past N: the last)
+            w[i] = p.w + (int64_t)min(n0 + ((i * NT + t) >> 2), p.N - 1) * p.w_n + 4 * (t & 3);
+    }
+    // (chunks are whole in the packed rows: k0 is a multiple of 32 below kp)
+    __device__ __forceinline__ void load(Raw& r, int k0) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.w[i] = *reinterpret_cast<const uint32_t*>(w[i] + (k0 >> 1));
+    }
+    __device__ __forceinline__ void store(const Raw& r, char* buf) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            *reinterpret_cast<u32x4*>(buf + (t & 3) * kGroup + ((i * NT + t) >> 2) * 16) =
+                q4_unpack(r.w[i]);
+    }
+};
 
-// Many rows: tiles of BM x BN, waves of 64x64 (or 32x64).
 template <int BM, int BN, int WM, int WN, int G, bool Q8>
 __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) q4_gemm(Q4Params p) {
     constexpr int P = Q8 ? 1 : 3;
     constexpr int WAVES_N = BN / WN, NT = BM / WM * WAVES_N * 64;
     constexpr int MB = WM / 32, NB = WN / 32;
-    constexpr int NA = BM * 4 / NT, NBI = BN * 4 / NT;     // items of eight k per thread
-    static_assert(NA * NT == BM * 4 && NBI * NT == BN * 4, "whole items per thread");
-    constexpr int BUF = P * lb_plane<BM>() + lb_plane<BN>();
-    __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+    using LA = Q4X<Q8, BM, NT>;
+    using LB = Q4W<BN, NT>;
+    __shared__ __attribute__((aligned(16))) char smem[2 * (P * LA::kBytes + LB::kBytes)];
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int ra = wave / WAVES_N * WM, rb = wave % WAVES_N * WN;
@@ -315,119 +299,48 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) q4_gemm(Q4Params 
     lb_tile(blockIdx.x - split * tiles_m * tiles_n, tiles_m, tiles_n, im, in);
     const int m0 = im * BM, n0 = in * BN;
     const int kb = split * p.k_per_split, ke = min(p.K, kb + p.k_per_split);
-    const int nk = (ke - kb + 31) >> 5;
-    const int kp = (p.K + 31) & ~31;
-
-    // (rows past M or N: the last row's values, not stored)
-    struct Items {
-        rowf4 a[Q8 ? 1 : NA][2];
-        uint32_t q[Q8 ? NA : 1][2];
-        uint32_t w[NBI];
-    };
-    auto load = [&](Items& x, int k0) {
-#pragma unroll
-        for (int i = 0; i < NA; ++i) {
-            const int v = i * NT + t, m = min(m0 + (v >> 2), p.M - 1), k = k0 + 8 * (v & 3);
-            if constexpr (Q8) q4_q8(p, m, k, x.q[i][0], x.q[i][1]);
-            else q4_x8(p, m, k, x.a[i][0], x.a[i][1]);
-        }
-#pragma unroll
-        for (int i = 0; i < NBI; ++i) {
-            const int v = i * NT + t, n = min(n0 + (v >> 2), p.N - 1), k = k0 + 8 * (v & 3);
-            x.w[i] = k < kp ? *reinterpret_cast<const uint32_t*>(p.w + (int64_t)n * p.w_n + (k >> 1))
-                            : 0u;
-        }
-    };
-    auto store = [&](const Items& x, char* buf) {
-#pragma unroll
-        for (int i = 0; i < NA; ++i) {
-            const int v = i * NT + t;
-            char* const d = buf + (v & 3) * lb_group<BM>() + (v >> 2) * 16;
-            if constexpr (Q8) {
-                *reinterpret_cast<u32x4*>(d) = q8_bf16(x.q[i][0], x.q[i][1]);
-            } else {
-                u32x4 h, m, l;
-                cut8(x.a[i][0], x.a[i][1], h, m, l);
-                *reinterpret_cast<u32x4*>(d) = h;
-                *reinterpret_cast<u32x4*>(d + lb_plane<BM>()) = m;
-                *reinterpret_cast<u32x4*>(d + 2 * lb_plane<BM>()) = l;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < NBI; ++i) {
-            const int v = i * NT + t;
-            *reinterpret_cast<u32x4*>(buf + P * lb_plane<BM>() + (v & 3) * lb_group<BN>() +
-                                      (v >> 2) * 16) = q4_unpack(x.w[i]);
-        }
-    };
-
+    LA la(p, m0, t);
+    LB lb(p, n0, t);
     f32x16 sum[MB][NB], acc[MB][NB];
     zero_blocks<MB, NB>(sum);
-    zero_blocks<MB, NB>(acc);
-    constexpr int GC = G / 32;                             // chunks per group
+    // the scale of the lane's columns in the group that is being summed
     const float* sr[NB];
+    float sc[NB];
 #pragma unroll
-    for (int jn = 0; jn < NB; ++jn)
-        sr[jn] = p.s + (int64_t)min(n0 + rb + 32 * jn + (lane & 31), p.N - 1) * p.s_n;
-    Items x;
-    load(x, kb);
-    store(x, smem);
-    for (int c = 0; c < nk; ++c) {
-        __syncthreads();
-        const bool more = c + 1 < nk;
-        if (more) load(x, kb + 32 * (c + 1));
-        lb_multiply<P, MB, NB, BM, BN>(smem + (c & 1) * BUF, ra, rb, lane, acc);
-        if (more) store(x, smem + ((c + 1) & 1) * BUF);
-        if ((c + 1) % GC == 0 || !more) {
-            const int g = (kb + 32 * c) / G;
-#pragma unroll
-            for (int jn = 0; jn < NB; ++jn) {
-                const float s = sr[jn][g] * kQ4Unit;
-#pragma unroll
-                for (int i = 0; i < MB; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        sum[i][jn][r] = __builtin_fmaf(acc[i][jn][r], s, sum[i][jn][r]);
-                        acc[i][jn][r] = 0.f;
-                    }
-            }
-        }
+    for (int j = 0; j < NB; ++j) {
+        sr[j] = p.s + (int64_t)min(n0 + rb + 32 * j + (lane & 31), p.N - 1) * p.s_n;
+        sc[j] = sr[j][kb / G];
     }
-    // block element r of a lane: row 8*(r/4) + 4*(lane/32) + r%4, column lane%32
+    lb_product<P, G / 32, MB, NB>(la, lb, smem, kb, ke, ra, rb, lane, acc, [&](int k) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const float s = sc[j] * kQ4Unit;
+            if (k < ke) sc[j] = sr[j][k / G];
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    sum[i][j][r] = __builtin_fmaf(acc[i][j][r], s, sum[i][j][r]);
+        }
+    });
     const bool part = p.splits > 1;
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int jn = 0; jn < NB; ++jn) {
-            const int n = n0 + rb + 32 * jn + (lane & 31);
+        for (int j = 0; j < NB; ++j) {
+            const int n = n0 + rb + 32 * j + (lane & 31);
             if (n >= p.N) continue;
             const float b = !part && p.bias ? p.bias[(int64_t)n * p.bias_stride] : 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int m = m0 + ra + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                const int m = m0 + ra + 32 * i + lb_row(lane, r);
                 if (m >= p.M) continue;
-                float v = sum[i][jn][r];
+                float v = sum[i][j][r];
                 if constexpr (Q8) v *= p.q_scale[m];
                 if (part) p.part[((int64_t)split * p.M + m) * p.N + n] = v;
                 else p.y[(int64_t)m * p.y_m + (int64_t)n * p.y_n] = v + b;
             }
         }
-}
-
-// y[m][n] = beta*y + bias[n] + the splits' partials [splits][M][N] in order (no
-// splits: part is not read).
-__global__ void __launch_bounds__(256)
-lb_sum(const float* part, int splits, int M, int N, const float* bias, int64_t bias_stride, float* y,
-       int64_t y_m, int64_t y_n, float beta) {
-    const int64_t n = (int64_t)M * N;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int m = (int)(i / N), c = (int)(i - (int64_t)m * N);
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += part[s * n + i];
-        if (bias) v += bias[(int64_t)c * bias_stride];
-        float* const d = y + (int64_t)m * y_m + (int64_t)c * y_n;
-        *d = beta != 0.f ? beta * *d + v : v;
-    }
 }
 
 // Codes and scales of a weight: a thread takes eight inputs (a dword of codes),
