@@ -106,14 +106,15 @@ struct Q4Plan {
     int bm, splits, kps;
     size_t ws;
 };
-Q4Plan q4_plan(int64_t M, int64_t N, int64_t K, bool q8) {
+Q4Plan q4_plan(int64_t M, int64_t N, int64_t K, int group, bool q8) {
     Q4Plan p{};
     const int64_t parts = q8 ? 1 : 3;
     if (M * parts <= 48) {
         p.few = true;
         return p;
     }
-    p.bm = ((M + 127) / 128) * ((N + 255) / 256) < kCus / 2 ? 64 : 128;
+    // (groups of 32: the wide tile's scales do not fit the registers)
+    p.bm = group == 32 || ((M + 127) / 128) * ((N + 255) / 256) < kCus / 2 ? 64 : 128;
     const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + 2 * p.bm - 1) / (2 * p.bm));
     // splits of whole blocks of 128 inputs, at least four of them
     const int64_t blocks = (K + 127) / 128;
@@ -143,7 +144,7 @@ void launch_gemm(const Q4Params& p, int bm, hipStream_t s) {
     if (bm == 64)
         hipLaunchKernelGGL((q4_gemm<64, 128, 32, 64, G, Q8>), dim3((unsigned)tiles), dim3(256), 0, s,
                            p);
-    else
+    else if constexpr (G > 32)
         hipLaunchKernelGGL((q4_gemm<128, 256, 32, 128, G, Q8>), dim3((unsigned)tiles), dim3(512), 0,
                            s, p);
 }
@@ -165,7 +166,7 @@ int run_q4(Q4Params p, int64_t M, const mt_weight_q4* W, const float* bias, int6
     p.M = (int)M;
     p.N = (int)W->n;
     p.K = (int)W->k;
-    const Q4Plan plan = q4_plan(M, W->n, W->k, Q8);
+    const Q4Plan plan = q4_plan(M, W->n, W->k, W->group, Q8);
     if (W->k == 0) {                                  // no inputs: the bias alone
         const unsigned blocks = (unsigned)std::min<int64_t>((M * W->n + 255) / 256, 4096);
         hipLaunchKernelGGL(lb_sum, dim3(blocks), dim3(256), 0, s, nullptr, 0, p.M, p.N, bias,
@@ -430,7 +431,10 @@ size_t mt_linear_q4_workspace(int64_t rows, int64_t in_f, int64_t out_f) {
     if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxDim - 128 ||
         out_f >= kMaxDim)
         return 0;
-    return std::max(q4_plan(rows, out_f, in_f, false).ws, q4_plan(rows, out_f, in_f, true).ws);
+    size_t ws = 0;
+    for (const int group : {32, 128})
+        for (const bool q8 : {false, true}) ws = std::max(ws, q4_plan(rows, out_f, in_f, group, q8).ws);
+    return ws;
 }
 
 int mt_linear_q4_f32(const mt_mat_f32* X, const mt_weight_q4* W, const float* bias,

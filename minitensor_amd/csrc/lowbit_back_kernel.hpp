@@ -24,12 +24,19 @@ struct BackParams {
     int splits, r_per_split;          // a multiple of 128
 };
 
+// A load of an address that is the same across the wave.
+__device__ __forceinline__ float uniform_load(const float* p) {
+    return *(const float __attribute__((address_space(4)))*)p;
+}
+
 // Both operands lie across k (= r).  dY: a thread takes eight rows of one output,
 // consecutive outputs on consecutive lanes.
 template <int BM, int NT>
 struct BackDy {
     static constexpr int N = BM * 4 / NT, kGroup = lb_group<BM>(), kBytes = lb_plane<BM>();
     static_assert(N * NT == BM * 4 && BM % 64 == 0, "whole items, rows the same across a wave");
+    static constexpr int kWork = N * 8 * 8;
+    static constexpr bool fast = true;
     struct Raw {
         float a[N][8], s[N][8];
     };
@@ -45,23 +52,27 @@ struct BackDy {
             src[i] = p.dy + (int64_t)min(m0 + (i * NT + t) % BM, p.O - 1) * p.dy_o;
         }
     }
-    __device__ __forceinline__ void load(Raw& x, int k0) const {
+    __device__ __forceinline__ void load_fast(Raw& x, int k0) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int r = k0 + 8 * g[i];
-            if (k0 + 32 <= R) {
-                const float* const q = src[i] + r * ld;
+            const float* const q = src[i] + r * ld;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x.a[i][e] = q[e * ld];
-                    x.s[i][e] = scale[r + e];
-                }
-            } else {
+            for (int e = 0; e < 8; ++e) {
+                x.a[i][e] = q[e * ld];
+                x.s[i][e] = uniform_load(scale + r + e);
+            }
+        }
+    }
+    __device__ __forceinline__ void load(Raw& x, int k0) const {
+        if (k0 + 32 <= R) return load_fast(x, k0);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x.a[i][e] = r + e < R ? src[i][(r + e) * ld] : 0.f;
-                    x.s[i][e] = r + e < R ? scale[r + e] : 0.f;
-                }
+        for (int i = 0; i < N; ++i) {
+            const int r = k0 + 8 * g[i];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x.a[i][e] = r + e < R ? src[i][(r + e) * ld] : 0.f;
+                x.s[i][e] = r + e < R ? uniform_load(scale + r + e) : 0.f;
             }
         }
     }
@@ -90,14 +101,16 @@ struct BackQ {
     static constexpr int N = BN * 2 / NT, kRun = BN / 4 + 2, kGroup = 4 * kRun * 16,
                          kBytes = 4 * kGroup;
     static_assert(N * NT == BN * 2, "whole items");
+    static constexpr int kWork = N * 16 * 2;
     struct Raw {
         uint32_t q[N][4];
     };
     const int8_t* src[N];             // the item's inputs, row 0
     int64_t ld;
     int R, t, left[N];                // inputs from the item's first on
+    bool fast;                        // whole items in this workgroup's tile
     __device__ __forceinline__ static int entry(int c) { return (c & 3) * kRun + (c >> 2); }
-    __device__ __forceinline__ BackQ(const BackParams& p, int n0, int t_) : ld(p.q_r), R(p.R), t(t_) {
+    __device__ __forceinline__ BackQ(const BackParams& p, int n0, int t_) : ld(p.q_r), R(p.R), t(t_), fast(n0 + BN <= p.C) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = n0 + (i * NT + t) % (BN / 4) * 4;
@@ -105,24 +118,31 @@ struct BackQ {
             left[i] = p.C - c;
         }
     }
+    __device__ __forceinline__ void load_fast(Raw& x, int k0) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int8_t* const q = src[i] + (k0 + 4 * ((i * NT + t) / (BN / 4))) * ld;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x.q[i][e] = *reinterpret_cast<const row_codes*>(q + e * ld);
+        }
+    }
     __device__ __forceinline__ void load(Raw& x, int k0) const {
+        if (k0 + 32 <= R && fast) return load_fast(x, k0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int r = k0 + 4 * ((i * NT + t) / (BN / 4));
-            if (k0 + 32 <= R && left[i] >= 4) {
-                const int8_t* const q = src[i] + r * ld;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x.q[i][e] = *reinterpret_cast<const row_codes*>(q + e * ld);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t v = 0;
+            for (int e = 0; e < 4; ++e) {
+                const int8_t* const q = src[i] + (r + e) * ld;
+                uint32_t v = 0;
+                if (r + e < R && left[i] >= 4) {
+                    v = *reinterpret_cast<const row_codes*>(q);
+                } else {
 #pragma unroll
                     for (int b = 0; b < 4; ++b)
-                        if (r + e < R && b < left[i])
-                            v |= (uint32_t)(uint8_t)src[i][(r + e) * ld + b] << (8 * b);
-                    x.q[i][e] = v;
+                        if (r + e < R && b < left[i]) v |= (uint32_t)(uint8_t)q[b] << (8 * b);
                 }
+                x.q[i][e] = v;
             }
         }
     }

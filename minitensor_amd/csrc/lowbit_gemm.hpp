@@ -22,17 +22,24 @@
 
 namespace mtk {
 
-// The parts of eight values.  What is left of an infinity or a NaN (a NaN) is
+// Keeps the compiler from taking a packed value apart again (it rounded the low half a second
+// time rather than shift it: two instructions more per pair).
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
+// The parts of eight values (6.5 instructions each).  What is left of an infinity or a NaN (a NaN) is
 // made zero, so that its products are those of fp32: the middle of (r, r, 0)
 // is r, and 0 where r is a NaN.
 __device__ __forceinline__ void cut8(const float (&x)[8], u32x4& h, u32x4& m, u32x4& l) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        h[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
+        h[i] = opaque(bf16_pair(x[2 * i], x[2 * i + 1]));
         float r0 = x[2 * i] - bf16_lo(h[i]), r1 = x[2 * i + 1] - bf16_hi(h[i]);
         r0 = __builtin_amdgcn_fmed3f(r0, r0, 0.f);
         r1 = __builtin_amdgcn_fmed3f(r1, r1, 0.f);
-        m[i] = bf16_pair(r0, r1);
+        m[i] = opaque(bf16_pair(r0, r1));
         l[i] = bf16_pair(r0 - bf16_lo(m[i]), r1 - bf16_hi(m[i]));
     }
 }
@@ -83,16 +90,25 @@ __device__ __forceinline__ void lb_tile(int b, int tm, int tn, int& im, int& in)
 
 // The loop.  LA, LB: loaders with
 //   Raw                          what a thread holds of a chunk
-//   load(Raw&, int k0)           chunk of 32 k from k0 on, zero past the end
+//   fast                         whether load_fast may be called at all
+//   load_fast(Raw&, int k0)      chunk of 32 k from k0 on, all of them below kEnd()
+//   load(Raw&, int k0)           any chunk, zero past the end
 //   store(const Raw&, char*)     converted, to its part of the buffer
-//   kBytes, entry(row)           LDS size of a part, and the entry of a row in a group
+//   kBytes, kGroup, entry(row)   LDS size of a part and of a group of eight k, and the
+//                                entry of a row in a group
+//   kWork                        vector instructions of store
 // P: parts of A.  GC: chunks (1, 2 or 4) whose sums are taken on the matrix unit;
-// flush(k) adds those that end before k to the result and is called in order.
+// flush(k) adds those of the group that holds k - 1 to the result; called in order, for
+// groups of four chunks a step late, beside the next group's first MFMAs (for
+// shorter ones that took more registers than there are).
 template <int P, int GC, int MB, int NB, class LA, class LB, class Flush>
 __device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_begin, int k_end, int ra,
                                            int rb, int lane, f32x16 (&acc)[MB][NB], Flush flush) {
     constexpr int BUF = P * LA::kBytes + LB::kBytes;
+    constexpr int NM = 2 * P * MB * NB, NR = P * MB + NB;     // MFMAs, and reads of half a chunk
     const int nk = (k_end - k_begin + 31) >> 5;
+    // chunks that load_fast takes: all but a partial one
+    const int whole = la.fast && lb.fast ? (k_end - k_begin) >> 5 : 0;
     const int half = lane >> 5, row = lane & 31;
     typename LA::Raw xa, ya;
     typename LB::Raw xb, yb;
@@ -137,28 +153,61 @@ __device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_beg
                     }
         }
     };
-    // Chunk c out of LDS; a, b hold chunk c+1 and take chunk c+3, na, nb hold c+2.
+    // Chunk c = 4n + s out of LDS; a, b hold chunk c+1, na, nb take chunk c+2.
     auto step = [&](int c, int s, typename LA::Raw& a, typename LB::Raw& b, typename LA::Raw& na,
-                    typename LB::Raw& nb) {
+                    typename LB::Raw& nb, auto fast) {
         lb_barrier();
-        fetch(na, nb, c + 2);
+        if constexpr (fast) {             // (past the last chunk: that chunk again)
+            const int k = k_begin + 32 * min(c + 2, nk - 1);
+            la.load_fast(na, k);
+            lb.load_fast(nb, k);
+            __builtin_amdgcn_sched_barrier(0);
+        } else {
+            fetch(na, nb, c + 2);
+        }
+        if (GC == 4 && s == 0 && c > 0) flush(k_begin + 32 * c);
         multiply(smem + (s & 1) * BUF, s % GC == 0);
-        if (c + 1 < nk) put(a, b, (s + 1) & 1);
-        if (s % GC == GC - 1 || c + 1 == nk) flush(k_begin + 32 * (c + 1));
+        if (fast || c + 1 < nk) put(a, b, (s + 1) & 1);
+        if constexpr (fast) {
+            // the conversions beside the MFMAs: after them, as the compiler has it,
+            // the matrix unit stood still meanwhile
+            constexpr int NV = (LA::kWork + LB::kWork + NM - 1) / NM + 1;
+            __builtin_amdgcn_sched_group_barrier(0x100, NR, 0);
+#pragma unroll
+            for (int g = 0; g < NM; ++g) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (g < NR) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, NV, 0);
+            }
+        }
+        if (GC < 4 && (s % GC == GC - 1 || c + 1 == nk)) {
+            if constexpr (fast) __builtin_amdgcn_sched_barrier(0);
+            flush(k_begin + 32 * (c + 1));
+        }
     };
     if (nk <= 0) return;
     fetch(xa, xb, 0);
     fetch(ya, yb, 1);
     put(xa, xb, 0);
-    for (int c = 0; c < nk; c += 4) {
-        step(c, 0, ya, yb, xa, xb);
-        if (c + 1 >= nk) break;
-        step(c + 1, 1, xa, xb, ya, yb);
-        if (c + 2 >= nk) break;
-        step(c + 2, 2, ya, yb, xa, xb);
-        if (c + 3 >= nk) break;
-        step(c + 3, 3, xa, xb, ya, yb);
+    int c = 0;
+    constexpr std::true_type kFast{};
+    constexpr std::false_type kAny{};
+    for (; c + 4 <= whole && (c + 6 <= whole || whole == nk); c += 4) {
+        step(c, 0, ya, yb, xa, xb, kFast);
+        step(c + 1, 1, xa, xb, ya, yb, kFast);
+        step(c + 2, 2, ya, yb, xa, xb, kFast);
+        step(c + 3, 3, xa, xb, ya, yb, kFast);
     }
+    for (; c < nk; c += 4) {
+        step(c, 0, ya, yb, xa, xb, kAny);
+        if (c + 1 >= nk) break;
+        step(c + 1, 1, xa, xb, ya, yb, kAny);
+        if (c + 2 >= nk) break;
+        step(c + 2, 2, ya, yb, xa, xb, kAny);
+        if (c + 3 >= nk) break;
+        step(c + 3, 3, xa, xb, ya, yb, kAny);
+    }
+    if (GC == 4) flush(k_end);
 }
 
 // Block element r of a lane: row 8*(r/4) + 4*(lane/32) + r%4, column lane%32.

@@ -36,15 +36,14 @@ struct Q4Params {
 };
 
 // The eight codes of a dword, over 16, as bf16 (exact): v_cvt_off_f32_i4 gives
-// a code over 16, whose low half as fp32 is zero.  19 instructions.
+// a code over 16, whose low half as fp32 is zero.  13 instructions.
 __device__ __forceinline__ u32x4 q4_unpack(uint32_t w) {
+    const uint32_t odd = w >> 4;
     u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t a = __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4(w >> (8 * i)));
-        const uint32_t b = __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4(w >> (8 * i + 4)));
-        r[i] = __builtin_amdgcn_perm(b, a, 0x07060302);
-    }
+    for (int i = 0; i < 4; ++i)
+        r[i] = bf16_exact(__builtin_amdgcn_cvt_off_f32_i4((w >> (8 * i)) & 0xff),
+                          __builtin_amdgcn_cvt_off_f32_i4((odd >> (8 * i)) & 0xff));
     return r;
 }
 constexpr float kQ4Unit = 16.f;
@@ -211,6 +210,7 @@ template <bool Q8, int BM, int NT>
 struct Q4X {
     static constexpr int N = BM * 4 / NT, kGroup = lb_group<BM>(), kBytes = lb_plane<BM>();
     static_assert(N * NT == BM * 4, "whole items");
+    static constexpr int kWork = N * 8 * (Q8 ? 2 : 7);
     struct Raw {
         float a[Q8 ? 1 : N][8];
         u32x2 q[Q8 ? N : 1];
@@ -219,8 +219,10 @@ struct Q4X {
     const float* x[N];
     const int8_t* q[N];
     int t;
+    bool fast;                        // a row's inputs are neighbours
     __device__ __forceinline__ static int entry(int row) { return row; }
-    __device__ __forceinline__ Q4X(const Q4Params& p_, int m0, int t_) : p(p_), t(t_) {
+    __device__ __forceinline__ Q4X(const Q4Params& p_, int m0, int t_)
+        : p(p_), t(t_), fast(Q8 || p_.x_k == 1) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {                      // (rows past M: the last, not stored)
             const int64_t m = min(m0 + ((i * NT + t) >> 2), p.M - 1);
@@ -228,7 +230,25 @@ struct Q4X {
             else x[i] = p.x + m * p.x_m;
         }
     }
+    __device__ __forceinline__ void load_fast(Raw& r, int k0) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int k = k0 + 8 * (t & 3);
+            if constexpr (Q8) {
+                r.q[i] = *reinterpret_cast<const u32x2_u*>(q[i] + k);
+            } else {
+                const rowf4 a = *reinterpret_cast<const rowf4_u*>(x[i] + k);
+                const rowf4 b = *reinterpret_cast<const rowf4_u*>(x[i] + k + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    r.a[i][e] = a[e];
+                    r.a[i][4 + e] = b[e];
+                }
+            }
+        }
+    }
     __device__ __forceinline__ void load(Raw& r, int k0) const {
+        if (fast && k0 + 32 <= p.K) return load_fast(r, k0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int k = k0 + 8 * (t & 3);
@@ -258,6 +278,8 @@ template <int BN, int NT>
 struct Q4W {
     static constexpr int N = BN * 4 / NT, kGroup = lb_group<BN>(), kBytes = lb_plane<BN>();
     static_assert(N * NT == BN * 4, "whole items");
+    static constexpr int kWork = N * 14;
+    static constexpr bool fast = true;
     struct Raw {
         uint32_t w[N];
     };
@@ -270,7 +292,8 @@ struct Q4W {
             w[i] = p.w + (int64_t)min(n0 + ((i * NT + t) >> 2), p.N - 1) * p.w_n + 4 * (t & 3);
     }
     // (chunks are whole in the packed rows: k0 is a multiple of 32 below kp)
-    __device__ __forceinline__ void load(Raw& r, int k0) const {
+    __device__ __forceinline__ void load(Raw& r, int k0) const { load_fast(r, k0); }
+    __device__ __forceinline__ void load_fast(Raw& r, int k0) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) r.w[i] = *reinterpret_cast<const uint32_t*>(w[i] + (k0 >> 1));
     }
@@ -303,24 +326,33 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) q4_gemm(Q4Params 
     LB lb(p, n0, t);
     f32x16 sum[MB][NB], acc[MB][NB];
     zero_blocks<MB, NB>(sum);
-    // the scale of the lane's columns in the group that is being summed
+    // the scales of the lane's columns, in the group that is being summed and the next one
+    const int last = (p.K - 1) / G;
     const float* sr[NB];
-    float sc[NB];
+    float sc[NB], next[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
         sr[j] = p.s + (int64_t)min(n0 + rb + 32 * j + (lane & 31), p.N - 1) * p.s_n;
         sc[j] = sr[j][kb / G];
+        next[j] = sr[j][min(kb / G + 1, last)];
     }
     lb_product<P, G / 32, MB, NB>(la, lb, smem, kb, ke, ra, rb, lane, acc, [&](int k) {
+        const int g = min((k - 1) / G + 2, last);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const float s = sc[j] * kQ4Unit;
-            if (k < ke) sc[j] = sr[j][k / G];
+            sc[j] = next[j];
+            next[j] = sr[j][g];
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     sum[i][j][r] = __builtin_fmaf(acc[i][j][r], s, sum[i][j][r]);
+            // here, and not four groups' together at the end of the loop, as the compiler
+            // had it: their sums do not fit the registers
+            if constexpr (G < 128)
+#pragma unroll
+                for (int i = 0; i < MB; ++i) asm volatile("" : "+v"(sum[i][j]));
         }
     });
     const bool part = p.splits > 1;
