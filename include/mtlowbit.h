@@ -40,7 +40,7 @@ typedef struct mt_rows_q8 {
  * the low half of byte packed[r*row_stride + i], input 2i+1 the high half,
  * two's complement (-8..7).  Rows are 16*ceil(k/32) bytes, the inputs past k in
  * the last 16 being read but not used.  packed and row_stride: multiples of 16;
- * n below 2^26. */
+ * n below 2^26, scale_stride below 2^22 unless n <= 1. */
 typedef struct mt_weight_q4 {
     uint8_t* packed;
     float* scale;

@@ -16,6 +16,7 @@ namespace {
 
 constexpr int64_t kMaxDim = (int64_t)1 << 31;   // extents are 32-bit inside the kernels
 constexpr int64_t kMaxOut = (int64_t)1 << 26;   // rows of a 4-bit weight (32 threads each in a grid)
+constexpr int64_t kMaxScaleStride = (int64_t)1 << 22;   // a tile's 256 rows of scales within 32 bits of bytes
 constexpr int kCus = 256;                       // what plans fill (MI355X)
 
 int launched() {
@@ -49,7 +50,7 @@ bool valid(const mt_weight_q4* W) {
         return false;
     if (W->n == 0 || W->k == 0) return true;
     if (!W->packed || !W->scale || ((uintptr_t)W->packed & 15) || (W->row_stride & 15)) return false;
-    return W->n == 1 || (W->row_stride >= (W->k + 31) / 32 * 16 &&
+    return W->n == 1 || (W->scale_stride < kMaxScaleStride && W->row_stride >= (W->k + 31) / 32 * 16 &&
                          W->scale_stride >= (W->k + W->group - 1) / W->group);
 }
 

@@ -36,42 +36,47 @@ struct BackDy {
     static constexpr int N = BM * 4 / NT, kGroup = lb_group<BM>(), kBytes = lb_plane<BM>();
     static_assert(N * NT == BM * 4 && BM % 64 == 0, "whole items, rows the same across a wave");
     static constexpr int kWork = N * 8 * 8;
-    static constexpr bool fast = true;
+    static constexpr bool kLate = true;
     struct Raw {
         float a[N][8], s[N][8];
     };
-    const float* src[N];              // output of the item, row 0
+    const float* base;                // output m0, row 0
+    uint32_t off[N];                  // of the item's output, in elements
     const float* scale;
-    int64_t ld;
-    int R, t, g[N];
+    int64_t ld, so;
+    int R, t, last, g[N];
+    bool fast;                        // the tile's outputs within 32 bits of bytes
     __device__ __forceinline__ static int entry(int row) { return row; }
-    __device__ __forceinline__ BackDy(const BackParams& p, int m0, int t_) : scale(p.scale), ld(p.dy_r), R(p.R), t(t_) {
+    __device__ __forceinline__ BackDy(const BackParams& p, int m0, int t_)
+        : base(p.dy + m0 * p.dy_o), scale(p.scale), ld(p.dy_r), so(p.dy_o), R(p.R), t(t_),
+          last(p.O - 1 - m0), fast(p.dy_o < (1 << 22)) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < N; ++i) {                      // (outputs past O: the last, not stored)
             g[i] = __builtin_amdgcn_readfirstlane((i * NT + t) / BM);
-            src[i] = p.dy + (int64_t)min(m0 + (i * NT + t) % BM, p.O - 1) * p.dy_o;
+            off[i] = (uint32_t)min((i * NT + t) % BM, last) * (uint32_t)so;
         }
     }
     __device__ __forceinline__ void load_fast(Raw& x, int k0) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int r = k0 + 8 * g[i];
-            const float* const q = src[i] + r * ld;
+            const float* q = base + r * ld;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x.a[i][e] = q[e * ld];
+            for (int e = 0; e < 8; ++e, q += ld) {
+                x.a[i][e] = q[off[i]];
                 x.s[i][e] = uniform_load(scale + r + e);
             }
         }
     }
     __device__ __forceinline__ void load(Raw& x, int k0) const {
-        if (k0 + 32 <= R) return load_fast(x, k0);
+        if (fast && k0 + 32 <= R) return load_fast(x, k0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int r = k0 + 8 * g[i];
+            const float* const q = base + min((i * NT + t) % BM, last) * so;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x.a[i][e] = r + e < R ? src[i][(r + e) * ld] : 0.f;
+                x.a[i][e] = r + e < R ? q[(r + e) * ld] : 0.f;
                 x.s[i][e] = r + e < R ? uniform_load(scale + r + e) : 0.f;
             }
         }
@@ -105,42 +110,46 @@ struct BackQ {
     struct Raw {
         uint32_t q[N][4];
     };
-    const int8_t* src[N];             // the item's inputs, row 0
+    const int8_t* base;               // input n0, row 0
+    uint32_t off[N];                  // of the item from its wave's first row on
     int64_t ld;
-    int R, t, left[N];                // inputs from the item's first on
+    int R, t, left, row[N];           // inputs from n0 on; the wave's first row in a chunk
     bool fast;                        // whole items in this workgroup's tile
     __device__ __forceinline__ static int entry(int c) { return (c & 3) * kRun + (c >> 2); }
-    __device__ __forceinline__ BackQ(const BackParams& p, int n0, int t_) : ld(p.q_r), R(p.R), t(t_), fast(n0 + BN <= p.C) {
+    __device__ __forceinline__ BackQ(const BackParams& p, int n0, int t_)
+        : base(p.q + n0), ld(p.q_r), R(p.R), t(t_), left(p.C - n0),
+          fast(BN <= left && p.q_r < (1 << 28)) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = n0 + (i * NT + t) % (BN / 4) * 4;
-            src[i] = p.q + c;
-            left[i] = p.C - c;
+            const int r = 4 * ((i * NT + t) / (BN / 4));
+            row[i] = __builtin_amdgcn_readfirstlane(r);
+            off[i] = (uint32_t)((i * NT + t) % (BN / 4) * 4) + (uint32_t)(r - row[i]) * (uint32_t)ld;
         }
     }
     __device__ __forceinline__ void load_fast(Raw& x, int k0) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int8_t* const q = src[i] + (k0 + 4 * ((i * NT + t) / (BN / 4))) * ld;
+            const int8_t* q = base + (k0 + row[i]) * ld;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x.q[i][e] = *reinterpret_cast<const row_codes*>(q + e * ld);
+            for (int e = 0; e < 4; ++e, q += ld)
+                x.q[i][e] = *reinterpret_cast<const row_codes*>(q + off[i]);
         }
     }
     __device__ __forceinline__ void load(Raw& x, int k0) const {
         if (k0 + 32 <= R && fast) return load_fast(x, k0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int r = k0 + 4 * ((i * NT + t) / (BN / 4));
+            const int r = k0 + 4 * ((i * NT + t) / (BN / 4)), c = (i * NT + t) % (BN / 4) * 4;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int8_t* const q = src[i] + (r + e) * ld;
+                const int8_t* const q = base + (r + e) * ld + c;
                 uint32_t v = 0;
-                if (r + e < R && left[i] >= 4) {
+                if (r + e < R && c + 4 <= left) {
                     v = *reinterpret_cast<const row_codes*>(q);
                 } else {
 #pragma unroll
                     for (int b = 0; b < 4; ++b)
-                        if (r + e < R && b < left[i]) v |= (uint32_t)(uint8_t)q[b] << (8 * b);
+                        if (r + e < R && c + b < left) v |= (uint32_t)(uint8_t)q[b] << (8 * b);
                 }
                 x.q[i][e] = v;
             }

@@ -95,7 +95,8 @@ __device__ __forceinline__ void lb_tile(int b, int tm, int tn, int& im, int& in)
 //   load(Raw&, int k0)           any chunk, zero past the end
 //   store(const Raw&, char*)     converted, to its part of the buffer
 //   kBytes, kGroup, entry(row)   LDS size of a part and of a group of eight k, and the
-//                                entry of a row in a group
+//                                entry of a row in a group: entry(32a + b) = entry(32a)
+//                                + entry(b)
 //   kWork                        vector instructions of store
 // P: parts of A.  GC: chunks (1, 2 or 4) whose sums are taken on the matrix unit;
 // flush(k) adds those of the group that holds k - 1 to the result; called in order, for
@@ -106,6 +107,7 @@ __device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_beg
                                            int rb, int lane, f32x16 (&acc)[MB][NB], Flush flush) {
     constexpr int BUF = P * LA::kBytes + LB::kBytes;
     constexpr int NM = 2 * P * MB * NB, NR = P * MB + NB;     // MFMAs, and reads of half a chunk
+    constexpr bool kLate = GC == 4 && (MB * NB < 4 || LA::kLate);
     const int nk = (k_end - k_begin + 31) >> 5;
     // chunks that load_fast takes: all but a partial one
     const int whole = la.fast && lb.fast ? (k_end - k_begin) >> 5 : 0;
@@ -131,12 +133,13 @@ __device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_beg
             for (int q = P - 1; q >= 0; --q)
 #pragma unroll
                 for (int i = 0; i < MB; ++i)
-                    a[q][i] = *reinterpret_cast<const u32x4*>(buf + q * LA::kBytes + g * LA::kGroup +
-                                                              LA::entry(ra + 32 * i + row) * 16);
+                    a[q][i] = *reinterpret_cast<const u32x4*>(
+                        buf + q * LA::kBytes + g * LA::kGroup +
+                        (LA::entry(row) + LA::entry(ra) + LA::entry(32 * i)) * 16);
 #pragma unroll
             for (int j = 0; j < NB; ++j)
-                b[j] = *reinterpret_cast<const u32x4*>(pb + g * LB::kGroup +
-                                                       LB::entry(rb + 32 * j + row) * 16);
+                b[j] = *reinterpret_cast<const u32x4*>(
+                    pb + g * LB::kGroup + (LB::entry(row) + LB::entry(rb) + LB::entry(32 * j)) * 16);
 #pragma unroll
             for (int q = P - 1; q >= 0; --q)
 #pragma unroll
@@ -153,35 +156,29 @@ __device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_beg
                     }
         }
     };
-    // Chunk c = 4n + s out of LDS; a, b hold chunk c+1, na, nb take chunk c+2.
+    // Chunk c = 4n + s, all of whose neighbours are whole: no branch, so that the
+    // conversions can go beside the MFMAs (after them, as the compiler had it, the
+    // matrix unit stood still meanwhile).  a, b hold chunk c+1, na, nb take chunk c+2.
     auto step = [&](int c, int s, typename LA::Raw& a, typename LB::Raw& b, typename LA::Raw& na,
-                    typename LB::Raw& nb, auto fast) {
+                    typename LB::Raw& nb) {
         lb_barrier();
-        if constexpr (fast) {             // (past the last chunk: that chunk again)
-            const int k = k_begin + 32 * min(c + 2, nk - 1);
-            la.load_fast(na, k);
-            lb.load_fast(nb, k);
-            __builtin_amdgcn_sched_barrier(0);
-        } else {
-            fetch(na, nb, c + 2);
-        }
-        if (GC == 4 && s == 0 && c > 0) flush(k_begin + 32 * c);
+        const int k = k_begin + 32 * min(c + 2, nk - 1);   // (past the last one: that again)
+        la.load_fast(na, k);
+        lb.load_fast(nb, k);
+        __builtin_amdgcn_sched_barrier(0);
+        if (kLate && s == 0 && c > 0) flush(k_begin + 32 * c);
         multiply(smem + (s & 1) * BUF, s % GC == 0);
-        if (fast || c + 1 < nk) put(a, b, (s + 1) & 1);
-        if constexpr (fast) {
-            // the conversions beside the MFMAs: after them, as the compiler has it,
-            // the matrix unit stood still meanwhile
-            constexpr int NV = (LA::kWork + LB::kWork + NM - 1) / NM + 1;
-            __builtin_amdgcn_sched_group_barrier(0x100, NR, 0);
+        put(a, b, (s + 1) & 1);
+        constexpr int NV = (LA::kWork + LB::kWork + NM - 1) / NM + 1;
+        __builtin_amdgcn_sched_group_barrier(0x100, NR, 0);
 #pragma unroll
-            for (int g = 0; g < NM; ++g) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                if (g < NR) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, NV, 0);
-            }
+        for (int g = 0; g < NM; ++g) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (g < NR) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, NV, 0);
         }
-        if (GC < 4 && (s % GC == GC - 1 || c + 1 == nk)) {
-            if constexpr (fast) __builtin_amdgcn_sched_barrier(0);
+        if (!kLate && s % GC == GC - 1) {
+            __builtin_amdgcn_sched_barrier(0);
             flush(k_begin + 32 * (c + 1));
         }
     };
@@ -190,24 +187,31 @@ __device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_beg
     fetch(ya, yb, 1);
     put(xa, xb, 0);
     int c = 0;
-    constexpr std::true_type kFast{};
-    constexpr std::false_type kAny{};
     for (; c + 4 <= whole && (c + 6 <= whole || whole == nk); c += 4) {
-        step(c, 0, ya, yb, xa, xb, kFast);
-        step(c + 1, 1, xa, xb, ya, yb, kFast);
-        step(c + 2, 2, ya, yb, xa, xb, kFast);
-        step(c + 3, 3, xa, xb, ya, yb, kFast);
+        step(c, 0, ya, yb, xa, xb);
+        step(c + 1, 1, xa, xb, ya, yb);
+        step(c + 2, 2, ya, yb, xa, xb);
+        step(c + 3, 3, xa, xb, ya, yb);
     }
-    for (; c < nk; c += 4) {
-        step(c, 0, ya, yb, xa, xb, kAny);
-        if (c + 1 >= nk) break;
-        step(c + 1, 1, xa, xb, ya, yb, kAny);
-        if (c + 2 >= nk) break;
-        step(c + 2, 2, ya, yb, xa, xb, kAny);
-        if (c + 3 >= nk) break;
-        step(c + 3, 3, xa, xb, ya, yb, kAny);
+    // the rest, in one rolled step
+    for (; c < nk; ++c) {
+        lb_barrier();
+        fetch(xa, xb, c + 2);
+        if (c % GC == 0) {
+            if (kLate && c > 0) flush(k_begin + 32 * c);
+            zero_blocks<MB, NB>(acc);
+        }
+        multiply(smem + (c & 1) * BUF, false);
+        if (c + 1 < nk) put(ya, yb, (c + 1) & 1);
+        const typename LA::Raw ta = xa;
+        const typename LB::Raw tb = xb;
+        xa = ya;
+        xb = yb;
+        ya = ta;
+        yb = tb;
+        if (!kLate && ((c + 1) % GC == 0 || c + 1 == nk)) flush(k_begin + 32 * (c + 1));
     }
-    if (GC == 4) flush(k_end);
+    if (kLate) flush(k_end);
 }
 
 // Block element r of a lane: row 8*(r/4) + 4*(lane/32) + r%4, column lane%32.

@@ -211,34 +211,40 @@ struct Q4X {
     static constexpr int N = BM * 4 / NT, kGroup = lb_group<BM>(), kBytes = lb_plane<BM>();
     static_assert(N * NT == BM * 4, "whole items");
     static constexpr int kWork = N * 8 * (Q8 ? 2 : 7);
-    struct Raw {
-        float a[Q8 ? 1 : N][8];
-        u32x2 q[Q8 ? N : 1];
+    static constexpr bool kLate = Q8;
+    struct RawX {
+        float a[N][8];
     };
+    struct RawQ {
+        u32x2 q[N];
+    };
+    using Raw = std::conditional_t<Q8, RawQ, RawX>;
+    using T = std::conditional_t<Q8, int8_t, float>;
     const Q4Params& p;
-    const float* x[N];
-    const int8_t* q[N];
-    int t;
-    bool fast;                        // a row's inputs are neighbours
+    const T* base;                    // row m0
+    uint32_t off[N];                  // of the item, in elements
+    int64_t ld;
+    int t, last;
+    bool fast;                        // a row's inputs are neighbours, the tile within 32 bits of bytes
     __device__ __forceinline__ static int entry(int row) { return row; }
-    __device__ __forceinline__ Q4X(const Q4Params& p_, int m0, int t_)
-        : p(p_), t(t_), fast(Q8 || p_.x_k == 1) {
+    __device__ __forceinline__ Q4X(const Q4Params& p_, int m0, int t_) : p(p_), t(t_), last(p_.M - 1 - m0) {
+        if constexpr (Q8) base = p.q, ld = p.q_m;
+        else base = p.x, ld = p.x_m;
+        base += m0 * ld;
+        fast = (Q8 || p.x_k == 1) && ld < (1 << 22);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {                      // (rows past M: the last, not stored)
-            const int64_t m = min(m0 + ((i * NT + t) >> 2), p.M - 1);
-            if constexpr (Q8) q[i] = p.q + m * p.q_m;
-            else x[i] = p.x + m * p.x_m;
-        }
+        for (int i = 0; i < N; ++i)                        // (rows past M: the last, not stored)
+            off[i] = (uint32_t)min((i * NT + t) >> 2, last) * (uint32_t)ld + 8 * (t & 3);
     }
     __device__ __forceinline__ void load_fast(Raw& r, int k0) const {
+        const T* const x = base + k0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int k = k0 + 8 * (t & 3);
             if constexpr (Q8) {
-                r.q[i] = *reinterpret_cast<const u32x2_u*>(q[i] + k);
+                r.q[i] = *reinterpret_cast<const u32x2_u*>(x + off[i]);
             } else {
-                const rowf4 a = *reinterpret_cast<const rowf4_u*>(x[i] + k);
-                const rowf4 b = *reinterpret_cast<const rowf4_u*>(x[i] + k + 4);
+                const rowf4 a = *reinterpret_cast<const rowf4_u*>(x + off[i]);
+                const rowf4 b = *reinterpret_cast<const rowf4_u*>(x + off[i] + 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     r.a[i][e] = a[e];
@@ -251,9 +257,9 @@ struct Q4X {
         if (fast && k0 + 32 <= p.K) return load_fast(r, k0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int k = k0 + 8 * (t & 3);
-            if constexpr (Q8) r.q[i] = q4_x8(p, q[i], k);
-            else q4_x8(p, x[i], k, r.a[i]);
+            const T* const x = base + min((i * NT + t) >> 2, last) * ld;
+            if constexpr (Q8) r.q[i] = q4_x8(p, x, k0 + 8 * (t & 3));
+            else q4_x8(p, x, k0 + 8 * (t & 3), r.a[i]);
         }
     }
     __device__ __forceinline__ void store(const Raw& r, char* buf) const {
@@ -279,23 +285,32 @@ struct Q4W {
     static constexpr int N = BN * 4 / NT, kGroup = lb_group<BN>(), kBytes = lb_plane<BN>();
     static_assert(N * NT == BN * 4, "whole items");
     static constexpr int kWork = N * 14;
-    static constexpr bool fast = true;
     struct Raw {
         uint32_t w[N];
     };
-    const uint8_t* w[N];
-    int kp, t;
+    const uint8_t* base;              // column n0
+    uint32_t off[N];                  // of the item, in bytes
+    int64_t ld;
+    int t, last;
+    bool fast;                        // the tile within 32 bits of bytes
     __device__ __forceinline__ static int entry(int c) { return c; }
-    __device__ __forceinline__ Q4W(const Q4Params& p, int n0, int t_) : kp((p.K + 31) & ~31), t(t_) {
+    __device__ __forceinline__ Q4W(const Q4Params& p, int n0, int t_)
+        : base(p.w + n0 * p.w_n), ld(p.w_n), t(t_), last(p.N - 1 - n0), fast(p.w_n < (1 << 23)) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)                        // (columns past N: the last)
-            w[i] = p.w + (int64_t)min(n0 + ((i * NT + t) >> 2), p.N - 1) * p.w_n + 4 * (t & 3);
+        for (int i = 0; i < N; ++i)                        // (columns past N: the last, not stored)
+            off[i] = (uint32_t)min((i * NT + t) >> 2, last) * (uint32_t)ld + 4 * (t & 3);
     }
-    // (chunks are whole in the packed rows: k0 is a multiple of 32 below kp)
-    __device__ __forceinline__ void load(Raw& r, int k0) const { load_fast(r, k0); }
+    // (chunks are whole in the packed rows)
     __device__ __forceinline__ void load_fast(Raw& r, int k0) const {
+        const uint8_t* const w = base + (k0 >> 1);
 #pragma unroll
-        for (int i = 0; i < N; ++i) r.w[i] = *reinterpret_cast<const uint32_t*>(w[i] + (k0 >> 1));
+        for (int i = 0; i < N; ++i) r.w[i] = *reinterpret_cast<const uint32_t*>(w + off[i]);
+    }
+    __device__ __forceinline__ void load(Raw& r, int k0) const {
+        const uint8_t* const w = base + (k0 >> 1) + 4 * (t & 3);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            r.w[i] = *reinterpret_cast<const uint32_t*>(w + min((i * NT + t) >> 2, last) * ld);
     }
     __device__ __forceinline__ void store(const Raw& r, char* buf) const {
 #pragma unroll
@@ -306,7 +321,8 @@ struct Q4W {
 };
 
 template <int BM, int BN, int WM, int WN, int G, bool Q8>
-__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) q4_gemm(Q4Params p) {
+__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, BM > 64 ? 2 : Q8 ? 4 : 3)
+q4_gemm(Q4Params p) {
     constexpr int P = Q8 ? 1 : 3;
     constexpr int WAVES_N = BN / WN, NT = BM / WM * WAVES_N * 64;
     constexpr int MB = WM / 32, NB = WN / 32;
@@ -328,13 +344,15 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) q4_gemm(Q4Params 
     zero_blocks<MB, NB>(sum);
     // the scales of the lane's columns, in the group that is being summed and the next one
     const int last = (p.K - 1) / G;
-    const float* sr[NB];
+    // (32-bit offsets from the tile's first column: the host limits s_n)
+    const float* const s0 = p.s + (int64_t)n0 * p.s_n;
+    uint32_t so[NB];
     float sc[NB], next[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-        sr[j] = p.s + (int64_t)min(n0 + rb + 32 * j + (lane & 31), p.N - 1) * p.s_n;
-        sc[j] = sr[j][kb / G];
-        next[j] = sr[j][min(kb / G + 1, last)];
+        so[j] = (uint32_t)min(rb + 32 * j + (lane & 31), p.N - 1 - n0) * (uint32_t)p.s_n;
+        sc[j] = (s0 + kb / G)[so[j]];
+        next[j] = (s0 + min(kb / G + 1, last))[so[j]];
     }
     lb_product<P, G / 32, MB, NB>(la, lb, smem, kb, ke, ra, rb, lane, acc, [&](int k) {
         const int g = min((k - 1) / G + 2, last);
@@ -342,7 +360,7 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) q4_gemm(Q4Params 
         for (int j = 0; j < NB; ++j) {
             const float s = sc[j] * kQ4Unit;
             sc[j] = next[j];
-            next[j] = sr[j][g];
+            next[j] = (s0 + g)[so[j]];
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
