@@ -106,7 +106,9 @@ struct BackQ {
     static constexpr int N = BN * 2 / NT, kRun = BN / 4 + 2, kGroup = 4 * kRun * 16,
                          kBytes = 4 * kGroup;
     static_assert(N * NT == BN * 2, "whole items");
-    static constexpr int kWork = N * 16 * 2;
+    static constexpr int kWork = N * 16 * 2, kReads = 0, kRaw = 0;
+    static constexpr bool kBlock = false;
+    struct Codes {};
     struct Raw {
         uint32_t q[N][4];
     };
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) back_dw(BackParam
     LB lb(p, n0, t);
     f32x16 sum[MB][NB], acc[MB][NB];
     zero_blocks<MB, NB>(sum);
-    lb_product<3, 4, MB, NB>(la, lb, smem, rbeg, rend, ra, rb, lane, acc, [&](int) {
+    lb_product<3, 4, MB, NB>(la, lb, smem, rbeg, rend, ra, rb, lane, acc, [&](auto, int) {
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll

@@ -29,6 +29,12 @@ __device__ __forceinline__ uint32_t opaque(uint32_t v) {
     return v;
 }
 
+// The value anew, for a path beside the loop: not kept in registers through it.
+__device__ __forceinline__ int anew(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // The parts of eight values (6.5 instructions each).  What is left of an infinity or a NaN (a NaN) is
 // made zero, so that its products are those of fp32: the middle of (r, r, 0)
 // is r, and 0 where r is a NaN.
@@ -88,40 +94,55 @@ __device__ __forceinline__ void lb_tile(int b, int tm, int tn, int& im, int& in)
     in = w / h;
 }
 
-// The loop.  LA, LB: loaders with
+// The loop.  LA: loader with
 //   Raw                          what a thread holds of a chunk
 //   fast                         whether load_fast may be called at all
-//   load_fast(Raw&, int k0)      chunk of 32 k from k0 on, all of them below kEnd()
+//   load_fast(Raw&, int k0)      chunk of 32 k from k0 on, all of them below k_end
 //   load(Raw&, int k0)           any chunk, zero past the end
 //   store(const Raw&, char*)     converted, to its part of the buffer
 //   kBytes, kGroup, entry(row)   LDS size of a part and of a group of eight k, and the
 //                                entry of a row in a group: entry(32a + b) = entry(32a)
 //                                + entry(b)
 //   kWork                        vector instructions of store
+// LB: the same, or (kBlock) with its values brought to LDS as they are, in blocks of four
+// chunks, from which each chunk is converted:
+//   load(Raw&, int k0)           block from k0 on; past the end anything
+//   stage(const Raw&, char*)     to LDS, kRaw bytes
+//   Codes, peek(Codes&, const char*, int s)   chunk s of the block there
+//   store(const Codes&, char*)
+// smem: two buffers of a chunk, and two of kRaw.
 // P: parts of A.  GC: chunks (1, 2 or 4) whose sums are taken on the matrix unit;
-// flush(k) adds those of the group that holds k - 1 to the result; called in order, for
-// groups of four chunks a step late, beside the next group's first MFMAs (for
-// shorter ones that took more registers than there are).
+// flush(i, block) adds those of group i of a block (from k_begin on) to the result; called
+// in order, with kLate a step late, beside the next group's first MFMAs.
 template <int P, int GC, int MB, int NB, class LA, class LB, class Flush>
 __device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_begin, int k_end, int ra,
                                            int rb, int lane, f32x16 (&acc)[MB][NB], Flush flush) {
     constexpr int BUF = P * LA::kBytes + LB::kBytes;
     constexpr int NM = 2 * P * MB * NB, NR = P * MB + NB;     // MFMAs, and reads of half a chunk
     constexpr bool kLate = GC == 4 && (MB * NB < 4 || LA::kLate);
-    const int nk = (k_end - k_begin + 31) >> 5;
+    const int nk = (k_end - k_begin + 31) >> 5, nb = (nk + 3) >> 2;
     // chunks that load_fast takes: all but a partial one
     const int whole = la.fast && lb.fast ? (k_end - k_begin) >> 5 : 0;
     const int half = lane >> 5, row = lane & 31;
+    char* const raw = smem + 2 * BUF;
     typename LA::Raw xa, ya;
-    typename LB::Raw xb, yb;
+    typename LB::Raw xb, yb;              // (kBlock: the next block is in xb)
     auto fetch = [&](typename LA::Raw& a, typename LB::Raw& b, int c) {
         if (c >= nk) return;
         la.load(a, k_begin + 32 * c);
-        lb.load(b, k_begin + 32 * c);
+        if constexpr (!LB::kBlock) lb.load(b, k_begin + 32 * c);
     };
-    auto put = [&](const typename LA::Raw& a, const typename LB::Raw& b, int buf) {
-        la.store(a, smem + buf * BUF);
-        lb.store(b, smem + buf * BUF + P * LA::kBytes);
+    // (what is read from LDS is read before anything is written there: the compiler
+    // keeps the order of the two)
+    typename LB::Codes codes;
+    auto peek = [&](int c) {
+        if constexpr (LB::kBlock) lb.peek(codes, raw + (c >> 2 & 1) * LB::kRaw, c & 3);
+    };
+    auto put = [&](const typename LA::Raw& a, const typename LB::Raw& b, int c) {
+        char* const buf = smem + (c & 1) * BUF;
+        la.store(a, buf);
+        if constexpr (LB::kBlock) lb.store(codes, buf + P * LA::kBytes);
+        else lb.store(b, buf + P * LA::kBytes);
     };
     auto multiply = [&](const char* buf, bool first) {
         const char* const pb = buf + P * LA::kBytes;
@@ -158,60 +179,93 @@ __device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_beg
     };
     // Chunk c = 4n + s, all of whose neighbours are whole: no branch, so that the
     // conversions can go beside the MFMAs (after them, as the compiler had it, the
-    // matrix unit stood still meanwhile).  a, b hold chunk c+1, na, nb take chunk c+2.
-    auto step = [&](int c, int s, typename LA::Raw& a, typename LB::Raw& b, typename LA::Raw& na,
-                    typename LB::Raw& nb) {
+    // matrix unit stood still meanwhile).  a, b hold chunk c+1, na, nxb take chunk c+2.
+    auto step = [&](int n, auto sc, typename LA::Raw& a, typename LB::Raw& b, typename LA::Raw& na,
+                    typename LB::Raw& nxb) {
+        constexpr int s = sc;
+        const int c = 4 * n + s;
         lb_barrier();
         const int k = k_begin + 32 * min(c + 2, nk - 1);   // (past the last one: that again)
         la.load_fast(na, k);
-        lb.load_fast(nb, k);
+        if constexpr (!LB::kBlock) lb.load_fast(nxb, k);
+        if constexpr (LB::kBlock)
+            if constexpr (s == 0) lb.load_fast(xb, k_begin + 128 * min(n + 1, nb - 1));
         __builtin_amdgcn_sched_barrier(0);
-        if (kLate && s == 0 && c > 0) flush(k_begin + 32 * c);
+        if constexpr (kLate && s == 0)
+            if (n > 0) flush(std::integral_constant<int, 0>{}, n - 1);
+        peek(c + 1);
         multiply(smem + (s & 1) * BUF, s % GC == 0);
-        put(a, b, (s + 1) & 1);
+        if constexpr (LB::kBlock)
+            if constexpr (s == 2) lb.stage(xb, raw + (n + 1 & 1) * LB::kRaw);
+        put(a, b, c + 1);
+        // (the second half's fragments as late as they may come: registers)
+        constexpr int R0 = NM / 2 > NR + 2 ? NM / 2 - NR - 2 : 0;
         constexpr int NV = (LA::kWork + LB::kWork + NM - 1) / NM + 1;
-        __builtin_amdgcn_sched_group_barrier(0x100, NR, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, NR + LB::kReads, 0);
 #pragma unroll
         for (int g = 0; g < NM; ++g) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (g < NR) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            if (g >= R0 && g < R0 + NR) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x002, NV, 0);
         }
-        if (!kLate && s % GC == GC - 1) {
+        if constexpr (!kLate && s % GC == GC - 1) {
             __builtin_amdgcn_sched_barrier(0);
-            flush(k_begin + 32 * (c + 1));
+            flush(std::integral_constant<int, s / GC>{}, n);
         }
     };
+    using std::integral_constant;
     if (nk <= 0) return;
     fetch(xa, xb, 0);
     fetch(ya, yb, 1);
+    if constexpr (LB::kBlock) {
+        lb.load(xb, k_begin);
+        lb.stage(xb, raw);
+        lb_barrier();
+    }
+    peek(0);
     put(xa, xb, 0);
-    int c = 0;
-    for (; c + 4 <= whole && (c + 6 <= whole || whole == nk); c += 4) {
-        step(c, 0, ya, yb, xa, xb);
-        step(c + 1, 1, xa, xb, ya, yb);
-        step(c + 2, 2, ya, yb, xa, xb);
-        step(c + 3, 3, xa, xb, ya, yb);
+    int n = 0;
+    for (; 4 * n + 4 <= whole && (4 * n + 6 <= whole || whole == nk); ++n) {
+        step(n, integral_constant<int, 0>{}, ya, yb, xa, xb);
+        step(n, integral_constant<int, 1>{}, xa, xb, ya, yb);
+        step(n, integral_constant<int, 2>{}, ya, yb, xa, xb);
+        step(n, integral_constant<int, 3>{}, xa, xb, ya, yb);
     }
     // the rest, in one rolled step
-    for (; c < nk; ++c) {
+    for (int c = 4 * n; c < nk; ++c) {
         lb_barrier();
         fetch(xa, xb, c + 2);
+        if constexpr (LB::kBlock)
+            if ((c & 3) == 0 && (c >> 2) + 1 < nb) lb.load(xb, k_begin + 32 * (c + 4));
         if (c % GC == 0) {
-            if (kLate && c > 0) flush(k_begin + 32 * c);
+            if (kLate && c > 0) flush(integral_constant<int, 0>{}, (c >> 2) - 1);
             zero_blocks<MB, NB>(acc);
         }
+        if (c + 1 < nk) peek(c + 1);
         multiply(smem + (c & 1) * BUF, false);
-        if (c + 1 < nk) put(ya, yb, (c + 1) & 1);
+        if constexpr (LB::kBlock)
+            if ((c & 3) == 2 && (c >> 2) + 1 < nb) lb.stage(xb, raw + ((c >> 2) + 1 & 1) * LB::kRaw);
+        if (c + 1 < nk) put(ya, yb, c + 1);
         const typename LA::Raw ta = xa;
-        const typename LB::Raw tb = xb;
         xa = ya;
-        xb = yb;
         ya = ta;
-        yb = tb;
-        if (!kLate && ((c + 1) % GC == 0 || c + 1 == nk)) flush(k_begin + 32 * (c + 1));
+        if constexpr (!LB::kBlock) {
+            const typename LB::Raw tb = xb;
+            xb = yb;
+            yb = tb;
+        }
+        if (!kLate && ((c + 1) % GC == 0 || c + 1 == nk)) {
+            const int i = (c & 3) / GC;
+            if (i == 0) flush(integral_constant<int, 0>{}, c >> 2);
+            if constexpr (GC < 4)
+                if (i == 1) flush(integral_constant<int, 1>{}, c >> 2);
+            if constexpr (GC < 2) {
+                if (i == 2) flush(integral_constant<int, 2>{}, c >> 2);
+                if (i == 3) flush(integral_constant<int, 3>{}, c >> 2);
+            }
+        }
     }
-    if (kLate) flush(k_end);
+    if (kLate) flush(integral_constant<int, 0>{}, nb - 1);
 }
 
 // Block element r of a lane: row 8*(r/4) + 4*(lane/32) + r%4, column lane%32.

@@ -255,11 +255,12 @@ struct Q4X {
     }
     __device__ __forceinline__ void load(Raw& r, int k0) const {
         if (fast && k0 + 32 <= p.K) return load_fast(r, k0);
+        const int v = anew(t);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const T* const x = base + min((i * NT + t) >> 2, last) * ld;
-            if constexpr (Q8) r.q[i] = q4_x8(p, x, k0 + 8 * (t & 3));
-            else q4_x8(p, x, k0 + 8 * (t & 3), r.a[i]);
+            const T* const x = base + min((i * NT + v) >> 2, last) * ld;
+            if constexpr (Q8) r.q[i] = q4_x8(p, x, k0 + 8 * (v & 3));
+            else q4_x8(p, x, k0 + 8 * (v & 3), r.a[i]);
         }
     }
     __device__ __forceinline__ void store(const Raw& r, char* buf) const {
@@ -279,56 +280,137 @@ struct Q4X {
     }
 };
 
-// The weight as B: a thread takes eight inputs (a dword of codes) of a column.
-template <int BN, int NT>
+// The weight as B: a thread converts eight inputs (a dword of codes) of a column per chunk.
+// BLOCK: blocks of 128 inputs of a column, 64 bytes, go to LDS as they lie in memory and are
+// converted from there: loaded chunk by chunk, each 64 bytes are asked for four times, and
+// the lines of a narrow tile, of which a CU holds several, do not stay in L1 meanwhile.
+// The 16-byte pieces of a column change places by its number, so that the dwords of 16
+// columns fall on different banks.  (The wide tile has no registers left for it.)
+template <int BN, int NT, bool BLOCK>
 struct Q4W {
     static constexpr int N = BN * 4 / NT, kGroup = lb_group<BN>(), kBytes = lb_plane<BN>();
     static_assert(N * NT == BN * 4, "whole items");
-    static constexpr int kWork = N * 14;
-    struct Raw {
+    static constexpr bool kBlock = BLOCK;
+    static constexpr int kWork = N * 14, kReads = BLOCK ? N : 0, kRaw = BLOCK ? BN * 64 : 0;
+    struct Codes {
         uint32_t w[N];
     };
+    struct Block {
+        u32x4 w[N];
+    };
+    using Raw = std::conditional_t<BLOCK, Block, Codes>;
     const uint8_t* base;              // column n0
-    uint32_t off[N];                  // of the item, in bytes
+    uint32_t off[N];                  // of the item's column, in bytes
     int64_t ld;
-    int t, last;
+    int t, last, end;                 // bytes of a row
     bool fast;                        // the tile within 32 bits of bytes
+    static constexpr int kStep = NT / 4;   // columns between a thread's items, a multiple of 16
     __device__ __forceinline__ static int entry(int c) { return c; }
+    __device__ __forceinline__ static int slot(int c, int piece) {
+        return c * 64 + ((piece ^ (c >> 2)) & 3) * 16;
+    }
     __device__ __forceinline__ Q4W(const Q4Params& p, int n0, int t_)
-        : base(p.w + n0 * p.w_n), ld(p.w_n), t(t_), last(p.N - 1 - n0), fast(p.w_n < (1 << 23)) {
+        : base(p.w + n0 * p.w_n), ld(p.w_n), t(t_), last(p.N - 1 - n0),
+          end(((p.K + 31) & ~31) >> 1), fast(p.w_n < (1 << 23)) {
 #pragma unroll
         for (int i = 0; i < N; ++i)                        // (columns past N: the last, not stored)
-            off[i] = (uint32_t)min((i * NT + t) >> 2, last) * (uint32_t)ld + 4 * (t & 3);
+            off[i] = (uint32_t)min((i * NT + t) >> 2, last) * (uint32_t)ld;
     }
-    // (chunks are whole in the packed rows)
+    // The thread's place in a row from input k0 on: a dword of a chunk (whole in a row), or a
+    // piece of a block (past the end of the row its last piece again: x is zero there).
+    __device__ __forceinline__ int place(int k0) const {
+        if constexpr (BLOCK) return min((k0 >> 1) + 16 * (t & 3), end - 16);
+        else return (k0 >> 1) + 4 * (t & 3);
+    }
+    using Item = std::conditional_t<BLOCK, u32x4, uint32_t>;
     __device__ __forceinline__ void load_fast(Raw& r, int k0) const {
-        const uint8_t* const w = base + (k0 >> 1);
 #pragma unroll
-        for (int i = 0; i < N; ++i) r.w[i] = *reinterpret_cast<const uint32_t*>(w + off[i]);
+        for (int i = 0; i < N; ++i)
+            r.w[i] = *reinterpret_cast<const Item*>(base + (off[i] + (uint32_t)place(k0)));
     }
     __device__ __forceinline__ void load(Raw& r, int k0) const {
-        const uint8_t* const w = base + (k0 >> 1) + 4 * (t & 3);
+        if (fast) return load_fast(r, k0);
+        const int v = anew(t);
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            r.w[i] = *reinterpret_cast<const uint32_t*>(w + min((i * NT + t) >> 2, last) * ld);
+            r.w[i] = *reinterpret_cast<const Item*>(base + min((i * NT + v) >> 2, last) * ld +
+                                                    place(k0));
     }
-    __device__ __forceinline__ void store(const Raw& r, char* buf) const {
+    __device__ __forceinline__ void stage(const Block& r, char* raw) const {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            *reinterpret_cast<u32x4*>(buf + (t & 3) * kGroup + ((i * NT + t) >> 2) * 16) =
-                q4_unpack(r.w[i]);
+            *reinterpret_cast<u32x4*>(raw + slot(t >> 2, t & 3) + i * kStep * 64) = r.w[i];
+    }
+    __device__ __forceinline__ void peek(Codes& x, const char* raw, int s) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            x.w[i] = *reinterpret_cast<const uint32_t*>(
+                raw + ((slot(t >> 2, 0) + 4 * (t & 3)) ^ (16 * s)) + i * kStep * 64);
+    }
+    __device__ __forceinline__ void store(const Codes& x, char* buf) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            *reinterpret_cast<u32x4*>(buf + (t & 3) * kGroup + (t >> 2) * 16 + i * kStep * 16) =
+                q4_unpack(x.w[i]);
+    }
+};
+
+// The scales of a lane's NB columns, NG groups at a time: those that are being summed, and
+// the next ones, on their way.
+template <int NB, int G, int NG>
+struct Q4Scales {
+    typedef float Vec __attribute__((ext_vector_type(NG), aligned(4)));
+    const float* s0;                  // column n0
+    uint32_t off[NB];                 // (32 bits: the host limits s_n)
+    int groups;
+    float cur[NB][NG], next[NB][NG];
+    __device__ __forceinline__ Q4Scales(const Q4Params& p, int n0, int col, int k0)
+        : s0(p.s + (int64_t)n0 * p.s_n), groups((p.K + G - 1) / G) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            off[j] = (uint32_t)min(col + 32 * j, p.N - 1 - n0) * (uint32_t)p.s_n;
+        load(cur, k0 / G);
+        load(next, k0 / G + NG);
+    }
+    // Groups g0.. of every column; those past the last are never used.  One load per column,
+    // which starts early enough to end with the row.
+    __device__ __forceinline__ void load(float (&x)[NB][NG], int g0) const {
+        const int g = max(min(g0, groups - NG), 0), late = g0 - g;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const float* const q = s0 + g + off[j];
+            if (NG == 1 || groups >= NG) {
+                const Vec v = *reinterpret_cast<const Vec*>(q);
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    x[j][i] = v[i];
+#pragma unroll
+                    for (int d = 1; i + d < NG; ++d) x[j][i] = late == d ? v[i + d] : x[j][i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) x[j][i] = q[min(i, groups - 1)];
+            }
+        }
+    }
+    __device__ __forceinline__ void advance(int g0) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int i = 0; i < NG; ++i) cur[j][i] = next[j][i];
+        load(next, g0);
     }
 };
 
 template <int BM, int BN, int WM, int WN, int G, bool Q8>
-__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, BM > 64 ? 2 : Q8 ? 4 : 3)
+__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, BM > 64 || G == 32 ? 2 : 3)
 q4_gemm(Q4Params p) {
     constexpr int P = Q8 ? 1 : 3;
     constexpr int WAVES_N = BN / WN, NT = BM / WM * WAVES_N * 64;
     constexpr int MB = WM / 32, NB = WN / 32;
     using LA = Q4X<Q8, BM, NT>;
-    using LB = Q4W<BN, NT>;
-    __shared__ __attribute__((aligned(16))) char smem[2 * (P * LA::kBytes + LB::kBytes)];
+    using LB = Q4W<BN, NT, BN == 128>;
+    __shared__ __attribute__((aligned(16))) char smem[2 * (P * LA::kBytes + LB::kBytes + LB::kRaw)];
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int ra = wave / WAVES_N * WM, rb = wave % WAVES_N * WN;
@@ -342,36 +424,25 @@ q4_gemm(Q4Params p) {
     LB lb(p, n0, t);
     f32x16 sum[MB][NB], acc[MB][NB];
     zero_blocks<MB, NB>(sum);
-    // the scales of the lane's columns, in the group that is being summed and the next one
-    const int last = (p.K - 1) / G;
-    // (32-bit offsets from the tile's first column: the host limits s_n)
-    const float* const s0 = p.s + (int64_t)n0 * p.s_n;
-    uint32_t so[NB];
-    float sc[NB], next[NB];
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        so[j] = (uint32_t)min(rb + 32 * j + (lane & 31), p.N - 1 - n0) * (uint32_t)p.s_n;
-        sc[j] = (s0 + kb / G)[so[j]];
-        next[j] = (s0 + min(kb / G + 1, last))[so[j]];
-    }
-    lb_product<P, G / 32, MB, NB>(la, lb, smem, kb, ke, ra, rb, lane, acc, [&](int k) {
-        const int g = min((k - 1) / G + 2, last);
+    // (one load for all groups of 128 inputs where there are registers for them)
+    constexpr int GB = 128 / G, NG = BN == 128 ? GB : 1;
+    Q4Scales<NB, G, NG> sc(p, n0, rb + (lane & 31), kb);
+    lb_product<P, G / 32, MB, NB>(la, lb, smem, kb, ke, ra, rb, lane, acc, [&](auto i, int block) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const float s = sc[j] * kQ4Unit;
-            sc[j] = next[j];
-            next[j] = (s0 + g)[so[j]];
+            const float s = sc.cur[j][i % NG] * kQ4Unit;
 #pragma unroll
-            for (int i = 0; i < MB; ++i)
+            for (int m = 0; m < MB; ++m)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    sum[i][j][r] = __builtin_fmaf(acc[i][j][r], s, sum[i][j][r]);
+                    sum[m][j][r] = __builtin_fmaf(acc[m][j][r], s, sum[m][j][r]);
             // here, and not four groups' together at the end of the loop, as the compiler
             // had it: their sums do not fit the registers
             if constexpr (G < 128)
 #pragma unroll
-                for (int i = 0; i < MB; ++i) asm volatile("" : "+v"(sum[i][j]));
+                for (int m = 0; m < MB; ++m) asm volatile("" : "+v"(sum[m][j]));
         }
+        if constexpr (i % NG == NG - 1) sc.advance(kb / G + block * GB + i + 1 + NG);
     });
     const bool part = p.splits > 1;
 #pragma unroll
