@@ -41,7 +41,7 @@ struct BackDy {
         float a[N][8], s[N][8];
     };
     const float* base;                // output m0, row 0
-    uint32_t off[N];                  // of the item's output, in elements
+    uint32_t off[N];                  // of the item's output, in bytes
     const float* scale;
     int64_t ld, so;
     int R, t, last, g[N];
@@ -53,7 +53,7 @@ struct BackDy {
 #pragma unroll
         for (int i = 0; i < N; ++i) {                      // (outputs past O: the last, not stored)
             g[i] = __builtin_amdgcn_readfirstlane((i * NT + t) / BM);
-            off[i] = (uint32_t)min((i * NT + t) % BM, last) * (uint32_t)so;
+            off[i] = (uint32_t)min((i * NT + t) % BM, last) * (uint32_t)so * 4u;
         }
     }
     __device__ __forceinline__ void load_fast(Raw& x, int k0) const {
@@ -63,17 +63,18 @@ struct BackDy {
             const float* q = base + r * ld;
 #pragma unroll
             for (int e = 0; e < 8; ++e, q += ld) {
-                x.a[i][e] = q[off[i]];
+                x.a[i][e] = *at_bytes(q, off[i]);
                 x.s[i][e] = uniform_load(scale + r + e);
             }
         }
     }
     __device__ __forceinline__ void load(Raw& x, int k0) const {
         if (fast && k0 + 32 <= R) return load_fast(x, k0);
+        const int u = anew(t);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int r = k0 + 8 * g[i];
-            const float* const q = base + min((i * NT + t) % BM, last) * so;
+            const float* const q = base + min((i * NT + u) % BM, last) * so;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 x.a[i][e] = r + e < R ? q[(r + e) * ld] : 0.f;
@@ -134,14 +135,15 @@ struct BackQ {
             const int8_t* q = base + (k0 + row[i]) * ld;
 #pragma unroll
             for (int e = 0; e < 4; ++e, q += ld)
-                x.q[i][e] = *reinterpret_cast<const row_codes*>(q + off[i]);
+                x.q[i][e] = *reinterpret_cast<const row_codes*>(at_bytes(q, off[i]));
         }
     }
     __device__ __forceinline__ void load(Raw& x, int k0) const {
         if (k0 + 32 <= R && fast) return load_fast(x, k0);
+        const int u = anew(t);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int r = k0 + 4 * ((i * NT + t) / (BN / 4)), c = (i * NT + t) % (BN / 4) * 4;
+            const int r = k0 + 4 * ((i * NT + u) / (BN / 4)), c = (i * NT + u) % (BN / 4) * 4;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int8_t* const q = base + (r + e) * ld + c;
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) back_dw(BackParam
     LB lb(p, n0, t);
     f32x16 sum[MB][NB], acc[MB][NB];
     zero_blocks<MB, NB>(sum);
-    lb_product<3, 4, MB, NB>(la, lb, smem, rbeg, rend, ra, rb, lane, acc, [&](auto, int) {
+    lb_product<3, 4, BM == 64 ? 4 : 2, MB, NB>(la, lb, smem, rbeg, rend, ra, rb, lane, acc, [&](auto, int) {
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll

@@ -3,9 +3,11 @@
 // an operand B in 8 or 4 bits, on the bf16 matrix units.
 //
 // Tiles of BM x BN over chunks of 32 k, in two LDS buffers: while chunk c is multiplied,
-// chunk c+1, loaded into registers a chunk before, is converted to bf16 and written to
-// the other buffer, and chunk c+2 is on its way from memory.  One barrier per chunk; it
-// waits for LDS alone, so that the loads stay in flight across it.
+// chunk c+1, loaded into registers before, is converted to bf16 and written to the other
+// buffer, and the chunks up to c+D are on their way from memory.  One barrier per chunk; it
+// waits for LDS alone, so that the loads stay in flight across it.  (A third buffer, from
+// which the next chunk's first fragments came before the barrier, cost more in addresses
+// than it saved in waiting: the 2048-row prompt 4096 -> 8192 took 435 us against 402.)
 //
 // Each wave multiplies WM x WN in blocks of 32x32.  A's parts make a row three times
 // as dear as a column in LDS reads (three fragments, one for B) and four to five times
@@ -27,6 +29,14 @@ namespace mtk {
 __device__ __forceinline__ uint32_t opaque(uint32_t v) {
     asm("" : "+v"(v));
     return v;
+}
+
+// p moved on by a 32-bit number of bytes: one register beside a uniform p (the compiler
+// kept the number's 64 bits through the loop).
+template <class T>
+__device__ __forceinline__ const T* at_bytes(const T* p, uint32_t bytes) {
+    asm volatile("" : "+v"(bytes));
+    return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + bytes);
 }
 
 // The value anew, for a path beside the loop: not kept in registers through it.
@@ -111,26 +121,27 @@ __device__ __forceinline__ void lb_tile(int b, int tm, int tn, int& im, int& in)
 //   Codes, peek(Codes&, const char*, int s)   chunk s of the block there
 //   store(const Codes&, char*)
 // smem: two buffers of a chunk, and two of kRaw.
-// P: parts of A.  GC: chunks (1, 2 or 4) whose sums are taken on the matrix unit;
+// P: parts of A.  D: chunks ahead (2 or 4).  GC: chunks (1, 2 or 4) whose sums are taken on the matrix unit;
 // flush(i, block) adds those of group i of a block (from k_begin on) to the result; called
 // in order, with kLate a step late, beside the next group's first MFMAs.
-template <int P, int GC, int MB, int NB, class LA, class LB, class Flush>
+template <int P, int GC, int D, int MB, int NB, class LA, class LB, class Flush>
 __device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_begin, int k_end, int ra,
                                            int rb, int lane, f32x16 (&acc)[MB][NB], Flush flush) {
+    using std::integral_constant;
     constexpr int BUF = P * LA::kBytes + LB::kBytes;
-    constexpr int NM = 2 * P * MB * NB, NR = P * MB + NB;     // MFMAs, and reads of half a chunk
+    constexpr int NH = P * MB * NB, NR = P * MB + NB;         // MFMAs and reads of half a chunk
     constexpr bool kLate = GC == 4 && (MB * NB < 4 || LA::kLate);
     const int nk = (k_end - k_begin + 31) >> 5, nb = (nk + 3) >> 2;
     // chunks that load_fast takes: all but a partial one
     const int whole = la.fast && lb.fast ? (k_end - k_begin) >> 5 : 0;
     const int half = lane >> 5, row = lane & 31;
     char* const raw = smem + 2 * BUF;
-    typename LA::Raw xa, ya;
-    typename LB::Raw xb, yb;              // (kBlock: the next block is in xb)
-    auto fetch = [&](typename LA::Raw& a, typename LB::Raw& b, int c) {
+    typename LA::Raw xa[D];               // chunk c in xa[c % D]
+    typename LB::Raw xb[LB::kBlock ? 1 : D];   // (kBlock: the next block)
+    auto fetch = [&](int c, int slot) {
         if (c >= nk) return;
-        la.load(a, k_begin + 32 * c);
-        if constexpr (!LB::kBlock) lb.load(b, k_begin + 32 * c);
+        la.load(xa[slot], k_begin + 32 * c);
+        if constexpr (!LB::kBlock) lb.load(xb[slot], k_begin + 32 * c);
     };
     // (what is read from LDS is read before anything is written there: the compiler
     // keeps the order of the two)
@@ -138,122 +149,132 @@ __device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_beg
     auto peek = [&](int c) {
         if constexpr (LB::kBlock) lb.peek(codes, raw + (c >> 2 & 1) * LB::kRaw, c & 3);
     };
-    auto put = [&](const typename LA::Raw& a, const typename LB::Raw& b, int c) {
+    auto put = [&](int c, int slot) {
         char* const buf = smem + (c & 1) * BUF;
-        la.store(a, buf);
+        la.store(xa[slot], buf);
         if constexpr (LB::kBlock) lb.store(codes, buf + P * LA::kBytes);
-        else lb.store(b, buf + P * LA::kBytes);
+        else lb.store(xb[slot], buf + P * LA::kBytes);
     };
-    auto multiply = [&](const char* buf, bool first) {
-        const char* const pb = buf + P * LA::kBytes;
+    // the fragments of half h of the chunk in buf, and its MFMAs
+    struct Frags {
+        u32x4 a[P][MB], b[NB];
+    };
+    auto read = [&](Frags& f, const char* buf, int h) {
+        const int g = 2 * h + half;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            u32x4 a[P][MB], b[NB];
-            const int g = 2 * s + half;
+        for (int q = P - 1; q >= 0; --q)
 #pragma unroll
-            for (int q = P - 1; q >= 0; --q)
+            for (int i = 0; i < MB; ++i)
+                f.a[q][i] = *reinterpret_cast<const u32x4*>(
+                    buf + q * LA::kBytes + g * LA::kGroup +
+                    (LA::entry(row) + LA::entry(ra) + LA::entry(32 * i)) * 16);
 #pragma unroll
-                for (int i = 0; i < MB; ++i)
-                    a[q][i] = *reinterpret_cast<const u32x4*>(
-                        buf + q * LA::kBytes + g * LA::kGroup +
-                        (LA::entry(row) + LA::entry(ra) + LA::entry(32 * i)) * 16);
+        for (int j = 0; j < NB; ++j)
+            f.b[j] = *reinterpret_cast<const u32x4*>(
+                buf + P * LA::kBytes + g * LB::kGroup +
+                (LB::entry(row) + LB::entry(rb) + LB::entry(32 * j)) * 16);
+    };
+    auto multiply = [&](const Frags& f, bool first) {
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
-                b[j] = *reinterpret_cast<const u32x4*>(
-                    pb + g * LB::kGroup + (LB::entry(row) + LB::entry(rb) + LB::entry(32 * j)) * 16);
+        for (int q = P - 1; q >= 0; --q)
 #pragma unroll
-            for (int q = P - 1; q >= 0; --q)
+            for (int i = 0; i < MB; ++i)
 #pragma unroll
-                for (int i = 0; i < MB; ++i)
+                for (int j = 0; j < NB; ++j) {
+                    f32x16 c = acc[i][j];
+                    if (first && q == P - 1)
 #pragma unroll
-                    for (int j = 0; j < NB; ++j) {
-                        f32x16 c = acc[i][j];
-                        if (first && s == 0 && q == P - 1)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) c[r] = 0.f;
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            __builtin_bit_cast(bf16x8, a[q][i]), __builtin_bit_cast(bf16x8, b[j]), c,
-                            0, 0, 0);
-                    }
-        }
+                        for (int r = 0; r < 16; ++r) c[r] = 0.f;
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        __builtin_bit_cast(bf16x8, f.a[q][i]), __builtin_bit_cast(bf16x8, f.b[j]), c,
+                        0, 0, 0);
+                }
     };
     // Chunk c = 4n + s, all of whose neighbours are whole: no branch, so that the
     // conversions can go beside the MFMAs (after them, as the compiler had it, the
-    // matrix unit stood still meanwhile).  a, b hold chunk c+1, na, nxb take chunk c+2.
-    auto step = [&](int n, auto sc, typename LA::Raw& a, typename LB::Raw& b, typename LA::Raw& na,
-                    typename LB::Raw& nxb) {
+    // matrix unit stood still meanwhile).
+    auto step = [&](int n, auto sc) {
         constexpr int s = sc;
         const int c = 4 * n + s;
         lb_barrier();
-        const int k = k_begin + 32 * min(c + 2, nk - 1);   // (past the last one: that again)
-        la.load_fast(na, k);
-        if constexpr (!LB::kBlock) lb.load_fast(nxb, k);
+        // (past the last chunk: that again)
+        const int k = k_begin + 32 * min(c + D, nk - 1);
+        la.load_fast(xa[s % D], k);
+        if constexpr (!LB::kBlock) lb.load_fast(xb[s % D], k);
         if constexpr (LB::kBlock)
-            if constexpr (s == 0) lb.load_fast(xb, k_begin + 128 * min(n + 1, nb - 1));
+            if constexpr (s == 3) lb.load_fast(xb[0], k_begin + 128 * min(n + 2, nb - 1));
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (kLate && s == 0)
-            if (n > 0) flush(std::integral_constant<int, 0>{}, n - 1);
+            if (n > 0) flush(integral_constant<int, 0>{}, n - 1);
+        const char* const buf = smem + (s & 1) * BUF;
+        Frags f, g;
         peek(c + 1);
-        multiply(smem + (s & 1) * BUF, s % GC == 0);
+        read(f, buf, 0);
+        read(g, buf, 1);
+        multiply(f, s % GC == 0);
+        multiply(g, false);
         if constexpr (LB::kBlock)
-            if constexpr (s == 2) lb.stage(xb, raw + (n + 1 & 1) * LB::kRaw);
-        put(a, b, c + 1);
+            if constexpr (s == 2) lb.stage(xb[0], raw + (n + 1 & 1) * LB::kRaw);
+        put(c + 1, (s + 1) % D);
+        constexpr int NV = (LA::kWork + LB::kWork + 2 * NH - 1) / (2 * NH) + 1;
         // (the second half's fragments as late as they may come: registers)
-        constexpr int R0 = NM / 2 > NR + 2 ? NM / 2 - NR - 2 : 0;
-        constexpr int NV = (LA::kWork + LB::kWork + NM - 1) / NM + 1;
-        __builtin_amdgcn_sched_group_barrier(0x100, NR + LB::kReads, 0);
+        constexpr int R0 = NH > NR + 2 ? NH - NR - 2 : 0;
+        __builtin_amdgcn_sched_group_barrier(0x100, LB::kReads + NR, 0);
 #pragma unroll
-        for (int g = 0; g < NM; ++g) {
+        for (int i = 0; i < 2 * NH; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (g >= R0 && g < R0 + NR) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            if (i >= R0 && i < R0 + NR) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x002, NV, 0);
         }
         if constexpr (!kLate && s % GC == GC - 1) {
             __builtin_amdgcn_sched_barrier(0);
-            flush(std::integral_constant<int, s / GC>{}, n);
+            flush(integral_constant<int, s / GC>{}, n);
         }
     };
-    using std::integral_constant;
     if (nk <= 0) return;
-    fetch(xa, xb, 0);
-    fetch(ya, yb, 1);
+#pragma unroll
+    for (int c = 0; c < D; ++c) fetch(c, c);
     if constexpr (LB::kBlock) {
-        lb.load(xb, k_begin);
-        lb.stage(xb, raw);
+        lb.load(xb[0], k_begin);
+        lb.stage(xb[0], raw);
+        if (nb > 1) lb.load(xb[0], k_begin + 128);
         lb_barrier();
     }
     peek(0);
-    put(xa, xb, 0);
+    put(0, 0);
     int n = 0;
-    for (; 4 * n + 4 <= whole && (4 * n + 6 <= whole || whole == nk); ++n) {
-        step(n, integral_constant<int, 0>{}, ya, yb, xa, xb);
-        step(n, integral_constant<int, 1>{}, xa, xb, ya, yb);
-        step(n, integral_constant<int, 2>{}, ya, yb, xa, xb);
-        step(n, integral_constant<int, 3>{}, xa, xb, ya, yb);
+    for (; 4 * n + 4 <= whole && (4 * n + 4 + D <= whole || whole == nk); ++n) {
+        step(n, integral_constant<int, 0>{});
+        step(n, integral_constant<int, 1>{});
+        step(n, integral_constant<int, 2>{});
+        step(n, integral_constant<int, 3>{});
     }
-    // the rest, in one rolled step
+    // the rest, in one rolled step; the chunks move up in their places instead
     for (int c = 4 * n; c < nk; ++c) {
         lb_barrier();
-        fetch(xa, xb, c + 2);
-        if constexpr (LB::kBlock)
-            if ((c & 3) == 0 && (c >> 2) + 1 < nb) lb.load(xb, k_begin + 32 * (c + 4));
+#pragma unroll
+        for (int i = 0; i + 1 < D; ++i) {
+            xa[i] = xa[i + 1];
+            if constexpr (!LB::kBlock) xb[i] = xb[i + 1];
+        }
+        fetch(c + D, D - 1);
         if (c % GC == 0) {
             if (kLate && c > 0) flush(integral_constant<int, 0>{}, (c >> 2) - 1);
             zero_blocks<MB, NB>(acc);
         }
         if (c + 1 < nk) peek(c + 1);
-        multiply(smem + (c & 1) * BUF, false);
-        if constexpr (LB::kBlock)
-            if ((c & 3) == 2 && (c >> 2) + 1 < nb) lb.stage(xb, raw + ((c >> 2) + 1 & 1) * LB::kRaw);
-        if (c + 1 < nk) put(ya, yb, c + 1);
-        const typename LA::Raw ta = xa;
-        xa = ya;
-        ya = ta;
-        if constexpr (!LB::kBlock) {
-            const typename LB::Raw tb = xb;
-            xb = yb;
-            yb = tb;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            Frags f;
+            read(f, smem + (c & 1) * BUF, h);
+            multiply(f, false);
         }
+        if constexpr (LB::kBlock) {
+            if ((c & 3) == 2 && (c >> 2) + 1 < nb)
+                lb.stage(xb[0], raw + ((c >> 2) + 1 & 1) * LB::kRaw);
+            if ((c & 3) == 3 && (c >> 2) + 2 < nb) lb.load(xb[0], k_begin + 32 * (c + 5));
+        }
+        if (c + 1 < nk) put(c + 1, 0);
         if (!kLate && ((c + 1) % GC == 0 || c + 1 == nk)) {
             const int i = (c & 3) / GC;
             if (i == 0) flush(integral_constant<int, 0>{}, c >> 2);

@@ -222,7 +222,7 @@ struct Q4X {
     using T = std::conditional_t<Q8, int8_t, float>;
     const Q4Params& p;
     const T* base;                    // row m0
-    uint32_t off[N];                  // of the item, in elements
+    uint32_t off[N];                  // of the item, in bytes
     int64_t ld;
     int t, last;
     bool fast;                        // a row's inputs are neighbours, the tile within 32 bits of bytes
@@ -234,17 +234,18 @@ struct Q4X {
         fast = (Q8 || p.x_k == 1) && ld < (1 << 22);
 #pragma unroll
         for (int i = 0; i < N; ++i)                        // (rows past M: the last, not stored)
-            off[i] = (uint32_t)min((i * NT + t) >> 2, last) * (uint32_t)ld + 8 * (t & 3);
+            off[i] = ((uint32_t)min((i * NT + t) >> 2, last) * (uint32_t)ld + 8 * (t & 3)) *
+                     (uint32_t)sizeof(T);
     }
     __device__ __forceinline__ void load_fast(Raw& r, int k0) const {
-        const T* const x = base + k0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
+            const T* const x = at_bytes(base + k0, off[i]);
             if constexpr (Q8) {
-                r.q[i] = *reinterpret_cast<const u32x2_u*>(x + off[i]);
+                r.q[i] = *reinterpret_cast<const u32x2_u*>(x);
             } else {
-                const rowf4 a = *reinterpret_cast<const rowf4_u*>(x + off[i]);
-                const rowf4 b = *reinterpret_cast<const rowf4_u*>(x + off[i] + 4);
+                const rowf4 a = *reinterpret_cast<const rowf4_u*>(x);
+                const rowf4 b = *reinterpret_cast<const rowf4_u*>(x + 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     r.a[i][e] = a[e];
@@ -361,14 +362,14 @@ template <int NB, int G, int NG>
 struct Q4Scales {
     typedef float Vec __attribute__((ext_vector_type(NG), aligned(4)));
     const float* s0;                  // column n0
-    uint32_t off[NB];                 // (32 bits: the host limits s_n)
+    uint32_t off[NB];                 // in bytes (the host limits s_n)
     int groups;
     float cur[NB][NG], next[NB][NG];
     __device__ __forceinline__ Q4Scales(const Q4Params& p, int n0, int col, int k0)
         : s0(p.s + (int64_t)n0 * p.s_n), groups((p.K + G - 1) / G) {
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-            off[j] = (uint32_t)min(col + 32 * j, p.N - 1 - n0) * (uint32_t)p.s_n;
+            off[j] = (uint32_t)min(col + 32 * j, p.N - 1 - n0) * (uint32_t)p.s_n * 4u;
         load(cur, k0 / G);
         load(next, k0 / G + NG);
     }
@@ -378,7 +379,7 @@ struct Q4Scales {
         const int g = max(min(g0, groups - NG), 0), late = g0 - g;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const float* const q = s0 + g + off[j];
+            const float* const q = at_bytes(s0 + g, off[j]);
             if (NG == 1 || groups >= NG) {
                 const Vec v = *reinterpret_cast<const Vec*>(q);
 #pragma unroll
@@ -410,7 +411,8 @@ q4_gemm(Q4Params p) {
     constexpr int MB = WM / 32, NB = WN / 32;
     using LA = Q4X<Q8, BM, NT>;
     using LB = Q4W<BN, NT, BN == 128>;
-    __shared__ __attribute__((aligned(16))) char smem[2 * (P * LA::kBytes + LB::kBytes + LB::kRaw)];
+    __shared__ __attribute__((aligned(16))) char smem[2 * (P * LA::kBytes + LB::kBytes) +
+                                                         2 * LB::kRaw];
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int ra = wave / WAVES_N * WM, rb = wave % WAVES_N * WN;
@@ -427,7 +429,8 @@ q4_gemm(Q4Params p) {
     // (one load for all groups of 128 inputs where there are registers for them)
     constexpr int GB = 128 / G, NG = BN == 128 ? GB : 1;
     Q4Scales<NB, G, NG> sc(p, n0, rb + (lane & 31), kb);
-    lb_product<P, G / 32, MB, NB>(la, lb, smem, kb, ke, ra, rb, lane, acc, [&](auto i, int block) {
+    lb_product<P, G / 32, BM == 64 ? 4 : 2, MB, NB>(
+        la, lb, smem, kb, ke, ra, rb, lane, acc, [&](auto i, int block) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const float s = sc.cur[j][i % NG] * kQ4Unit;
