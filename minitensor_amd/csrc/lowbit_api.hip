@@ -170,8 +170,8 @@ int run_q4(Q4Params p, int64_t M, const mt_weight_q4* W, const float* bias, int6
     const Q4Plan plan = q4_plan(M, W->n, W->k, W->group, Q8);
     if (W->k == 0) {                                  // no inputs: the bias alone
         const unsigned blocks = (unsigned)std::min<int64_t>((M * W->n + 255) / 256, 4096);
-        hipLaunchKernelGGL(lb_sum, dim3(blocks), dim3(256), 0, s, nullptr, 0, p.M, p.N, bias,
-                           bias_stride, p.y, p.y_m, p.y_n, 0.f);
+        hipLaunchKernelGGL(lb_sum, dim3(blocks), dim3(256), 0, s,
+                           LbSum{nullptr, 0, p.M, p.N, bias, bias_stride, p.y, p.y_m, p.y_n});
         return launched();
     }
     if (plan.ws > 0 && (!workspace || ws_bytes < plan.ws)) return MT_ERR_WORKSPACE;
@@ -188,8 +188,8 @@ int run_q4(Q4Params p, int64_t M, const mt_weight_q4* W, const float* bias, int6
     else go(std::integral_constant<int, 128>{});
     if (p.splits > 1) {
         const unsigned blocks = (unsigned)std::min<int64_t>((M * W->n + 255) / 256, 8192);
-        hipLaunchKernelGGL(lb_sum, dim3(blocks), dim3(256), 0, s, p.part, p.splits, p.M, p.N, bias,
-                           bias_stride, p.y, p.y_m, p.y_n, 0.f);
+        hipLaunchKernelGGL(lb_sum, dim3(blocks), dim3(256), 0, s,
+                           LbSum{p.part, p.splits, p.M, p.N, bias, bias_stride, p.y, p.y_m, p.y_n});
     }
     return launched();
 }
@@ -210,7 +210,7 @@ BackPlan back_plan(int64_t R, int64_t O, int64_t C) {
     s = std::max<int64_t>(1, (blocks + per - 1) / per);
     p.splits = (int)s;
     p.rps = (int)(per * 128);
-    p.ws = s > 1 ? (size_t)(s * O * C) * 4 : 0;
+    p.ws = s > 1 ? (size_t)(s * (O * C + O)) * 4 : 0;
     return p;
 }
 
@@ -375,11 +375,15 @@ int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const m
         p.C = (int)X->cols;
         p.splits = plan.splits;
         p.r_per_split = plan.rps;
-        const unsigned sum_blocks = (unsigned)std::min<int64_t>(((int64_t)p.O * p.C + 255) / 256, 8192);
-        if (p.R == 0) {                               // no rows: beta_w·dW
-            hipLaunchKernelGGL(lb_sum, dim3(sum_blocks), dim3(256), 0, s, nullptr, 0, p.O, p.C,
-                               nullptr, 0, p.dw, p.dw_o, p.dw_c, beta_w);
-        } else {
+        if (db) {
+            p.db = db;
+            p.db_stride = db_stride;
+            p.beta_b = beta_b;
+            p.part_b = p.part + (int64_t)p.splits * p.O * p.C;
+        }
+        const LbSum sum{p.part, p.R > 0 ? p.splits : 0, p.O, p.C, nullptr, 0, p.dw, p.dw_o, p.dw_c,
+                        beta_w, p.part_b, db, db_stride, beta_b, p.O};
+        if (p.R > 0) {
             const int64_t tiles = (int64_t)((p.O + plan.bm - 1) / plan.bm) *
                                   ((p.C + plan.bn - 1) / plan.bn) * p.splits;
             if (plan.bm == 64)
@@ -388,11 +392,13 @@ int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const m
             else
                 hipLaunchKernelGGL((back_dw<128, 256, 32, 128>), dim3((unsigned)tiles), dim3(512), 0,
                                    s, p);
-            if (p.splits > 1)
-                hipLaunchKernelGGL(lb_sum, dim3(sum_blocks), dim3(256), 0, s, p.part, p.splits, p.O,
-                                   p.C, nullptr, 0, p.dw, p.dw_o, p.dw_c, beta_w);
         }
-        if (launched() != MT_OK) return MT_ERR_HIP;
+        if (p.R == 0 || p.splits > 1) {               // (no rows: beta·dW, beta·db)
+            const int64_t n = (int64_t)p.O * p.C + p.O;
+            hipLaunchKernelGGL(lb_sum, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 8192)),
+                               dim3(256), 0, s, sum);
+        }
+        return launched();
     }
     if (db) return mt_colsum_f32(dY, db, db_stride, beta_b, stream);
     return MT_OK;

@@ -20,6 +20,10 @@ struct BackParams {
     int64_t dw_o, dw_c;
     float beta;
     float* part;                      // [splits][O][C] where splits > 1
+    float* db;                        // [O], nullptr: not wanted
+    int64_t db_stride;
+    float beta_b;
+    float* part_b;                    // [splits][O]
     int R, O, C;
     int splits, r_per_split;          // a multiple of 128
 };
@@ -30,8 +34,9 @@ __device__ __forceinline__ float uniform_load(const float* p) {
 }
 
 // Both operands lie across k (= r).  dY: a thread takes eight rows of one output,
-// consecutive outputs on consecutive lanes.
-template <int BM, int NT>
+// consecutive outputs on consecutive lanes.  SUM: the rows of each output added up as they
+// pass (the bias gradient; dY is read once for both).
+template <int BM, int NT, bool SUM>
 struct BackDy {
     static constexpr int N = BM * 4 / NT, kGroup = lb_group<BM>(), kBytes = lb_plane<BM>();
     static_assert(N * NT == BM * 4 && BM % 64 == 0, "whole items, rows the same across a wave");
@@ -45,6 +50,7 @@ struct BackDy {
     const float* scale;
     int64_t ld, so;
     int R, t, last, g[N];
+    float sum[N];
     bool fast;                        // the tile's outputs within 32 bits of bytes
     __device__ __forceinline__ static int entry(int row) { return row; }
     __device__ __forceinline__ BackDy(const BackParams& p, int m0, int t_)
@@ -54,6 +60,7 @@ struct BackDy {
         for (int i = 0; i < N; ++i) {                      // (outputs past O: the last, not stored)
             g[i] = __builtin_amdgcn_readfirstlane((i * NT + t) / BM);
             off[i] = (uint32_t)min((i * NT + t) % BM, last) * (uint32_t)so * 4u;
+            sum[i] = 0.f;
         }
     }
     __device__ __forceinline__ void load_fast(Raw& x, int k0) const {
@@ -82,9 +89,14 @@ struct BackDy {
             }
         }
     }
-    __device__ __forceinline__ void store(const Raw& x, char* buf) const {
+    __device__ __forceinline__ void store(const Raw& x, char* buf, bool live) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
+            if constexpr (SUM) {
+                const float* const a = x.a[i];
+                const float v = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
+                sum[i] += live ? v : 0.f;
+            }
             float a[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) a[e] = x.a[i][e] * x.s[i][e];
@@ -180,7 +192,7 @@ template <int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) back_dw(BackParams p) {
     constexpr int WAVES_N = BN / WN, NT = BM / WM * WAVES_N * 64;
     constexpr int MB = WM / 32, NB = WN / 32;
-    using LA = BackDy<BM, NT>;
+    using LA = BackDy<BM, NT, true>;
     using LB = BackQ<BN, NT>;
     __shared__ __attribute__((aligned(16))) char smem[2 * (3 * LA::kBytes + LB::kBytes)];
     const int t = threadIdx.x, lane = t & 63;
@@ -192,38 +204,66 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) back_dw(BackParam
     lb_tile(blockIdx.x - split * tiles_m * tiles_n, tiles_m, tiles_n, im, in);
     const int m0 = im * BM, n0 = in * BN;
     const int rbeg = split * p.r_per_split, rend = min(p.R, rbeg + p.r_per_split);
-    LA la(p, m0, t);
+    const bool part = p.splits > 1;
     LB lb(p, n0, t);
     f32x16 sum[MB][NB], acc[MB][NB];
     zero_blocks<MB, NB>(sum);
-    lb_product<3, 4, BM == 64 ? 4 : 2, MB, NB>(la, lb, smem, rbeg, rend, ra, rb, lane, acc, [&](auto, int) {
+    auto product = [&](auto& la) {
+        lb_product<3, 4, BM == 64 ? 4 : 2, MB, NB>(
+            la, lb, smem, rbeg, rend, ra, rb, lane, acc, [&](auto, int) {
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int j = 0; j < NB; ++j)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) sum[i][j][r] += acc[i][j][r];
+            });
+    };
+    if (p.db && in == 0) {
+        LA la(p, m0, t);
+        product(la);
+        // the four groups of rows of each output
+        float* const red = reinterpret_cast<float*>(smem);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < LA::N; ++i) red[i * NT + t] = la.sum[i];
+        __syncthreads();
+        if (t < BM && m0 + t < p.O) {
+            const float v = (red[t] + red[BM + t]) + (red[2 * BM + t] + red[3 * BM + t]);
+            if (part) {
+                p.part_b[(int64_t)split * p.O + m0 + t] = v;
+            } else {
+                float* const d = p.db + (int64_t)(m0 + t) * p.db_stride;
+                *d = p.beta_b != 0.f ? p.beta_b * *d + v : v;
+            }
+        }
+    } else {
+        BackDy<BM, NT, false> la(p, m0, t);
+        product(la);
+    }
+    auto each = [&](auto put) {
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
+            for (int j = 0; j < NB; ++j) {
+                const int n = n0 + rb + 32 * j + (lane & 31);
+                if (n >= p.C) continue;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sum[i][j][r] += acc[i][j][r];
-    });
-    const bool part = p.splits > 1;
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            const int n = n0 + rb + 32 * j + (lane & 31);
-            if (n >= p.C) continue;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int m = m0 + ra + 32 * i + lb_row(lane, r);
-                if (m >= p.O) continue;
-                const float v = sum[i][j][r];
-                if (part) {
-                    p.part[((int64_t)split * p.O + m) * p.C + n] = v;
-                } else {
-                    float* const d = p.dw + (int64_t)m * p.dw_o + (int64_t)n * p.dw_c;
-                    *d = p.beta != 0.f ? p.beta * *d + v : v;
+                for (int r = 0; r < 16; ++r) {
+                    const int m = m0 + ra + 32 * i + lb_row(lane, r);
+                    if (m < p.O) put(m, n, sum[i][j][r]);
                 }
             }
-        }
+    };
+    float* const out = part ? p.part + (int64_t)split * p.O * p.C : p.dw;
+    const int64_t om = part ? p.C : p.dw_o, on = part ? 1 : p.dw_c;
+    if (part || p.beta == 0.f)
+        each([&](int m, int n, float v) { out[m * om + n * on] = v; });
+    else
+        each([&](int m, int n, float v) {
+            float* const d = out + (m * om + n * on);
+            *d = p.beta * *d + v;
+        });
 }
 
 }  // namespace mtk

@@ -109,7 +109,8 @@ __device__ __forceinline__ void lb_tile(int b, int tm, int tn, int& im, int& in)
 //   fast                         whether load_fast may be called at all
 //   load_fast(Raw&, int k0)      chunk of 32 k from k0 on, all of them below k_end
 //   load(Raw&, int k0)           any chunk, zero past the end
-//   store(const Raw&, char*)     converted, to its part of the buffer
+//   store(const Raw&, char*, live)   converted, to its part of the buffer (live: not a
+//                                chunk that is there only again)
 //   kBytes, kGroup, entry(row)   LDS size of a part and of a group of eight k, and the
 //                                entry of a row in a group: entry(32a + b) = entry(32a)
 //                                + entry(b)
@@ -151,7 +152,7 @@ __device__ __forceinline__ void lb_product(LA& la, LB& lb, char* smem, int k_beg
     };
     auto put = [&](int c, int slot) {
         char* const buf = smem + (c & 1) * BUF;
-        la.store(xa[slot], buf);
+        la.store(xa[slot], buf, c < nk);
         if constexpr (LB::kBlock) lb.store(codes, buf + P * LA::kBytes);
         else lb.store(xb[slot], buf + P * LA::kBytes);
     };
@@ -294,19 +295,37 @@ __device__ __forceinline__ int lb_row(int lane, int r) {
     return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
 }
 
-// y[m][n] = beta*y + bias[n] + the splits' partials [splits][M][N] in order (no
-// splits: part is not read).
-__global__ void __launch_bounds__(256)
-lb_sum(const float* part, int splits, int M, int N, const float* bias, int64_t bias_stride, float* y,
-       int64_t y_m, int64_t y_n, float beta) {
-    const int64_t n = (int64_t)M * N;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int m = (int)(i / N), c = (int)(i - (int64_t)m * N);
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += part[s * n + i];
-        if (bias) v += bias[(int64_t)c * bias_stride];
-        float* const d = y + (int64_t)m * y_m + (int64_t)c * y_n;
-        *d = beta != 0.f ? beta * *d + v : v;
+// y[m][n] = beta*y + bias[n] + the splits' partials [splits][M][N] in order, and
+// v[i] = beta_v*v + those of part_v [splits][L] (no splits: nothing is read).
+struct LbSum {
+    const float* part;
+    int splits, M, N;
+    const float* bias;                // nullptr: none
+    int64_t bias_stride;
+    float* y;
+    int64_t y_m, y_n;
+    float beta;
+    const float* part_v;
+    float* v;                         // nullptr: none
+    int64_t v_stride;
+    float beta_v;
+    int L;
+};
+__global__ void __launch_bounds__(256) lb_sum(LbSum p) {
+    const int64_t n = (int64_t)p.M * p.N, all = n + (p.v ? p.L : 0);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all;
+         i += (int64_t)gridDim.x * 256) {
+        const bool vec = i >= n;
+        const float* const part = vec ? p.part_v + (i - n) : p.part + i;
+        const int64_t stride = vec ? p.L : n;
+        float s = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < p.splits; ++k) s += part[k * stride];
+        const int m = (int)(i / p.N), c = (int)(i - (int64_t)m * p.N);
+        if (p.bias && !vec) s += p.bias[(int64_t)c * p.bias_stride];
+        float* const d = vec ? p.v + (i - n) * p.v_stride : p.y + (int64_t)m * p.y_m + (int64_t)c * p.y_n;
+        const float beta = vec ? p.beta_v : p.beta;
+        *d = beta != 0.f ? beta * *d + s : s;
     }
 }
 

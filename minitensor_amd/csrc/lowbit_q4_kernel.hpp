@@ -264,7 +264,7 @@ struct Q4X {
             else q4_x8(p, x, k0 + 8 * (v & 3), r.a[i]);
         }
     }
-    __device__ __forceinline__ void store(const Raw& r, char* buf) const {
+    __device__ __forceinline__ void store(const Raw& r, char* buf, bool) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             char* const d = buf + (t & 3) * kGroup + ((i * NT + t) >> 2) * 16;
