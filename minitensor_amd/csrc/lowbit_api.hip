@@ -102,30 +102,57 @@ int64_t row_groups(int64_t rows, int64_t cols) {
     return (std::min(rows, most) + 3) / 4 * 4;
 }
 
+// Tiles and splits of a product over chunks of 32 k.  Measured times of a chunk in us, by
+// workgroups on a CU, where each holds as many as its LDS and registers allow: the tile
+// and the number of splits that come out fastest, workgroups going in rounds over the CUs,
+// with the partials' sum at 4 TB/s and a launch.  (1024 rows, 4096 -> 4096: 128x256 tiles
+// in 2 splits 100 us, 64x128 unsplit 118; 1027 8-bit rows, 2048 -> 4096: 64x128 unsplit 50,
+// 128x256 61 unsplit and 79 in 3 splits.)
+struct Tiling {
+    int bm;                           // of bm x 2·bm
+    int per_cu;
+    double alone, full;               // a chunk's time: one workgroup on the CU, all of them
+};
+struct Tiled {
+    int bm, splits, k_per_split;
+    size_t partials;                  // floats, 0 without splits
+};
+Tiled plan_tiles(int64_t M, int64_t N, int64_t K, const Tiling* t, int n) {
+    Tiled best{};
+    double least = 0;
+    const int64_t blocks = std::max<int64_t>(1, (K + 127) / 128);
+    for (int i = 0; i < n; ++i) {
+        const int64_t tiles = ((M + t[i].bm - 1) / t[i].bm) * ((N + 2 * t[i].bm - 1) / (2 * t[i].bm));
+        for (int64_t s = 1; s <= std::min<int64_t>(blocks, 32); ++s) {
+            const int64_t per = (blocks + s - 1) / s;
+            if ((blocks + per - 1) / per != s) continue;
+            const int64_t wgs = tiles * s, slots = (int64_t)kCus * t[i].per_cu;
+            const int64_t rest = wgs % slots;
+            double rounds = (double)(wgs / slots) * t[i].full;
+            if (rest > kCus) rounds += t[i].full;
+            else if (rest > 0) rounds += t[i].alone;
+            double us = (double)std::min<int64_t>(4 * per, (K + 31) / 32) * rounds;
+            if (s > 1) us += 2.5 + (double)(s + 1) * (double)M * (double)N * 1e-6;
+            if (least == 0 || us < least) {
+                least = us;
+                best = {t[i].bm, (int)s, (int)(per * 128), s > 1 ? (size_t)(s * M * N) : 0};
+            }
+            if (wgs >= 4 * slots) break;
+        }
+    }
+    return best;
+}
+
 struct Q4Plan {
     bool few;
-    int bm, splits, kps;
-    size_t ws;
+    Tiled tiled;
 };
 Q4Plan q4_plan(int64_t M, int64_t N, int64_t K, int group, bool q8) {
-    Q4Plan p{};
-    const int64_t parts = q8 ? 1 : 3;
-    if (M * parts <= 48) {
-        p.few = true;
-        return p;
-    }
+    if (M * (q8 ? 1 : 3) <= 48) return {true, {}};
     // (groups of 32: the wide tile's scales do not fit the registers)
-    p.bm = group == 32 || ((M + 127) / 128) * ((N + 255) / 256) < kCus / 2 ? 64 : 128;
-    const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + 2 * p.bm - 1) / (2 * p.bm));
-    // splits of whole blocks of 128 inputs, at least four of them
-    const int64_t blocks = (K + 127) / 128;
-    int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * kCus / std::max<int64_t>(tiles, 1), blocks / 4));
-    const int64_t per = (blocks + s - 1) / s;
-    s = std::max<int64_t>(1, (blocks + per - 1) / std::max<int64_t>(per, 1));
-    p.splits = (int)s;
-    p.kps = (int)(per * 128);
-    p.ws = s > 1 ? (size_t)(s * M * N) * 4 : 0;
-    return p;
+    static const Tiling f32[] = {{64, 2, 0.5, 0.92}, {128, 1, 1.2, 1.2}};
+    static const Tiling int8[] = {{64, 3, 0.5, 0.78}, {128, 1, 0.84, 0.84}};
+    return {false, plan_tiles(M, N, K, q8 ? int8 : f32, group == 32 ? 1 : 2)};
 }
 
 template <bool Q8, int G>
@@ -174,14 +201,15 @@ int run_q4(Q4Params p, int64_t M, const mt_weight_q4* W, const float* bias, int6
                            LbSum{nullptr, 0, p.M, p.N, bias, bias_stride, p.y, p.y_m, p.y_n});
         return launched();
     }
-    if (plan.ws > 0 && (!workspace || ws_bytes < plan.ws)) return MT_ERR_WORKSPACE;
-    p.splits = plan.few ? 1 : plan.splits;
-    p.k_per_split = plan.kps;
+    const size_t need = plan.tiled.partials * 4;
+    if (need > 0 && (!workspace || ws_bytes < need)) return MT_ERR_WORKSPACE;
+    p.splits = plan.few ? 1 : plan.tiled.splits;
+    p.k_per_split = plan.tiled.k_per_split;
     p.part = static_cast<float*>(workspace);
     auto go = [&](auto g) {
         constexpr int G = decltype(g)::value;
         if (plan.few) launch_few<Q8, G>(p, s);
-        else launch_gemm<Q8, G>(p, plan.bm, s);
+        else launch_gemm<Q8, G>(p, plan.tiled.bm, s);
     };
     if (W->group == 32) go(std::integral_constant<int, 32>{});
     else if (W->group == 64) go(std::integral_constant<int, 64>{});
@@ -194,24 +222,13 @@ int run_q4(Q4Params p, int64_t M, const mt_weight_q4* W, const float* bias, int6
     return launched();
 }
 
-struct BackPlan {
-    int bm, bn, splits, rps;
-    size_t ws;
-};
-BackPlan back_plan(int64_t R, int64_t O, int64_t C) {
-    BackPlan p{};
-    const bool small = ((O + 127) / 128) * ((C + 255) / 256) < kCus / 2;
-    p.bm = small ? 64 : 128;
-    p.bn = 2 * p.bm;
-    const int64_t tiles = ((O + p.bm - 1) / p.bm) * ((C + p.bn - 1) / p.bn);
-    const int64_t blocks = (R + 127) / 128;
-    int64_t s = std::max<int64_t>(1, std::min<int64_t>(2 * kCus / std::max<int64_t>(tiles, 1), blocks / 4));
-    const int64_t per = std::max<int64_t>(1, (blocks + s - 1) / s);
-    s = std::max<int64_t>(1, (blocks + per - 1) / per);
-    p.splits = (int)s;
-    p.rps = (int)(per * 128);
-    p.ws = s > 1 ? (size_t)(s * (O * C + O)) * 4 : 0;
-    return p;
+// The weight gradient [O][C] over R rows, and the floats of its workspace: the splits'
+// partial products and row sums.
+Tiled back_plan(int64_t R, int64_t O, int64_t C) {
+    static const Tiling tiles[] = {{64, 2, 0.8, 1.0}, {128, 1, 1.35, 1.35}};
+    Tiled t = plan_tiles(O, C, R, tiles, 2);
+    if (t.partials) t.partials += (size_t)t.splits * O;
+    return t;
 }
 
 }  // namespace
@@ -335,7 +352,7 @@ int mt_dequantize_q8_f32(const mt_rows_q8* Q, const mt_mat_f32* Y, void* stream)
 size_t mt_linear_backward_q8_workspace_f32(int64_t rows, int64_t in_f, int64_t out_f) {
     if (rows < 0 || in_f < 0 || out_f < 0 || rows >= kMaxDim || in_f >= kMaxDim || out_f >= kMaxDim)
         return 0;
-    return std::max(mt_linear_workspace_f32(rows, in_f, out_f), back_plan(rows, out_f, in_f).ws);
+    return std::max(mt_linear_workspace_f32(rows, in_f, out_f), back_plan(rows, out_f, in_f).partials * 4);
 }
 
 int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const mt_mat_f32* W,
@@ -349,8 +366,9 @@ int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const m
     if (dW && (!valid(dW, true) || dW->rows != dY->cols || dW->cols != X->cols))
         return MT_ERR_INVALID;
     if (db && (db_stride < 0 || (dY->cols > 1 && db_stride == 0))) return MT_ERR_INVALID;
-    const BackPlan plan = back_plan(X->rows, dY->cols, X->cols);
-    if (dW && plan.ws > 0 && (!workspace || ws_bytes < plan.ws)) return MT_ERR_WORKSPACE;
+    const Tiled plan = back_plan(X->rows, dY->cols, X->cols);
+    if (dW && plan.partials > 0 && (!workspace || ws_bytes < plan.partials * 4))
+        return MT_ERR_WORKSPACE;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (dX) {
         const int rc = mt_gemm_f32(dY, W, dX, nullptr, workspace, ws_bytes, stream);
@@ -374,7 +392,7 @@ int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const m
         p.O = (int)dY->cols;
         p.C = (int)X->cols;
         p.splits = plan.splits;
-        p.r_per_split = plan.rps;
+        p.r_per_split = plan.k_per_split;
         if (db) {
             p.db = db;
             p.db_stride = db_stride;
@@ -385,7 +403,7 @@ int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const m
                         beta_w, p.part_b, db, db_stride, beta_b, p.O};
         if (p.R > 0) {
             const int64_t tiles = (int64_t)((p.O + plan.bm - 1) / plan.bm) *
-                                  ((p.C + plan.bn - 1) / plan.bn) * p.splits;
+                                  ((p.C + 2 * plan.bm - 1) / (2 * plan.bm)) * p.splits;
             if (plan.bm == 64)
                 hipLaunchKernelGGL((back_dw<64, 128, 32, 64>), dim3((unsigned)tiles), dim3(256), 0, s,
                                    p);
@@ -438,10 +456,11 @@ size_t mt_linear_q4_workspace(int64_t rows, int64_t in_f, int64_t out_f) {
     if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxDim - 128 ||
         out_f >= kMaxDim)
         return 0;
-    size_t ws = 0;
+    size_t n = 0;
     for (const int group : {32, 128})
-        for (const bool q8 : {false, true}) ws = std::max(ws, q4_plan(rows, out_f, in_f, group, q8).ws);
-    return ws;
+        for (const bool q8 : {false, true})
+            n = std::max(n, q4_plan(rows, out_f, in_f, group, q8).tiled.partials);
+    return n * 4;
 }
 
 int mt_linear_q4_f32(const mt_mat_f32* X, const mt_weight_q4* W, const float* bias,

@@ -114,7 +114,9 @@ struct BackDy {
 // which change places in registers.  The entries of four neighbouring inputs lie
 // in four runs, so that consecutive lanes write consecutive entries; the runs start 32
 // bytes apart modulo 128, so that a fragment's rows fall on different banks.
-template <int BN, int NT>
+// EDGE: a tile that reaches past the last input (four inputs or more in all).  Items there
+// start early enough to end with the row, and are shifted back into place.
+template <int BN, int NT, bool EDGE>
 struct BackQ {
     static constexpr int N = BN * 2 / NT, kRun = BN / 4 + 2, kGroup = 4 * kRun * 16,
                          kBytes = 4 * kGroup;
@@ -129,16 +131,23 @@ struct BackQ {
     uint32_t off[N];                  // of the item from its wave's first row on
     int64_t ld;
     int R, t, left, row[N];           // inputs from n0 on; the wave's first row in a chunk
-    bool fast;                        // whole items in this workgroup's tile
+    int shift[EDGE ? N : 1];          // of an edge item, in bits
+    bool fast;                        // rows within 32 bits of bytes, and four inputs or more
     __device__ __forceinline__ static int entry(int c) { return (c & 3) * kRun + (c >> 2); }
     __device__ __forceinline__ BackQ(const BackParams& p, int n0, int t_)
         : base(p.q + n0), ld(p.q_r), R(p.R), t(t_), left(p.C - n0),
-          fast(BN <= left && p.q_r < (1 << 28)) {
+          fast(p.C >= 4 && p.q_r < (1 << 28)) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int r = 4 * ((i * NT + t) / (BN / 4));
             row[i] = __builtin_amdgcn_readfirstlane(r);
-            off[i] = (uint32_t)((i * NT + t) % (BN / 4) * 4) + (uint32_t)(r - row[i]) * (uint32_t)ld;
+            int c = (i * NT + t) % (BN / 4) * 4;
+            if constexpr (EDGE) {                          // (inputs past C: anything, not stored)
+                const int early = min(c, left - 4);
+                shift[i] = 8 * (c - early) & 31;
+                c = early;
+            }
+            off[i] = (uint32_t)c + (uint32_t)(r - row[i]) * (uint32_t)ld;
         }
     }
     __device__ __forceinline__ void load_fast(Raw& x, int k0) const {
@@ -146,8 +155,12 @@ struct BackQ {
         for (int i = 0; i < N; ++i) {
             const int8_t* q = base + (k0 + row[i]) * ld;
 #pragma unroll
-            for (int e = 0; e < 4; ++e, q += ld)
-                x.q[i][e] = *reinterpret_cast<const row_codes*>(at_bytes(q, off[i]));
+            for (int e = 0; e < 4; ++e, q += ld) {
+                if constexpr (EDGE)                        // (off may be negative)
+                    x.q[i][e] = *reinterpret_cast<const row_codes*>(q + (int32_t)off[i]);
+                else
+                    x.q[i][e] = *reinterpret_cast<const row_codes*>(at_bytes(q, off[i]));
+            }
         }
     }
     __device__ __forceinline__ void load(Raw& x, int k0) const {
@@ -167,7 +180,7 @@ struct BackQ {
                     for (int b = 0; b < 4; ++b)
                         if (r + e < R && c + b < left) v |= (uint32_t)(uint8_t)q[b] << (8 * b);
                 }
-                x.q[i][e] = v;
+                x.q[i][e] = EDGE ? v << shift[i] : v;
             }
         }
     }
@@ -176,11 +189,14 @@ struct BackQ {
         for (int i = 0; i < N; ++i) {
             const int v = i * NT + t, c4 = v % (BN / 4), kq = v / (BN / 4);
             char* const d = buf + (kq >> 1) * kGroup + c4 * 16 + (kq & 1) * 8;
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = EDGE ? x.q[i][e] >> shift[i] : x.q[i][e];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 float f[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(x.q[i][e] >> (8 * b));
+                for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(w[e] >> (8 * b));
                 *reinterpret_cast<u32x2*>(d + b * kRun * 16) =
                     u32x2{bf16_exact(f[0], f[1]), bf16_exact(f[2], f[3])};
             }
@@ -193,7 +209,7 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) back_dw(BackParam
     constexpr int WAVES_N = BN / WN, NT = BM / WM * WAVES_N * 64;
     constexpr int MB = WM / 32, NB = WN / 32;
     using LA = BackDy<BM, NT, true>;
-    using LB = BackQ<BN, NT>;
+    using LB = BackQ<BN, NT, false>;
     __shared__ __attribute__((aligned(16))) char smem[2 * (3 * LA::kBytes + LB::kBytes)];
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -205,10 +221,9 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) back_dw(BackParam
     const int m0 = im * BM, n0 = in * BN;
     const int rbeg = split * p.r_per_split, rend = min(p.R, rbeg + p.r_per_split);
     const bool part = p.splits > 1;
-    LB lb(p, n0, t);
     f32x16 sum[MB][NB], acc[MB][NB];
     zero_blocks<MB, NB>(sum);
-    auto product = [&](auto& la) {
+    auto multiply = [&](auto& la, auto lb) {
         lb_product<3, 4, BM == 64 ? 4 : 2, MB, NB>(
             la, lb, smem, rbeg, rend, ra, rb, lane, acc, [&](auto, int) {
 #pragma unroll
@@ -218,6 +233,10 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) back_dw(BackParam
 #pragma unroll
                         for (int r = 0; r < 16; ++r) sum[i][j][r] += acc[i][j][r];
             });
+    };
+    auto product = [&](auto& la) {
+        if (n0 + BN <= p.C) multiply(la, LB(p, n0, t));
+        else multiply(la, BackQ<BN, NT, true>(p, n0, t));
     };
     if (p.db && in == 0) {
         LA la(p, m0, t);
