@@ -15,6 +15,7 @@ using namespace mtk;
 namespace {
 
 constexpr int64_t kMaxDim = (int64_t)1 << 31;   // extents are 32-bit inside the kernels
+constexpr int64_t kMaxIn = kMaxDim - (1 << 16);  // inputs of one (blocks past the end stay below 2^31)
 constexpr int64_t kMaxOut = (int64_t)1 << 26;   // rows of a 4-bit weight (32 threads each in a grid)
 constexpr int64_t kMaxScaleStride = (int64_t)1 << 22;   // a tile's 256 rows of scales within 32 bits of bytes
 constexpr int kCus = 256;                       // what plans fill (MI355X)
@@ -44,7 +45,7 @@ bool valid(const mt_rows_q8* Q) {
     return Q->rows == 0 || (Q->scale && (Q->cols == 0 || Q->q));
 }
 bool valid(const mt_weight_q4* W) {
-    if (!W || W->n < 0 || W->k < 0 || W->n >= kMaxOut || W->k >= kMaxDim - 128 ||
+    if (!W || W->n < 0 || W->k < 0 || W->n >= kMaxOut || W->k >= kMaxIn ||
         (W->group != 32 && W->group != 64 && W->group != 128) || W->row_stride < 0 ||
         W->scale_stride < 0)
         return false;
@@ -157,14 +158,29 @@ Q4Plan q4_plan(int64_t M, int64_t N, int64_t K, int group, bool q8) {
 
 template <bool Q8, int G>
 void launch_few(const Q4Params& p, hipStream_t s) {
-    const unsigned grid = (unsigned)((p.N + 15) / 16);
-    const int rows = p.M * (Q8 ? 1 : 3);
-    if (rows <= 16)
-        hipLaunchKernelGGL((q4_few<1, G, Q8, 8>), dim3(grid), dim3(512), 0, s, p);
+    const int rows = p.M * (Q8 ? 1 : 3), cols = (p.N + 15) / 16;
+    // column blocks per workgroup, where that leaves one for every CU
+    // (four of them, and 48 rows, do not fit the registers)
+    const int nc = rows <= 6 ? 1 : cols >= 4 * kCus && rows <= 32 ? 4 : cols >= 2 * kCus ? 2 : 1;
+    const dim3 grid((unsigned)((cols + nc - 1) / nc)), block(512);
+    auto go = [&](auto cap, auto u) {
+        if constexpr (cap() <= 32)
+            if (nc == 4) {
+                hipLaunchKernelGGL((q4_few<cap(), 1, 4, G, Q8, 8>), grid, block, 0, s, p);
+                return;
+            }
+        if (nc == 2) hipLaunchKernelGGL((q4_few<cap(), 1, 2, G, Q8, 8>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((q4_few<cap(), u(), 1, G, Q8, 8>), grid, block, 0, s, p);
+    };
+    using std::integral_constant;
+    if (rows <= 6)
+        hipLaunchKernelGGL((q4_few<6, 4, 1, G, Q8, 8>), grid, block, 0, s, p);
+    else if (rows <= 16)
+        go(integral_constant<int, Q8 ? 16 : 15>{}, integral_constant<int, 2>{});
     else if (rows <= 32)
-        hipLaunchKernelGGL((q4_few<2, G, Q8, 8>), dim3(grid), dim3(512), 0, s, p);
+        go(integral_constant<int, Q8 ? 32 : 30>{}, integral_constant<int, 1>{});
     else
-        hipLaunchKernelGGL((q4_few<3, G, Q8, 8>), dim3(grid), dim3(512), 0, s, p);
+        go(integral_constant<int, 48>{}, integral_constant<int, 1>{});
 }
 template <bool Q8, int G>
 void launch_gemm(const Q4Params& p, int bm, hipStream_t s) {
@@ -453,7 +469,7 @@ int mt_dequantize_q4_f32(const mt_weight_q4* Q, const mt_mat_f32* W, void* strea
 }
 
 size_t mt_linear_q4_workspace(int64_t rows, int64_t in_f, int64_t out_f) {
-    if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxDim - 128 ||
+    if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxIn ||
         out_f >= kMaxDim)
         return 0;
     size_t n = 0;

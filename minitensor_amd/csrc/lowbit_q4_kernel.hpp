@@ -79,126 +79,211 @@ __device__ __forceinline__ f32x4 mfma_16(const u32x4& a, const u32x4& b, const f
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Few rows.  A workgroup owns 16 columns n and all of K, in blocks of 128: wave
-// w takes the blocks w, w + W, ...; the waves' sums meet in LDS in wave order.
-// The parts of x are rows of their own (row 3m + part; row m for 8-bit x): one
-// MFMA of 16x16x32 covers five rows of fp32 x.  Each wave stages its block of x in an LDS region
-// of its own, so that nothing waits for another wave until the end.
+// Few rows.  A workgroup owns NC blocks of 16 columns n and all of K, in blocks of 128, of
+// which each wave takes up to four neighbouring ones at a time; the waves' sums meet in LDS
+// in wave order.  The parts of x are rows of their own (row 3m + part; row m for 8-bit x), so
+// that one MFMA of 16x16x32 covers five rows of fp32 x.  Each wave stages U blocks of x at a
+// time in an LDS region of its own, so that nothing waits for another wave until the end.
+// CAP: rows that a block there has room for; the MFMAs' rows past it are its last one again,
+// their sums not used.
 //
-// Lane (n = lane % 16, j = lane / 16) reads its weights as they lie: with
-// groups of 128 the 16 bytes of k = 32j..32j+31 (four MFMAs), with smaller ones
-// 8 or 4 bytes of each group, so that the 32 inputs of an MFMA are of one group.
-template <int MB, int G, bool Q8, int W>
+// NC = 1: the loads of all four blocks are in flight at once (one row, 4096 -> 4096: 6.7 us
+// block by block, 5.5 so).  NC > 1: a block of all NC at a time, the next one on its way; x
+// is cut once for 16·NC columns, which is what many rows cost most.
+//
+// Lane (n = lane % 16, j = lane / 16) reads 16 bytes of a block's 64, and the 32 inputs of an
+// MFMA have to be of one group: with smaller groups than 128 the four lanes of a column
+// exchange dwords (loads of 4 bytes, each lane's in place, took 34 us where these take 16).
+template <int G>
+struct Q4Lanes {
+    static constexpr int LW = G / 32, NL = 4 / LW;    // dwords per group and lane, groups
+    // dword i·LW + d of lane j: piece (of eight inputs) of the block
+    __device__ __forceinline__ static int piece(int i, int d, int j) {
+        return G == 128 ? 4 * j + d : G == 64 ? 8 * i + 4 * (j & 1) + 2 * (j >> 1) + d : 4 * i + j;
+    }
+    // from dword 4j + r in register r of lane j
+    __device__ __forceinline__ static void exchange(uint32_t (&w)[4]) {
+        if constexpr (G < 128) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const auto x = __builtin_amdgcn_permlane32_swap(w[r], w[r + 2], false, false);
+                w[r] = x[0];
+                w[r + 2] = x[1];
+            }
+        }
+        if constexpr (G < 64) {
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+                const auto x = __builtin_amdgcn_permlane16_swap(w[r], w[r + 1], false, false);
+                w[r] = x[0];
+                w[r + 1] = x[1];
+            }
+        }
+    }
+};
+
+template <int CAP, int U, int NC, int G, bool Q8, int W>
 __global__ void __launch_bounds__(64 * W) q4_few(Q4Params p) {
-    constexpr int P = Q8 ? 1 : 3;
-    constexpr int LW = G / 32;                        // dwords per load, MFMAs per group
-    constexpr int NL = 4 / LW;                        // loads (groups) per block
+    using Lanes = Q4Lanes<G>;
+    constexpr int P = Q8 ? 1 : 3, MB = (CAP + 15) / 16;
+    constexpr int LW = Lanes::LW, NL = Lanes::NL;
     constexpr int RS = 256 + 16;                      // bytes of a row of a staged block
-    constexpr int XB = 16 * MB * RS;
-    constexpr int RED = W * 16 * MB * 16 * 4;
+    constexpr int XB = U * CAP * RS;
+    constexpr int RED = W * 16 * MB * 16 * NC * 4;
+    constexpr int AHEAD = NC == 1 ? 4 : 2;            // blocks of weights in registers
+    static_assert(NC == 1 || U == 1, "several columns go block by block");
     __shared__ __attribute__((aligned(16))) char smem[W * XB > RED ? W * XB : RED];
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int col = lane & 15, j = lane >> 4;
-    const int n0 = blockIdx.x * 16;
-    const int n = min(n0 + col, p.N - 1);             // (columns past N are not stored)
-    const uint8_t* const wr = p.w + (int64_t)n * p.w_n;
-    const float* const sr = p.s + (int64_t)n * p.s_n;
+    const int n0 = blockIdx.x * (16 * NC);
+    const uint8_t* wr[NC];
+    const float* sr[NC];
+#pragma unroll
+    for (int q = 0; q < NC; ++q) {                    // (columns past N: the last, not stored)
+        const int64_t n = min(n0 + 16 * q + col, p.N - 1);
+        wr[q] = p.w + n * p.w_n;
+        sr[q] = p.s + n * p.s_n;
+    }
     const int kp = (p.K + 31) & ~31;                  // inputs that the packed row holds
     const int groups = (p.K + G - 1) / G;
     const int blocks = (p.K + 127) >> 7;
+    const int per = min(4, (blocks + W - 1) / W);     // a wave's neighbouring blocks
     char* const xs = smem + wave * XB;
 
-    f32x4 sum[MB];
+    f32x4 sum[NC][MB];
 #pragma unroll
-    for (int b = 0; b < MB; ++b) sum[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < NC; ++q)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) sum[q][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    for (int kb = wave; kb < blocks; kb += W) {
-        const int k0 = kb * 128;
-        uint32_t cw[4];
-        float sc[NL];
+    // Pieces of eight inputs of x: 16 per row and block.  A lane takes the pieces lane, lane +
+    // 64, ... of U blocks, MAXP of them at most.
+    constexpr int MAXP = (CAP / P * 16 * U + 63) / 64;
+    using Piece = std::conditional_t<Q8, u32x2, float[8]>;
+    typedef float Scales __attribute__((ext_vector_type(NL), aligned(4)));
+    for (int kb0 = wave * per; kb0 < blocks; kb0 += per * W) {
+        const int end = min(kb0 + per, blocks);
+        Piece x[MAXP];
+        auto load_x = [&](int kb) {                   // U blocks from kb on (zeros past K)
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int k = k0 + G * i + 8 * LW * j;    // of the load's first dword
-            const uint32_t* const src = reinterpret_cast<const uint32_t*>(wr + (k >> 1));
+            for (int i = 0; i < MAXP; ++i) {
+                const int e = lane + 64 * i, m = e / (16 * U);
+                if (m >= p.M) break;
+                const int k = 128 * (kb + (e >> 4) % U) + 8 * (e & 15);
+                if constexpr (Q8) x[i] = q4_x8(p, p.q + (int64_t)m * p.q_m, k);
+                else q4_x8(p, p.x + (int64_t)m * p.x_m, k, x[i]);
+            }
+        };
+        uint32_t cw[AHEAD][NC][4];
+        float sc[AHEAD][NC][NL];
+        auto load_w = [&](int kb, uint32_t (&w)[NC][4], float (&s)[NC][NL]) {
 #pragma unroll
-            for (int d = 0; d < LW; ++d) cw[LW * i + d] = 0;
-            if (k < kp) {
-                if constexpr (LW == 4) {
-                    const u32x4 v = *reinterpret_cast<const u32x4*>(src);
+            for (int q = 0; q < NC; ++q) {
+                const int k = 128 * kb + 32 * j;
+                u32x4 v = {0u, 0u, 0u, 0u};
+                if (k < kp) v = *reinterpret_cast<const u32x4*>(wr[q] + (k >> 1));
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) cw[d] = v[d];
-                } else if constexpr (LW == 2) {
-                    const u32x2 v = *reinterpret_cast<const u32x2*>(src);
-                    cw[2 * i] = v[0];
-                    cw[2 * i + 1] = v[1];
+                for (int d = 0; d < 4; ++d) w[q][d] = v[d];
+                const int g = kb * NL;
+                if (g + NL <= groups) {
+                    const Scales f = *reinterpret_cast<const Scales*>(sr[q] + g);
+#pragma unroll
+                    for (int i = 0; i < NL; ++i) s[q][i] = f[i];
                 } else {
-                    cw[i] = *src;
+#pragma unroll
+                    for (int i = 0; i < NL; ++i) s[q][i] = g + i < groups ? sr[q][g + i] : 0.f;
                 }
             }
-            const int g = kb * NL + i;
-            sc[i] = g < groups ? sr[g] * kQ4Unit : 0.f;
-        }
-        // the block of x: 16 pieces of eight inputs per row
-        for (int e = lane; e < p.M * 16; e += 64) {
-            const int m = e >> 4, piece = e & 15;
-            char* const d = xs + P * m * RS + piece * 16;
-            if constexpr (Q8) {
-                *reinterpret_cast<u32x4*>(d) =
-                    q8_bf16(q4_x8(p, p.q + (int64_t)m * p.q_m, k0 + 8 * piece));
-            } else {
-                float x[8];
-                u32x4 h, mm, l;
-                q4_x8(p, p.x + (int64_t)m * p.x_m, k0 + 8 * piece, x);
-                cut8(x, h, mm, l);
-                *reinterpret_cast<u32x4*>(d) = h;
-                *reinterpret_cast<u32x4*>(d + RS) = mm;
-                *reinterpret_cast<u32x4*>(d + 2 * RS) = l;
-            }
-        }
-        // (the wave's own region: its LDS accesses are in order)
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        f32x4 acc[MB];
+        };
+        load_x(kb0);
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
+        for (int u = 0; u < (NC == 1 ? 4 : 1); ++u)
+            if (u == 0 || kb0 + u < end) load_w(kb0 + u, cw[u], sc[u]);
 #pragma unroll
-            for (int d = 0; d < LW; ++d) {
-                const u32x4 b = q4_unpack(cw[LW * i + d]);
-                const int piece = (G * i + 8 * LW * j + 8 * d) >> 3;
+        for (int h = 0; h < 4; h += U) {
+            if (kb0 + h >= end) break;                // (uniform)
 #pragma unroll
-                for (int mb = 0; mb < MB; ++mb) {
-                    // (rows past the last one hold what they hold: their sums are not used)
-                    const u32x4 a = *reinterpret_cast<const u32x4*>(xs + (16 * mb + col) * RS +
-                                                                    piece * 16);
-                    acc[mb] = mfma_16(a, b, d == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[mb]);
+            for (int i = 0; i < MAXP; ++i) {
+                const int e = lane + 64 * i, m = e / (16 * U);
+                if (m >= p.M) break;
+                char* const d = xs + ((e >> 4) % U * CAP + P * m) * RS + (e & 15) * 16;
+                if constexpr (Q8) {
+                    *reinterpret_cast<u32x4*>(d) = q8_bf16(x[i]);
+                } else {
+                    u32x4 hi, mi, lo;
+                    cut8(x[i], hi, mi, lo);
+                    *reinterpret_cast<u32x4*>(d) = hi;
+                    *reinterpret_cast<u32x4*>(d + RS) = mi;
+                    *reinterpret_cast<u32x4*>(d + 2 * RS) = lo;
                 }
             }
+            if (kb0 + h + U < end) {
+                load_x(kb0 + h + U);
+                if constexpr (NC > 1) load_w(kb0 + h + 1, cw[(h + 1) & 1], sc[(h + 1) & 1]);
+            }
+            // (the wave's own region: its LDS accesses are in order)
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-            for (int mb = 0; mb < MB; ++mb) sum[mb] += acc[mb] * sc[i];
+            for (int u = 0; u < U; ++u) {
+                if (u > 0 && kb0 + h + u >= end) break;
+                auto& w = cw[NC == 1 ? h + u : h & 1];
+                auto& s = sc[NC == 1 ? h + u : h & 1];
+#pragma unroll
+                for (int q = 0; q < NC; ++q) Lanes::exchange(w[q]);
+#pragma unroll
+                for (int i = 0; i < NL; ++i) {
+                    f32x4 acc[NC][MB];
+#pragma unroll
+                    for (int d = 0; d < LW; ++d) {
+                        u32x4 b[NC];
+#pragma unroll
+                        for (int q = 0; q < NC; ++q) b[q] = q4_unpack(w[q][LW * i + d]);
+#pragma unroll
+                        for (int mb = 0; mb < MB; ++mb) {
+                            const u32x4 a = *reinterpret_cast<const u32x4*>(
+                                xs + (u * CAP + min(16 * mb + col, CAP - 1)) * RS +
+                                Lanes::piece(i, d, j) * 16);
+#pragma unroll
+                            for (int q = 0; q < NC; ++q)
+                                acc[q][mb] = mfma_16(a, b[q], d == 0 ? f32x4{0.f, 0.f, 0.f, 0.f}
+                                                                     : acc[q][mb]);
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < NC; ++q)
+#pragma unroll
+                        for (int mb = 0; mb < MB; ++mb)
+                            sum[q][mb] += acc[q][mb] * (s[q][i] * kQ4Unit);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
     __syncthreads();
     // [wave][row][column]
+    constexpr int C = 16 * NC;
     float* const red = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
+    for (int q = 0; q < NC; ++q)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            red[(wave * 16 * MB + 16 * mb + 4 * j + r) * 16 + col] = sum[mb][r];
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                red[(wave * 16 * MB + 16 * mb + 4 * j + r) * C + 16 * q + col] = sum[q][mb][r];
     __syncthreads();
-    for (int e = t; e < p.M * 16; e += 64 * W) {
-        const int m = e >> 4, c = e & 15;
+    for (int e = t; e < p.M * C; e += 64 * W) {
+        const int m = e / C, c = e % C;
         if (n0 + c >= p.N) continue;
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w)
 #pragma unroll
-            for (int q = P - 1; q >= 0; --q) v += red[(w * 16 * MB + P * m + q) * 16 + c];
+            for (int q = P - 1; q >= 0; --q) v += red[(w * 16 * MB + P * m + q) * C + c];
         if constexpr (Q8) v *= p.q_scale[m];
         if (p.bias) v += p.bias[(int64_t)(n0 + c) * p.bias_stride];
         p.y[(int64_t)m * p.y_m + (int64_t)(n0 + c) * p.y_n] = v;
