@@ -95,11 +95,14 @@ void launch_rows(const RowParams& p, bool units, hipStream_t s) {
     });
 }
 
-// Row groups of the backward kernel, each of which keeps a part of dweight: a
-// multiple of four, whether a workgroup holds four groups or one.
+// Row groups of the backward kernel, each of which keeps a part of dweight: enough to keep
+// the loads in flight, few enough that the parts weigh little (2048 x 4096, 256 to 2048
+// groups: 31, 29, 32, 41 us; 8192 x 2048: 67, 48, 46, 53; 1024 x 8192: 29, 35, 45, 45;
+// 8192 x 512: 51, 30, 20, 20).  A multiple of four, whether a
+// workgroup holds four groups or one.
 int64_t row_groups(int64_t rows, int64_t cols) {
     const int nt = row_threads(cols);
-    const int64_t most = nt == 64 ? 2048 : nt == 256 ? 1024 : 512;
+    const int64_t most = nt == 64 ? 2048 : nt == 256 ? 640 : 256;
     return (std::min(rows, most) + 3) / 4 * 4;
 }
 
@@ -173,7 +176,9 @@ void launch_few(const Q4Params& p, hipStream_t s) {
         else hipLaunchKernelGGL((q4_few<cap(), u(), 1, G, Q8, 8>), grid, block, 0, s, p);
     };
     using std::integral_constant;
-    if (rows <= 6)
+    if (rows <= 3)
+        hipLaunchKernelGGL((q4_few<3, 4, 1, G, Q8, 8>), grid, block, 0, s, p);
+    else if (rows <= 6)
         hipLaunchKernelGGL((q4_few<6, 4, 1, G, Q8, 8>), grid, block, 0, s, p);
     else if (rows <= 16)
         go(integral_constant<int, Q8 ? 16 : 15>{}, integral_constant<int, 2>{});
@@ -325,7 +330,7 @@ int mt_rms_norm_backward_f32(const mt_mat_f32* dY, const mt_mat_f32* H, const fl
         });
     }
     if (dweight)
-        hipLaunchKernelGGL(rms_dweight_sum, dim3((unsigned)((p.cols + 63) / 64)), dim3(1024), 0, s,
+        hipLaunchKernelGGL(rms_dweight_sum, dim3((unsigned)((p.cols + 15) / 16)), dim3(1024), 0, s,
                            p.part, p.rows > 0 ? (int)groups : 0, p.cols, dweight, dweight_stride,
                            beta);
     return launched();
@@ -351,17 +356,16 @@ int mt_dequantize_q8_f32(const mt_rows_q8* Q, const mt_mat_f32* Y, void* stream)
         return MT_ERR_INVALID;
     if (Y->rows == 0 || Y->cols == 0) return MT_OK;
     const RowView y = view(Y);
-    const int v = y.cs != 1 ? 1 : (Y->cols & 15) == 0 ? 16 : (Y->cols & 3) == 0 ? 4 : 1;
-    const int64_t n = Y->rows * (Y->cols / v);
-    const unsigned blocks = (unsigned)std::min<int64_t>((n + 255) / 256, 1 << 16);
-    auto go = [&](auto w) {
-        hipLaunchKernelGGL(dequantize_q8<w()>, dim3(blocks), dim3(256), 0,
-                           static_cast<hipStream_t>(stream), Q->q, Q->row_stride, Q->scale, y,
-                           Y->rows, (int)Y->cols);
-    };
-    if (v == 16) go(std::integral_constant<int, 16>{});
-    else if (v == 4) go(std::integral_constant<int, 4>{});
-    else go(std::integral_constant<int, 1>{});
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t waves = Y->rows * ((Y->cols + 1023) / 1024), n = Y->rows * Y->cols;
+    if (y.cs == 1)
+        hipLaunchKernelGGL(dequantize_q8<true>,
+                           dim3((unsigned)std::min<int64_t>((waves + 3) / 4, 1 << 20)), dim3(256), 0,
+                           s, Q->q, Q->row_stride, Q->scale, y, Y->rows, (int)Y->cols);
+    else
+        hipLaunchKernelGGL(dequantize_q8<false>,
+                           dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 16)), dim3(256), 0,
+                           s, Q->q, Q->row_stride, Q->scale, y, Y->rows, (int)Y->cols);
     return launched();
 }
 

@@ -123,7 +123,7 @@ struct Q4Lanes {
 };
 
 template <int CAP, int U, int NC, int G, bool Q8, int W>
-__global__ void __launch_bounds__(64 * W) q4_few(Q4Params p) {
+__global__ void __launch_bounds__(64 * W, CAP <= 4 && G > 32 ? 8 : 2) q4_few(Q4Params p) {
     using Lanes = Q4Lanes<G>;
     constexpr int P = Q8 ? 1 : 3, MB = (CAP + 15) / 16;
     constexpr int LW = Lanes::LW, NL = Lanes::NL;

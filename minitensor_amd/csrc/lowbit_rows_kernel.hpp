@@ -303,15 +303,16 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) rms_backward(RowBwdParams
         if constexpr (RES) {
             T g[NI], xh[NI];
             float s = 0.f;
+            // (the next row's loads ahead of this one's sums cost a wave of the four: 61 us
+            // against 50 for 8192 x 2048)
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int c = (i * NT + t) * V;
                 g[i] = c < p.cols ? row_load<MODE>(p.dy, r, c, p.cols) : zero;
-                xh[i] = c < p.cols ? row_load<MODE>(p.h, r, c, p.cols) : zero;
+                xh[i] = (c < p.cols ? row_load<MODE>(p.h, r, c, p.cols) : zero) * rstd;
             }
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                xh[i] = xh[i] * rstd;
                 dw[i] += g[i] * xh[i];
                 g[i] = g[i] * w[i];
                 s += row_dot(g[i], xh[i]);
@@ -361,49 +362,76 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) rms_backward(RowBwdParams
     }
 }
 
-// out[c] = beta*out[c] + sum over n parts, in order within each of 16 slices
-// and then over the slices: 64 columns per workgroup of 1024 threads.
+// out[c] = beta*out[c] + sum over n parts, in order within each of 64 slices and then over
+// the slices: 16 columns per workgroup of 1024 threads.  (64 columns and 16 slices left
+// most CUs without work: 5.4 us for 1024 parts of 2048.)
 __global__ void __launch_bounds__(1024)
 rms_dweight_sum(const float* part, int n, int cols, float* out, int64_t os, float beta) {
-    __shared__ float red[16][64];
-    const int l = threadIdx.x & 63, q = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + l;
+    __shared__ float red[64][17];
+    const int l = threadIdx.x & 15, q = threadIdx.x >> 4;
+    const int c = blockIdx.x * 16 + l;
     float s = 0.f;
     if (c < cols) {
 #pragma unroll 8
-        for (int i = q; i < n; i += 16) s += part[(int64_t)i * cols + c];
+        for (int i = q; i < n; i += 64) s += part[(int64_t)i * cols + c];
     }
     red[q][l] = s;
     __syncthreads();
-    if (q != 0 || c >= cols) return;
-    for (int i = 1; i < 16; ++i) s += red[i][l];
+    if (q >= 4 || c >= cols) return;                   // (one wave)
+    for (int i = q + 4; i < 64; i += 4) s += red[i][l];
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if (q != 0) return;
     float* const d = out + (int64_t)c * os;
     *d = beta != 0.f ? beta * *d + s : s;
 }
 
-// y = q·scale, V elements per thread: 16, or 4, of rows of a multiple of that,
-// or single ones at any strides.
-template <int V>
+// y = q·scale.  UNIT: a wave takes 1024 elements of a row, four dwords of codes per lane,
+// each load and store over neighbouring lanes' bytes (16 codes per lane, stored as four
+// pieces 64 bytes apart, took 42 us for 8192 x 4096 where these take 26); otherwise single
+// elements at any strides.
+template <bool UNIT>
 __global__ void __launch_bounds__(256)
 dequantize_q8(const int8_t* q, int64_t qs, const float* scale, RowView y, int64_t rows, int cols) {
-    typedef uint32_t codes __attribute__((ext_vector_type(V > 4 ? V / 4 : 1), aligned(1)));
-    const int64_t per = cols / V, n = rows * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per;
-        const int c = (int)(i - r * per) * V;
-        const float s = scale[r];
-        const int8_t* const src = q + r * qs + c;
-        if constexpr (V > 1) {
-            const codes w = *reinterpret_cast<const codes*>(src);
+    if constexpr (UNIT) {
+        const int lane = threadIdx.x & 63;
+        const int64_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+        const int segs = (cols + 1023) >> 10;
+        const int64_t n = rows * segs, step = (int64_t)gridDim.x * 4;
+        for (int64_t i = wave; i < n; i += step) {
+            const int64_t r = i / segs;
+            const int c0 = (int)(i - r * segs) * 1024 + 4 * lane;
+            const int8_t* const src = q + r * qs;
+            uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < V / 4; ++j) {
+            for (int j = 0; j < 4; ++j) {
+                const int c = c0 + 256 * j;
+                w[j] = 0;
+                if (c + 4 <= cols) {
+                    w[j] = *reinterpret_cast<const row_codes*>(src + c);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        if (c + e < cols) w[j] |= (uint32_t)(uint8_t)src[c + e] << (8 * e);
+                }
+            }
+            const float s = scale[r];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = c0 + 256 * j;
                 rowf4 o;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = (float)(int8_t)(w[j] >> (8 * e)) * s;
-                row_store<R_VEC>(y, r, c + 4 * j, cols, o);
+                if (c < cols) row_store<R_TAIL>(y, r, c, cols, o);
             }
-        } else {
-            y.p[r * y.rs + (int64_t)c * y.cs] = (float)*src * s;
+        }
+    } else {
+        const int64_t n = rows * cols;
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n;
+             i += (int64_t)gridDim.x * 256) {
+            const int64_t r = i / cols;
+            const int c = (int)(i - r * cols);
+            y.p[r * y.rs + (int64_t)c * y.cs] = (float)q[r * qs + c] * scale[r];
         }
     }
 }
