@@ -9,8 +9,8 @@
  * None of these has a counterpart in the reference, whose tensors are fp32
  * only; their fp32 operands are mt_mat_f32 views with batch 1.
  *
- * Sums and norms are fp32.  An output must not
- * overlap an input unless said otherwise.
+ * Sums and norms are fp32.  Extents are below 2^31 - 2^16, and a product has
+ * fewer than 2^23 tiles of 64 x 128 (strides and offsets are 64-bit).  An output must not overlap an input unless said otherwise.
  */
 #ifndef MTLOWBIT_H
 #define MTLOWBIT_H

@@ -14,11 +14,12 @@ using namespace mtk;
 
 namespace {
 
-constexpr int64_t kMaxDim = (int64_t)1 << 31;   // extents are 32-bit inside the kernels
-constexpr int64_t kMaxIn = kMaxDim - (1 << 16);  // inputs of one (blocks past the end stay below 2^31)
+// Extents are 32-bit inside the kernels, and blocks past an end stay below 2^31.
+constexpr int64_t kMaxDim = ((int64_t)1 << 31) - (1 << 16);
 constexpr int64_t kMaxOut = (int64_t)1 << 26;   // rows of a 4-bit weight (32 threads each in a grid)
 constexpr int64_t kMaxScaleStride = (int64_t)1 << 22;   // a tile's 256 rows of scales within 32 bits of bytes
 constexpr int kCus = 256;                       // what plans fill (MI355X)
+constexpr int64_t kMaxTiles = (int64_t)1 << 23; // of 512 threads: a grid's threads are a 32-bit number
 
 int launched() {
     // (as mt_gemm_f32: a launch recorded by a stream capture reports this)
@@ -45,7 +46,7 @@ bool valid(const mt_rows_q8* Q) {
     return Q->rows == 0 || (Q->scale && (Q->cols == 0 || Q->q));
 }
 bool valid(const mt_weight_q4* W) {
-    if (!W || W->n < 0 || W->k < 0 || W->n >= kMaxOut || W->k >= kMaxIn ||
+    if (!W || W->n < 0 || W->k < 0 || W->n >= kMaxOut || W->k >= kMaxDim ||
         (W->group != 32 && W->group != 64 && W->group != 128) || W->row_stride < 0 ||
         W->scale_stride < 0)
         return false;
@@ -98,8 +99,7 @@ void launch_rows(const RowParams& p, bool units, hipStream_t s) {
 // Row groups of the backward kernel, each of which keeps a part of dweight: enough to keep
 // the loads in flight, few enough that the parts weigh little (2048 x 4096, 256 to 2048
 // groups: 31, 29, 32, 41 us; 8192 x 2048: 67, 48, 46, 53; 1024 x 8192: 29, 35, 45, 45;
-// 8192 x 512: 51, 30, 20, 20).  A multiple of four, whether a
-// workgroup holds four groups or one.
+// 8192 x 512: 51, 30, 20, 20).  A multiple of four, whether a workgroup holds four groups or one.
 int64_t row_groups(int64_t rows, int64_t cols) {
     const int nt = row_threads(cols);
     const int64_t most = nt == 64 ? 2048 : nt == 256 ? 640 : 256;
@@ -119,6 +119,7 @@ struct Tiling {
 };
 struct Tiled {
     int bm, splits, k_per_split;
+    int64_t tiles;                    // the splits' among them
     size_t partials;                  // floats, 0 without splits
 };
 Tiled plan_tiles(int64_t M, int64_t N, int64_t K, const Tiling* t, int n) {
@@ -139,7 +140,7 @@ Tiled plan_tiles(int64_t M, int64_t N, int64_t K, const Tiling* t, int n) {
             if (s > 1) us += 2.5 + (double)(s + 1) * (double)M * (double)N * 1e-6;
             if (least == 0 || us < least) {
                 least = us;
-                best = {t[i].bm, (int)s, (int)(per * 128), s > 1 ? (size_t)(s * M * N) : 0};
+                best = {t[i].bm, (int)s, (int)(per * 128), wgs, s > 1 ? (size_t)(s * M * N) : 0};
             }
             if (wgs >= 4 * slots) break;
         }
@@ -188,14 +189,12 @@ void launch_few(const Q4Params& p, hipStream_t s) {
         go(integral_constant<int, 48>{}, integral_constant<int, 1>{});
 }
 template <bool Q8, int G>
-void launch_gemm(const Q4Params& p, int bm, hipStream_t s) {
-    const int64_t tiles = (int64_t)((p.M + bm - 1) / bm) * ((p.N + 2 * bm - 1) / (2 * bm)) * p.splits;
-    if (bm == 64)
-        hipLaunchKernelGGL((q4_gemm<64, 128, 32, 64, G, Q8>), dim3((unsigned)tiles), dim3(256), 0, s,
-                           p);
+void launch_gemm(const Q4Params& p, const Tiled& plan, hipStream_t s) {
+    const dim3 grid((unsigned)plan.tiles);
+    if (plan.bm == 64)
+        hipLaunchKernelGGL((q4_gemm<64, 128, 32, 64, G, Q8>), grid, dim3(256), 0, s, p);
     else if constexpr (G > 32)
-        hipLaunchKernelGGL((q4_gemm<128, 256, 32, 128, G, Q8>), dim3((unsigned)tiles), dim3(512), 0,
-                           s, p);
+        hipLaunchKernelGGL((q4_gemm<128, 256, 32, 128, G, Q8>), grid, dim3(512), 0, s, p);
 }
 
 template <bool Q8>
@@ -223,6 +222,7 @@ int run_q4(Q4Params p, int64_t M, const mt_weight_q4* W, const float* bias, int6
         return launched();
     }
     const size_t need = plan.tiled.partials * 4;
+    if (plan.tiled.tiles >= kMaxTiles) return MT_ERR_INVALID;
     if (need > 0 && (!workspace || ws_bytes < need)) return MT_ERR_WORKSPACE;
     p.splits = plan.few ? 1 : plan.tiled.splits;
     p.k_per_split = plan.tiled.k_per_split;
@@ -230,7 +230,7 @@ int run_q4(Q4Params p, int64_t M, const mt_weight_q4* W, const float* bias, int6
     auto go = [&](auto g) {
         constexpr int G = decltype(g)::value;
         if (plan.few) launch_few<Q8, G>(p, s);
-        else launch_gemm<Q8, G>(p, plan.tiled.bm, s);
+        else launch_gemm<Q8, G>(p, plan.tiled, s);
     };
     if (W->group == 32) go(std::integral_constant<int, 32>{});
     else if (W->group == 64) go(std::integral_constant<int, 64>{});
@@ -387,6 +387,7 @@ int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const m
         return MT_ERR_INVALID;
     if (db && (db_stride < 0 || (dY->cols > 1 && db_stride == 0))) return MT_ERR_INVALID;
     const Tiled plan = back_plan(X->rows, dY->cols, X->cols);
+    if (dW && plan.tiles >= kMaxTiles) return MT_ERR_INVALID;
     if (dW && plan.partials > 0 && (!workspace || ws_bytes < plan.partials * 4))
         return MT_ERR_WORKSPACE;
     const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -422,14 +423,11 @@ int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const m
         const LbSum sum{p.part, p.R > 0 ? p.splits : 0, p.O, p.C, nullptr, 0, p.dw, p.dw_o, p.dw_c,
                         beta_w, p.part_b, db, db_stride, beta_b, p.O};
         if (p.R > 0) {
-            const int64_t tiles = (int64_t)((p.O + plan.bm - 1) / plan.bm) *
-                                  ((p.C + 2 * plan.bm - 1) / (2 * plan.bm)) * p.splits;
+            const dim3 grid((unsigned)plan.tiles);
             if (plan.bm == 64)
-                hipLaunchKernelGGL((back_dw<64, 128, 32, 64>), dim3((unsigned)tiles), dim3(256), 0, s,
-                                   p);
+                hipLaunchKernelGGL((back_dw<64, 128, 32, 64>), grid, dim3(256), 0, s, p);
             else
-                hipLaunchKernelGGL((back_dw<128, 256, 32, 128>), dim3((unsigned)tiles), dim3(512), 0,
-                                   s, p);
+                hipLaunchKernelGGL((back_dw<128, 256, 32, 128>), grid, dim3(512), 0, s, p);
         }
         if (p.R == 0 || p.splits > 1) {               // (no rows: beta·dW, beta·db)
             const int64_t n = (int64_t)p.O * p.C + p.O;
@@ -473,7 +471,7 @@ int mt_dequantize_q4_f32(const mt_weight_q4* Q, const mt_mat_f32* W, void* strea
 }
 
 size_t mt_linear_q4_workspace(int64_t rows, int64_t in_f, int64_t out_f) {
-    if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxIn ||
+    if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxDim ||
         out_f >= kMaxDim)
         return 0;
     size_t n = 0;

@@ -400,6 +400,23 @@ py::object quantize_q8(py::handle px, py::handle stream) {
     return py::make_tuple(tensor(q), tensor(scale));
 }
 
+py::object dequantize_q8(py::handle pq, py::handle pscale, py::handle pout, py::handle stream) {
+    bool ok = true;
+    const at::Tensor q = rows_arg(pq, at::kChar, 2, &ok);
+    const at::Tensor scale = rows_arg(pscale, at::kFloat, 1, &ok);
+    at::Tensor out = arg(pout, &ok);
+    if (!ok || scale.size(0) != q.size(0) || !shaped(out, q.size(0), q.size(1))) return py::none();
+    void* const s = stream_of(stream);
+    {
+        const py::gil_scoped_release nogil;
+        if (!out.defined()) out = empty(q.sizes(), q);
+        const mt_rows_q8 mq = rows_q8(q, scale);
+        const mt_mat_f32 my = mat(out);
+        check(mt_dequantize_q8_f32(&mq, &my, s), "mt_dequantize_q8_f32");
+    }
+    return pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout);
+}
+
 py::object linear_backward_q8(py::handle pdy, py::handle pq, py::handle pscale, py::handle pw,
                               bool need_dw, bool need_db, py::handle pdx, py::handle pdw,
                               py::handle pdb, float beta_w, float beta_b, py::handle pws,
@@ -500,6 +517,7 @@ PYBIND11_MODULE(_native, m) {
     m.def("rms_norm", &rms_norm);
     m.def("rms_norm_backward", &rms_norm_backward);
     m.def("quantize_q8", &quantize_q8);
+    m.def("dequantize_q8", &dequantize_q8);
     m.def("linear_backward_q8", &linear_backward_q8);
     m.def("linear_q4", &linear_q4);
 }

@@ -239,6 +239,9 @@ def quantize_q8(x: torch.Tensor, out: Optional[Q8Rows] = None, stream=None) -> Q
 @_api
 def dequantize_q8(xq: Q8Rows, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """q·scale in float32."""
+    r = native().dequantize_q8(xq[0], xq[1], out, _handle(stream))
+    if r is not None:
+        return r
     d = _rows(xq)
     if out is None:
         out = _empty(xq.q.shape, xq.q)

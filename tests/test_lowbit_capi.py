@@ -38,6 +38,7 @@ BAD_QUANTIZE = {
     "negative stride": (M(4, 8, rs=-8), Q(4, 8)),
     "no x": (M(4, 8, base=0), Q(4, 8)),
     "past 32 bits": (M(1 << 31, 8), Q(1 << 31, 8)),
+    "blocks past 32 bits": (M(1, (1 << 31) - (1 << 16)), Q(1, (1 << 31) - (1 << 16))),
 }
 
 
@@ -102,6 +103,7 @@ BAD_WEIGHT = {
     "negative n": W(-1, 64),
     "n past 2^26": W(1 << 26, 64),
     "k past 32 bits": W(4, (1 << 31) - 1),
+    "scales far apart": W(4, 64, ss=1 << 22),
 }
 
 
@@ -122,6 +124,9 @@ def test_linear_q4_refuses():
     assert f(R(M(3, 64)), R(W(4, 64)), None, 0, R(M(3, 4, cs=0)), None, 0, None) == INVALID
     assert f(R(M(3, 64)), R(W(4, 64)), 0x100, -1, R(M(3, 4)), None, 0, None) == INVALID
     assert g(R(Q(3, 64, rs=10)), R(W(4, 64)), None, 0, R(M(3, 4)), None, 0, None) == INVALID
+    many = 1 << 30                    # more tiles than a grid has threads
+    assert f(R(M(many, 64)), R(W(4, 64)), None, 0, R(M(many, 4)), None, 0, None) == INVALID
+    assert g(R(Q(many, 64)), R(W(4, 64)), None, 0, R(M(many, 4)), None, 0, None) == INVALID
     assert f(R(M(0, 64)), R(W(4, 64)), None, 0, R(M(0, 4)), None, 0, None) == OK
     assert g(R(Q(0, 64)), R(W(4, 64)), None, 0, R(M(0, 4)), None, 0, None) == OK
     assert f(R(M(3, 64)), R(W(0, 64)), None, 0, R(M(3, 0)), None, 0, None) == OK
