@@ -106,16 +106,17 @@ int64_t row_groups(int64_t rows, int64_t cols) {
     return (std::min(rows, most) + 3) / 4 * 4;
 }
 
-// Tiles and splits of a product over chunks of 32 k.  Measured times of a chunk in us, by
-// workgroups on a CU, where each holds as many as its LDS and registers allow: the tile
-// and the number of splits that come out fastest, workgroups going in rounds over the CUs,
-// with the partials' sum at 4 TB/s and a launch.  (1024 rows, 4096 -> 4096: 128x256 tiles
-// in 2 splits 100 us, 64x128 unsplit 118; 1027 8-bit rows, 2048 -> 4096: 64x128 unsplit 50,
-// 128x256 61 unsplit and 79 in 3 splits.)
+// Tiles and splits of a product over chunks of 32 k, from measured times in us: of a chunk,
+// by workgroups on a CU, where each holds as many as its LDS and registers allow, and of a
+// round's beginning and end.  The tile and the number of splits that come out fastest,
+// workgroups going in rounds over the CUs, with a launch and the partials' sum.  (4096 ->
+// 4096: 1024 fp32 rows, 128x256 tiles in 2 splits 100 us, 64x128 unsplit 118; 1024 8-bit
+// rows 53 and 46, 2048 of them unsplit 63 and 84, 256 of them, 64x128 in 2 splits 28,
+// unsplit 31.)
 struct Tiling {
     int bm;                           // of bm x 2·bm
     int per_cu;
-    double alone, full;               // a chunk's time: one workgroup on the CU, all of them
+    double alone, more;               // a chunk's time: one workgroup on the CU, each further one
 };
 struct Tiled {
     int bm, splits, k_per_split;
@@ -132,12 +133,14 @@ Tiled plan_tiles(int64_t M, int64_t N, int64_t K, const Tiling* t, int n) {
             const int64_t per = (blocks + s - 1) / s;
             if ((blocks + per - 1) / per != s) continue;
             const int64_t wgs = tiles * s, slots = (int64_t)kCus * t[i].per_cu;
-            const int64_t rest = wgs % slots;
-            double rounds = (double)(wgs / slots) * t[i].full;
-            if (rest > kCus) rounds += t[i].full;
-            else if (rest > 0) rounds += t[i].alone;
-            double us = (double)std::min<int64_t>(4 * per, (K + 31) / 32) * rounds;
-            if (s > 1) us += 2.5 + (double)(s + 1) * (double)M * (double)N * 1e-6;
+            const double chunks = (double)std::min<int64_t>(4 * per, (K + 31) / 32);
+            auto round = [&](int64_t n) {             // with n workgroups on a CU
+                return chunks * (t[i].alone + (double)(n - 1) * t[i].more) + 5 +
+                       (double)(n * t[i].bm / 32);
+            };
+            double us = (double)(wgs / slots) * round(t[i].per_cu);
+            if (wgs % slots) us += round((wgs % slots + kCus - 1) / kCus);
+            if (s > 1) us += 4 + (double)(s + 1) * (double)M * (double)N * 1.2e-6;
             if (least == 0 || us < least) {
                 least = us;
                 best = {t[i].bm, (int)s, (int)(per * 128), wgs, s > 1 ? (size_t)(s * M * N) : 0};
@@ -155,9 +158,12 @@ struct Q4Plan {
 Q4Plan q4_plan(int64_t M, int64_t N, int64_t K, int group, bool q8) {
     if (M * (q8 ? 1 : 3) <= 48) return {true, {}};
     // (groups of 32: the wide tile's scales do not fit the registers)
-    static const Tiling f32[] = {{64, 2, 0.5, 0.92}, {128, 1, 1.2, 1.2}};
-    static const Tiling int8[] = {{64, 3, 0.5, 0.78}, {128, 1, 0.84, 0.84}};
-    return {false, plan_tiles(M, N, K, q8 ? int8 : f32, group == 32 ? 1 : 2)};
+    static const Tiling f32[] = {{64, 2, 0.5, 0.42}, {128, 1, 1.2, 0}};
+    static const Tiling int8_32[] = {{64, 4, 0.3, 0.13}};
+    static const Tiling int8_64[] = {{64, 4, 0.25, 0.1}, {128, 1, 0.53, 0}};
+    static const Tiling int8_128[] = {{64, 4, 0.18, 0.117}, {128, 1, 0.38, 0}};
+    const Tiling* const t = !q8 ? f32 : group == 32 ? int8_32 : group == 64 ? int8_64 : int8_128;
+    return {false, plan_tiles(M, N, K, t, group == 32 ? 1 : 2)};
 }
 
 template <bool Q8, int G>
@@ -191,10 +197,15 @@ void launch_few(const Q4Params& p, hipStream_t s) {
 template <bool Q8, int G>
 void launch_gemm(const Q4Params& p, const Tiled& plan, hipStream_t s) {
     const dim3 grid((unsigned)plan.tiles);
-    if (plan.bm == 64)
-        hipLaunchKernelGGL((q4_gemm<64, 128, 32, 64, G, Q8>), grid, dim3(256), 0, s, p);
+    if constexpr (Q8) {
+        if (plan.bm == 64)
+            hipLaunchKernelGGL((q4_gemm_q8<64, 128, 32, 64, G>), grid, dim3(256), 0, s, p);
+        else if constexpr (G > 32)
+            hipLaunchKernelGGL((q4_gemm_q8<128, 256, 64, 64, G>), grid, dim3(512), 0, s, p);
+    } else if (plan.bm == 64)
+        hipLaunchKernelGGL((q4_gemm<64, 128, 32, 64, G>), grid, dim3(256), 0, s, p);
     else if constexpr (G > 32)
-        hipLaunchKernelGGL((q4_gemm<128, 256, 32, 128, G, Q8>), grid, dim3(512), 0, s, p);
+        hipLaunchKernelGGL((q4_gemm<128, 256, 32, 128, G>), grid, dim3(512), 0, s, p);
 }
 
 template <bool Q8>
@@ -246,7 +257,7 @@ int run_q4(Q4Params p, int64_t M, const mt_weight_q4* W, const float* bias, int6
 // The weight gradient [O][C] over R rows, and the floats of its workspace: the splits'
 // partial products and row sums.
 Tiled back_plan(int64_t R, int64_t O, int64_t C) {
-    static const Tiling tiles[] = {{64, 2, 0.8, 1.0}, {128, 1, 1.35, 1.35}};
+    static const Tiling tiles[] = {{64, 2, 0.8, 0.2}, {128, 1, 1.35, 0}};
     Tiled t = plan_tiles(O, C, R, tiles, 2);
     if (t.partials) t.partials += (size_t)t.splits * O;
     return t;
@@ -475,7 +486,7 @@ size_t mt_linear_q4_workspace(int64_t rows, int64_t in_f, int64_t out_f) {
         out_f >= kMaxDim)
         return 0;
     size_t n = 0;
-    for (const int group : {32, 128})
+    for (const int group : {32, 64, 128})
         for (const bool q8 : {false, true})
             n = std::max(n, q4_plan(rows, out_f, in_f, group, q8).tiled.partials);
     return n * 4;

@@ -1,6 +1,6 @@
 // lowbit_gemm.hpp -- the product that the operators of include/mtlowbit.h share: an
-// operand A in fp32, cut into three bf16 values, or in 8 bits (exact in bf16), times
-// an operand B in 8 or 4 bits, on the bf16 matrix units.
+// operand A in fp32, cut into three bf16 values, times an operand B in 8 or 4 bits
+// (exact in bf16), on the bf16 matrix units.
 //
 // Tiles of BM x BN over chunks of 32 k, in two LDS buffers: while chunk c is multiplied,
 // chunk c+1, loaded into registers before, is converted to bf16 and written to the other
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(256) lb_sum(LbSum p) {
         const float* const part = vec ? p.part_v + (i - n) : p.part + i;
         const int64_t stride = vec ? p.L : n;
         float s = 0.f;
-#pragma unroll 4
+#pragma unroll 8
         for (int k = 0; k < p.splits; ++k) s += part[k * stride];
         const int m = (int)(i / p.N), c = (int)(i - (int64_t)m * p.N);
         if (p.bias && !vec) s += p.bias[(int64_t)c * p.bias_stride];

@@ -4,12 +4,13 @@
 // A 4-bit code is exact in bf16, and an fp32 x is the sum of three bf16 values
 // h + m + l (gemm_split.hpp): the product is three bf16 products on the matrix
 // units, each exact, with fp32's precision (six for two fp32 operands); an
-// 8-bit x is exact in bf16 by itself, one product, and its sums within a group
-// are whole numbers below 2^24, exact too.  The sums of a group are taken on
-// the matrix unit from zero and added to the fp32 result with one fused
-// multiply-add by the group's scale.
+// 8-bit x takes one product, whose sums within a group are whole numbers below
+// 2^24, exact too.  The sums of a group are taken on the matrix unit from zero
+// and added to the fp32 result with one fused multiply-add by the group's
+// scale.
 //
-// q4_few: few rows of x, bound by the weight's bytes.  q4_gemm: the rest.
+// q4_few: few rows of x, bound by the weight's bytes.  The rest: q4_gemm, fp32
+// rows, and q4_gemm_q8, 8-bit ones.
 #pragma once
 
 #include "lowbit_gemm.hpp"
@@ -290,52 +291,40 @@ __global__ void __launch_bounds__(64 * W, CAP <= 4 && G > 32 ? 8 : 2) q4_few(Q4P
     }
 }
 
-// Many rows: x as A, in fp32 or in 8 bits; a thread takes eight inputs of a row.
-template <bool Q8, int BM, int NT>
+// Many rows of fp32: x as A; a thread takes eight inputs of a row.
+template <int BM, int NT>
 struct Q4X {
     static constexpr int N = BM * 4 / NT, kGroup = lb_group<BM>(), kBytes = lb_plane<BM>();
     static_assert(N * NT == BM * 4, "whole items");
-    static constexpr int kWork = N * 8 * (Q8 ? 2 : 7);
-    static constexpr bool kLate = Q8;
-    struct RawX {
+    static constexpr int kWork = N * 56;
+    static constexpr bool kLate = false;
+    struct Raw {
         float a[N][8];
     };
-    struct RawQ {
-        u32x2 q[N];
-    };
-    using Raw = std::conditional_t<Q8, RawQ, RawX>;
-    using T = std::conditional_t<Q8, int8_t, float>;
     const Q4Params& p;
-    const T* base;                    // row m0
+    const float* base;                // row m0
     uint32_t off[N];                  // of the item, in bytes
     int64_t ld;
     int t, last;
     bool fast;                        // a row's inputs are neighbours, the tile within 32 bits of bytes
     __device__ __forceinline__ static int entry(int row) { return row; }
-    __device__ __forceinline__ Q4X(const Q4Params& p_, int m0, int t_) : p(p_), t(t_), last(p_.M - 1 - m0) {
-        if constexpr (Q8) base = p.q, ld = p.q_m;
-        else base = p.x, ld = p.x_m;
-        base += m0 * ld;
-        fast = (Q8 || p.x_k == 1) && ld < (1 << 22);
+    __device__ __forceinline__ Q4X(const Q4Params& p_, int m0, int t_)
+        : p(p_), base(p_.x + m0 * p_.x_m), ld(p_.x_m), t(t_), last(p_.M - 1 - m0),
+          fast(p_.x_k == 1 && p_.x_m < (1 << 22)) {
 #pragma unroll
         for (int i = 0; i < N; ++i)                        // (rows past M: the last, not stored)
-            off[i] = ((uint32_t)min((i * NT + t) >> 2, last) * (uint32_t)ld + 8 * (t & 3)) *
-                     (uint32_t)sizeof(T);
+            off[i] = ((uint32_t)min((i * NT + t) >> 2, last) * (uint32_t)ld + 8 * (t & 3)) * 4u;
     }
     __device__ __forceinline__ void load_fast(Raw& r, int k0) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const T* const x = at_bytes(base + k0, off[i]);
-            if constexpr (Q8) {
-                r.q[i] = *reinterpret_cast<const u32x2_u*>(x);
-            } else {
-                const rowf4 a = *reinterpret_cast<const rowf4_u*>(x);
-                const rowf4 b = *reinterpret_cast<const rowf4_u*>(x + 4);
+            const float* const x = at_bytes(base + k0, off[i]);
+            const rowf4 a = *reinterpret_cast<const rowf4_u*>(x);
+            const rowf4 b = *reinterpret_cast<const rowf4_u*>(x + 4);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    r.a[i][e] = a[e];
-                    r.a[i][4 + e] = b[e];
-                }
+            for (int e = 0; e < 4; ++e) {
+                r.a[i][e] = a[e];
+                r.a[i][4 + e] = b[e];
             }
         }
     }
@@ -343,25 +332,18 @@ struct Q4X {
         if (fast && k0 + 32 <= p.K) return load_fast(r, k0);
         const int v = anew(t);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const T* const x = base + min((i * NT + v) >> 2, last) * ld;
-            if constexpr (Q8) r.q[i] = q4_x8(p, x, k0 + 8 * (v & 3));
-            else q4_x8(p, x, k0 + 8 * (v & 3), r.a[i]);
-        }
+        for (int i = 0; i < N; ++i)
+            q4_x8(p, base + min((i * NT + v) >> 2, last) * ld, k0 + 8 * (v & 3), r.a[i]);
     }
     __device__ __forceinline__ void store(const Raw& r, char* buf, bool) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             char* const d = buf + (t & 3) * kGroup + ((i * NT + t) >> 2) * 16;
-            if constexpr (Q8) {
-                *reinterpret_cast<u32x4*>(d) = q8_bf16(r.q[i]);
-            } else {
-                u32x4 h, m, l;
-                cut8(r.a[i], h, m, l);
-                *reinterpret_cast<u32x4*>(d) = h;
-                *reinterpret_cast<u32x4*>(d + kBytes) = m;
-                *reinterpret_cast<u32x4*>(d + 2 * kBytes) = l;
-            }
+            u32x4 h, m, l;
+            cut8(r.a[i], h, m, l);
+            *reinterpret_cast<u32x4*>(d) = h;
+            *reinterpret_cast<u32x4*>(d + kBytes) = m;
+            *reinterpret_cast<u32x4*>(d + 2 * kBytes) = l;
         }
     }
 };
@@ -488,13 +470,13 @@ struct Q4Scales {
     }
 };
 
-template <int BM, int BN, int WM, int WN, int G, bool Q8>
+template <int BM, int BN, int WM, int WN, int G>
 __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, BM > 64 || G == 32 ? 2 : 3)
 q4_gemm(Q4Params p) {
-    constexpr int P = Q8 ? 1 : 3;
+    constexpr int P = 3;
     constexpr int WAVES_N = BN / WN, NT = BM / WM * WAVES_N * 64;
     constexpr int MB = WM / 32, NB = WN / 32;
-    using LA = Q4X<Q8, BM, NT>;
+    using LA = Q4X<BM, NT>;
     using LB = Q4W<BN, NT, BN == 128>;
     __shared__ __attribute__((aligned(16))) char smem[2 * (P * LA::kBytes + LB::kBytes) +
                                                          2 * LB::kRaw];
@@ -544,8 +526,198 @@ q4_gemm(Q4Params p) {
             for (int r = 0; r < 16; ++r) {
                 const int m = m0 + ra + 32 * i + lb_row(lane, r);
                 if (m >= p.M) continue;
-                float v = sum[i][j][r];
-                if constexpr (Q8) v *= p.q_scale[m];
+                const float v = sum[i][j][r];
+                if (part) p.part[((int64_t)split * p.M + m) * p.N + n] = v;
+                else p.y[(int64_t)m * p.y_m + (int64_t)n * p.y_n] = v + b;
+            }
+        }
+}
+
+// Many 8-bit rows: both operands in int8 on the integer matrix unit, at twice bf16's rate and
+// half its bytes in LDS; the sums of a group are whole numbers below 2^21.  A code goes in as
+// 16 times itself, the high half of a byte: two masks and a shift for the eight of a dword,
+// four even inputs and four odd ones, in which order x is put to LDS too.  The codes stay
+// packed there, and each wave unpacks the columns that it multiplies.
+//
+// Chunks of 64 k in two LDS buffers, as lb_product, and two on their way.  What bounds it is
+// the vector unit, which turns each sum into fp32 and adds it, in groups of 32 three
+// instructions of four (1536 rows, 4096 -> 4096: 93% of its cycles), so four workgroups of
+// the narrow tile share a CU.  2048 rows, 4096 -> 8192, groups of 128, 64 and
+// 32: 121, 157 and 205 us (on the bf16 units, x and codes converted: 211, 219 and, of 32,
+// 1027 rows, 2047 -> 4096, 64 where this takes 48).  Sums added beside the next group's
+// MFMAs, from accumulators of their own, took as long.
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_u __attribute__((aligned(1)));
+
+template <int BM, int BN, int WM, int WN, int G>
+__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, BM > 64 ? 2 : 4) q4_gemm_q8(Q4Params p) {
+    constexpr int WAVES_N = BN / WN, NT = BM / WM * WAVES_N * 64;
+    constexpr int MB = WM / 32, NB = WN / 32;
+    static_assert(BM * 4 == NT && BN * 2 == NT, "16 bytes of x and of the weight per thread");
+    constexpr int XG = lb_group<BM>(), WG = lb_group<BN>(), BUF = 4 * XG + 2 * WG;
+    __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+    const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int ra = wave / WAVES_N * WM, rb = wave % WAVES_N * WN;
+    const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
+    const int split = blockIdx.x / (tiles_m * tiles_n);
+    int im, in;
+    lb_tile(blockIdx.x - split * tiles_m * tiles_n, tiles_m, tiles_n, im, in);
+    const int m0 = im * BM, n0 = in * BN;
+    const int kb = split * p.k_per_split, ke = min(p.K, kb + p.k_per_split);
+
+    // (rows and columns past the end: the last, not stored)
+    const int row = min(t >> 2, p.M - 1 - m0), col = min(t >> 1, p.N - 1 - n0);
+    const int8_t* const xt = p.q + m0 * p.q_m;
+    const uint8_t* const wt = p.w + n0 * p.w_n;
+    const bool fast = p.q_m < (1 << 22) && p.w_n < (1 << 23);   // the tile within 32 bits of bytes
+    const uint32_t xo = (uint32_t)row * (uint32_t)p.q_m + 16 * (t & 3);
+    const uint32_t wo = (uint32_t)col * (uint32_t)p.w_n + 16 * (t & 1);
+    const int w_end = ((p.K + 31) & ~31) >> 1;                  // bytes of a row of codes
+    u32x4 xr[2], wr[2];                                         // chunk c in [c % 2]
+    auto load_fast = [&](int slot, int c) {
+        const int k0 = kb + 64 * c;
+        xr[slot] = *reinterpret_cast<const u32x4_u*>(at_bytes(xt + k0, xo));
+        wr[slot] = *reinterpret_cast<const u32x4*>(at_bytes(wt + (k0 >> 1), wo));
+    };
+    auto load = [&](int slot, int c) {                          // x zero past K, so that codes do not matter
+        const int k0 = kb + 64 * c;
+        if (fast && k0 + 64 <= p.K) return load_fast(slot, c);
+        const int v = anew(t), k = k0 + 16 * (v & 3);
+        const int8_t* const x = xt + min(v >> 2, p.M - 1 - m0) * p.q_m + k;
+        if (k + 16 <= p.K) {
+            xr[slot] = *reinterpret_cast<const u32x4_u*>(x);
+        } else {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                uint32_t b = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (k + 4 * d + e < p.K) b |= (uint32_t)(uint8_t)x[4 * d + e] << (8 * e);
+                xr[slot][d] = b;
+            }
+        }
+        wr[slot] = *reinterpret_cast<const u32x4*>(wt + min(v >> 1, p.N - 1 - n0) * p.w_n +
+                                                   min((k0 >> 1) + 16 * (v & 1), w_end - 16));
+    };
+    auto put = [&](int slot, int b) {
+        char* const buf = smem + b * BUF;
+        const u32x4 x = xr[slot];
+        u32x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            o[i] = __builtin_amdgcn_perm(x[i + 1], x[i], 0x06040200);
+            o[i + 1] = __builtin_amdgcn_perm(x[i + 1], x[i], 0x07050301);
+        }
+        *reinterpret_cast<u32x4*>(buf + (t & 3) * XG + (t >> 2) * 16) = o;
+        *reinterpret_cast<u32x4*>(buf + 4 * XG + (t & 1) * WG + (t >> 1) * 16) = wr[slot];
+    };
+
+    f32x16 sum[MB][NB];
+    i32x16 acc[MB][NB];
+    zero_blocks<MB, NB>(sum);
+    constexpr int GB = 128 / G;
+    Q4Scales<NB, G, GB> sc(p, n0, rb + (lane & 31), kb);
+    // group i of a block of 128 inputs has its sums
+    auto flush = [&](auto i, int block) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const float s = sc.cur[j][i] * (1.f / 16);
+#pragma unroll
+            for (int m = 0; m < MB; ++m)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    sum[m][j][r] = __builtin_fmaf((float)acc[m][j][r], s, sum[m][j][r]);
+#pragma unroll
+            for (int m = 0; m < MB; ++m) asm volatile("" : "+v"(sum[m][j]));   // (as q4_gemm)
+        }
+        if constexpr (i == GB - 1) sc.advance(kb / G + (block + 2) * GB);
+    };
+    using std::integral_constant;
+    // chunk c, c % 2 = s
+    auto multiply = [&](int c, auto s) {
+        const char* const buf = smem + s() * BUF;
+        u32x4 a[2][MB];
+        u32x2 w[2][NB];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {                           // 32 k each
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+                a[h][i] = *reinterpret_cast<const u32x4*>(buf + (2 * h + half) * XG +
+                                                          (ra + 32 * i + (lane & 31)) * 16);
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                w[h][j] = *reinterpret_cast<const u32x2*>(
+                    buf + 4 * XG + h * WG + (rb + 32 * j + (lane & 31)) * 16 + 8 * half);
+        }
+        auto part = [&](auto h) {
+            constexpr int group = (2 * s() + h()) * 32 / G;
+            constexpr bool first = (2 * s() + h()) * 32 % G == 0;
+            constexpr bool whole = (2 * s() + h() + 1) * 32 % G == 0;
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                u32x4 b;
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    b[2 * d] = (w[h()][j][d] << 4) & 0xf0f0f0f0u;
+                    b[2 * d + 1] = w[h()][j][d] & 0xf0f0f0f0u;
+                }
+#pragma unroll
+                for (int i = 0; i < MB; ++i) {
+                    i32x16 o = acc[i][j];
+                    if constexpr (first)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[r] = 0;
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(
+                        __builtin_bit_cast(i32x4, a[h()][i]), __builtin_bit_cast(i32x4, b), o, 0, 0, 0);
+                }
+            }
+            if constexpr (whole) flush(integral_constant<int, group>{}, c >> 1);
+        };
+        part(integral_constant<int, 0>{});
+        part(integral_constant<int, 1>{});
+    };
+    const int nk = (ke - kb + 127) >> 7 << 1;                   // (an odd one's last chunk: zeros)
+    const int whole = fast ? (ke - kb) >> 6 : 0;
+    load(0, 0);
+    load(1, 1);
+    put(0, 0);
+    auto step = [&](int c, auto s) {
+        lb_barrier();
+        load_fast(s(), min(c + 2, nk - 1));                     // (past the last chunk: that again)
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(c, s);
+        put(~s() & 1, ~s() & 1);
+    };
+    int c = 0;
+    for (; c + 4 <= whole || (c < whole && whole == nk); c += 2) {
+        step(c, integral_constant<int, 0>{});
+        step(c + 1, integral_constant<int, 1>{});
+    }
+    for (; c < nk; c += 2) {
+        lb_barrier();
+        if (c + 2 < nk) load(0, c + 2);
+        multiply(c, integral_constant<int, 0>{});
+        put(1, 1);
+        lb_barrier();
+        if (c + 3 < nk) load(1, c + 3);
+        multiply(c + 1, integral_constant<int, 1>{});
+        if (c + 2 < nk) put(0, 0);
+    }
+    const bool part = p.splits > 1;
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int n = n0 + rb + 32 * j + (lane & 31);
+            if (n >= p.N) continue;
+            const float b = !part && p.bias ? p.bias[(int64_t)n * p.bias_stride] : 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int m = m0 + ra + 32 * i + lb_row(lane, r);
+                if (m >= p.M) continue;
+                const float v = sum[i][j][r] * p.q_scale[m];
                 if (part) p.part[((int64_t)split * p.M + m) * p.N + n] = v;
                 else p.y[(int64_t)m * p.y_m + (int64_t)n * p.y_n] = v + b;
             }
