@@ -102,7 +102,7 @@ void launch_rows(const RowParams& p, bool units, hipStream_t s) {
 // 8192 x 512: 51, 30, 20, 20).  A multiple of four, whether a workgroup holds four groups or one.
 int64_t row_groups(int64_t rows, int64_t cols) {
     const int nt = row_threads(cols);
-    const int64_t most = nt == 64 ? 2048 : nt == 256 ? 640 : 256;
+    const int64_t most = nt == 64 ? 2048 : nt == 256 ? 768 : 256;
     return (std::min(rows, most) + 3) / 4 * 4;
 }
 

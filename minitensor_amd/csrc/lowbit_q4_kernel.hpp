@@ -541,9 +541,9 @@ q4_gemm(Q4Params p) {
 //
 // Chunks of 64 k in two LDS buffers, as lb_product, and two on their way.  What bounds it is
 // the vector unit, which turns each sum into fp32 and adds it, in groups of 32 three
-// instructions of four (1536 rows, 4096 -> 4096: 93% of its cycles), so four workgroups of
+// instructions of four (1536 rows, 4096 -> 4096: 91% of its cycles), so four workgroups of
 // the narrow tile share a CU.  2048 rows, 4096 -> 8192, groups of 128, 64 and
-// 32: 121, 157 and 205 us (on the bf16 units, x and codes converted: 211, 219 and, of 32,
+// 32: 121, 157 and 200 us (on the bf16 units, x and codes converted: 211, 219 and, of 32,
 // 1027 rows, 2047 -> 4096, 64 where this takes 48).  Sums added beside the next group's
 // MFMAs, from accumulators of their own, took as long.
 typedef int i32x16 __attribute__((ext_vector_type(16)));
