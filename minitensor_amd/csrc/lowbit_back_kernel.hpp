@@ -270,19 +270,23 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) back_dw(BackParam
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int m = m0 + ra + 32 * i + lb_row(lane, r);
-                    if (m < p.O) put(m, n, sum[i][j][r]);
+                    float v = sum[i][j][r], old = acc[i][j][r];
+                    if (m < p.O) put(m, n, v, old);
+                    sum[i][j][r] = v;
+                    acc[i][j][r] = old;
                 }
             }
     };
     float* const out = part ? p.part + (int64_t)split * p.O * p.C : p.dw;
     const int64_t om = part ? p.C : p.dw_o, on = part ? 1 : p.dw_c;
-    if (part || p.beta == 0.f)
-        each([&](int m, int n, float v) { out[m * om + n * on] = v; });
-    else
-        each([&](int m, int n, float v) {
-            float* const d = out + (m * om + n * on);
-            *d = p.beta * *d + v;
-        });
+    // (the old values first, all on their way at once: with loads and stores in turn 256 rows,
+    // 2048 -> 1000, took 14.8 us, so 13.4)
+    const float beta = part ? 0.f : p.beta;
+    if (beta != 0.f) {
+        each([&](int m, int n, float& v, float& old) { old = out[m * om + n * on]; });
+        each([&](int m, int n, float& v, float& old) { v = beta * old + v; });
+    }
+    each([&](int m, int n, float& v, float&) { out[m * om + n * on] = v; });
 }
 
 }  // namespace mtk
