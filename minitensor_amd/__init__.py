@@ -232,6 +232,18 @@ def workspace(nbytes: int, device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
+def _require_ws(ws: Optional[torch.Tensor]) -> None:
+    """A caller's workspace is memory that the GPU reaches, there to its last element (an
+    expanded view's is not)."""
+    if ws is None:
+        return
+    if not isinstance(ws, torch.Tensor) or not (
+            ws.is_cuda or ws.numel() == 0 or (ws.device.type == "cpu" and ws.is_pinned())):
+        raise ValueError("a workspace must be a GPU tensor")
+    if ws.untyped_storage().nbytes() < (ws.storage_offset() + ws.numel()) * ws.element_size():
+        raise ValueError("a workspace must not be an expanded view")
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -245,6 +257,7 @@ def gemm(A: torch.Tensor, B: torch.Tensor, out: Optional[torch.Tensor] = None,
     if r is not None:
         return r
     _require_gpu(A, B, out, bias)
+    _require_ws(ws)
     if A.dim() != B.dim() or A.dim() not in (2, 3):
         raise ValueError("gemm: A and B must both be 2-D or both 3-D")
     if A.shape[-1] != B.shape[-2]:
@@ -303,6 +316,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = None,
     if r is not None:
         return r
     _require_gpu(x, w, b, out)
+    _require_ws(ws)
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise ValueError("linear: expected x [B,in] and w [out,in]")
     if b is not None and (b.dim() != 1 or b.shape[0] != w.shape[0]):
@@ -328,6 +342,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, need_dx:
     if r is not None:
         return r
     _require_gpu(dy, x, w, dx, dw, db)
+    _require_ws(ws)
     Bn, in_f, out_f = x.shape[0], x.shape[1], w.shape[0]
     dev = x.device
     if need_dx and dx is None:
@@ -377,6 +392,7 @@ def conv2d(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = None, s
     if r is not None:
         return r
     _require_gpu(x, w, b)
+    _require_ws(ws)
     if x.dim() != 4 or w.dim() != 4 or x.shape[1] != w.shape[1]:
         raise ValueError("conv2d: expected input [N,C,H,W] and weight [Cout,C,kh,kw]")
     if b is not None and (b.dim() != 1 or b.shape[0] != w.shape[0]):
@@ -412,6 +428,7 @@ def conv2d_backward(x: torch.Tensor, w: torch.Tensor, dy: torch.Tensor, stride: 
     if r is not None:
         return r
     _require_gpu(x, w, dy)
+    _require_ws(ws)
     x, w, dy = x.contiguous(), w.contiguous(), dy.contiguous()
     n, c, h, wd = x.shape
     co, _, kh, kw = w.shape

@@ -74,10 +74,17 @@ struct Workspace {
     }
 };
 
-// The caller's workspace (nothing for None); `ok` is cleared for no tensor.
+// The caller's workspace (nothing for None); `ok` is cleared for anything but memory that the
+// GPU reaches (its own, or pinned) and that is there to its last element (not an expanded view).
 at::Tensor given_ws(py::handle h, bool* ok) {
     if (h.is_none()) return {};
-    if (THPVariable_Check(h.ptr())) return THPVariable_Unpack(h.ptr());
+    if (THPVariable_Check(h.ptr())) {
+        at::Tensor t = THPVariable_Unpack(h.ptr());
+        if (t.defined() && t.has_storage() &&
+            (t.is_cuda() || t.numel() == 0 || (t.is_cpu() && t.is_pinned())) &&
+            t.storage().nbytes() >= (size_t)(t.storage_offset() + t.numel()) * t.element_size())
+            return t;
+    }
     *ok = false;
     return {};
 }

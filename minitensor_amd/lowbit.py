@@ -20,7 +20,8 @@ from typing import NamedTuple, Optional, Union
 
 import torch
 
-from . import MatF32, _api, _check, _handle, _ptr, _require_gpu, _stream, lib, mat, native, workspace
+from . import (MatF32, _api, _check, _handle, _ptr, _require_gpu, _require_ws, _stream, lib, mat,
+               native, workspace)
 
 
 class Q8Rows(NamedTuple):
@@ -139,6 +140,7 @@ def _empty(shape, like, dtype=torch.float32):
 
 
 def _ws(ws, need, like):
+    _require_ws(ws)
     return ws if ws is not None else workspace(need, like.device)
 
 
