@@ -244,6 +244,10 @@ def _require_ws(ws: Optional[torch.Tensor]) -> None:
         raise ValueError("a workspace must not be an expanded view")
 
 
+def _nbytes(ws: Optional[torch.Tensor]) -> int:
+    return 0 if ws is None else ws.numel() * ws.element_size()
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -282,7 +286,7 @@ def gemm(A: torch.Tensor, B: torch.Tensor, out: Optional[torch.Tensor] = None,
     if ws is None:
         ws = workspace(lib().mt_gemm_workspace_f32(ma, mb, mc), A.device)
     rc = lib().mt_gemm_f32(ma, mb, mc, ctypes.byref(ep) if ep is not None else None,
-                           _ptr(ws), ws.numel() if ws is not None else 0, _stream(stream))
+                           _ptr(ws), _nbytes(ws), _stream(stream))
     _check(rc, "mt_gemm_f32")
     return out
 
@@ -326,8 +330,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = None,
     if ws is None:
         ws = workspace(lib().mt_linear_workspace_f32(x.shape[0], x.shape[1], w.shape[0]), x.device)
     rc = lib().mt_linear_forward_f32(mat(x), mat(w), _ptr(b), b.stride(0) if b is not None else 0,
-                                     mat(out), _ptr(ws), ws.numel() if ws is not None else 0,
-                                     _stream(stream))
+                                     mat(out), _ptr(ws), _nbytes(ws), _stream(stream))
     _check(rc, "mt_linear_forward_f32")
     return out
 
@@ -358,7 +361,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, need_dx:
         ctypes.byref(mat(dx)) if need_dx else None,
         ctypes.byref(mat(dw)) if need_dw else None, float(beta_w),
         _ptr(db) if need_db else None, db.stride(0) if need_db else 0, float(beta_b),
-        _ptr(ws), ws.numel() if ws is not None else 0, _stream(stream))
+        _ptr(ws), _nbytes(ws), _stream(stream))
     _check(rc, "mt_linear_backward_f32")
     return dx, dw, db
 
@@ -409,7 +412,7 @@ def conv2d(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = None, s
     strides = (ctypes.c_int64 * 4)(*x.stride())
     rc = lib().mt_conv2d_fwd_strided_f32(ctypes.byref(d), x.data_ptr(), strides, w.data_ptr(),
                                          _ptr(b), out.data_ptr(), _ptr(ws),
-                                         ws.numel() if ws is not None else 0, _stream(stream))
+                                         _nbytes(ws), _stream(stream))
     _check(rc, "mt_conv2d_fwd_strided_f32")
     return out
 
@@ -438,7 +441,7 @@ def conv2d_backward(x: torch.Tensor, w: torch.Tensor, dy: torch.Tensor, stride: 
         raise ValueError("conv2d_backward: grad_output has the wrong shape")
     if ws is None:
         ws = workspace(lib().mt_conv2d_bwd_workspace_f32(ctypes.byref(d)), x.device)
-    wp, wn = _ptr(ws), (ws.numel() if ws is not None else 0)
+    wp, wn = _ptr(ws), _nbytes(ws)
     dx = db = None
     if not need_dw:
         dw = None

@@ -66,7 +66,7 @@ struct Workspace {
     Workspace(const at::Tensor& given, const at::Tensor& like, Need need) {
         if (given.defined()) {
             own = given;
-            n = (size_t)own.numel();
+            n = own.nbytes();
         } else if ((n = need()) > 0) {
             own = at::empty({(int64_t)n}, at::TensorOptions().dtype(at::kByte).device(like.device()));
         }

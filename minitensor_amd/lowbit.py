@@ -20,8 +20,8 @@ from typing import NamedTuple, Optional, Union
 
 import torch
 
-from . import (MatF32, _api, _check, _handle, _ptr, _require_gpu, _require_ws, _stream, lib, mat,
-               native, workspace)
+from . import (MatF32, _api, _check, _handle, _nbytes, _ptr, _require_gpu, _require_ws, _stream, lib,
+               mat, native, workspace)
 
 
 class Q8Rows(NamedTuple):
@@ -144,10 +144,6 @@ def _ws(ws, need, like):
     return ws if ws is not None else workspace(need, like.device)
 
 
-def _size(ws):
-    return ws.numel() * ws.element_size() if ws is not None else 0
-
-
 @_api
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
              residual: Optional[torch.Tensor] = None, eps: float = 1e-6, y: bool = True,
@@ -213,7 +209,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: Optional[torch.
     rc = lib().mt_rms_norm_backward_f32(
         mat(dy), mat(h), w, wst, rp, _matrix(dh, dy.shape, "rms_norm_backward: dh"),
         _matrix(out if need_dh else None, dy.shape, "rms_norm_backward: out"), dwp, dws, float(beta),
-        _ptr(ws), _size(ws), _stream(stream))
+        _ptr(ws), _nbytes(ws), _stream(stream))
     _check(rc, "mt_rms_norm_backward_f32")
     return out if need_dh else None, dw if need_dw else None
 
@@ -285,7 +281,7 @@ def linear_backward_q8(dy: torch.Tensor, xq: Q8Rows, w: Optional[torch.Tensor] =
         mat(dy), ctypes.byref(x), wm,
         _matrix(dx if w is not None else None, (n, fin), "linear_backward_q8: dx"),
         _matrix(dw if need_dw else None, (fout, fin), "linear_backward_q8: dw"), float(beta_w), dbp,
-        dbs, float(beta_b), _ptr(ws), _size(ws), _stream(stream))
+        dbs, float(beta_b), _ptr(ws), _nbytes(ws), _stream(stream))
     _check(rc, "mt_linear_backward_q8_f32")
     return dx if w is not None else None, dw if need_dw else None, db if need_db else None
 
@@ -343,6 +339,6 @@ def linear_q4(x: Union[torch.Tensor, Q8Rows], wq: Q4Weight, b: Optional[torch.Te
     y = _matrix(out, (rows, d.n), "linear_q4: out")
     ws = _ws(ws, lib().mt_linear_q4_workspace(rows, d.k, d.n), wq.packed)
     fn = lib().mt_linear_q4_q8 if q8 else lib().mt_linear_q4_f32
-    rc = fn(ctypes.byref(xd), ctypes.byref(d), bp, bs, y, _ptr(ws), _size(ws), _stream(stream))
+    rc = fn(ctypes.byref(xd), ctypes.byref(d), bp, bs, y, _ptr(ws), _nbytes(ws), _stream(stream))
     _check(rc, "mt_linear_q4_q8" if q8 else "mt_linear_q4_f32")
     return out

@@ -51,3 +51,17 @@ def test_a_slice_of_gpu_memory_is_taken(dev):
     x = torch.randn(200, 4096, device=dev)
     wq = mt.quantize_q4(torch.randn(64, 4096, device=dev))
     assert torch.equal(mt.linear_q4(x, wq, ws=big[64:]), mt.linear_q4(x, wq))
+
+
+@pytest.mark.gpu
+def test_a_workspace_of_floats_counts_in_bytes(dev):
+    x, dy = torch.randn(4096, 64, device=dev), torch.randn(4096, 64, device=dev)
+    xq = mt.quantize_q8(x)
+    need = mt.lib().mt_linear_backward_q8_workspace_f32(4096, 64, 64)
+    assert need > 0
+    ws = torch.empty((need + 3) // 4, device=dev)
+    assert torch.equal(mt.linear_backward_q8(dy, xq, ws=ws)[1], mt.linear_backward_q8(dy, xq)[1])
+    a, b = torch.randn(64, 65536, device=dev), torch.randn(65536, 64, device=dev)
+    need = mt.lib().mt_gemm_workspace_f32(mt.mat(a), mt.mat(b), mt.mat(torch.empty(64, 64, device=dev)))
+    assert need > 0
+    assert torch.equal(mt.gemm(a, b, ws=torch.empty((need + 3) // 4, device=dev)), mt.gemm(a, b))
