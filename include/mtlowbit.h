@@ -26,7 +26,8 @@ extern "C" {
  *   scale = max(a * (1/127), 2^-126),   q = x * (1/scale) to the nearest (ties
  *   to even), so |q| <= 127 and |x - q*scale| <= (0.5 + 2^-16) * scale.
  * A row that holds an infinity or a NaN has the scale inf or NaN and zero codes
- * wherever x*(1/scale) is none: it reads back as NaN throughout.
+ * wherever x*(1/scale) is none: it reads back as NaN throughout.  A row of no
+ * columns has a = 0.
  * Readers take any finite scale and any q, -128 among them. */
 typedef struct mt_rows_q8 {
     int8_t* q;
@@ -56,7 +57,8 @@ typedef struct mt_weight_q4 {
  * R, weight, H, Y, Q, rstd may each be NULL: no addition, a weight of ones, an
  * output that is not wanted.  H may be the same view as X or as R (the residual
  * stream updated in place).  Sums of squares past the fp32 range (|h| near
- * 1e19 and more) are infinite: such a row's y is zero. */
+ * 1e19 and more) are infinite: such a row's y is zero.  A row of no columns has
+ * the mean square 0: rstd = 1/sqrt(eps). */
 int mt_rms_norm_f32(const mt_mat_f32* X, const mt_mat_f32* R, const float* weight,
                     int64_t weight_stride, float eps, const mt_mat_f32* H, const mt_mat_f32* Y,
                     const mt_rows_q8* Q, float* rstd, void* stream);

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 #include "lowbit_back_kernel.hpp"
@@ -69,6 +70,14 @@ bool row_resident(int64_t cols) { return cols <= 16384; }
 // (workgroups beyond these take a second row: a grid's threads are a 32-bit number)
 unsigned row_blocks(int64_t rows, int nt) {
     return (unsigned)std::min<int64_t>(nt == 64 ? (rows + 3) / 4 : rows, 1 << 20);
+}
+
+// The scales and rstd of rows without columns (nullptr: not wanted).
+int empty_rows(int64_t rows, const mt_rows_q8* Q, float* rstd, float eps, void* stream) {
+    int rc = MT_OK;
+    if (Q) rc = mt_fill_f32(Q->scale, rows, kScaleMin, stream);
+    if (rc == MT_OK && rstd) rc = mt_fill_f32(rstd, rows, 1.f / std::sqrt(eps), stream);
+    return rc;
 }
 
 // Calls go(NT, MODE, RES) as constants: see lowbit_rows_kernel.hpp.
@@ -276,7 +285,8 @@ int mt_rms_norm_f32(const mt_mat_f32* X, const mt_mat_f32* R, const float* weigh
         (Q && (!valid(Q) || Q->rows != X->rows || Q->cols != X->cols)) || weight_stride < 0 ||
         !(eps >= 0.f))
         return MT_ERR_INVALID;
-    if (X->rows == 0 || X->cols == 0) return MT_OK;
+    if (X->rows == 0) return MT_OK;
+    if (X->cols == 0) return empty_rows(X->rows, Q, rstd, eps, stream);
     RowParams p{};
     p.x = view(X);
     p.r = view(R);
@@ -350,7 +360,8 @@ int mt_rms_norm_backward_f32(const mt_mat_f32* dY, const mt_mat_f32* H, const fl
 int mt_quantize_q8_f32(const mt_mat_f32* X, const mt_rows_q8* Q, void* stream) {
     if (!valid(X, false) || !valid(Q) || Q->rows != X->rows || Q->cols != X->cols)
         return MT_ERR_INVALID;
-    if (X->rows == 0 || X->cols == 0) return MT_OK;
+    if (X->rows == 0) return MT_OK;
+    if (X->cols == 0) return empty_rows(X->rows, Q, nullptr, 0.f, stream);
     RowParams p{};
     p.x = view(X);
     p.q = Q->q;
