@@ -83,7 +83,9 @@ int mt_dequantize_q8_f32(const mt_rows_q8* Q, const mt_mat_f32* Y, void* stream)
 /* A Linear layer's gradients from an input that was kept in 8 bits (the layout
  * of mt_linear_backward_f32): dX = dY·W, dW = dYᵀ·(scale*q) (+ beta_w·dW_old),
  * db = sum of dY's rows (+ beta_b·db_old).  Any of dX, dW, db may be NULL, and
- * W where dX is. */
+ * W where dX is.  dW takes dY·scale first, rounded to fp32 and infinite past its
+ * range; below 2^-102 what that has past its first 16 bits may be dropped where it
+ * is below 2^-126. */
 int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const mt_mat_f32* W,
                               const mt_mat_f32* dX, const mt_mat_f32* dW, float beta_w, float* db,
                               int64_t db_stride, float beta_b, void* workspace, size_t ws_bytes,
@@ -100,9 +102,9 @@ int mt_quantize_q4_f32(const mt_mat_f32* W, const mt_weight_q4* Q, void* stream)
 int mt_dequantize_q4_f32(const mt_weight_q4* Q, const mt_mat_f32* W, void* stream);
 
 /* Y = X·Wᵀ + bias (bias NULL: none), X in fp32 or in 8 bits.  k == 0 writes the bias
- * or zeros.  An fp32 input above 3.38e38 in magnitude counts as infinite; what an
- * input below 2^-102 has past its first 16 bits may be dropped where that is
- * below 2^-126. */
+ * or zeros.  What an fp32 input below 2^-102 has past its first 16 bits may be dropped
+ * where that is below 2^-126; a NaN whose set bits are all in its lower half (a
+ * signalling one) counts as an infinity. */
 int mt_linear_q4_f32(const mt_mat_f32* X, const mt_weight_q4* W, const float* bias,
                      int64_t bias_stride, const mt_mat_f32* Y, void* workspace, size_t ws_bytes,
                      void* stream);

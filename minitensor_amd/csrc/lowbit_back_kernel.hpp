@@ -202,7 +202,7 @@ struct BackQ {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(w[e] >> (8 * b));
                 *reinterpret_cast<u32x2*>(d + b * kRun * 16) =
-                    u32x2{bf16_exact(f[0], f[1]), bf16_exact(f[2], f[3])};
+                    u32x2{bf16_cut(f[0], f[1]), bf16_cut(f[2], f[3])};
             }
         }
     }

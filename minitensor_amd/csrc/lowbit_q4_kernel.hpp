@@ -43,7 +43,7 @@ __device__ __forceinline__ u32x4 q4_unpack(uint32_t w) {
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        r[i] = bf16_exact(__builtin_amdgcn_cvt_off_f32_i4((w >> (8 * i)) & 0xff),
+        r[i] = bf16_cut(__builtin_amdgcn_cvt_off_f32_i4((w >> (8 * i)) & 0xff),
                           __builtin_amdgcn_cvt_off_f32_i4((odd >> (8 * i)) & 0xff));
     return r;
 }

@@ -50,3 +50,30 @@ def test_rows_of_no_columns(dev, r):
         n = mt.rms_norm(x, torch.empty(0, device=dev), residual=x, eps=0.25, q8=q8)
         assert bool((n.rstd == 2.0).all()) and n.y.shape == n.h.shape == (r, 0)
         assert not q8 or bool((n.q8.scale == 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize("m,n,k,group", [(2, 40, 300, 64), (16, 33, 260, 128), (80, 70, 300, 32),
+                                         (130, 140, 257, 128)])
+def test_linear_q4_of_the_largest_inputs(dev, m, n, k, group):
+    """One input per row past the largest bf16 value, some of its codes zero: finite
+    products of finite values."""
+    g = rng(1, m, n, k, group)
+    code = g.integers(-8, 8, (n, k)).astype(np.int8)
+    scale = (1e-3 * (g.random((n, -(-k // group))) + 0.5)).astype(np.float32)
+    x = g.standard_normal((m, k)).astype(np.float32)
+    for i in range(m):
+        x[i, (7 * i + 3) % k] = (FLT_MAX, -FLT_MAX, 3.397e38, -3.4e38, 3.39e38)[i % 5]
+    code[:, 3], code[0, 3] = 7, 0
+    wq = mt.Q4Weight(gpu(ref.pack_q4(code), dev), gpu(scale, dev), k, group)
+    near(mt.linear_q4(gpu(x, dev), wq), x.astype(np.float64), ref.weight_q4(code, scale, group), group, 3)
+
+
+@pytest.mark.parametrize("r,fin,fout", [(50, 64, 40), (300, 130, 70)])
+def test_linear_backward_q8_of_the_largest_gradients(dev, r, fin, fout):
+    g = rng(2, r)
+    q = g.integers(-1, 2, (r, fin)).astype(np.int8)
+    s = np.ones(r, np.float32)
+    dy = g.standard_normal((r, fout)).astype(np.float32)
+    dy[5, 3], dy[6, 4], dy[r - 1, 39], dy[7, 0] = FLT_MAX, -FLT_MAX, 3.397e38, 3.39e38
+    _, dw, _ = mt.linear_backward_q8(gpu(dy, dev), mt.Q8Rows(gpu(q, dev), gpu(s, dev)))
+    near(dw, dy.T.astype(np.float64), q.T.astype(np.float64), 128, 3)
