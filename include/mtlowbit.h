@@ -104,7 +104,9 @@ int mt_dequantize_q4_f32(const mt_weight_q4* Q, const mt_mat_f32* W, void* strea
 /* Y = X·Wᵀ + bias (bias NULL: none), X in fp32 or in 8 bits.  k == 0 writes the bias
  * or zeros.  What an fp32 input below 2^-102 has past its first 16 bits may be dropped
  * where that is below 2^-126; a NaN whose set bits are all in its lower half (a
- * signalling one) counts as an infinity. */
+ * signalling one) counts as an infinity.  Sums are held in fp32, those over 8-bit rows
+ * without the row's scale; below 2^-122 they, and with 8-bit rows a group's scale, may
+ * be rounded to multiples of 2^-145. */
 int mt_linear_q4_f32(const mt_mat_f32* X, const mt_weight_q4* W, const float* bias,
                      int64_t bias_stride, const mt_mat_f32* Y, void* workspace, size_t ws_bytes,
                      void* stream);

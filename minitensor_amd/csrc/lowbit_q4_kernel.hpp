@@ -37,7 +37,8 @@ struct Q4Params {
 };
 
 // The eight codes of a dword, over 16, as bf16 (exact): v_cvt_off_f32_i4 gives
-// a code over 16, whose low half as fp32 is zero.  13 instructions.
+// a code over 16, whose low half as fp32 is zero.  13 instructions.  The factor comes back at
+// a sum's end: times 16 a group's scale may leave fp32's range.
 __device__ __forceinline__ u32x4 q4_unpack(uint32_t w) {
     const uint32_t odd = w >> 4;
     u32x4 r;
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(64 * W, CAP <= 4 && G > 32 ? 8 : 2) q4_few(Q4P
                     for (int q = 0; q < NC; ++q)
 #pragma unroll
                         for (int mb = 0; mb < MB; ++mb)
-                            sum[q][mb] += acc[q][mb] * (s[q][i] * kQ4Unit);
+                            sum[q][mb] += acc[q][mb] * s[q][i];
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -285,6 +286,7 @@ __global__ void __launch_bounds__(64 * W, CAP <= 4 && G > 32 ? 8 : 2) q4_few(Q4P
         for (int w = 0; w < W; ++w)
 #pragma unroll
             for (int q = P - 1; q >= 0; --q) v += red[(w * 16 * MB + P * m + q) * C + c];
+        v *= kQ4Unit;
         if constexpr (Q8) v *= p.q_scale[m];
         if (p.bias) v += p.bias[(int64_t)(n0 + c) * p.bias_stride];
         p.y[(int64_t)m * p.y_m + (int64_t)(n0 + c) * p.y_n] = v;
@@ -502,7 +504,7 @@ q4_gemm(Q4Params p) {
         la, lb, smem, kb, ke, ra, rb, lane, acc, [&](auto i, int block) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const float s = sc.cur[j][i % NG] * kQ4Unit;
+            const float s = sc.cur[j][i % NG];
 #pragma unroll
             for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -528,7 +530,7 @@ q4_gemm(Q4Params p) {
             for (int r = 0; r < 16; ++r) {
                 const int m = m0 + ra + 32 * i + lb_row(lane, r);
                 if (m >= p.M) continue;
-                const float v = sum[i][j][r];
+                const float v = sum[i][j][r] * kQ4Unit;
                 if (part) p.part[((int64_t)split * p.M + m) * p.N + n] = v;
                 else p.y[(int64_t)m * p.y_m + (int64_t)n * p.y_n] = v + b;
             }

@@ -77,3 +77,31 @@ def test_linear_backward_q8_of_the_largest_gradients(dev, r, fin, fout):
     dy[5, 3], dy[6, 4], dy[r - 1, 39], dy[7, 0] = FLT_MAX, -FLT_MAX, 3.397e38, 3.39e38
     _, dw, _ = mt.linear_backward_q8(gpu(dy, dev), mt.Q8Rows(gpu(q, dev), gpu(s, dev)))
     near(dw, dy.T.astype(np.float64), q.T.astype(np.float64), 128, 3)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 3, 16, 80, 200])
+def test_linear_q4_of_the_largest_weights(dev, m, group):
+    """A group near 3e38 and its scale: finite products of finite values, and zero where
+    the group's codes are."""
+    g = rng(3, m, group)
+    n, k = 50, 200
+    w = g.standard_normal((n, k)).astype(np.float32)
+    w[3, :128] *= 1e38
+    w[3, 5], w[20, 131] = 3e38, -3.3e38
+    x = (1e-4 * g.standard_normal((m, k))).astype(np.float32)
+    wq = mt.quantize_q4(gpu(w, dev), group)
+    wd = cpu(mt.dequantize_q4(wq)).astype(np.float64)
+    assert np.isfinite(wd).all()
+    near(mt.linear_q4(gpu(x, dev), wq), x.astype(np.float64), wd, group, 3)
+    # any finite scale; rows in 8 bits too, one input of each sign in a group
+    code = np.zeros((n, k), np.int8)
+    code[:, 5], code[:, 150] = 1, -1
+    scale = np.full((n, -(-k // group)), 1.5e38, np.float32)
+    code[7] = 0
+    wq = mt.Q4Weight(gpu(ref.pack_q4(code), dev), gpu(scale, dev), k, group)
+    wd = ref.weight_q4(code, scale, group)
+    near(mt.linear_q4(gpu(x, dev), wq), x.astype(np.float64), wd, group, 3)
+    q = g.integers(-1, 2, (m, k)).astype(np.int8)
+    y = mt.linear_q4(mt.Q8Rows(gpu(q, dev), torch.full((m,), 0.5, device=dev)), wq)
+    near(y, 0.5 * q, wd, group, 1)
