@@ -115,6 +115,10 @@ int64_t row_groups(int64_t rows, int64_t cols) {
     return (std::min(rows, most) + 3) / 4 * 4;
 }
 
+// Workgroups of the parts' sum, 16 columns each at a time (a grid's threads are a 32-bit
+// number: 64 a column, one column in each, were 2^32 of them from 2^26 columns on).
+unsigned dweight_blocks(int64_t cols) { return (unsigned)std::min<int64_t>((cols + 15) / 16, 1 << 20); }
+
 // Tiles and splits of a product over chunks of 32 k, from measured times in us: of a chunk,
 // by workgroups on a CU, where each holds as many as its LDS and registers allow, and of a
 // round's beginning and end.  The tile and the number of splits that come out fastest,
@@ -351,9 +355,8 @@ int mt_rms_norm_backward_f32(const mt_mat_f32* dY, const mt_mat_f32* H, const fl
         });
     }
     if (dweight)
-        hipLaunchKernelGGL(rms_dweight_sum, dim3((unsigned)((p.cols + 15) / 16)), dim3(1024), 0, s,
-                           p.part, p.rows > 0 ? (int)groups : 0, p.cols, dweight, dweight_stride,
-                           beta);
+        hipLaunchKernelGGL(rms_dweight_sum, dim3(dweight_blocks(p.cols)), dim3(1024), 0, s, p.part,
+                           p.rows > 0 ? (int)groups : 0, p.cols, dweight, dweight_stride, beta);
     return launched();
 }
 

@@ -366,27 +366,30 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) rms_backward(RowBwdParams
 }
 
 // out[c] = beta*out[c] + sum over n parts, in order within each of 64 slices and then over
-// the slices: 16 columns per workgroup of 1024 threads.  (64 columns and 16 slices left
-// most CUs without work: 5.4 us for 1024 parts of 2048.)
+// the slices: 16 columns per workgroup of 1024 threads at a time.  (64 columns and 16 slices
+// left most CUs without work: 5.4 us for 1024 parts of 2048.)
 __global__ void __launch_bounds__(1024)
 rms_dweight_sum(const float* part, int n, int cols, float* out, int64_t os, float beta) {
     __shared__ float red[64][17];
     const int l = threadIdx.x & 15, q = threadIdx.x >> 4;
-    const int c = blockIdx.x * 16 + l;
-    float s = 0.f;
-    if (c < cols) {
+    for (int64_t c0 = (int64_t)blockIdx.x * 16; c0 < cols; c0 += (int64_t)gridDim.x * 16) {
+        const int64_t c = c0 + l;
+        float s = 0.f;
+        if (c < cols) {
 #pragma unroll 8
-        for (int i = q; i < n; i += 64) s += part[(int64_t)i * cols + c];
+            for (int i = q; i < n; i += 64) s += part[(int64_t)i * cols + c];
+        }
+        __syncthreads();                               // the readers of the columns before are done
+        red[q][l] = s;
+        __syncthreads();
+        if (q >= 4 || c >= cols) continue;             // (one wave)
+        for (int i = q + 4; i < 64; i += 4) s += red[i][l];
+        s += __shfl_xor(s, 16);
+        s += __shfl_xor(s, 32);
+        if (q != 0) continue;
+        float* const d = out + c * os;
+        *d = beta != 0.f ? beta * *d + s : s;
     }
-    red[q][l] = s;
-    __syncthreads();
-    if (q >= 4 || c >= cols) return;                   // (one wave)
-    for (int i = q + 4; i < 64; i += 4) s += red[i][l];
-    s += __shfl_xor(s, 16);
-    s += __shfl_xor(s, 32);
-    if (q != 0) return;
-    float* const d = out + (int64_t)c * os;
-    *d = beta != 0.f ? beta * *d + s : s;
 }
 
 // y = q·scale.  UNIT: a wave takes 1024 elements of a row, four dwords of codes per lane,

@@ -105,3 +105,22 @@ def test_linear_q4_of_the_largest_weights(dev, m, group):
     q = g.integers(-1, 2, (m, k)).astype(np.int8)
     y = mt.linear_q4(mt.Q8Rows(gpu(q, dev), torch.full((m,), 0.5, device=dev)), wq)
     near(y, 0.5 * q, wd, group, 1)
+
+
+@pytest.mark.parametrize("c", [(1 << 24) + 5, (1 << 26) + 37])
+def test_rms_norm_backward_of_very_wide_rows(dev, c):
+    """The weight gradient's sum takes its columns in several rounds from 2^24 of them on (a
+    grid's threads are a 32-bit number)."""
+    g = torch.Generator(device=dev).manual_seed(c)
+    dy, h = (torch.randn(2, c, device=dev, generator=g) for _ in range(2))
+    rstd = torch.tensor([0.5, 2.0], device=dev)
+    dw0 = torch.randn(c, device=dev, generator=g)
+    dw = dw0.clone()
+    mt.rms_norm_backward(dy, h, None, rstd, need_dh=False, dw=dw, beta=0.5)
+    # a product, its row's 1/rms, the two rows' sum, the old gradient's share
+    for a in range(0, c, 1 << 24):
+        s = slice(a, a + (1 << 24))
+        terms = dy[:, s].double() * h[:, s].double() * rstd.double()[:, None]
+        want = terms.sum(0) + 0.5 * dw0[s].double()
+        size = terms.abs().sum(0) + 0.5 * dw0[s].double().abs()
+        assert bool(((dw[s].double() - want).abs() <= 6 * ref.EPS32 * size).all())
