@@ -124,3 +124,18 @@ def test_rms_norm_backward_of_very_wide_rows(dev, c):
         want = terms.sum(0) + 0.5 * dw0[s].double()
         size = terms.abs().sum(0) + 0.5 * dw0[s].double().abs()
         assert bool(((dw[s].double() - want).abs() <= 6 * ref.EPS32 * size).all())
+
+
+@pytest.mark.parametrize("r,fin,fout", [(20000, 4096, 2048), (20000, 70, 100)])
+def test_linear_backward_q8_bias_gradient_of_many_rows(dev, r, fin, fout):
+    """Rows of one sign and one value an output, whose additions all round the same way: a sum of
+    eight rows (3 roundings), a compensated one over those (2, and 1 at its end), four groups
+    (2), the splits (at most 32 of them) and what the compensation itself rounds (1)."""
+    a = torch.linspace(1, 2, fout, device=dev)
+    dy = a.expand(r, fout).contiguous()
+    xq = mt.Q8Rows(torch.zeros(r, fin, dtype=torch.int8, device=dev), torch.ones(r, device=dev))
+    _, dw, db = mt.linear_backward_q8(dy, xq)
+    assert bool((dw == 0).all())
+    want = r * a.double()
+    split = mt.lib().mt_linear_backward_q8_workspace_f32(r, fin, fout) > 0 and fin < 4096
+    assert bool(((db.double() - want).abs() <= (9 + 32 * split) * ref.EPS32 * want).all())
