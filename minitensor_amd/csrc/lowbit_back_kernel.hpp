@@ -113,7 +113,7 @@ struct BackDy {
 #pragma unroll
             for (int e = 0; e < 8; ++e) a[e] = x.a[i][e] * x.s[i][e];
             u32x4 h, m, l;
-            cut8(a, h, m, l);
+            cut8<(BM > 64)>(a, h, m, l);
             char* const d = buf + g[i] * kGroup + (i * NT + t) % BM * 16;
             *reinterpret_cast<u32x4*>(d) = h;
             *reinterpret_cast<u32x4*>(d + kBytes) = m;

@@ -52,20 +52,43 @@ __device__ __forceinline__ uint32_t bf16_cut(float a, float b) {
 
 // The parts of eight values, h + m + l = x (6.5 instructions each): eight of its 24 bits each,
 // cut off and not rounded; with h rounded the values above bf16's largest, 3.39e38, would
-// become infinite.  (8192 rows, 4096 -> 4096, the weight gradient: 683 us against 679
-// rounded.)  What is left of an infinity or a NaN (a NaN) is made zero, so that its products
-// are those of fp32: the middle of (r, r, 0) is r, and 0 where r is a NaN.  (A NaN whose set
-// bits are all in the lower half, a signalling one, would count as an infinity; no operation
-// gives such a one.)
+// become infinite.  What is left of an infinity or a NaN (a NaN) is made zero, so that its
+// products are those of fp32: the middle of (r, r, 0) is r, and 0 where r is a NaN.  (A NaN
+// whose set bits are all in the lower half, a signalling one, would count as an infinity; no
+// operation gives such a one.)
+// WIDE: the cut values are kept for the subtractions and converted, rather than packed by
+// v_perm and taken apart again: as many instructions and two registers more (the weight
+// gradient's 128x256 tile, 8192 rows, 4096 -> 4096: 672 us against 683; its 64x128 tile, 256
+// rows, 2048 -> 1000 with dX: 41.1 against 40.6).
+template <bool WIDE>
 __device__ __forceinline__ void cut8(const float (&x)[8], u32x4& h, u32x4& m, u32x4& l) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        h[i] = opaque(bf16_cut(x[2 * i], x[2 * i + 1]));
-        float r0 = x[2 * i] - bf16_lo(h[i]), r1 = x[2 * i + 1] - bf16_hi(h[i]);
+        const float x0 = x[2 * i], x1 = x[2 * i + 1];
+        float h0, h1, m0, m1;
+        if constexpr (WIDE) {
+            h0 = bf16_hi(__float_as_uint(x0));
+            h1 = bf16_hi(__float_as_uint(x1));
+            h[i] = bf16_pair(h0, h1);
+        } else {
+            h[i] = opaque(bf16_cut(x0, x1));
+            h0 = bf16_lo(h[i]);
+            h1 = bf16_hi(h[i]);
+        }
+        float r0 = x0 - h0, r1 = x1 - h1;
         r0 = __builtin_amdgcn_fmed3f(r0, r0, 0.f);
         r1 = __builtin_amdgcn_fmed3f(r1, r1, 0.f);
-        m[i] = opaque(bf16_cut(r0, r1));
-        l[i] = bf16_cut(r0 - bf16_lo(m[i]), r1 - bf16_hi(m[i]));
+        if constexpr (WIDE) {
+            m0 = bf16_hi(__float_as_uint(r0));
+            m1 = bf16_hi(__float_as_uint(r1));
+            m[i] = bf16_pair(m0, m1);
+            l[i] = bf16_pair(r0 - m0, r1 - m1);
+        } else {
+            m[i] = opaque(bf16_cut(r0, r1));
+            m0 = bf16_lo(m[i]);
+            m1 = bf16_hi(m[i]);
+            l[i] = bf16_cut(r0 - m0, r1 - m1);
+        }
     }
 }
 

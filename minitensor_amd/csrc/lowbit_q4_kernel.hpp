@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(64 * W, CAP <= 4 && G > 32 ? 8 : 2) q4_few(Q4P
                     *reinterpret_cast<u32x4*>(d) = q8_bf16(x[i]);
                 } else {
                     u32x4 hi, mi, lo;
-                    cut8(x[i], hi, mi, lo);
+                    cut8<false>(x[i], hi, mi, lo);
                     *reinterpret_cast<u32x4*>(d) = hi;
                     *reinterpret_cast<u32x4*>(d + RS) = mi;
                     *reinterpret_cast<u32x4*>(d + 2 * RS) = lo;
@@ -342,7 +342,7 @@ struct Q4X {
         for (int i = 0; i < N; ++i) {
             char* const d = buf + (t & 3) * kGroup + ((i * NT + t) >> 2) * 16;
             u32x4 h, m, l;
-            cut8(r.a[i], h, m, l);
+            cut8<(BM > 64)>(r.a[i], h, m, l);
             *reinterpret_cast<u32x4*>(d) = h;
             *reinterpret_cast<u32x4*>(d + kBytes) = m;
             *reinterpret_cast<u32x4*>(d + 2 * kBytes) = l;
