@@ -438,7 +438,7 @@ py::object linear_backward_q8(py::handle pdy, py::handle pq, py::handle pscale, 
     const int64_t n = q.size(0), fin = q.size(1), fout = dy.size(1);
     const bool need_dx = w.defined();
     if (dy.size(0) != n || scale.size(0) != n || !shaped(w, fout, fin) || !shaped(dx, n, fin) ||
-        !shaped(dw, fout, fin) || !vec_of(db, fout) ||
+        !shaped(dw, fout, fin) || !vec_of(db, fout) || (dx.defined() && !need_dx) ||
         (need_dw && !dw.defined() && beta_w != 0.f) || (need_db && !db.defined() && beta_b != 0.f))
         return py::none();
     void* const s = stream_of(stream);

@@ -265,6 +265,8 @@ def linear_backward_q8(dy: torch.Tensor, xq: Q8Rows, w: Optional[torch.Tensor] =
         raise ValueError("linear_backward_q8: expected dy [B, out] and rows [B, in]")
     n, fin, fout = x.rows, x.cols, dy.shape[1]
     wm = _matrix(w, (fout, fin), "linear_backward_q8: w")
+    if w is None and dx is not None:
+        raise ValueError("linear_backward_q8: a dx to write to without the w that gives it")
     if w is not None and dx is None:
         dx = _empty((n, fin), dy)
     if need_dw and dw is None:

@@ -126,6 +126,15 @@ def test_rms_norm_backward_of_very_wide_rows(dev, c):
         assert bool(((dw[s].double() - want).abs() <= 6 * ref.EPS32 * size).all())
 
 
+def test_a_place_for_dx_needs_the_weight(dev):
+    """linear_backward_q8 gives dX from the weight alone: a dx to write to without one is
+    refused, not left as it was."""
+    dy, xq = torch.ones(4, 8, device=dev), mt.quantize_q8(torch.ones(4, 16, device=dev))
+    dx = torch.full((4, 16), 5.0, device=dev)
+    with pytest.raises(ValueError):
+        mt.linear_backward_q8(dy, xq, dx=dx)
+
+
 @pytest.mark.parametrize("r,fin,fout", [(20000, 4096, 2048), (20000, 70, 100)])
 def test_linear_backward_q8_bias_gradient_of_many_rows(dev, r, fin, fout):
     """Rows of one sign and one value an output, whose additions all round the same way: a sum of
