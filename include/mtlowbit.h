@@ -116,6 +116,19 @@ int mt_linear_q4_q8(const mt_rows_q8* X, const mt_weight_q4* W, const float* bia
 /* Workspace of either call for `rows` rows of X. */
 size_t mt_linear_q4_workspace(int64_t rows, int64_t in_features, int64_t out_features);
 
+/* ---- diagnostics ---------------------------------------------------------------
+ * Which kernel a product's call takes, by its sizes, for tests and benchmarks (as
+ * mt_last_config, but nothing runs): of the 4-bit product, and of dW. */
+typedef struct mt_lowbit_plan {
+    int32_t tile_rows;      /* 64 or 128, by twice as many columns; 0: the few-rows kernel */
+    int32_t splits;         /* of the summed axis, added up by a launch of their own */
+    int32_t column_blocks;  /* of 16 columns, a workgroup of the few-rows kernel; 0 with tiles */
+} mt_lowbit_plan;
+int mt_linear_q4_plan(int64_t rows, int64_t in_features, int64_t out_features, int group,
+                      int x_in_8_bits, mt_lowbit_plan* plan);
+int mt_linear_backward_q8_plan(int64_t batch_rows, int64_t in_features, int64_t out_features,
+                               mt_lowbit_plan* plan);
+
 #ifdef __cplusplus
 }
 #endif

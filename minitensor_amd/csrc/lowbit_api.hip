@@ -179,12 +179,16 @@ Q4Plan q4_plan(int64_t M, int64_t N, int64_t K, int group, bool q8) {
     return {false, plan_tiles(M, N, K, t, group == 32 ? 1 : 2)};
 }
 
+// Column blocks of a workgroup for few rows (of parts), where that leaves one for every CU
+// (four of them, and 48 rows, do not fit the registers).
+int few_columns(int rows, int64_t N) {
+    const int64_t cols = (N + 15) / 16;
+    return rows <= 6 ? 1 : cols >= 4 * kCus && rows <= 32 ? 4 : cols >= 2 * kCus ? 2 : 1;
+}
+
 template <bool Q8, int G>
 void launch_few(const Q4Params& p, hipStream_t s) {
-    const int rows = p.M * (Q8 ? 1 : 3), cols = (p.N + 15) / 16;
-    // column blocks per workgroup, where that leaves one for every CU
-    // (four of them, and 48 rows, do not fit the registers)
-    const int nc = rows <= 6 ? 1 : cols >= 4 * kCus && rows <= 32 ? 4 : cols >= 2 * kCus ? 2 : 1;
+    const int rows = p.M * (Q8 ? 1 : 3), cols = (p.N + 15) / 16, nc = few_columns(rows, p.N);
     const dim3 grid((unsigned)((cols + nc - 1) / nc)), block(512);
     auto go = [&](auto cap, auto u) {
         if constexpr (cap() <= 32)
@@ -504,6 +508,26 @@ size_t mt_linear_q4_workspace(int64_t rows, int64_t in_f, int64_t out_f) {
         for (const bool q8 : {false, true})
             n = std::max(n, q4_plan(rows, out_f, in_f, group, q8).tiled.partials);
     return n * 4;
+}
+
+int mt_linear_q4_plan(int64_t rows, int64_t in_f, int64_t out_f, int group, int x_in_8_bits,
+                      mt_lowbit_plan* plan) {
+    if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxDim ||
+        out_f >= kMaxOut || (group != 32 && group != 64 && group != 128) || !plan)
+        return MT_ERR_INVALID;
+    const Q4Plan p = q4_plan(rows, out_f, in_f, group, x_in_8_bits != 0);
+    if (p.few) *plan = {0, 1, few_columns((int)rows * (x_in_8_bits ? 1 : 3), out_f)};
+    else *plan = {p.tiled.bm, p.tiled.splits, 0};
+    return MT_OK;
+}
+
+int mt_linear_backward_q8_plan(int64_t rows, int64_t in_f, int64_t out_f, mt_lowbit_plan* plan) {
+    if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxDim ||
+        out_f >= kMaxDim || !plan)
+        return MT_ERR_INVALID;
+    const Tiled t = back_plan(rows, out_f, in_f);
+    *plan = {t.bm, t.splits, 0};
+    return MT_OK;
 }
 
 int mt_linear_q4_f32(const mt_mat_f32* X, const mt_weight_q4* W, const float* bias,

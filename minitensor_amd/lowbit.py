@@ -60,6 +60,11 @@ class WeightQ4(ctypes.Structure):
                 ("scale_stride", ctypes.c_int64), ("group", ctypes.c_int32)]
 
 
+class LowbitPlan(ctypes.Structure):
+    _fields_ = [("tile_rows", ctypes.c_int32), ("splits", ctypes.c_int32),
+                ("column_blocks", ctypes.c_int32)]
+
+
 _P, _V, _I64, _F = ctypes.POINTER, ctypes.c_void_p, ctypes.c_int64, ctypes.c_float
 _M, _Q, _W = _P(MatF32), _P(RowsQ8), _P(WeightQ4)
 SIGS = {
@@ -77,6 +82,8 @@ SIGS = {
     "mt_linear_q4_f32": (ctypes.c_int, [_M, _W, _V, _I64, _M, _V, ctypes.c_size_t, _V]),
     "mt_linear_q4_q8": (ctypes.c_int, [_Q, _W, _V, _I64, _M, _V, ctypes.c_size_t, _V]),
     "mt_linear_q4_workspace": (ctypes.c_size_t, [_I64] * 3),
+    "mt_linear_q4_plan": (ctypes.c_int, [_I64] * 3 + [ctypes.c_int] * 2 + [_P(LowbitPlan)]),
+    "mt_linear_backward_q8_plan": (ctypes.c_int, [_I64] * 3 + [_P(LowbitPlan)]),
 }
 
 
