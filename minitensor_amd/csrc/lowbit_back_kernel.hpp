@@ -4,7 +4,7 @@
 // The row's scale goes to dY (one fp32 rounding), and q is exact in bf16: three
 // bf16 products in fp32's precision (lowbit_gemm.hpp), where a product of two fp32
 // operands takes six.  The matrix unit bounds it, at the clock that its power
-// allows: 8192 rows, 4096 -> 4096, 677-721 us (a bf16 product of that size and
+// allows: 8192 rows, 4096 -> 4096, 661-718 us (a bf16 product of that size and
 // three parts at a library's rate: 650); dY is read down its columns, 8 rows of an
 // output per thread, and cut there, which costs four to five times what q does, so
 // the tiles are wider in inputs than in outputs.

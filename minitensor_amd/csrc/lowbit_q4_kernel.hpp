@@ -2,7 +2,7 @@
 // (include/mtlowbit.h): y[m][n] = bias[n] + sum_g s[n][g] sum_{k in g} x[m][k] c[n][k].
 //
 // A 4-bit code is exact in bf16, and an fp32 x is the sum of three bf16 values
-// h + m + l (gemm_split.hpp): the product is three bf16 products on the matrix
+// h + m + l (lowbit_gemm.hpp): the product is three bf16 products on the matrix
 // units, each exact, with fp32's precision (six for two fp32 operands); an
 // 8-bit x takes one product, whose sums within a group are whole numbers below
 // 2^24, exact too.  The sums of a group are taken on the matrix unit from zero
@@ -472,7 +472,7 @@ struct Q4Scales {
     }
 };
 
-// 2048 rows, 4096 -> 8192, groups of 128: 347 us, the matrix unit's power (three bf16
+// 2048 rows, 4096 -> 8192, groups of 128: 342 us, the matrix unit's power (three bf16
 // products at a library's rate: 325).  (Groups of 32: registers for two workgroups a CU.)
 template <int BM, int BN, int WM, int WN, int G>
 __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, BM > 64 || G == 32 ? 2 : 3)
@@ -547,7 +547,7 @@ q4_gemm(Q4Params p) {
 // the vector unit, which turns each sum into fp32 and adds it, in groups of 32 three
 // instructions of four (1536 rows, 4096 -> 4096: 91% of its cycles), so four workgroups of
 // the narrow tile share a CU.  2048 rows, 4096 -> 8192, groups of 128, 64 and
-// 32: 121, 157 and 200 us (on the bf16 units, x and codes converted: 211, 219 and, of 32,
+// 32: 124, 158 and 201 us, where the unit's rate would take 54 (on the bf16 units, x and codes converted: 211, 219 and, of 32,
 // 1027 rows, 2047 -> 4096, 64 where this takes 48).  Sums added beside the next group's
 // MFMAs, from accumulators of their own, took as long.
 typedef int i32x16 __attribute__((ext_vector_type(16)));
@@ -729,7 +729,8 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, BM > 64 ? 2 : 4) q4_
 }
 
 // Codes and scales of a weight: a thread takes eight inputs (a dword of codes),
-// G/8 neighbouring threads a group.
+// G/8 neighbouring threads a group.  4096 x 16384: 119 us for 302 MB (a copy's rate: 58),
+// bound by its single loads, 32 bytes apart between lanes.
 template <int G>
 __global__ void __launch_bounds__(256)
 quantize_q4(const float* w, int64_t w_n, int64_t w_k, uint8_t* out, int64_t o_n, float* s,
@@ -763,6 +764,8 @@ quantize_q4(const float* w, int64_t w_n, int64_t w_k, uint8_t* out, int64_t o_n,
     }
 }
 
+// w = code·scale, a thread a dword of codes.  4096 x 16384: 166 us for 302 MB, bound by its
+// single stores, 32 bytes apart between lanes.
 __global__ void __launch_bounds__(256)
 dequantize_q4(const uint8_t* w, int64_t w_n, const float* s, int64_t s_n, int group, float* y,
               int64_t y_n, int64_t y_k, int N, int K) {
