@@ -83,9 +83,8 @@ int mt_dequantize_q8_f32(const mt_rows_q8* Q, const mt_mat_f32* Y, void* stream)
 /* A Linear layer's gradients from an input that was kept in 8 bits (the layout
  * of mt_linear_backward_f32): dX = dY·W, dW = dYᵀ·(scale*q) (+ beta_w·dW_old),
  * db = sum of dY's rows (+ beta_b·db_old).  Any of dX, dW, db may be NULL, and
- * W where dX is.  dW takes dY·scale first, rounded to fp32 and infinite past its
- * range; below 2^-102 what that has past its first 16 bits may be dropped where it
- * is below 2^-126. */
+ * W where dX is.  dW takes dY·scale first, rounded to fp32 (infinite past its
+ * range) and to a multiple of 2^-133. */
 int mt_linear_backward_q8_f32(const mt_mat_f32* dY, const mt_rows_q8* X, const mt_mat_f32* W,
                               const mt_mat_f32* dX, const mt_mat_f32* dW, float beta_w, float* db,
                               int64_t db_stride, float beta_b, void* workspace, size_t ws_bytes,
@@ -102,8 +101,8 @@ int mt_quantize_q4_f32(const mt_mat_f32* W, const mt_weight_q4* Q, void* stream)
 int mt_dequantize_q4_f32(const mt_weight_q4* Q, const mt_mat_f32* W, void* stream);
 
 /* Y = X·Wᵀ + bias (bias NULL: none), X in fp32 or in 8 bits.  k == 0 writes the bias
- * or zeros.  What an fp32 input below 2^-102 has past its first 16 bits may be dropped
- * where that is below 2^-126; a NaN whose set bits are all in its lower half (a
+ * or zeros.  An fp32 input is taken to the nearest multiple of 2^-133 (which one below
+ * 2^-110 need not be); a NaN whose set bits are all in its lower half (a
  * signalling one) counts as an infinity.  Sums are held in fp32, those over 8-bit rows
  * without the row's scale; below 2^-122 they, and with 8-bit rows a group's scale, may
  * be rounded to multiples of 2^-145. */

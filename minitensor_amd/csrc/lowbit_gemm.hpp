@@ -52,7 +52,8 @@ __device__ __forceinline__ uint32_t bf16_cut(float a, float b) {
 
 // The parts of eight values, h + m + l = x (6.5 instructions each): eight of its 24 bits each,
 // cut off and not rounded; with h rounded the values above bf16's largest, 3.39e38, would
-// become infinite.  What is left of an infinity or a NaN (a NaN) is made zero, so that its
+// become infinite.  Only l is, to the nearest: below 2^-110 it may reach past bf16's last
+// place, 2^-133.  What is left of an infinity or a NaN (a NaN) is made zero, so that its
 // products are those of fp32: the middle of (r, r, 0) is r, and 0 where r is a NaN.  (A NaN
 // whose set bits are all in the lower half, a signalling one, would count as an infinity; no
 // operation gives such a one.)
@@ -87,7 +88,7 @@ __device__ __forceinline__ void cut8(const float (&x)[8], u32x4& h, u32x4& m, u3
             m[i] = opaque(bf16_cut(r0, r1));
             m0 = bf16_lo(m[i]);
             m1 = bf16_hi(m[i]);
-            l[i] = bf16_cut(r0 - m0, r1 - m1);
+            l[i] = bf16_pair(r0 - m0, r1 - m1);
         }
     }
 }

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import lowbit_reference as ref
+import lowbit_variants as var
 import minitensor_amd as mt
 
 pytestmark = pytest.mark.gpu
@@ -148,3 +149,40 @@ def test_linear_backward_q8_bias_gradient_of_many_rows(dev, r, fin, fout):
     want = r * a.double()
     split = mt.lib().mt_linear_backward_q8_workspace_f32(r, fin, fout) > 0 and fin < 4096
     assert bool(((db.double() - want).abs() <= (9 + 32 * split) * ref.EPS32 * want).all())
+
+
+def smallest(dev, key, n, k):
+    """[n, k], in each row one value from 2^-149 to 2^-100 with all its bits; it, its column."""
+    g = torch.Generator(device=dev).manual_seed(key)
+    e = torch.arange(n, device=dev) % 50 - 149
+    v = ((1 + torch.rand(n, device=dev, generator=g)).double() * 2.0 ** e.double()).float()
+    at = (torch.arange(n, device=dev) * 37 + 11) % k
+    x = torch.zeros(n, k, device=dev)
+    x[torch.arange(n, device=dev), at] = v
+    return x, v.double(), at
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** 60])
+@pytest.mark.parametrize("m,n,k,group", [(16, 64, 300, 64), (100, 130, 300, 128), (100, 130, 300, 32),
+                                         (2047, 2050, 300, 128)])
+def test_linear_q4_of_the_smallest_inputs(dev, m, n, k, group, scale):
+    """To the nearest multiple of 2^-133, subnormal ones too; the product's roundings
+    (lowbit_variants.SINGLE), and a subnormal sum's (2^-146: half of 2^-145)."""
+    x, v, at = smallest(dev, m, m, k)
+    code = rng(8, n, k).integers(-8, 8, (n, k)).astype(np.int8)
+    s = np.full((n, -(-k // group)), scale, np.float32)
+    wq = mt.Q4Weight(gpu(ref.pack_q4(code), dev), gpu(s, dev), k, group)
+    w = gpu(ref.weight_q4(code, s, group), dev)[:, at].t()
+    want = v[:, None] * w
+    err = (mt.linear_q4(x, wq).double() - want).abs()
+    assert bool((err <= 2.0 ** -134 * w.abs() + var.SINGLE * want.abs() + 2.0 ** -146).all())
+
+
+@pytest.mark.parametrize("r,fin,fout", [(300, 130, 70), (300, 2050, 2050)])
+def test_linear_backward_q8_of_the_smallest_gradients(dev, r, fin, fout):
+    x, v, at = smallest(dev, r + fin, fout, r)
+    q = gpu(rng(9, r, fin).integers(-128, 128, (r, fin)).astype(np.int8), dev)
+    _, dw, _ = mt.linear_backward_q8(x.t().contiguous(), mt.Q8Rows(q, torch.ones(r, device=dev)))
+    want = v[:, None] * q[at].double()
+    err = (dw.double() - want).abs()
+    assert bool((err <= 2.0 ** -134 * q[at].double().abs() + var.SINGLE * want.abs() + 2.0 ** -149).all())
