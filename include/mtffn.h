@@ -1,0 +1,76 @@
+/*
+ * mtffn.h -- C ABI of a gated feed-forward block and of what a training step does with its
+ * gradients (libmtgemm.so, beside mtgemm.h and mtlowbit.h, whose conventions hold here too:
+ * device pointers, element offsets and strides read in place, work enqueued on `stream`, no
+ * allocation, no synchronisation, workspaces sized by the matching query, negative mt_status
+ * on error, nothing thrown, every sum in a fixed order).
+ *
+ * None of these has a counterpart in the reference.  fp32 operands are mt_mat_f32 views with
+ * batch 1 unless said otherwise; extents are below 2^31 - 2^16.  An output must not overlap an
+ * input unless said otherwise.
+ */
+#ifndef MTFFN_H
+#define MTFFN_H
+
+#include "mtgemm.h"
+#include "mtlowbit.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Activations, and their formulas: s(a) = 1/(1 + exp(-a)). */
+typedef enum mt_activation {
+    MT_ACT_SILU = 0,        /* a*s(a) */
+    MT_ACT_GELU = 1,        /* a*(1 + erf(a/sqrt 2))/2 */
+    MT_ACT_GELU_TANH = 2,   /* a*(1 + tanh(sqrt(2/pi)*(a + 0.044715 a^3)))/2 */
+    MT_ACT_RELU = 3,        /* max(a, 0) */
+    MT_ACT_SIGMOID = 4      /* s(a) */
+} mt_activation;
+
+/* ---- gated feed-forward block ----------------------------------------------------
+ * GU = X·Wᵀ + bias with W [2F][in], the gates' rows first;  H = act(GU[:, :F]) * GU[:, F:].
+ * GU NULL: not wanted (training keeps it for the backward pass).  bias NULL: none.  No
+ * inputs (in = 0): GU is the bias, or zeros.
+ * The products are those of mt_linear_forward_f32 and mt_linear_q8.
+ * workspace: a multiple of 4; aligned to 16 bytes it is written 16 at a time. */
+int mt_gated_linear_f32(const mt_mat_f32* X, const mt_mat_f32* W, const float* bias,
+                        int64_t bias_stride, int act, const mt_mat_f32* H, const mt_mat_f32* GU,
+                        void* workspace, size_t ws_bytes, void* stream);
+size_t mt_gated_linear_workspace_f32(int64_t rows, int64_t in_features, int64_t features);
+int mt_gated_linear_q8(const mt_rows_q8* X, const mt_rows_q8* W, const float* bias,
+                       int64_t bias_stride, int act, const mt_mat_f32* H, const mt_mat_f32* GU,
+                       void* workspace, size_t ws_bytes, void* stream);
+size_t mt_gated_linear_q8_workspace(int64_t rows, int64_t in_features, int64_t features);
+/* The kernel that a call takes (as mt_linear_q8_plan). */
+int mt_gated_linear_q8_plan(int64_t rows, int64_t in_features, int64_t features,
+                            mt_lowbit_plan* plan);
+
+/* H = act(GU[:, :F]) * GU[:, F:] of projections that are there already, and the gradient
+ * at them:  dG = dH * U * act'(G),  dU = dH * act(G).  dGU may be the same view as GU. */
+int mt_gate_f32(const mt_mat_f32* GU, int act, const mt_mat_f32* H, void* stream);
+int mt_gate_backward_f32(const mt_mat_f32* dH, const mt_mat_f32* GU, int act,
+                         const mt_mat_f32* dGU, void* stream);
+
+/* ---- gradients of a whole model ----------------------------------------------------
+ * norm = sqrt(sum of the squares of every element of every tensor), held in fp64 until it is
+ * rounded to fp32.  Tensors are views of up to three axes (batch, rows, cols), each below 2^42
+ * elements, at most 2^20 of them; `grads` is read before the call returns.
+ * workspace: a multiple of 8. */
+int mt_grad_norm_f32(const mt_mat_f32* grads, int64_t count, float* norm, void* workspace,
+                     size_t ws_bytes, void* stream);
+/* ... and out[i] = grads[i] * c with c = min(1, max_norm / (norm + eps)) in fp64, rounded
+ * to fp32 (a NaN norm gives NaN throughout; an infinite one 0, and NaN where the gradient is
+ * infinite).  out NULL: in place; with c = 1 nothing is written then.  Otherwise out[i] has the
+ * shape of grads[i], and may be the same view.  No output may appear twice.  norm is that
+ * before the scaling. */
+int mt_clip_grad_norm_f32(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count,
+                          float max_norm, float eps, float* norm, void* workspace, size_t ws_bytes,
+                          void* stream);
+size_t mt_grad_norm_workspace_f32(int64_t count);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* MTFFN_H */

@@ -130,7 +130,7 @@ def lib() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build it with `python -m minitensor_amd.build` "
                 "(there is no CPU fallback)")
         h = ctypes.CDLL(str(LIB_PATH))
-        for name, (res, args) in {**_SIGS, **_LOWBIT_SIGS}.items():
+        for name, (res, args) in {**_SIGS, **_LOWBIT_SIGS, **_FFN_SIGS}.items():
             fn = getattr(h, name)
             fn.restype = res
             fn.argtypes = args
@@ -510,6 +510,9 @@ def tolerance(K: int, amax: float, bmax: float) -> float:
 
 
 from .lowbit import (Q4Weight, Q8Rows, RmsNorm, dequantize_q4, dequantize_q8,  # noqa: E402, F401
-                     linear_backward_q8, linear_q4, quantize_q4, quantize_q8, rms_norm,
-                     rms_norm_backward)
+                     linear_backward_q8, linear_q4, linear_q8, quantize_q4, quantize_q8,
+                     rms_norm, rms_norm_backward)
 from .lowbit import SIGS as _LOWBIT_SIGS  # noqa: E402
+from .ffn import (GatedLinear, clip_grad_norm, gate, gate_backward, gated_linear,  # noqa: E402, F401
+                  gated_linear_backward, grad_norm)
+from .ffn import SIGS as _FFN_SIGS  # noqa: E402

@@ -1,0 +1,147 @@
+// gate_kernel.hpp -- activations of a gated feed-forward block and its elementwise passes
+// (include/mtffn.h): h = act(g) * u, and its gradients.
+//
+// The passes are bound by memory: 12 and 20 bytes per element of h.  exp and erfc are the
+// device library's; a quotient by 1 + e, 1 <= 1 + e <= 2, is a product with v_rcp_f32 (1 ulp).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "row_access.hpp"
+
+namespace mtk {
+
+enum : int { ACT_SILU = 0, ACT_GELU = 1, ACT_GELU_TANH = 2, ACT_RELU = 3, ACT_SIGMOID = 4, kActs = 5 };
+
+// 1/(1 + exp(-a)) and, in rest, 1/(1 + exp(a)), neither by a difference.
+__device__ __forceinline__ float logistic(float a, float& rest) {
+    const float e = expf(-__builtin_fabsf(a)), r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
+    rest = a < 0.f ? r : s;
+    return a < 0.f ? s : r;
+}
+
+constexpr float kGeluC = 0.7978845608028654f;        // sqrt(2/pi)
+constexpr float kGeluA = 0.044715f;
+constexpr float kHalfRoot = 0.7071067811865476f;     // sqrt(1/2)
+constexpr float kNormalPeak = 0.3989422804014327f;   // 1/sqrt(2 pi)
+
+// act(a) and, with SLOPE, its derivative in d.
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ float act_at(float a, float& d) {
+    float q;
+    if constexpr (ACT == ACT_SILU || ACT == ACT_SIGMOID) {
+        const float t = logistic(a, q);
+        // (where t*q is zero, a may be infinite)
+        const float p = t * q;
+        if constexpr (SLOPE) d = ACT == ACT_SIGMOID ? p : p == 0.f ? t : __builtin_fmaf(a, p, t);
+        return ACT == ACT_SIGMOID ? t : a * t;
+    } else if constexpr (ACT == ACT_GELU) {
+        const float t = 0.5f * erfcf(-kHalfRoot * a);
+        if constexpr (SLOPE) {
+            const float p = kNormalPeak * expf(-0.5f * a * a);
+            d = p == 0.f ? t : __builtin_fmaf(a, p, t);
+        }
+        return a * t;
+    } else if constexpr (ACT == ACT_GELU_TANH) {
+        // (1 + tanh z)/2 = 1/(1 + exp(-2z))
+        const float a2 = a * a;
+        const float t = logistic(2.f * kGeluC * a * __builtin_fmaf(kGeluA, a2, 1.f), q);
+        if constexpr (SLOPE) {
+            const float p = t * q;
+            d = p == 0.f ? t
+                         : __builtin_fmaf(2.f * kGeluC * a * p, __builtin_fmaf(3.f * kGeluA, a2, 1.f), t);
+        }
+        return a * t;
+    } else {
+        if constexpr (SLOPE) d = a > 0.f ? 1.f : 0.f;
+        return a <= 0.f ? 0.f : a;                   // (a NaN stays)
+    }
+}
+
+// Calls f(constant) for a run-time activation (the same throughout a launch).
+template <class F>
+__device__ __forceinline__ void with_act(int act, F f) {
+    using std::integral_constant;
+    switch (act) {
+        case ACT_SILU: return f(integral_constant<int, ACT_SILU>{});
+        case ACT_GELU: return f(integral_constant<int, ACT_GELU>{});
+        case ACT_GELU_TANH: return f(integral_constant<int, ACT_GELU_TANH>{});
+        case ACT_RELU: return f(integral_constant<int, ACT_RELU>{});
+        default: return f(integral_constant<int, ACT_SIGMOID>{});
+    }
+}
+
+// h = act(g)*u of four elements.
+__device__ __forceinline__ rowf4 gate4(int act, const rowf4& g, const rowf4& u) {
+    rowf4 h;
+    with_act(act, [&](auto a) {
+        float d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = act_at<a(), false>(g[e], d) * u[e];
+    });
+    return h;
+}
+
+struct GateParams {
+    RowView gu;                       // [M][2F], the gates first
+    RowView dh;                       // backward
+    RowView out;                      // h [M][F], or the gradients [M][2F] (gu itself, if need be)
+    int64_t M;
+    int F, act;
+};
+
+// VEC: elements of a row are neighbours in every operand: a thread takes four of them, the
+// last of a row one by one.
+template <bool VEC, bool BACK>
+__global__ void __launch_bounds__(256) gate_rows(GateParams p) {
+    const int per = VEC ? (p.F + 3) / 4 : p.F;
+    const int64_t total = p.M * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+         i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / per;
+        const int f = (int)(i - m * per) * (VEC ? 4 : 1);
+        constexpr int MODE = VEC ? R_TAIL : R_STRIDED;
+        // (the up columns as rows of their own, so that a row's end is theirs)
+        const RowView up{p.gu.p + (int64_t)p.F * p.gu.cs, p.gu.rs, p.gu.cs};
+        const auto g = row_load<MODE>(p.gu, m, f, p.F), u = row_load<MODE>(up, m, f, p.F);
+        if constexpr (!BACK) {
+            auto h = g;
+            with_act(p.act, [&](auto a) {
+                float d;
+                if constexpr (VEC) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) h[e] = act_at<a(), false>(g[e], d) * u[e];
+                } else {
+                    h = act_at<a(), false>(g, d) * u;
+                }
+            });
+            row_store<MODE>(p.out, m, f, p.F, h);
+        } else {
+            const auto dh = row_load<MODE>(p.dh, m, f, p.F);
+            auto dg = g, du = u;
+            with_act(p.act, [&](auto a) {
+                if constexpr (VEC) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float d;
+                        const float v = act_at<a(), true>(g[e], d);
+                        dg[e] = dh[e] * u[e] * d;
+                        du[e] = dh[e] * v;
+                    }
+                } else {
+                    float d;
+                    const float v = act_at<a(), true>(g, d);
+                    dg = dh * u * d;
+                    du = dh * v;
+                }
+            });
+            const RowView dup{p.out.p + (int64_t)p.F * p.out.cs, p.out.rs, p.out.cs};
+            row_store<MODE>(p.out, m, f, p.F, dg);
+            row_store<MODE>(dup, m, f, p.F, du);
+        }
+    }
+}
+
+}  // namespace mtk

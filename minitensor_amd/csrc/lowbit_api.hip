@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdint>
 
+#include "api_checks.hpp"
 #include "lowbit_back_kernel.hpp"
 #include "lowbit_q4_kernel.hpp"
 #include "lowbit_rows_kernel.hpp"
@@ -15,37 +16,11 @@ using namespace mtk;
 
 namespace {
 
-// Extents are 32-bit inside the kernels, and blocks past an end stay below 2^31.
-constexpr int64_t kMaxDim = ((int64_t)1 << 31) - (1 << 16);
+using mtk::valid;
+
 constexpr int64_t kMaxOut = (int64_t)1 << 26;   // rows of a 4-bit weight (32 threads each in a grid)
 constexpr int64_t kMaxScaleStride = (int64_t)1 << 22;   // a tile's 256 rows of scales within 32 bits of bytes
-constexpr int kCus = 256;                       // what plans fill (MI355X)
-constexpr int64_t kMaxTiles = (int64_t)1 << 23; // of 512 threads: a grid's threads are a 32-bit number
 
-int launched() {
-    // (as mt_gemm_f32: a launch recorded by a stream capture reports this)
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess || e == hipErrorStreamCaptureUnsupported ? MT_OK : MT_ERR_HIP;
-}
-
-// A 2-D fp32 view; written: no two elements on one address.
-bool valid(const mt_mat_f32* X, bool written) {
-    if (!X || X->batch != 1 || X->rows < 0 || X->cols < 0 || X->row_stride < 0 ||
-        X->col_stride < 0 || X->offset < 0 || X->rows >= kMaxDim || X->cols >= kMaxDim)
-        return false;
-    if (X->rows == 0 || X->cols == 0) return true;
-    if (!X->base) return false;
-    return !written || ((X->rows <= 1 || X->row_stride > 0) && (X->cols <= 1 || X->col_stride > 0));
-}
-bool same_shape(const mt_mat_f32* A, const mt_mat_f32* B) {
-    return A->rows == B->rows && A->cols == B->cols;
-}
-bool valid(const mt_rows_q8* Q) {
-    if (!Q || Q->rows < 0 || Q->cols < 0 || Q->rows >= kMaxDim || Q->cols >= kMaxDim ||
-        Q->row_stride < 0 || (Q->rows > 1 && Q->row_stride < Q->cols))
-        return false;
-    return Q->rows == 0 || (Q->scale && (Q->cols == 0 || Q->q));
-}
 bool valid(const mt_weight_q4* W) {
     if (!W || W->n < 0 || W->k < 0 || W->n >= kMaxOut || W->k >= kMaxDim ||
         (W->group != 32 && W->group != 64 && W->group != 128) || W->row_stride < 0 ||
@@ -56,13 +31,6 @@ bool valid(const mt_weight_q4* W) {
     return W->n == 1 || (W->scale_stride < kMaxScaleStride && W->row_stride >= (W->k + 31) / 32 * 16 &&
                          W->scale_stride >= (W->k + W->group - 1) / W->group);
 }
-
-RowView view(const mt_mat_f32* X) {
-    if (!X) return {nullptr, 0, 0};
-    return {const_cast<float*>(X->base) + X->offset, X->row_stride, X->col_stride};
-}
-// Rows whose elements are neighbours (or absent).
-bool unit(const RowView& v) { return !v.p || v.cs == 1; }
 
 // Threads of a row: 16 values each (lowbit_rows_kernel.hpp).
 int row_threads(int64_t cols) { return cols <= 1024 ? 64 : cols <= 4096 ? 256 : 1024; }

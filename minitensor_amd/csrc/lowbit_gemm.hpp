@@ -21,29 +21,9 @@
 
 #include "gemm_split.hpp"
 #include "lowbit_rows_kernel.hpp"
+#include "tile_helpers.hpp"
 
 namespace mtk {
-
-// Keeps the compiler from taking a packed value apart again (it rounded the low half a second
-// time rather than shift it: two instructions more per pair).
-__device__ __forceinline__ uint32_t opaque(uint32_t v) {
-    asm("" : "+v"(v));
-    return v;
-}
-
-// p moved on by a 32-bit number of bytes: one register beside a uniform p (the compiler
-// kept the number's 64 bits through the loop).
-template <class T>
-__device__ __forceinline__ const T* at_bytes(const T* p, uint32_t bytes) {
-    asm volatile("" : "+v"(bytes));
-    return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + bytes);
-}
-
-// The value anew, for a path beside the loop: not kept in registers through it.
-__device__ __forceinline__ int anew(int v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
 
 // Two floats' upper halves: themselves where they are exact in bf16, else cut off.
 __device__ __forceinline__ uint32_t bf16_cut(float a, float b) {
@@ -104,13 +84,6 @@ __device__ __forceinline__ u32x4 q8_bf16(const u32x2& q) {
     return r;
 }
 
-// A barrier that orders LDS alone.
-__device__ __forceinline__ void lb_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 // LDS of a chunk: per part four groups of eight k, each a column of 16-byte entries, one
 // per row, and two entries more, so that the groups of a row start 32 bytes apart modulo
 // the banks' 128.
@@ -118,19 +91,6 @@ template <int ROWS>
 constexpr int lb_group() { return (ROWS + 2) * 16; }
 template <int ROWS>
 constexpr int lb_plane() { return 4 * lb_group<ROWS>(); }
-
-// The tile of a workgroup: eight XCDs take consecutive workgroups in turn; each
-// gets a run of tiles, walked down eight rows of tiles at a time, so that the
-// tiles in flight on one L2 share their operands.
-__device__ __forceinline__ void lb_tile(int b, int tm, int tn, int& im, int& in) {
-    const int n = tm * tn;
-    const int xcd = b & 7, q = n >> 3, rem = n & 7;
-    b = xcd * q + min(xcd, rem) + (b >> 3);
-    const int band = 8 * tn, first = b / band * 8, h = min(8, tm - first);
-    const int w = b % band;
-    im = first + w % h;
-    in = w / h;
-}
 
 // The loop.  LA: loader with
 //   Raw                          what a thread holds of a chunk

@@ -21,18 +21,13 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "row_access.hpp"
+
 namespace mtk {
 
 constexpr int kRowVals = 16;          // values of a row per thread
 constexpr float kQ8Inv = 1.f / 127.f;
 constexpr float kScaleMin = 0x1p-126f;
-
-typedef float rowf4 __attribute__((ext_vector_type(4)));
-
-struct RowView {                      // fp32 rows (base nullptr: none)
-    float* p;
-    int64_t rs, cs;
-};
 
 struct RowParams {
     RowView x, r, h, y;               // forward: inputs x, r; outputs h, y
@@ -58,49 +53,6 @@ struct RowBwdParams {
     int row_step;                     // rows between a row group's consecutive rows
 };
 
-enum { R_STRIDED = 0, R_TAIL = 1, R_VEC = 2 };
-
-typedef rowf4 rowf4_u __attribute__((aligned(4)));
-typedef uint32_t row_codes __attribute__((aligned(1)));
-
-// What a thread takes at a time: four elements of row r from column c, or one.
-template <int MODE>
-using RowV = std::conditional_t<MODE == R_STRIDED, float, rowf4>;
-
-template <int MODE>
-__device__ __forceinline__ RowV<MODE> run_load(const float* p, int64_t cs, int c, int cols) {
-    if constexpr (MODE == R_STRIDED) return p[(int64_t)c * cs];
-    else if (MODE == R_VEC || c + 4 <= cols) return *reinterpret_cast<const rowf4_u*>(p + c);
-    else {
-        rowf4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 3; ++e)
-            if (c + e < cols) x[e] = p[c + e];
-        return x;
-    }
-}
-template <int MODE>
-__device__ __forceinline__ RowV<MODE> row_load(const RowView& v, int64_t r, int c, int cols) {
-    return run_load<MODE>(v.p + r * v.rs, v.cs, c, cols);
-}
-template <int MODE>
-__device__ __forceinline__ void row_store(const RowView& v, int64_t r, int c, int cols,
-                                          const RowV<MODE>& x) {
-    float* const p = v.p + r * v.rs;
-    if constexpr (MODE == R_STRIDED) p[(int64_t)c * v.cs] = x;
-    else if (MODE == R_VEC || c + 4 <= cols) *reinterpret_cast<rowf4_u*>(p + c) = x;
-    else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e)
-            if (c + e < cols) p[c + e] = x[e];
-    }
-}
-template <int MODE>
-__device__ __forceinline__ RowV<MODE> weight_load(const float* w, int64_t ws, int c, int cols) {
-    if (w) return run_load<MODE>(w, ws, c, cols);
-    if constexpr (MODE == R_STRIDED) return 1.f;
-    else return rowf4{1.f, 1.f, 1.f, 1.f};
-}
 __device__ __forceinline__ float row_dot(const rowf4& a, const rowf4& b) {
     return (a[0] * b[0] + a[1] * b[1]) + (a[2] * b[2] + a[3] * b[3]);
 }

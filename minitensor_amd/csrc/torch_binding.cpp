@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
+#include "mtffn.h"
 #include "mtgemm.h"
 #include "mtlowbit.h"
 
@@ -513,6 +514,150 @@ py::object linear_q4(py::handle px, py::handle pxscale, py::handle ppacked, py::
     return pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout);
 }
 
+// Whether all tensors given are on the current device, whose stream the work goes to.
+template <class... T>
+bool here(const T&... t) {
+    const auto d = c10::hip::current_device();
+    return ((!t.defined() || t.get_device() == d) && ...);
+}
+
+py::object linear_q8(py::handle pq, py::handle pscale, py::handle pw, py::handle pwscale,
+                     py::handle pb, py::handle pout, py::handle pws, py::handle stream) {
+    bool ok = true;
+    const at::Tensor gws = given_ws(pws, &ok);
+    const at::Tensor q = rows_arg(pq, at::kChar, 2, &ok), w = rows_arg(pw, at::kChar, 2, &ok);
+    const at::Tensor scale = rows_arg(pscale, at::kFloat, 1, &ok),
+                     wscale = rows_arg(pwscale, at::kFloat, 1, &ok), b = arg(pb, &ok);
+    at::Tensor out = arg(pout, &ok);
+    if (!ok || !here(q, scale, w, wscale, b, out)) return py::none();
+    const int64_t rows = q.size(0), k = q.size(1), n = w.size(0);
+    if (w.size(1) != k || scale.size(0) != rows || wscale.size(0) != n || !vec_of(b, n) ||
+        !shaped(out, rows, n))
+        return py::none();
+    void* const s = stream_of(stream);
+    {
+        const py::gil_scoped_release nogil;
+        if (!out.defined()) out = empty({rows, n}, q);
+        const mt_rows_q8 mx = rows_q8(q, scale), mw = rows_q8(w, wscale);
+        const mt_mat_f32 my = mat(out);
+        const Workspace ws(gws, q, [&] { return mt_linear_q8_workspace(rows, k, n); });
+        check(mt_linear_q8(&mx, &mw, ptr(b), step(b), &my, ws.p, ws.n, s), "mt_linear_q8");
+    }
+    return pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout);
+}
+
+// ---- include/mtffn.h -----------------------------------------------------------
+
+// x and w: fp32 (no scales), or 8-bit rows.
+py::object gated_linear(py::handle px, py::handle pxscale, py::handle pw, py::handle pwscale,
+                        py::handle pb, int act, bool keep, py::handle pout, py::handle pws,
+                        py::handle stream) {
+    bool ok = true;
+    const bool q8 = !pxscale.is_none();
+    const at::Tensor gws = given_ws(pws, &ok);
+    const at::Tensor x = q8 ? rows_arg(px, at::kChar, 2, &ok) : arg(px, &ok);
+    const at::Tensor w = q8 ? rows_arg(pw, at::kChar, 2, &ok) : arg(pw, &ok);
+    at::Tensor xscale, wscale;
+    if (q8) {
+        xscale = rows_arg(pxscale, at::kFloat, 1, &ok);
+        wscale = rows_arg(pwscale, at::kFloat, 1, &ok);
+    }
+    const at::Tensor b = arg(pb, &ok);
+    at::Tensor out = arg(pout, &ok), gu;
+    if (!ok || !x.defined() || !w.defined() || x.dim() != 2 || w.dim() != 2 ||
+        !here(x, w, xscale, wscale, b, out))
+        return py::none();
+    const int64_t rows = x.size(0), k = x.size(1), f2 = w.size(0), f = f2 / 2;
+    if (w.size(1) != k || f2 % 2 != 0 || !vec_of(b, f2) || !shaped(out, rows, f) ||
+        (q8 && (xscale.size(0) != rows || wscale.size(0) != f2)))
+        return py::none();
+    void* const s = stream_of(stream);
+    {
+        const py::gil_scoped_release nogil;
+        if (!out.defined()) out = empty({rows, f}, x);
+        if (keep) gu = empty({rows, f2}, x);
+        mt_mat_f32 mg{};
+        if (keep) mg = mat(gu);
+        const mt_mat_f32 mh = mat(out);
+        const Workspace ws(gws, x, [&] {
+            return q8 ? mt_gated_linear_q8_workspace(rows, k, f)
+                      : mt_gated_linear_workspace_f32(rows, k, f);
+        });
+        if (q8) {
+            const mt_rows_q8 mx = rows_q8(x, xscale), mw = rows_q8(w, wscale);
+            check(mt_gated_linear_q8(&mx, &mw, ptr(b), step(b), act, &mh, keep ? &mg : nullptr, ws.p,
+                                     ws.n, s),
+                  "mt_gated_linear_q8");
+        } else {
+            const mt_mat_f32 mx = mat(x), mw = mat(w);
+            check(mt_gated_linear_f32(&mx, &mw, ptr(b), step(b), act, &mh, keep ? &mg : nullptr, ws.p,
+                                      ws.n, s),
+                  "mt_gated_linear_f32");
+        }
+    }
+    return py::make_tuple(pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout),
+                          tensor(gu));
+}
+
+py::object gate_backward(py::handle pdh, py::handle pgu, int act, py::handle pout,
+                         py::handle stream) {
+    bool ok = true;
+    const at::Tensor dh = arg(pdh, &ok), gu = arg(pgu, &ok);
+    at::Tensor out = arg(pout, &ok);
+    if (!ok || !dh.defined() || !gu.defined() || dh.dim() != 2 || !here(dh, gu, out) ||
+        !shaped(gu, dh.size(0), 2 * dh.size(1)) || !shaped(out, dh.size(0), 2 * dh.size(1)))
+        return py::none();
+    void* const s = stream_of(stream);
+    {
+        const py::gil_scoped_release nogil;
+        if (!out.defined()) out = empty(gu.sizes(), gu);
+        const mt_mat_f32 md = mat(dh), mg = mat(gu), mo = mat(out);
+        check(mt_gate_backward_f32(&md, &mg, act, &mo, s), "mt_gate_backward_f32");
+    }
+    return pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout);
+}
+
+// Lists of tensors that are each one run of elements, in the same order in both; anything
+// else is the caller's.
+py::object clip(py::handle pgrads, py::handle pout, bool scale, float most, float eps,
+                py::handle pws, py::handle stream) {
+    bool ok = true;
+    const at::Tensor gws = given_ws(pws, &ok);
+    const bool own = !pout.is_none();
+    if (!ok || !PyList_Check(pgrads.ptr()) || (own && !PyList_Check(pout.ptr()))) return py::none();
+    const Py_ssize_t n = PyList_GET_SIZE(pgrads.ptr());
+    if (n == 0 || (own && PyList_GET_SIZE(pout.ptr()) != n)) return py::none();
+    std::vector<mt_mat_f32> g((size_t)n), o(own ? (size_t)n : 0);
+    at::Tensor first;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const at::Tensor t = arg(PyList_GET_ITEM(pgrads.ptr(), i), &ok);
+        if (!ok || !t.defined() || !t.is_contiguous() || !here(t)) return py::none();
+        const int64_t e = t.numel();
+        g[(size_t)i] = mt_mat_f32{ptr(t), 0, 1, e, e, 1, 1, 0};
+        if (own) {
+            const at::Tensor u = arg(PyList_GET_ITEM(pout.ptr(), i), &ok);
+            if (!ok || !u.defined() || !u.is_contiguous() || !here(u) || u.sizes() != t.sizes())
+                return py::none();
+            o[(size_t)i] = mt_mat_f32{ptr(u), 0, 1, e, e, 1, 1, 0};
+        }
+        if (i == 0) first = t;
+    }
+    void* const s = stream_of(stream);
+    at::Tensor norm;
+    {
+        const py::gil_scoped_release nogil;
+        norm = empty({}, first);
+        const Workspace ws(gws, first, [&] { return mt_grad_norm_workspace_f32(n); });
+        if (scale)
+            check(mt_clip_grad_norm_f32(g.data(), own ? o.data() : nullptr, n, most, eps,
+                                        out_ptr(norm), ws.p, ws.n, s),
+                  "mt_clip_grad_norm_f32");
+        else
+            check(mt_grad_norm_f32(g.data(), n, out_ptr(norm), ws.p, ws.n, s), "mt_grad_norm_f32");
+    }
+    return tensor(norm);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -527,4 +672,8 @@ PYBIND11_MODULE(_native, m) {
     m.def("dequantize_q8", &dequantize_q8);
     m.def("linear_backward_q8", &linear_backward_q8);
     m.def("linear_q4", &linear_q4);
+    m.def("linear_q8", &linear_q8);
+    m.def("gated_linear", &gated_linear);
+    m.def("gate_backward", &gate_backward);
+    m.def("clip", &clip);
 }

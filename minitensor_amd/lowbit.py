@@ -1,5 +1,5 @@
 """Operators around a Linear layer whose activations are kept in 8 bits and
-whose weights are served in 4 (include/mtlowbit.h):
+whose weights are served in 4 or 8 (include/mtlowbit.h):
 
   rms_norm, rms_norm_backward   RMS norm with the residual's addition, its rows
                                 in fp32, in 8 bits, or both
@@ -7,6 +7,7 @@ whose weights are served in 4 (include/mtlowbit.h):
   linear_backward_q8            a Linear layer's gradients from such rows
   quantize_q4, dequantize_q4    a weight in 4 bits with a scale per group
   linear_q4                     F::linear over it, from fp32 or 8-bit rows
+  linear_q8                     F::linear of 8-bit rows over an 8-bit weight
 
 Like the rest of the package: GPU tensors, views read in place, work on the
 current stream or on `stream`, ValueError for wrong shapes, types and devices,
@@ -25,7 +26,8 @@ from . import (MatF32, _api, _check, _handle, _nbytes, _ptr, _require_gpu, _requ
 
 
 class Q8Rows(NamedTuple):
-    """Rows in 8 bits: x[r, c] ~ q[r, c]·scale[r]; q int8 [R, C], scale float32 [R]."""
+    """Rows in 8 bits: x[r, c] ~ q[r, c]·scale[r]; q int8 [R, C], scale float32 [R].  A
+    weight's rows are its output channels."""
     q: torch.Tensor
     scale: torch.Tensor
 
@@ -82,6 +84,9 @@ SIGS = {
     "mt_linear_q4_f32": (ctypes.c_int, [_M, _W, _V, _I64, _M, _V, ctypes.c_size_t, _V]),
     "mt_linear_q4_q8": (ctypes.c_int, [_Q, _W, _V, _I64, _M, _V, ctypes.c_size_t, _V]),
     "mt_linear_q4_workspace": (ctypes.c_size_t, [_I64] * 3),
+    "mt_linear_q8": (ctypes.c_int, [_Q, _Q, _V, _I64, _M, _V, ctypes.c_size_t, _V]),
+    "mt_linear_q8_workspace": (ctypes.c_size_t, [_I64] * 3),
+    "mt_linear_q8_plan": (ctypes.c_int, [_I64] * 3 + [_P(LowbitPlan)]),
     "mt_linear_q4_plan": (ctypes.c_int, [_I64] * 3 + [ctypes.c_int] * 2 + [_P(LowbitPlan)]),
     "mt_linear_backward_q8_plan": (ctypes.c_int, [_I64] * 3 + [_P(LowbitPlan)]),
 }
@@ -350,4 +355,28 @@ def linear_q4(x: Union[torch.Tensor, Q8Rows], wq: Q4Weight, b: Optional[torch.Te
     fn = lib().mt_linear_q4_q8 if q8 else lib().mt_linear_q4_f32
     rc = fn(ctypes.byref(xd), ctypes.byref(d), bp, bs, y, _ptr(ws), _nbytes(ws), _stream(stream))
     _check(rc, "mt_linear_q4_q8" if q8 else "mt_linear_q4_f32")
+    return out
+
+
+@_api
+def linear_q8(x: Q8Rows, w: Q8Rows, b: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, ws=None, stream=None) -> torch.Tensor:
+    """F::linear in 8-bit integers: y = x·wᵀ + b, x [B, in] and w [out, in] in 8 bits with a
+    scale per row (quantize_q8 of a weight gives its).  The sums are exact."""
+    r = native().linear_q8(x[0], x[1], w[0], w[1], b, out, ws, _handle(stream))
+    if r is not None:
+        return r
+    xd, wd = _rows(x), _rows(w)
+    if any(t is not None and t.get_device() != torch.cuda.current_device() for t in (*x, *w, b, out)):
+        raise ValueError("tensors must be on the current device")
+    if xd.cols != wd.cols:
+        raise ValueError(f"linear_q8: x has {xd.cols} inputs, the weight {wd.cols}")
+    bp, bs = _vector(b, wd.rows, "linear_q8: bias")
+    if out is None:
+        out = _empty((xd.rows, wd.rows), x[0])
+    y = _matrix(out, (xd.rows, wd.rows), "linear_q8: out")
+    ws = _ws(ws, lib().mt_linear_q8_workspace(xd.rows, xd.cols, wd.rows), x[0])
+    rc = lib().mt_linear_q8(ctypes.byref(xd), ctypes.byref(wd), bp, bs, y, _ptr(ws), _nbytes(ws),
+                            _stream(stream))
+    _check(rc, "mt_linear_q8")
     return out

@@ -1,0 +1,138 @@
+"""include/mtffn.h and mt_linear_q8 without a GPU: what the entry points refuse before they
+touch the device, what they take as nothing to do, and the queries."""
+import ctypes
+
+import pytest
+
+import minitensor_amd as mt
+from minitensor_amd.lowbit import LowbitPlan, RowsQ8
+
+OK, INVALID, WORKSPACE = mt.MT_OK, mt.MT_ERR_INVALID, mt.MT_ERR_WORKSPACE
+
+
+def M(rows, cols, rs=None, cs=1, batch=1, bs=0, off=0, base=0x1000):
+    return mt.MatF32(base, off, rows, cols, cols if rs is None else rs, cs, batch, bs)
+
+
+def Q(rows, cols, rs=None, q=0x1000, scale=0x2000):
+    return RowsQ8(q, scale, rows, cols, cols if rs is None else rs)
+
+
+def R(x):
+    return ctypes.byref(x) if x is not None else None
+
+
+def plan_q8(m, k, n, gated=False):
+    """(rows of a tile or 0, splits) that linear_q8 (gated_linear of 8-bit rows) takes."""
+    p = LowbitPlan()
+    f = mt.lib().mt_gated_linear_q8_plan if gated else mt.lib().mt_linear_q8_plan
+    assert f(m, k, n, R(p)) == OK
+    return p.tile_rows, p.splits
+
+
+def test_linear_q8_refuses():
+    def call(x=Q(4, 64), w=Q(8, 64), y=M(4, 8), b=None, bs=0, ws=None, n=0):
+        return mt.lib().mt_linear_q8(R(x), R(w), b, bs, R(y), ws, n, None)
+    assert call(w=Q(8, 63)) == INVALID
+    assert call(y=M(4, 9)) == INVALID
+    assert call(y=M(5, 8)) == INVALID
+    assert call(y=M(4, 8, cs=0)) == INVALID
+    assert call(x=Q(4, 64, q=0)) == INVALID
+    assert call(w=Q(8, 64, scale=0)) == INVALID
+    assert call(w=Q(8, 64, rs=63)) == INVALID
+    assert call(b=0x3000, bs=-1) == INVALID
+    assert call(x=None) == INVALID and call(w=None) == INVALID and call(y=None) == INVALID
+    assert call(x=Q(1 << 31, 64), y=M(1 << 31, 8)) == INVALID
+    assert call(x=Q(0, 64), y=M(0, 8)) == OK
+    assert call(w=Q(0, 64), y=M(4, 0)) == OK
+    assert plan_q8(64, 65536, 64)[1] > 1
+    assert call(x=Q(64, 65536), w=Q(64, 65536), y=M(64, 64)) == WORKSPACE
+
+
+def test_gated_linear_refuses():
+    f32, q8 = mt.lib().mt_gated_linear_f32, mt.lib().mt_gated_linear_q8
+
+    def call(f, x, w, h=M(4, 4), gu=None, act=0, b=None, bs=0, ws=None, n=0):
+        return f(R(x), R(w), b, bs, act, R(h), R(gu), ws, n, None)
+    for f, X in ((f32, M), (q8, Q)):
+        assert call(f, X(4, 64), X(7, 64)) == INVALID
+        assert call(f, X(4, 64), X(8, 60)) == INVALID
+        assert call(f, X(4, 64), X(8, 64), act=5) == INVALID
+        assert call(f, X(4, 64), X(8, 64), act=-1) == INVALID
+        assert call(f, X(4, 64), X(8, 64), h=M(4, 8)) == INVALID
+        assert call(f, X(4, 64), X(8, 64), h=M(4, 4, rs=0)) == INVALID
+        assert call(f, X(4, 64), X(8, 64), gu=M(4, 4)) == INVALID
+        assert call(f, X(4, 64), X(8, 64), gu=M(4, 8, cs=0)) == INVALID
+        assert call(f, X(4, 64), X(8, 64), b=0x3000, bs=-1) == INVALID
+        assert call(f, None, X(8, 64)) == INVALID
+        assert call(f, X(0, 64), X(8, 64), h=M(0, 4)) == OK
+        assert call(f, X(4, 64), X(0, 64), h=M(4, 0)) == OK
+
+
+def test_gate_refuses():
+    g, b = mt.lib().mt_gate_f32, mt.lib().mt_gate_backward_f32
+    assert g(R(M(4, 8)), 0, R(M(4, 5)), None) == INVALID
+    assert g(R(M(4, 8)), 9, R(M(4, 4)), None) == INVALID
+    assert g(R(M(4, 8)), 0, R(M(4, 4, cs=0)), None) == INVALID
+    assert g(R(M(4, 8, base=0)), 0, R(M(4, 4)), None) == INVALID
+    assert g(R(M(0, 8)), 0, R(M(0, 4)), None) == OK
+    assert b(R(M(4, 4)), R(M(4, 8)), 0, R(M(4, 6)), None) == INVALID
+    assert b(R(M(4, 3)), R(M(4, 8)), 0, R(M(4, 8)), None) == INVALID
+    assert b(R(M(4, 4)), R(M(4, 8)), 0, R(M(4, 8, rs=0)), None) == INVALID
+    assert b(R(M(4, 0)), R(M(4, 0)), 0, R(M(4, 0)), None) == OK
+
+
+def test_clip_refuses():
+    def call(g, o=None, n=None, most=1.0, eps=1e-6, norm=0x9000, ws=0x10000, size=1 << 30, alone=False):
+        a = (mt.MatF32 * max(len(g), 1))(*g)
+        b = (mt.MatF32 * max(len(o), 1))(*o) if o is not None else None
+        n = len(g) if n is None else n
+        if alone:
+            return mt.lib().mt_grad_norm_f32(a, n, norm, ws, size, None)
+        return mt.lib().mt_clip_grad_norm_f32(a, b, n, most, eps, norm, ws, size, None)
+    x = M(4, 8)
+    assert call([x], n=-1) == INVALID
+    assert call([x], n=(1 << 20) + 1) == INVALID
+    assert call([x], norm=None) == INVALID
+    assert call([x], most=-1.0) == INVALID
+    assert call([x], most=float("nan")) == INVALID
+    assert call([x], eps=-1.0) == INVALID
+    assert call([x, x]) == INVALID                                   # scaled twice
+    assert call([x, M(4, 8, base=0x8000)], [M(4, 8), M(4, 8)]) == INVALID
+    assert call([x], [M(4, 9)]) == INVALID
+    assert call([M(4, 8, rs=0)]) == INVALID                          # rows on one address
+    assert call([M(4, 8, base=0)]) == INVALID
+    assert call([M(4, 8, rs=-8)]) == INVALID
+    assert call([M(1 << 40, 1 << 40)], alone=True) == INVALID
+    assert call([x], ws=None) == WORKSPACE
+    assert call([x], size=8) == WORKSPACE
+    assert call([x], ws=0x10004) == WORKSPACE                        # not a multiple of 8
+    assert call([x], ws=None, alone=True) == WORKSPACE
+
+
+def test_queries():
+    lib = mt.lib()
+    for f in (lib.mt_linear_q8_workspace, lib.mt_gated_linear_q8_workspace, lib.mt_gated_linear_workspace_f32):
+        assert f(0, 8, 8) == 0 and f(-1, 8, 8) == 0 and f(1 << 31, 8, 8) == 0
+    assert lib.mt_grad_norm_workspace_f32(-1) == 0
+    assert 0 < lib.mt_grad_norm_workspace_f32(1) <= lib.mt_grad_norm_workspace_f32(1000)
+    p = LowbitPlan()
+    assert lib.mt_linear_q8_plan(4, 8, 8, None) == INVALID
+    assert lib.mt_linear_q8_plan(0, 8, 8, R(p)) == INVALID
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_q8_plans(gated):
+    """Few rows on their kernel, up to the inputs that its sums hold; a split never holds more
+    terms than 32 bits do; workspaces of whole tiles."""
+    assert plan_q8(1, 4096, 4096, gated)[0] == 0
+    assert plan_q8(2048, 4096, 8192, gated)[0] == 256
+    for m in (1, 40, 300):
+        for k in (1, 131071, 200000, 1 << 20, 1 << 27):
+            tile, splits = plan_q8(m, k, 100, gated)
+            assert tile == 0 and k < 1 << 19 or splits * ((1 << 17) - 128) >= k
+            f = mt.lib().mt_gated_linear_q8_workspace if gated else mt.lib().mt_linear_q8_workspace
+            ws = f(m, k, 100)
+            assert (ws > 0) == (splits > 1)
+            if splits > 1:
+                assert ws >= 4 * splits * m * 100 * (1 + gated)
