@@ -33,7 +33,7 @@ typedef enum mt_activation {
  * GU NULL: not wanted (training keeps it for the backward pass).  bias NULL: none.  No
  * inputs (in = 0): GU is the bias, or zeros.
  * The products are those of mt_linear_forward_f32 and mt_linear_q8.
- * workspace: a multiple of 4; aligned to 16 bytes it is written 16 at a time. */
+ * workspace (fp32): a multiple of 4. */
 int mt_gated_linear_f32(const mt_mat_f32* X, const mt_mat_f32* W, const float* bias,
                         int64_t bias_stride, int act, const mt_mat_f32* H, const mt_mat_f32* GU,
                         void* workspace, size_t ws_bytes, void* stream);
@@ -41,10 +41,9 @@ size_t mt_gated_linear_workspace_f32(int64_t rows, int64_t in_features, int64_t 
 int mt_gated_linear_q8(const mt_rows_q8* X, const mt_rows_q8* W, const float* bias,
                        int64_t bias_stride, int act, const mt_mat_f32* H, const mt_mat_f32* GU,
                        void* workspace, size_t ws_bytes, void* stream);
-size_t mt_gated_linear_q8_workspace(int64_t rows, int64_t in_features, int64_t features);
+size_t mt_gated_linear_q8_workspace(const mt_rows_q8* X, const mt_rows_q8* W);
 /* The kernel that a call takes (as mt_linear_q8_plan). */
-int mt_gated_linear_q8_plan(int64_t rows, int64_t in_features, int64_t features,
-                            mt_lowbit_plan* plan);
+int mt_gated_linear_q8_plan(int64_t rows, int64_t in_features, int64_t features, mt_q8_plan* plan);
 
 /* H = act(GU[:, :F]) * GU[:, F:] of projections that are there already, and the gradient
  * at them:  dG = dH * U * act'(G),  dU = dH * act(G).  dGU may be the same view as GU. */

@@ -119,26 +119,30 @@ size_t mt_linear_q4_workspace(int64_t rows, int64_t in_features, int64_t out_fea
  * Y = X·Wᵀ + bias, both operands in 8 bits: W's rows are the output channels, a scale
  * each (mt_quantize_q8_f32 of the weight gives them):
  *   y[m][n] = (sum_k X.q[m][k]·W.q[n][k]) * (X.scale[m]·W.scale[n]) + bias[n].
- * The sum is exact, whatever its length, and rounded to fp32 once.  Rows at any
- * address; those on multiples of 16 bytes go to LDS without a trip through registers.
- * workspace: a multiple of 4. */
+ * The sum is exact, whatever its length, and rounded to fp32 once.  Rows may lie at any
+ * address; of more than 32 rows of X, an operand whose rows do not start on multiples of 16
+ * bytes is first copied to the workspace. */
 int mt_linear_q8(const mt_rows_q8* X, const mt_rows_q8* W, const float* bias, int64_t bias_stride,
                  const mt_mat_f32* Y, void* workspace, size_t ws_bytes, void* stream);
-size_t mt_linear_q8_workspace(int64_t rows, int64_t in_features, int64_t out_features);
+size_t mt_linear_q8_workspace(const mt_rows_q8* X, const mt_rows_q8* W);
 
 /* ---- diagnostics ---------------------------------------------------------------
  * Which kernel a product's call takes, by its sizes, for tests and benchmarks (as
  * mt_last_config, but nothing runs): of the 4-bit product, and of dW. */
 typedef struct mt_lowbit_plan {
-    int32_t tile_rows;      /* 64 or 128, by twice as many columns (8-bit weights: 64x128, 128x128
-                               or 256x256); 0: the few-rows kernel */
+    int32_t tile_rows;      /* 64 or 128, by twice as many columns; 0: the few-rows kernel */
     int32_t splits;         /* of the summed axis, added up by a launch of their own */
     int32_t column_blocks;  /* of 16 columns, a workgroup of the few-rows kernel; 0 with tiles */
 } mt_lowbit_plan;
+/* Of a product with 8-bit weights: 64x128, 128x128, 128x256 or 256x256; 0: a kernel without
+ * tiles. */
+typedef struct mt_q8_plan {
+    int32_t tile_rows, tile_cols;
+    int32_t splits;
+} mt_q8_plan;
 int mt_linear_q4_plan(int64_t rows, int64_t in_features, int64_t out_features, int group,
                       int x_in_8_bits, mt_lowbit_plan* plan);
-int mt_linear_q8_plan(int64_t rows, int64_t in_features, int64_t out_features,
-                      mt_lowbit_plan* plan);
+int mt_linear_q8_plan(int64_t rows, int64_t in_features, int64_t out_features, mt_q8_plan* plan);
 int mt_linear_backward_q8_plan(int64_t batch_rows, int64_t in_features, int64_t out_features,
                                mt_lowbit_plan* plan);
 

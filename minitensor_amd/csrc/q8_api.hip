@@ -16,47 +16,58 @@ namespace {
 
 // A product's sums are 32-bit below this many terms: a split holds no more.
 constexpr int64_t kMaxTerms = ((int64_t)1 << 17) - 128;
+// Bytes between a tile's rows: their offsets, 255 of them and a chunk, are 32-bit.
+constexpr int64_t kMaxRow = ((int64_t)1 << 24) - 256;
+constexpr int64_t kFewRows = 32;
 
+enum Kind { FEW, LONG, TILES };
 struct Q8Plan {
-    bool few;
+    Kind kind;
     int bm, bn;
     int splits, k_per_split;
     int64_t tiles;                    // the splits' among them
     int64_t part_n;
-    size_t partials;                  // of 4 bytes, 0 without splits
+    size_t partials;                  // bytes, 0 without splits
 };
 
+// Times in us by workgroups on a CU, of a chunk of 128 inputs and of a workgroup's beginning
+// and end, from products of 64-4096 rows, 1000-16384 columns, 512 and 4096 inputs; workgroups
+// go in rounds over the CUs.  (2048 x 4096 -> 8192: 256x256 tiles 66-69 us, 128x256 73-78,
+// 128x128 90-100, 64x128 117-124; 1024 x 4096 -> 4096: 49, 33, 26, 33; 256 x 4096 -> 4096:
+// 46, 28, 21, 15.)
 struct Q8Tile {
     int bm, bn, per_cu;
-    double alone, more;               // us a chunk of 128 inputs: one workgroup on the CU, each further one
+    double alone, more, fixed;        // one workgroup on the CU, each further one; a workgroup
 };
-constexpr Q8Tile kTiles[] = {{64, 128, 3, 0.30, 0.14}, {128, 128, 2, 0.36, 0.22}, {256, 256, 1, 1.0, 0}};
+constexpr Q8Tile kTiles[] = {{64, 128, 2, 0.34, 0.45, 2.2},
+                             {128, 128, 2, 0.56, 0.70, 4},
+                             {128, 256, 1, 0.88, 0, 6.5},
+                             {256, 256, 1, 1.6, 0, 10}};
 
 // cols: columns of the launch (gated: whole blocks of 32 features, twice).
 Q8Plan q8_plan(int64_t M, int64_t cols, int64_t K) {
-    if (M <= 32 && K < ((int64_t)1 << 19)) return {true, 0, 0, 1, 0, 0, 0, 0};
+    if (K > kMaxRow) return {LONG, 0, 0, 1, 0, 0, 0, 0};
+    if (M <= kFewRows && K < kQ8Segment) return {FEW, 0, 0, 1, 0, 0, 0, 0};
     Q8Plan best{};
     double least = 0;
     const int64_t chunks = std::max<int64_t>(1, (K + 127) / 128);
-    const int64_t fewest = (K + kMaxTerms - 1) / kMaxTerms;
+    const int64_t fewest = std::max<int64_t>(1, (K + kMaxTerms - 1) / kMaxTerms);
     for (const Q8Tile& t : kTiles) {
         const int64_t tm = (M + t.bm - 1) / t.bm, tn = (cols + t.bn - 1) / t.bn;
-        for (int64_t s = std::max<int64_t>(1, fewest); s <= std::max<int64_t>(fewest, std::min<int64_t>(chunks, 32)); ++s) {
-            const int64_t per = (chunks + s - 1) / s;
-            if ((chunks + per - 1) / per != s && s != fewest) continue;
-            const int64_t splits = (chunks + per - 1) / per, wgs = tm * tn * splits;
-            const int64_t slots = (int64_t)kCus * t.per_cu;
+        for (int64_t s = fewest; s <= std::max(fewest, std::min<int64_t>(chunks, 32)); ++s) {
+            const int64_t per = (chunks + s - 1) / s, splits = (chunks + per - 1) / per;
+            if (splits != s && s != fewest) continue;
+            const int64_t wgs = tm * tn * splits, slots = (int64_t)kCus * t.per_cu;
             auto round = [&](int64_t n) {
-                return (double)per * (t.alone + (double)(n - 1) * t.more) + 3 +
-                       (double)n * t.bm * t.bn * 1.5e-4;
+                return (double)per * (t.alone + (double)(n - 1) * t.more) + t.fixed * (0.4 + 0.6 * (double)n);
             };
             double us = (double)(wgs / slots) * round(t.per_cu);
             if (wgs % slots) us += round((wgs % slots + kCus - 1) / kCus);
-            if (splits > 1) us += 4 + (double)(splits + 1) * (double)M * (double)cols * 1.2e-6;
+            if (splits > 1) us += 4 + (double)(2 * splits + 1) * (double)M * (double)cols * 0.9e-6;
             if (least == 0 || us < least) {
                 least = us;
-                best = {false, t.bm, t.bn, (int)splits, (int)(per * 128), wgs, tn * t.bn,
-                        splits > 1 ? (size_t)(splits * M) * (size_t)(tn * t.bn) : 0};
+                best = {TILES, t.bm, t.bn, (int)splits, (int)(per * 128), wgs, tn * t.bn,
+                        splits > 1 ? (size_t)(splits * M) * (size_t)(tn * t.bn) * 4 : 0};
             }
             if (wgs >= 4 * slots) break;
         }
@@ -65,58 +76,102 @@ Q8Plan q8_plan(int64_t M, int64_t cols, int64_t K) {
 }
 int64_t launch_cols(int64_t n, bool gated) { return gated ? (n + 31) / 32 * 64 : n; }
 
-// Rows on multiples of 16 bytes.
-bool aligned16(const int8_t* p, int64_t stride, int64_t rows) {
-    return ((uintptr_t)p & 15) == 0 && (rows <= 1 || (stride & 15) == 0);
+// Rows on multiples of `bytes`.
+bool on(int bytes, const mt_rows_q8* r) {
+    return r->cols == 0 || (((uintptr_t)r->q % bytes) == 0 && (r->rows <= 1 || r->row_stride % bytes == 0));
+}
+// Whether the tiles take the rows as they lie.
+bool in_place(const mt_rows_q8* r) { return on(16, r) && (r->rows <= 1 || r->row_stride <= kMaxRow); }
+int64_t padded(int64_t k) { return (k + 15) / 16 * 16; }
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+// The workspace: the splits' sums, then rows of x and of the weight that do not lie as the
+// tiles take them.
+struct Q8Space {
+    size_t x, w, all;
+};
+Q8Space q8_space(const Q8Plan& plan, const mt_rows_q8* X, const mt_rows_q8* W) {
+    Q8Space s{};
+    if (plan.kind != TILES) return s;
+    s.x = round16(plan.partials);
+    s.w = s.x + (in_place(X) ? 0 : (size_t)(X->rows * padded(X->cols)));
+    s.all = s.w + (in_place(W) ? 0 : (size_t)(W->rows * padded(W->cols)));
+    if (s.all) s.all += 15;           // (from any address)
+    return s;
 }
 
 template <bool GATED>
-void launch_few(const Q8Params& p, hipStream_t s) {
+void launch_few(const Q8Params& p, bool words, hipStream_t s) {
     using std::integral_constant;
-    auto go = [&](auto mb, auto nc) {
-        constexpr int F = GATED ? 8 * nc() : 16 * nc();
-        hipLaunchKernelGGL((q8_few<mb(), nc(), GATED>), dim3((unsigned)((p.N + F - 1) / F)), dim3(512),
-                           0, s, p);
+    auto go = [&](auto mb, auto kind) {
+        constexpr int NC = GATED ? 2 : 1, F = 16;
+        const dim3 grid((unsigned)((p.N + F - 1) / F));
+        hipLaunchKernelGGL((q8_few<mb(), NC, GATED, kind()>), grid, dim3(512), 0, s, p);
     };
-    if constexpr (GATED) {
-        if (p.M <= 16) go(integral_constant<int, 1>{}, integral_constant<int, 2>{});
-        else go(integral_constant<int, 2>{}, integral_constant<int, 2>{});
-    } else {
-        if (p.M <= 16) go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-        else go(integral_constant<int, 2>{}, integral_constant<int, 1>{});
-    }
+    auto rows = [&](auto kind) {
+        if (p.M <= 16) go(integral_constant<int, 1>{}, kind);
+        else go(integral_constant<int, 2>{}, kind);
+    };
+    if (words) rows(integral_constant<int, Q8_WORDS>{});
+    else rows(integral_constant<int, Q8_BYTES>{});
 }
-template <bool GATED, bool DMA>
+template <bool GATED>
 void launch_tiles(const Q8Params& p, const Q8Plan& plan, hipStream_t s) {
     const dim3 grid((unsigned)plan.tiles);
     if (plan.bm == 64)
-        hipLaunchKernelGGL((q8_gemm<64, 128, 32, 128, 2, DMA, GATED>), grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL((q8_gemm<64, 128, 32, 64, 64, 5, GATED>), grid, dim3(256), 0, s, p);
+    else if (plan.bm == 128 && plan.bn == 128)
+        hipLaunchKernelGGL((q8_gemm<128, 128, 64, 64, 64, 5, GATED>), grid, dim3(256), 0, s, p);
     else if (plan.bm == 128)
-        hipLaunchKernelGGL((q8_gemm<128, 128, 64, 128, 2, DMA, GATED>), grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL((q8_gemm<128, 256, 64, 64, 128, 2, GATED>), grid, dim3(512), 0, s, p);
     else
-        hipLaunchKernelGGL((q8_gemm<256, 256, 128, 128, 2, DMA, GATED>), grid, dim3(512), 0, s, p);
+        hipLaunchKernelGGL((q8_gemm<256, 256, 64, 128, 128, 2, GATED>), grid, dim3(512), 0, s, p);
 }
 
 template <bool GATED>
-int run_q8(Q8Params& p, void* workspace, size_t ws_bytes, hipStream_t s) {
+int run_q8(Q8Params& p, const mt_rows_q8* X, const mt_rows_q8* W, void* workspace, size_t ws_bytes,
+           hipStream_t s) {
     const Q8Plan plan = q8_plan(p.M, launch_cols(p.N, GATED), p.K);
-    if (plan.few) {
-        p.splits = 1;
-        launch_few<GATED>(p, s);
+    p.splits = 1;
+    if (plan.kind == FEW) {
+        launch_few<GATED>(p, on(4, X) && on(4, W), s);
+        return launched();
+    }
+    if (plan.kind == LONG) {
+        const int64_t blocks = ((int64_t)p.M + 15) / 16 * (((int64_t)p.N + 15) / 16);
+        if (blocks >= kMaxTiles) return MT_ERR_INVALID;
+        hipLaunchKernelGGL((q8_few<1, GATED ? 2 : 1, GATED, Q8_LONG>), dim3((unsigned)blocks), dim3(512),
+                           0, s, p);
         return launched();
     }
     if (plan.tiles >= kMaxTiles) return MT_ERR_INVALID;
-    const size_t need = plan.partials * 4;
-    if (need > 0 && (!workspace || ws_bytes < need || ((uintptr_t)workspace & 3)))
-        return MT_ERR_WORKSPACE;
+    const Q8Space space = q8_space(plan, X, W);
+    if (space.all > 0 && (!workspace || ws_bytes < space.all)) return MT_ERR_WORKSPACE;
+    char* const ws = reinterpret_cast<char*>(round16((uintptr_t)workspace));
+    Q8Align a{};
+    a.ld_dst = padded(p.K);
+    a.K = p.K;
+    auto align = [&](int i, const mt_rows_q8* r, size_t at, const int8_t*& q, int64_t& ld) {
+        if (in_place(r)) return;
+        a.src[i] = r->q;
+        a.ld[i] = r->row_stride;
+        a.rows[i] = r->rows;
+        a.dst[i] = reinterpret_cast<int8_t*>(ws + at);
+        q = a.dst[i];
+        ld = padded(p.K);
+    };
+    align(0, X, space.x, p.x, p.x_m);
+    align(1, W, space.w, p.w, p.w_n);
+    if (const int64_t n = a.rows[0] + a.rows[1]; n > 0) {
+        a.wave_blocks = p.K >= 16 ? (int)std::min<int64_t>((n + 3) / 4, 1 << 16) : 0;
+        const int64_t parts = p.K % 16 ? std::min<int64_t>((n + 255) / 256, 1 << 12) : 0;
+        hipLaunchKernelGGL(q8_align_rows<>, dim3((unsigned)(a.wave_blocks + parts)), dim3(256), 0, s, a);
+    }
     p.splits = plan.splits;
     p.k_per_split = plan.k_per_split;
-    p.part = static_cast<int32_t*>(workspace);
+    p.part = reinterpret_cast<int32_t*>(ws);
     p.part_n = plan.part_n;
-    if (aligned16(p.x, p.x_m, p.M) && aligned16(p.w, p.w_n, GATED ? 2 * (int64_t)p.N : p.N))
-        launch_tiles<GATED, true>(p, plan, s);
-    else
-        launch_tiles<GATED, false>(p, plan, s);
+    launch_tiles<GATED>(p, plan, s);
     if (plan.splits > 1) {
         const int64_t n = (int64_t)p.M * ((p.N + 3) / 4);
         hipLaunchKernelGGL(q8_sum<GATED>, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 8192)),
@@ -142,18 +197,18 @@ Q8Params q8_params(const mt_rows_q8* X, const mt_rows_q8* W, const float* bias, 
     p.K = (int)X->cols;
     return p;
 }
-size_t workspace_of(int64_t rows, int64_t in_f, int64_t out_f, bool gated) {
-    if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxDim ||
-        out_f >= (gated ? kMaxDim / 2 : kMaxDim))
+size_t workspace_of(const mt_rows_q8* X, const mt_rows_q8* W, bool gated) {
+    if (!valid(X) || !valid(W) || X->cols != W->cols || X->rows == 0 || W->rows < (gated ? 2 : 1))
         return 0;
-    return q8_plan(rows, launch_cols(out_f, gated), in_f).partials * 4;
+    const Q8Plan plan = q8_plan(X->rows, launch_cols(gated ? W->rows / 2 : W->rows, gated), X->cols);
+    return q8_space(plan, X, W).all;
 }
-int plan_of(int64_t rows, int64_t in_f, int64_t out_f, bool gated, mt_lowbit_plan* plan) {
+int plan_of(int64_t rows, int64_t in_f, int64_t out_f, bool gated, mt_q8_plan* plan) {
     if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxDim ||
         out_f >= (gated ? kMaxDim / 2 : kMaxDim) || !plan)
         return MT_ERR_INVALID;
     const Q8Plan p = q8_plan(rows, launch_cols(out_f, gated), in_f);
-    *plan = {p.bm, p.splits, p.few ? 1 : 0};
+    *plan = {p.bm, p.bn, p.splits};
     return MT_OK;
 }
 
@@ -168,13 +223,13 @@ int mt_linear_q8(const mt_rows_q8* X, const mt_rows_q8* W, const float* bias, in
         return MT_ERR_INVALID;
     if (Y->rows == 0 || Y->cols == 0) return MT_OK;
     Q8Params p = q8_params(X, W, bias, bias_stride, Y);
-    return run_q8<false>(p, workspace, ws_bytes, static_cast<hipStream_t>(stream));
+    return run_q8<false>(p, X, W, workspace, ws_bytes, static_cast<hipStream_t>(stream));
 }
 
-size_t mt_linear_q8_workspace(int64_t rows, int64_t in_f, int64_t out_f) {
-    return workspace_of(rows, in_f, out_f, false);
+size_t mt_linear_q8_workspace(const mt_rows_q8* X, const mt_rows_q8* W) {
+    return workspace_of(X, W, false);
 }
-int mt_linear_q8_plan(int64_t rows, int64_t in_f, int64_t out_f, mt_lowbit_plan* plan) {
+int mt_linear_q8_plan(int64_t rows, int64_t in_f, int64_t out_f, mt_q8_plan* plan) {
     return plan_of(rows, in_f, out_f, false, plan);
 }
 
@@ -190,13 +245,13 @@ int mt_gated_linear_q8(const mt_rows_q8* X, const mt_rows_q8* W, const float* bi
     Q8Params p = q8_params(X, W, bias, bias_stride, H);
     p.gu = view(GU);
     p.act = act;
-    return run_q8<true>(p, workspace, ws_bytes, static_cast<hipStream_t>(stream));
+    return run_q8<true>(p, X, W, workspace, ws_bytes, static_cast<hipStream_t>(stream));
 }
 
-size_t mt_gated_linear_q8_workspace(int64_t rows, int64_t in_f, int64_t features) {
-    return workspace_of(rows, in_f, features, true);
+size_t mt_gated_linear_q8_workspace(const mt_rows_q8* X, const mt_rows_q8* W) {
+    return workspace_of(X, W, true);
 }
-int mt_gated_linear_q8_plan(int64_t rows, int64_t in_f, int64_t features, mt_lowbit_plan* plan) {
+int mt_gated_linear_q8_plan(int64_t rows, int64_t in_f, int64_t features, mt_q8_plan* plan) {
     return plan_of(rows, in_f, features, true, plan);
 }
 

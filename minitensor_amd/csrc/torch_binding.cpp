@@ -540,7 +540,7 @@ py::object linear_q8(py::handle pq, py::handle pscale, py::handle pw, py::handle
         if (!out.defined()) out = empty({rows, n}, q);
         const mt_rows_q8 mx = rows_q8(q, scale), mw = rows_q8(w, wscale);
         const mt_mat_f32 my = mat(out);
-        const Workspace ws(gws, q, [&] { return mt_linear_q8_workspace(rows, k, n); });
+        const Workspace ws(gws, q, [&] { return mt_linear_q8_workspace(&mx, &mw); });
         check(mt_linear_q8(&mx, &mw, ptr(b), step(b), &my, ws.p, ws.n, s), "mt_linear_q8");
     }
     return pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout);
@@ -579,13 +579,17 @@ py::object gated_linear(py::handle px, py::handle pxscale, py::handle pw, py::ha
         mt_mat_f32 mg{};
         if (keep) mg = mat(gu);
         const mt_mat_f32 mh = mat(out);
+        mt_rows_q8 qx{}, qw{};
+        if (q8) {
+            qx = rows_q8(x, xscale);
+            qw = rows_q8(w, wscale);
+        }
         const Workspace ws(gws, x, [&] {
-            return q8 ? mt_gated_linear_q8_workspace(rows, k, f)
+            return q8 ? mt_gated_linear_q8_workspace(&qx, &qw)
                       : mt_gated_linear_workspace_f32(rows, k, f);
         });
         if (q8) {
-            const mt_rows_q8 mx = rows_q8(x, xscale), mw = rows_q8(w, wscale);
-            check(mt_gated_linear_q8(&mx, &mw, ptr(b), step(b), act, &mh, keep ? &mg : nullptr, ws.p,
+            check(mt_gated_linear_q8(&qx, &qw, ptr(b), step(b), act, &mh, keep ? &mg : nullptr, ws.p,
                                      ws.n, s),
                   "mt_gated_linear_q8");
         } else {

@@ -22,7 +22,7 @@ import torch
 
 from . import (MatF32, _api, _check, _handle, _nbytes, _ptr, _require_gpu, _stream, lib,
                linear_backward, mat, native)
-from .lowbit import (LowbitPlan, Q8Rows, RowsQ8, _empty, _matrix, _rows, _vector, _ws,
+from .lowbit import (Q8Plan, Q8Rows, RowsQ8, _empty, _matrix, _rows, _vector, _ws,
                      linear_backward_q8)
 
 ACTIVATIONS = ("silu", "gelu", "gelu_tanh", "relu", "sigmoid")   # mt_activation
@@ -41,8 +41,8 @@ SIGS = {
     "mt_gated_linear_f32": (_I, [_M, _M, _V, _I64, _I, _M, _M, _V, _S, _V]),
     "mt_gated_linear_workspace_f32": (_S, [_I64] * 3),
     "mt_gated_linear_q8": (_I, [_Q, _Q, _V, _I64, _I, _M, _M, _V, _S, _V]),
-    "mt_gated_linear_q8_workspace": (_S, [_I64] * 3),
-    "mt_gated_linear_q8_plan": (_I, [_I64] * 3 + [_P(LowbitPlan)]),
+    "mt_gated_linear_q8_workspace": (_S, [_Q, _Q]),
+    "mt_gated_linear_q8_plan": (_I, [_I64] * 3 + [_P(Q8Plan)]),
     "mt_gate_f32": (_I, [_M, _I, _M, _V]),
     "mt_gate_backward_f32": (_I, [_M, _M, _I, _M, _V]),
     "mt_grad_norm_f32": (_I, [_M, _I64, _V, _V, _S, _V]),
@@ -109,7 +109,8 @@ def gated_linear(x: Union[torch.Tensor, Q8Rows], w: Union[torch.Tensor, Q8Rows],
     if out is None:
         out = _empty((n, f), like)
     gu = _empty((n, f2), like) if keep else None
-    need = (lib().mt_gated_linear_q8_workspace if q8 else lib().mt_gated_linear_workspace_f32)(n, k, f)
+    need = (lib().mt_gated_linear_q8_workspace(ctypes.byref(xd), ctypes.byref(wd)) if q8 else
+            lib().mt_gated_linear_workspace_f32(n, k, f))
     ws = _ws(ws, need, like)
     fn, name = ((lib().mt_gated_linear_q8, "mt_gated_linear_q8") if q8 else
                 (lib().mt_gated_linear_f32, "mt_gated_linear_f32"))

@@ -67,6 +67,11 @@ class LowbitPlan(ctypes.Structure):
                 ("column_blocks", ctypes.c_int32)]
 
 
+class Q8Plan(ctypes.Structure):
+    _fields_ = [("tile_rows", ctypes.c_int32), ("tile_cols", ctypes.c_int32),
+                ("splits", ctypes.c_int32)]
+
+
 _P, _V, _I64, _F = ctypes.POINTER, ctypes.c_void_p, ctypes.c_int64, ctypes.c_float
 _M, _Q, _W = _P(MatF32), _P(RowsQ8), _P(WeightQ4)
 SIGS = {
@@ -85,8 +90,8 @@ SIGS = {
     "mt_linear_q4_q8": (ctypes.c_int, [_Q, _W, _V, _I64, _M, _V, ctypes.c_size_t, _V]),
     "mt_linear_q4_workspace": (ctypes.c_size_t, [_I64] * 3),
     "mt_linear_q8": (ctypes.c_int, [_Q, _Q, _V, _I64, _M, _V, ctypes.c_size_t, _V]),
-    "mt_linear_q8_workspace": (ctypes.c_size_t, [_I64] * 3),
-    "mt_linear_q8_plan": (ctypes.c_int, [_I64] * 3 + [_P(LowbitPlan)]),
+    "mt_linear_q8_workspace": (ctypes.c_size_t, [_Q, _Q]),
+    "mt_linear_q8_plan": (ctypes.c_int, [_I64] * 3 + [_P(Q8Plan)]),
     "mt_linear_q4_plan": (ctypes.c_int, [_I64] * 3 + [ctypes.c_int] * 2 + [_P(LowbitPlan)]),
     "mt_linear_backward_q8_plan": (ctypes.c_int, [_I64] * 3 + [_P(LowbitPlan)]),
 }
@@ -375,7 +380,7 @@ def linear_q8(x: Q8Rows, w: Q8Rows, b: Optional[torch.Tensor] = None,
     if out is None:
         out = _empty((xd.rows, wd.rows), x[0])
     y = _matrix(out, (xd.rows, wd.rows), "linear_q8: out")
-    ws = _ws(ws, lib().mt_linear_q8_workspace(xd.rows, xd.cols, wd.rows), x[0])
+    ws = _ws(ws, lib().mt_linear_q8_workspace(ctypes.byref(xd), ctypes.byref(wd)), x[0])
     rc = lib().mt_linear_q8(ctypes.byref(xd), ctypes.byref(wd), bp, bs, y, _ptr(ws), _nbytes(ws),
                             _stream(stream))
     _check(rc, "mt_linear_q8")

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 import minitensor_amd as mt
-from minitensor_amd.lowbit import LowbitPlan, RowsQ8
+from minitensor_amd.lowbit import Q8Plan, RowsQ8
 
 OK, INVALID, WORKSPACE = mt.MT_OK, mt.MT_ERR_INVALID, mt.MT_ERR_WORKSPACE
 
@@ -23,11 +23,11 @@ def R(x):
 
 
 def plan_q8(m, k, n, gated=False):
-    """(rows of a tile or 0, splits) that linear_q8 (gated_linear of 8-bit rows) takes."""
-    p = LowbitPlan()
+    """(rows and columns of a tile or 0, splits) that linear_q8 (gated_linear of 8-bit rows) takes."""
+    p = Q8Plan()
     f = mt.lib().mt_gated_linear_q8_plan if gated else mt.lib().mt_linear_q8_plan
     assert f(m, k, n, R(p)) == OK
-    return p.tile_rows, p.splits
+    return (p.tile_rows, p.tile_cols), p.splits
 
 
 def test_linear_q8_refuses():
@@ -112,11 +112,20 @@ def test_clip_refuses():
 
 def test_queries():
     lib = mt.lib()
-    for f in (lib.mt_linear_q8_workspace, lib.mt_gated_linear_q8_workspace, lib.mt_gated_linear_workspace_f32):
-        assert f(0, 8, 8) == 0 and f(-1, 8, 8) == 0 and f(1 << 31, 8, 8) == 0
+    f = lib.mt_gated_linear_workspace_f32
+    assert f(0, 8, 8) == 0 and f(-1, 8, 8) == 0 and f(1 << 31, 8, 8) == 0
+    for f in (lib.mt_linear_q8_workspace, lib.mt_gated_linear_q8_workspace):
+        assert f(R(Q(0, 8)), R(Q(8, 8))) == 0 and f(R(Q(8, 8)), R(Q(0, 8))) == 0
+        assert f(R(Q(8, 8)), R(Q(8, 9))) == 0 and f(None, R(Q(8, 8))) == 0
+        # rows that lie as the tiles take them need none, others a copy
+        assert f(R(Q(100, 64)), R(Q(96, 64))) == 0
+        assert 100 * 64 <= f(R(Q(100, 63)), R(Q(96, 63, rs=64))) < 100 * 64 + 32
+        assert 196 * 64 <= f(R(Q(100, 64, q=0x1008)), R(Q(96, 64, rs=72))) < 196 * 64 + 32
+        assert 96 * 64 <= f(R(Q(100, 64)), R(Q(96, 64, rs=1 << 24))) < 96 * 64 + 32
+        assert f(R(Q(32, 63)), R(Q(96, 63))) == 0
     assert lib.mt_grad_norm_workspace_f32(-1) == 0
     assert 0 < lib.mt_grad_norm_workspace_f32(1) <= lib.mt_grad_norm_workspace_f32(1000)
-    p = LowbitPlan()
+    p = Q8Plan()
     assert lib.mt_linear_q8_plan(4, 8, 8, None) == INVALID
     assert lib.mt_linear_q8_plan(0, 8, 8, R(p)) == INVALID
 
@@ -125,14 +134,14 @@ def test_queries():
 def test_q8_plans(gated):
     """Few rows on their kernel, up to the inputs that its sums hold; a split never holds more
     terms than 32 bits do; workspaces of whole tiles."""
-    assert plan_q8(1, 4096, 4096, gated)[0] == 0
-    assert plan_q8(2048, 4096, 8192, gated)[0] == 256
+    assert plan_q8(1, 4096, 4096, gated)[0] == (0, 0)
+    assert plan_q8(2048, 4096, 8192, gated)[0] == (256, 256)
     for m in (1, 40, 300):
         for k in (1, 131071, 200000, 1 << 20, 1 << 27):
             tile, splits = plan_q8(m, k, 100, gated)
-            assert tile == 0 and k < 1 << 19 or splits * ((1 << 17) - 128) >= k
+            assert tile == (0, 0) and (k < 1 << 19 or k > 1 << 24) or splits * ((1 << 17) - 128) >= k
             f = mt.lib().mt_gated_linear_q8_workspace if gated else mt.lib().mt_linear_q8_workspace
-            ws = f(m, k, 100)
+            ws = f(R(Q(m, k, rs=(k + 15) // 16 * 16)), R(Q(200 if gated else 100, k, rs=(k + 15) // 16 * 16)))
             assert (ws > 0) == (splits > 1)
             if splits > 1:
                 assert ws >= 4 * splits * m * 100 * (1 + gated)

@@ -96,14 +96,15 @@ def test_linear_q8(dev, m, n, k):
 
 
 # ... and outputs large enough for the larger tiles
-Q8_LARGE = [(2048, 2048, 256), (1900, 4000, 200), (2000, 8190, 300), (2048, 8192, 256)]
+Q8_LARGE = [(1000, 4000, 1100), (1900, 4000, 200), (2000, 8190, 300), (2048, 8192, 256)]
 
 
 def test_linear_q8_kernels():
     """Which sizes take which kernel, so that the tests here reach all of them."""
     from test_ffn_capi import plan_q8
     plans = [plan_q8(m, k, n) for m, n, k in Q8_SIZES + Q8_LARGE]
-    assert {p[0] for p in plans} == {0, 64, 128, 256}, plans
+    tiles = {(0, 0), (64, 128), (128, 128), (128, 256), (256, 256)}
+    assert {p[0] for p in plans} == tiles, plans
     assert any(p[1] > 1 for p in plans)
 
 
@@ -131,6 +132,26 @@ def test_linear_q8_sums_past_32_bits(dev, m, k):
     y = cpu(mt.linear_q8(mt.Q8Rows(q, one), mt.Q8Rows(w, torch.ones(5, device=dev))))
     want = np.array([k * 16384, k * -128 * 127] + [k * 16384] * 3, np.float64)
     assert np.array_equal(y, np.broadcast_to(want.astype(np.float32), (m, 5)))
+
+
+def test_linear_q8_long_rows(dev):
+    """Rows of 2^24 inputs and more, and rows that far apart: neither goes to the tiles as it is."""
+    k = (1 << 24) + 77
+    q = torch.full((35, k), -128, dtype=torch.int8, device=dev)
+    w = torch.full((3, k), 127, dtype=torch.int8, device=dev)
+    q[33, -1] = 5
+    y = cpu(mt.linear_q8(mt.Q8Rows(q, torch.ones(35, device=dev)), mt.Q8Rows(w, torch.ones(3, device=dev))))
+    want = np.full((35, 3), -128.0 * 127 * k)
+    want[33] += 127 * 133
+    assert np.array_equal(y, want.astype(np.float32))
+    g = rng(31)
+    codes, s = g.integers(-128, 128, (35, 100)).astype(np.int8), g.random(35).astype(np.float32)
+    far = q.flatten()[:35 * (1 << 24)].view(35, 1 << 24)[:, :100]
+    far.copy_(gpu(codes, dev))
+    wq, ws, wt = rows8(g, 64, 100, dev)
+    check(mt.linear_q8(mt.Q8Rows(far, gpu(s, dev)), wt), *ref.linear_q8(codes, s, wq, ws))
+    gu, e = ref.linear_q8(codes, s / 256, wq, ws)
+    check(mt.gated_linear(mt.Q8Rows(far, gpu(s / 256, dev)), wt).h, *ref.gate("silu", gu, e))
 
 
 def test_linear_q8_same_for_any_tile(dev):
