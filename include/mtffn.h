@@ -37,12 +37,17 @@ typedef enum mt_activation {
 int mt_gated_linear_f32(const mt_mat_f32* X, const mt_mat_f32* W, const float* bias,
                         int64_t bias_stride, int act, const mt_mat_f32* H, const mt_mat_f32* GU,
                         void* workspace, size_t ws_bytes, void* stream);
-size_t mt_gated_linear_workspace_f32(int64_t rows, int64_t in_features, int64_t features);
+size_t mt_gated_linear_workspace_f32(const mt_mat_f32* X, const mt_mat_f32* W);
 int mt_gated_linear_q8(const mt_rows_q8* X, const mt_rows_q8* W, const float* bias,
                        int64_t bias_stride, int act, const mt_mat_f32* H, const mt_mat_f32* GU,
                        void* workspace, size_t ws_bytes, void* stream);
 size_t mt_gated_linear_q8_workspace(const mt_rows_q8* X, const mt_rows_q8* W);
-/* The kernel that a call takes (as mt_linear_q8_plan). */
+/* The kernel that a call takes (as mt_linear_q8_plan); in fp32: kind 0 few rows, 1 tiles, 2 the
+ * product first, then the gate (operands with no unit stride, no inputs). */
+typedef struct mt_gate_plan {
+    int32_t kind, tile_rows, tile_cols, splits;
+} mt_gate_plan;
+int mt_gated_linear_plan_f32(const mt_mat_f32* X, const mt_mat_f32* W, mt_gate_plan* plan);
 int mt_gated_linear_q8_plan(int64_t rows, int64_t in_features, int64_t features, mt_q8_plan* plan);
 
 /* H = act(GU[:, :F]) * GU[:, F:] of projections that are there already, and the gradient

@@ -34,6 +34,7 @@ COMMON = [
 ]
 
 N_CFG = 3      # register-staged tile configurations (TileCfg)
+GATE_CFG = (0, 1, 2)             # gated gemm_f32_sp tiles (GateCfg)
 SP_CFG = (0, 1, 2, 3, 4, 6, 7)   # gemm_f32_sp tile configurations (SpCfg)
 
 
@@ -43,6 +44,9 @@ def _units():
         units.append((CSRC / "gemm_instances.hip", OBJDIR / f"gemm_cfg{cfg}.o", [f"-DMT_CFG={cfg}"]))
     for cfg in SP_CFG:
         units.append((CSRC / "gemm_sp_instances.hip", OBJDIR / f"gemm_sp_cfg{cfg}.o",
+                      [f"-DMT_CFG={cfg}"]))
+    for cfg in GATE_CFG:
+        units.append((CSRC / "gemm_gate_instances.hip", OBJDIR / f"gemm_gate_cfg{cfg}.o",
                       [f"-DMT_CFG={cfg}"]))
     units.append((CSRC / "gemm_dl_instances.hip", OBJDIR / "gemm_dl.o", []))
     units.append((CSRC / "gemm_dlp_instances.hip", OBJDIR / "gemm_dlp.o", []))

@@ -9,7 +9,9 @@
 
 #include "api_checks.hpp"
 #include "clip_kernel.hpp"
+#include "gate_f32_kernel.hpp"
 #include "gate_kernel.hpp"
+#include "gemm_configs.hpp"
 #include "mtffn.h"
 
 using namespace mtk;
@@ -29,6 +31,167 @@ int run_gate(const mt_mat_f32* GU, const mt_mat_f32* dH, const mt_mat_f32* out, 
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (units) hipLaunchKernelGGL((gate_rows<true, BACK>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((gate_rows<false, BACK>), grid, dim3(256), 0, s, p);
+    return launched();
+}
+
+// ---- gated projections in fp32 ---------------------------------------------------------
+
+// How a call goes: few rows (the vector units, the fp32 matrix units), tiles of gemm_f32_sp with the gate in their
+// epilogue, or (operands with no neighbouring elements either way, or too far apart for the
+// tiles' 32-bit offsets) the product to memory first.
+enum GateKind { GATE_FEW, GATE_TILES, GATE_APART };
+constexpr int64_t kGemvRows = 4, kFewRows = 48;
+
+// Times in us by workgroups on a CU, of a chunk of 16 inputs -- one workgroup on every fourth
+// CU or fewer, on every CU, each further one there -- and of a workgroup's beginning and end.
+// From products of 64-4096 rows, 512-4096 features, 256 and 2048 inputs.  (4096 x 2048 ->
+// 2 x 4096: 128x256 687 us, 128x128 748, 64x128 1072; 1024 x 2048 -> 2 x 2048: 135, 104, 125;
+// 256 x 2048 -> 2 x 2048: 114, 78, 67.)
+struct GateTile {
+    int bm, bn, per_cu;
+    double sparse, full, more, fixed;
+    GemmLaunchFn (*launcher)(int, int);
+};
+template <int C>
+constexpr GateTile gate_tile(int per_cu, double sparse, double full, double more, double fixed,
+                             GemmLaunchFn (*fn)(int, int)) {
+    return {GateCfg<C>::BM, GateCfg<C>::BN, per_cu, sparse, full, more, fixed, fn};
+}
+constexpr GateTile kGateTiles[kNumGateCfg] = {
+    gate_tile<0>(3, 0.45, 0.515, 0.40, 4, gate_launcher_cfg0),
+    gate_tile<1>(2, 0.52, 0.73, 0.65, 6.5, gate_launcher_cfg1),
+    gate_tile<2>(1, 0.79, 1.27, 0, 8, gate_launcher_cfg2)};
+
+struct GatePlan {
+    GateKind kind;
+    int tile, tiles_m, tiles_n, splits, k_per_split;
+    size_t partials;                  // bytes, 0 without splits
+};
+GatePlan gate_tiles_plan(int64_t M, int64_t F, int64_t K) {
+    GatePlan best{};
+    double least = 0;
+    const int64_t cols = (F + 31) / 32 * 64, chunks = (K + 15) / 16;
+    for (int i = 0; i < kNumGateCfg; ++i) {
+        const GateTile& t = kGateTiles[i];
+        const int64_t tm = (M + t.bm - 1) / t.bm, tn = (cols + t.bn - 1) / t.bn;
+        for (int64_t s = 1; s <= std::min<int64_t>(std::max<int64_t>(chunks / 4, 1), 32); ++s) {
+            const int64_t per = (chunks + s - 1) / s;
+            if ((chunks + per - 1) / per != s) continue;
+            const int64_t wgs = tm * tn * s, slots = (int64_t)kCus * t.per_cu;
+            const double fill = std::min(1.0, (double)wgs / kCus);
+            auto round = [&](int64_t n) {
+                const double one = t.sparse + (t.full - t.sparse) * std::max(0.0, (fill - 0.25) / 0.75);
+                return (double)per * (one + (double)(n - 1) * t.more) + t.fixed;
+            };
+            double us = (double)(wgs / slots) * round(t.per_cu);
+            if (wgs % slots) us += round((wgs % slots + kCus - 1) / kCus);
+            if (s > 1) us += 4 + (double)(s + 1) * (double)M * (double)cols * 0.9e-6;
+            if (least == 0 || us < least) {
+                least = us;
+                best = {GATE_TILES, i, (int)tm, (int)tn, (int)s, (int)(per * 16),
+                        s > 1 ? (size_t)(s * M * cols) * 4 : 0};
+            }
+            if (wgs >= 4 * slots) break;
+        }
+    }
+    return best;
+}
+// The layout in which the tiles read an operand (rows of a tile at most `rows`, the last of
+// them `span` rows from the first), or -1.
+int gate_layout(const RowView& v, int64_t K, int64_t span, bool weight) {
+    if ((v.cs == 1 || K == 1) && span * v.rs < ((int64_t)1 << 30) - 16) return weight ? L_GKV : L_KV;
+    if (v.rs == 1 && span < ((int64_t)1 << 30)) return weight ? L_GMV : L_MV;
+    return -1;
+}
+// Whether the kernels of few rows take a product, whose waves walk all of K and read x for 16
+// features each.  (Against the tiles, us: 16 rows 2048 -> 2 x 4096 14 and 23, 32 rows 19 and 24,
+// 48 rows 25 and 26, 500 -> 2 x 1000 8 and 11; but 4096 -> 2 x 8192 32 rows 67 and 62, 48 rows 95
+// and 69, 8192 -> 2 x 512 8 rows 38 and 19, and 5632 -> 2 x 2048 16 rows 32 and 35, 32 rows 42
+// and 35.)
+bool few_rows(int64_t M, int64_t F, int64_t K) {
+    if (M <= kGemvRows) return true;
+    return M <= 16 ? K <= 4 * F : M <= kFewRows && K <= F && F * K <= (int64_t)12 << 20;
+}
+GatePlan gate_plan(const mt_mat_f32* X, const mt_mat_f32* W, int* la, int* lb) {
+    const int64_t M = X->rows, F = W->rows / 2, K = X->cols;
+    const RowView x = view(X), w = view(W);
+    if (K > 0 && (x.cs == 1 || K == 1) && (w.cs == 1 || K == 1) && few_rows(M, F, K)) return {GATE_FEW};
+    // (a tile's rows; of the weight those of 128 features, and their up rows)
+    *la = gate_layout(x, K, std::min<int64_t>(M, 256), false);
+    *lb = gate_layout(w, K, F + std::min<int64_t>(F, 128), true);
+    if (K == 0 || *la < 0 || *lb < 0) return {GATE_APART};
+    const GatePlan p = gate_tiles_plan(M, F, K);
+    if ((int64_t)p.tiles_m * p.tiles_n * p.splits >= kMaxTiles) return {GATE_APART};
+    return p;
+}
+size_t apart_bytes(const mt_mat_f32* X, const mt_mat_f32* W) {
+    return (size_t)X->rows * (size_t)W->rows * 4;
+}
+
+int run_gated(const mt_mat_f32* X, const mt_mat_f32* W, const float* bias, int64_t bias_stride,
+              int act, const mt_mat_f32* H, const mt_mat_f32* GU, void* workspace, size_t ws_bytes,
+              hipStream_t s) {
+    int la = -1, lb = -1;
+    const GatePlan plan = gate_plan(X, W, &la, &lb);
+    const RowView x = view(X), w = view(W), h = view(H), gu = view(GU);
+    const int M = (int)X->rows, F = (int)H->cols, K = (int)X->cols;
+    if (plan.kind == GATE_FEW) {
+        const GateGemv p{x.p, x.rs, w.p, w.rs, bias, bias_stride, h, gu, M, F, K, act};
+        const auto blocks = [&](int features) { return dim3((unsigned)((F + features - 1) / features)); };
+        if (M == 1) hipLaunchKernelGGL((gate_gemv<1, 4>), blocks(4), dim3(512), 0, s, p);
+        else if (M == 2) hipLaunchKernelGGL((gate_gemv<2, 4>), blocks(4), dim3(512), 0, s, p);
+        else if (M <= kGemvRows) hipLaunchKernelGGL((gate_gemv<4, 4>), blocks(4), dim3(512), 0, s, p);
+        else if (M <= 16) hipLaunchKernelGGL(gate_few<1>, blocks(16), dim3(512), 0, s, p);
+        else if (M <= 32) hipLaunchKernelGGL(gate_few<2>, blocks(16), dim3(512), 0, s, p);
+        else hipLaunchKernelGGL(gate_few<3>, blocks(16), dim3(512), 0, s, p);
+        return launched();
+    }
+    if (plan.kind == GATE_APART) {
+        mt_mat_f32 to;
+        char* ws = static_cast<char*>(workspace);
+        if (GU) {
+            to = *GU;
+        } else {
+            const size_t own = apart_bytes(X, W);
+            if (!ws || ws_bytes < own) return MT_ERR_WORKSPACE;
+            to = mt_mat_f32{reinterpret_cast<float*>(ws), 0, X->rows, W->rows, W->rows, 1, 1, 0};
+            ws += own;
+            ws_bytes -= own;
+        }
+        const int rc = mt_linear_forward_f32(X, W, bias, bias_stride, &to, ws, ws_bytes, s);
+        return rc == MT_OK ? mt_gate_f32(&to, act, H, s) : rc;
+    }
+    if (plan.partials > 0 && (!workspace || ws_bytes < plan.partials)) return MT_ERR_WORKSPACE;
+    GemmParams p{};
+    p.A = x.p;
+    p.a_mn = x.rs;
+    p.a_k = x.cs;
+    p.B = w.p;
+    p.b_mn = w.rs;
+    p.b_k = w.cs;
+    p.M = M;
+    p.N = (F + 31) / 32 * 64;
+    p.K = K;
+    p.batch = 1;
+    p.c_n_inner = p.N;
+    p.bias = bias;
+    p.bias_stride = bias_stride;
+    p.splits = plan.splits;
+    p.k_per_split = plan.k_per_split;
+    p.ws = static_cast<float*>(workspace);
+    p.ws_vec = ((uintptr_t)workspace & 15) == 0;
+    p.tiles_m = plan.tiles_m;
+    p.tiles_n = plan.tiles_n;
+    p.group_m = 4;
+    p.gate = {h.p, h.rs, h.cs, gu.p, gu.rs, gu.cs, F, act};
+    const GemmLaunchFn fn = kGateTiles[plan.tile].launcher(la, lb);
+    hipError_t e = fn(p, (unsigned)(plan.tiles_m * plan.tiles_n * plan.splits), s);
+    if (e != hipSuccess && e != hipErrorStreamCaptureUnsupported) return MT_ERR_HIP;
+    if (plan.splits > 1) {
+        const int64_t n = (int64_t)M * ((F + 3) / 4);
+        hipLaunchKernelGGL(gate_sum<>, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 8192)), dim3(256),
+                           0, s, GateSum{p.ws, p.N, p.splits, bias, bias_stride, h, gu, M, F, act});
+    }
     return launched();
 }
 
@@ -169,11 +332,27 @@ int mt_gate_backward_f32(const mt_mat_f32* dH, const mt_mat_f32* GU, int act, co
     return run_gate<true>(GU, dH, dGU, dH->cols, act, stream);
 }
 
-size_t mt_gated_linear_workspace_f32(int64_t rows, int64_t in_f, int64_t features) {
-    if (rows <= 0 || in_f < 0 || features <= 0 || rows >= kMaxDim || in_f >= kMaxDim ||
-        features >= kMaxDim / 2)
+size_t mt_gated_linear_workspace_f32(const mt_mat_f32* X, const mt_mat_f32* W) {
+    if (!valid(X, false) || !valid(W, false) || X->cols != W->cols || X->rows == 0 || W->rows < 2)
         return 0;
-    return (size_t)rows * (size_t)features * 8 + mt_linear_workspace_f32(rows, in_f, 2 * features);
+    int la, lb;
+    const GatePlan p = gate_plan(X, W, &la, &lb);
+    if (p.kind != GATE_APART) return p.partials;
+    return apart_bytes(X, W) + mt_linear_workspace_f32(X->rows, X->cols, W->rows);
+}
+
+int mt_gated_linear_plan_f32(const mt_mat_f32* X, const mt_mat_f32* W, mt_gate_plan* plan) {
+    if (!valid(X, false) || !valid(W, false) || X->cols != W->cols || X->rows == 0 || W->rows < 2 ||
+        !plan)
+        return MT_ERR_INVALID;
+    int la, lb;
+    const GatePlan p = gate_plan(X, W, &la, &lb);
+    *plan = {p.kind, 0, 0, p.kind == GATE_TILES ? p.splits : 1};
+    if (p.kind == GATE_TILES) {
+        plan->tile_rows = kGateTiles[p.tile].bm;
+        plan->tile_cols = kGateTiles[p.tile].bn;
+    }
+    return MT_OK;
 }
 
 int mt_gated_linear_f32(const mt_mat_f32* X, const mt_mat_f32* W, const float* bias,
@@ -181,23 +360,12 @@ int mt_gated_linear_f32(const mt_mat_f32* X, const mt_mat_f32* W, const float* b
                         void* workspace, size_t ws_bytes, void* stream) {
     if (!valid(X, false) || !valid(W, false) || !valid(H, true) || !valid_act(act) ||
         X->cols != W->cols || W->rows % 2 != 0 || H->rows != X->rows || H->cols != W->rows / 2 ||
-        (bias && bias_stride < 0) ||
+        (bias && bias_stride < 0) || ((uintptr_t)workspace & 3) != 0 ||
         (GU && (!valid(GU, true) || GU->rows != X->rows || GU->cols != W->rows)))
         return MT_ERR_INVALID;
     if (H->rows == 0 || H->cols == 0) return MT_OK;
-    mt_mat_f32 gu;
-    char* ws = static_cast<char*>(workspace);
-    if (GU) {
-        gu = *GU;
-    } else {
-        const size_t own = (size_t)H->rows * (size_t)W->rows * 4;
-        if (!ws || ws_bytes < own) return MT_ERR_WORKSPACE;
-        gu = mt_mat_f32{reinterpret_cast<float*>(ws), 0, H->rows, W->rows, W->rows, 1, 1, 0};
-        ws += own;
-        ws_bytes -= own;
-    }
-    const int rc = mt_linear_forward_f32(X, W, bias, bias_stride, &gu, ws, ws_bytes, stream);
-    return rc == MT_OK ? mt_gate_f32(&gu, act, H, stream) : rc;
+    return run_gated(X, W, bias, bias_stride, act, H, GU, workspace, ws_bytes,
+                     static_cast<hipStream_t>(stream));
 }
 
 size_t mt_grad_norm_workspace_f32(int64_t count) {

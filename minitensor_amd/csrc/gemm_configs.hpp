@@ -132,6 +132,17 @@ GemmLaunchFn dl_convwi_launcher_cfg1();
 // (GemmParams::rowsum).
 GemmLaunchFn dl_rowsum_launcher_cfg2(bool kv);
 
+// A gated block's projections (GateOut): gemm_f32_sp's tiles for la in {L_KV, L_MV}, lb in
+// {L_GKV, L_GMV}.  (256x128 took what 128x256 takes.)
+template <int CFG> struct GateCfg;
+template <> struct GateCfg<0> { static constexpr int BM = 64, BN = 128, WM = 32, WN = 64, WPE = 3; };
+template <> struct GateCfg<1> { static constexpr int BM = 128, BN = 128, WM = 64, WN = 64, WPE = 2; };
+template <> struct GateCfg<2> { static constexpr int BM = 128, BN = 256, WM = 64, WN = 64, WPE = 2; };
+constexpr int kNumGateCfg = 3;
+GemmLaunchFn gate_launcher_cfg0(int la, int lb);
+GemmLaunchFn gate_launcher_cfg1(int la, int lb);
+GemmLaunchFn gate_launcher_cfg2(int la, int lb);
+
 // Wave-split kernel (gemm_ksw_kernel.hpp): tile (R*MB) x (R*NB) of R x R
 // MFMA blocks (R = 32: gemm_f32_ksw, R = 16: gemm_f32_ksw16), W waves
 // splitting the tile's K range, D chunks in flight per wave.  Any operand

@@ -63,6 +63,8 @@ enum : int {
                // patch of the input
     L_IM4 = 9, // B only, gemm_f32_sp: L_IM's operand for any c % 4 == 0
     L_IMQ = 10, // B only, gemm_f32_sp: L_IMW's operand, four columns per load (256-column tiles)
+    L_GKV = 11, // B only, gemm_f32_sp: a gated block's weight (GateOut), k contiguous
+    L_GMV = 12, // ... mn contiguous
     L_KVI = 8  // A only, direct-to-LDS kernels: k-contiguous rows split into images,
                // A(m, k) = A[(k / a_hw)*a_img + m*a_mn + k % a_hw] (dY of a
                // convolution read in NCHW as [c_out][n*h_out*w_out])
@@ -136,6 +138,16 @@ __host__ __device__ inline int dlh_lds_floats(const ConvGeom& g) {
 }
 
 
+// A gated product (B of layout L_GKV or L_GMV): rows f of B's first half are gates, rows
+// F + f of its second the same features' up columns.  The launch's columns (GemmParams::N, a
+// multiple of 64) take 32 gates and their 32 up columns in turn.  h = act(gate) * up, and gu
+// [M][2F] the two themselves.
+struct GateOut {
+    float* h; int64_t h_m, h_n;
+    float* gu; int64_t gu_m, gu_n;            // nullptr: not wanted
+    int F, act;
+};
+
 struct GemmParams {
     const float* A; int64_t a_mn, a_k, a_b;   // A(m,k) = A[m*a_mn + k*a_k + b*a_b]
     int64_t a_img; int a_hw;                  // L_KVI: image stride, k per image
@@ -175,6 +187,7 @@ struct GemmParams {
     // slabs of csum_rows[slab*M + m] (the GEMM's row-sum partials) instead.
     const float* csum_rows;
     int tiles_m, tiles_n, group_m;
+    GateOut gate;                             // B of layout L_GKV or L_GMV only
 };
 
 template <int L>

@@ -22,11 +22,13 @@
 //   * A workgroup whose sums are not finite takes its tile again with fp32
 //     MFMAs, from the same loaders.
 // Operand forms: L_KV / L_MV (any alignment and, across, any stride), L_IM,
-// L_IMW, L_IMR and L_KVI as in gemm_dl_kernel.hpp, and L_IM4 and L_IMQ.
+// L_IMW, L_IMR and L_KVI as in gemm_dl_kernel.hpp, and L_IM4 and L_IMQ; L_GKV and L_GMV,
+// with an epilogue of their own.
 #pragma once
 
 #include <type_traits>
 
+#include "gate_kernel.hpp"
 #include "gemm_dl_kernel.hpp"
 #include "gemm_split.hpp"
 
@@ -42,7 +44,11 @@ __device__ __forceinline__ T sp_global(const float* p) {
 }
 
 template <int L>
-constexpr bool sp_kc() { return L == L_KV || L == L_KVI || L == L_IM || L == L_IM4; }
+constexpr bool sp_kc() {
+    return L == L_KV || L == L_KVI || L == L_IM || L == L_IM4 || L == L_GKV;
+}
+template <int L>
+constexpr bool sp_gated() { return L == L_GKV || L == L_GMV; }
 
 // Items of four consecutive k of one row: BMN x 4 per chunk.  k-contiguous
 // forms put the four items of a row on consecutive lanes; the others put
@@ -160,6 +166,42 @@ struct SpLoader<L_MV, BMN, NT> {
                 }
         }
         base += adv ? 16 * sk : 0;
+    }
+};
+
+// A gated block's weight: the loaders of contiguous operands with the tile's rows in pairs of
+// blocks, gates and up rows (GateOut); mn0, a multiple of 64, counts both.  32-bit offsets
+// from the first gate on (the host checks that the last up row is within them).
+template <int BMN, int NT>
+struct SpLoader<L_GKV, BMN, NT> : SpLoader<L_KV, BMN, NT> {
+    using I = SpItems<L_GKV, BMN, NT>;
+    __device__ __forceinline__ void init(const GemmParams& p, const float* X, int64_t s_mn, int64_t,
+                                         int, int mn0, int k0, int t) {
+        const int f0 = mn0 >> 1;
+        this->base = reinterpret_cast<const char*>(X + (int64_t)f0 * s_mn + k0);
+        this->kq = t & 3;
+#pragma unroll
+        for (int i = 0; i < I::NI; ++i) {
+            const int r = I::row(i, t), f = min((r >> 6) * 32 + (r & 31), p.gate.F - 1 - f0);
+            this->off[i] = ((uint32_t)(f + (r & 32 ? p.gate.F : 0)) * (uint32_t)s_mn +
+                            4u * this->kq) * 4u;
+        }
+    }
+};
+template <int BMN, int NT>
+struct SpLoader<L_GMV, BMN, NT> : SpLoader<L_MV, BMN, NT> {
+    using I = SpItems<L_GMV, BMN, NT>;
+    __device__ __forceinline__ void init(const GemmParams& p, const float* X, int64_t, int64_t s_k,
+                                         int, int mn0, int k0, int t) {
+        const int f0 = mn0 >> 1;
+        this->base = X + (int64_t)k0 * s_k + f0;
+        this->sk = s_k;
+#pragma unroll
+        for (int i = 0; i < I::NI; ++i) {
+            const int r = I::row(i, t), f = min((r >> 6) * 32 + (r & 31), p.gate.F - 1 - f0);
+            this->off[i] = (uint32_t)(f + (r & 32 ? p.gate.F : 0));
+            this->kq[i] = I::kq(i, t);
+        }
     }
 };
 
@@ -541,6 +583,64 @@ __device__ __forceinline__ void sp_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// The epilogue of a gated tile: each wave turns a gate block and its up block round in a part
+// of LDS of its own (as store_tile_lds, without its barriers), and eight lanes write 32
+// features of a row.  (m, n): the wave's first row and column.
+template <int MB, int NB, int NW, int LDS>
+__device__ __forceinline__ void store_gated(const GemmParams& p, const f32x16 (&acc)[MB][NB],
+                                            char* lds, int m1, int n1, int wave, int lane) {
+    static_assert(NW * 32 * 64 * 4 <= LDS && NB % 2 == 0, "the staging must fit the ring");
+    const GateOut& o = p.gate;
+    const RowView h{o.h, o.h_m, o.h_n}, gu{o.gu, o.gu_m, o.gu_n};
+    rowf4* const stage = reinterpret_cast<rowf4*>(lds) + wave * 32 * 16;
+    const int half = lane >> 5, c = lane & 31, g = lane & 7, r0 = lane >> 3;
+    __syncthreads();
+#pragma unroll
+    for (int jj = 0; jj < NB; jj += 2) {
+        const int f = (n1 + 32 * jj) / 2 + 4 * g;
+        rowf4 bias[2] = {rowf4{0.f, 0.f, 0.f, 0.f}, rowf4{0.f, 0.f, 0.f, 0.f}};
+        if (p.bias)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    bias[x][e] = p.bias[((int64_t)x * o.F + min(f + e, o.F - 1)) * p.bias_stride];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    stage[c * 16 + ((8 * j + 2 * q + half) ^ (c & 15))] =
+                        rowf4{acc[i][jj + j][4 * q], acc[i][jj + j][4 * q + 1],
+                              acc[i][jj + j][4 * q + 2], acc[i][jj + j][4 * q + 3]};
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            rowf4 a[4], u[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int r = r0 + 8 * k;
+                a[k] = stage[r * 16 + (g ^ (r & 15))] + bias[0];
+                u[k] = stage[r * 16 + ((g + 8) ^ (r & 15))] + bias[1];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int m = m1 + 32 * i + r0 + 8 * k;
+                if (m >= p.M || f >= o.F) continue;
+                if (gu.p) {
+                    put4(gu, m, f, o.F, a[k]);
+                    put4(gu, m, (int64_t)o.F + f, 2 * (int64_t)o.F, u[k]);
+                }
+                put4(h, m, f, o.F, gate4(o.act, a[k], u[k]));
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        }
+    }
+}
+
 // BN: columns of the tile's blocks; BNT <= BN: columns of the tile.
 // RS: also the row sums of A (GemmParams::rowsum).
 template <int BM, int BN, int BNT, int WM, int WN, int LA, int LB, int WPE, bool RS = false>
@@ -796,6 +896,11 @@ gemm_f32_sp(GemmParams p) {
         }
     }
 
+    if constexpr (sp_gated<LB>())
+        if (p.splits == 1) {
+            store_gated<MB, NB, NW, 2 * BUF>(p, acc, smem, m0 + ra, n0 + rb, wave, lane);
+            return;
+        }
     store_tile_lds<MB, NB, NW, WAVES_N, WM, WN, 2 * BUF / 4>(
         p, acc, reinterpret_cast<float*>(smem), m0, n0, wave, lane, id.split, id.bz, n_end);
 }

@@ -63,7 +63,7 @@ Q8Plan q8_plan(int64_t M, int64_t cols, int64_t K) {
             };
             double us = (double)(wgs / slots) * round(t.per_cu);
             if (wgs % slots) us += round((wgs % slots + kCus - 1) / kCus);
-            if (splits > 1) us += 4 + (double)(2 * splits + 1) * (double)M * (double)cols * 0.9e-6;
+            if (splits > 1) us += 4 + (double)(splits + 1) * (double)M * (double)cols * 0.9e-6;
             if (least == 0 || us < least) {
                 least = us;
                 best = {TILES, t.bm, t.bn, (int)splits, (int)(per * 128), wgs, tn * t.bn,

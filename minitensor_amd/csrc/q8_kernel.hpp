@@ -74,31 +74,20 @@ struct Q8Cols {
             }
     }
 };
-__device__ __forceinline__ void q8_put4(const RowView& v, int64_t m, int64_t n, int64_t end,
-                                        const rowf4& x) {
-    float* const d = v.p + m * v.rs + n * v.cs;
-    if (v.cs == 1 && n + 4 <= end) {
-        *reinterpret_cast<rowf4_u*>(d) = x;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (n + e < end) d[e * v.cs] = x[e];
-    }
-}
 // Four sums of row m, of scale s, to y; gated: a of the gates, b of the up columns.
 template <bool GATED>
 __device__ __forceinline__ void q8_finish4(const Q8Params& p, int m, int n, float s,
                                            const Q8Cols<GATED>& c, const rowf4& a, const rowf4& b) {
     const rowf4 g = q8_value(a, s, c.s[0], c.b[0]);
     if constexpr (!GATED) {
-        q8_put4(p.y, m, n, p.N, g);
+        put4(p.y, m, n, p.N, g);
     } else {
         const rowf4 u = q8_value(b, s, c.s[1], c.b[1]);
         if (p.gu.p) {
-            q8_put4(p.gu, m, n, p.N, g);
-            q8_put4(p.gu, m, (int64_t)p.N + n, 2 * (int64_t)p.N, u);
+            put4(p.gu, m, n, p.N, g);
+            put4(p.gu, m, (int64_t)p.N + n, 2 * (int64_t)p.N, u);
         }
-        q8_put4(p.y, m, n, p.N, gate4(p.act, g, u));
+        put4(p.y, m, n, p.N, gate4(p.act, g, u));
     }
 }
 

@@ -59,4 +59,17 @@ __device__ __forceinline__ RowV<MODE> weight_load(const float* w, int64_t ws, in
     else return rowf4{1.f, 1.f, 1.f, 1.f};
 }
 
+// Four neighbouring columns n.. of row m, those before `end`.
+__device__ __forceinline__ void put4(const RowView& v, int64_t m, int64_t n, int64_t end,
+                                        const rowf4& x) {
+    float* const d = v.p + m * v.rs + n * v.cs;
+    if (v.cs == 1 && n + 4 <= end) {
+        *reinterpret_cast<rowf4_u*>(d) = x;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < end) d[e * v.cs] = x[e];
+    }
+}
+
 }  // namespace mtk

@@ -580,20 +580,23 @@ py::object gated_linear(py::handle px, py::handle pxscale, py::handle pw, py::ha
         if (keep) mg = mat(gu);
         const mt_mat_f32 mh = mat(out);
         mt_rows_q8 qx{}, qw{};
+        mt_mat_f32 mx{}, mw{};
         if (q8) {
             qx = rows_q8(x, xscale);
             qw = rows_q8(w, wscale);
+        } else {
+            mx = mat(x);
+            mw = mat(w);
         }
         const Workspace ws(gws, x, [&] {
             return q8 ? mt_gated_linear_q8_workspace(&qx, &qw)
-                      : mt_gated_linear_workspace_f32(rows, k, f);
+                      : mt_gated_linear_workspace_f32(&mx, &mw);
         });
         if (q8) {
             check(mt_gated_linear_q8(&qx, &qw, ptr(b), step(b), act, &mh, keep ? &mg : nullptr, ws.p,
                                      ws.n, s),
                   "mt_gated_linear_q8");
         } else {
-            const mt_mat_f32 mx = mat(x), mw = mat(w);
             check(mt_gated_linear_f32(&mx, &mw, ptr(b), step(b), act, &mh, keep ? &mg : nullptr, ws.p,
                                       ws.n, s),
                   "mt_gated_linear_f32");

@@ -34,12 +34,18 @@ class GatedLinear(NamedTuple):
     gu: Optional[torch.Tensor]
 
 
+class GatePlan(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int32), ("tile_rows", ctypes.c_int32),
+                ("tile_cols", ctypes.c_int32), ("splits", ctypes.c_int32)]
+
+
 _P, _V, _I64, _F, _S = (ctypes.POINTER, ctypes.c_void_p, ctypes.c_int64, ctypes.c_float,
                         ctypes.c_size_t)
 _M, _Q, _I = _P(MatF32), _P(RowsQ8), ctypes.c_int
 SIGS = {
     "mt_gated_linear_f32": (_I, [_M, _M, _V, _I64, _I, _M, _M, _V, _S, _V]),
-    "mt_gated_linear_workspace_f32": (_S, [_I64] * 3),
+    "mt_gated_linear_workspace_f32": (_S, [_M, _M]),
+    "mt_gated_linear_plan_f32": (_I, [_M, _M, _P(GatePlan)]),
     "mt_gated_linear_q8": (_I, [_Q, _Q, _V, _I64, _I, _M, _M, _V, _S, _V]),
     "mt_gated_linear_q8_workspace": (_S, [_Q, _Q]),
     "mt_gated_linear_q8_plan": (_I, [_I64] * 3 + [_P(Q8Plan)]),
@@ -109,8 +115,8 @@ def gated_linear(x: Union[torch.Tensor, Q8Rows], w: Union[torch.Tensor, Q8Rows],
     if out is None:
         out = _empty((n, f), like)
     gu = _empty((n, f2), like) if keep else None
-    need = (lib().mt_gated_linear_q8_workspace(ctypes.byref(xd), ctypes.byref(wd)) if q8 else
-            lib().mt_gated_linear_workspace_f32(n, k, f))
+    query = lib().mt_gated_linear_q8_workspace if q8 else lib().mt_gated_linear_workspace_f32
+    need = query(ctypes.byref(xd), ctypes.byref(wd))
     ws = _ws(ws, need, like)
     fn, name = ((lib().mt_gated_linear_q8, "mt_gated_linear_q8") if q8 else
                 (lib().mt_gated_linear_f32, "mt_gated_linear_f32"))

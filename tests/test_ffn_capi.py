@@ -5,6 +5,7 @@ import ctypes
 import pytest
 
 import minitensor_amd as mt
+from minitensor_amd.ffn import GatePlan
 from minitensor_amd.lowbit import Q8Plan, RowsQ8
 
 OK, INVALID, WORKSPACE = mt.MT_OK, mt.MT_ERR_INVALID, mt.MT_ERR_WORKSPACE
@@ -28,6 +29,28 @@ def plan_q8(m, k, n, gated=False):
     f = mt.lib().mt_gated_linear_q8_plan if gated else mt.lib().mt_linear_q8_plan
     assert f(m, k, n, R(p)) == OK
     return (p.tile_rows, p.tile_cols), p.splits
+
+
+def plan_gate(x, w):
+    """(kind, (rows and columns of a tile), splits) of gated_linear in fp32."""
+    p = GatePlan()
+    assert mt.lib().mt_gated_linear_plan_f32(R(x), R(w), R(p)) == OK
+    return p.kind, (p.tile_rows, p.tile_cols), p.splits
+
+
+def test_gate_plans():
+    assert plan_gate(M(1, 4096), M(8192, 4096))[0] == 0
+    assert plan_gate(M(8, 64), M(64, 64))[0] == 0
+    assert plan_gate(M(48, 64), M(64, 64))[0] == 0
+    assert plan_gate(M(49, 64), M(64, 64))[0] == 1
+    assert plan_gate(M(8, 64, rs=1, cs=8), M(64, 64))[0] == 1          # x across its rows
+    assert plan_gate(M(100, 64), M(64, 64, rs=1, cs=64))[0] == 1
+    assert plan_gate(M(100, 64, rs=128, cs=2), M(64, 64))[0] == 2
+    assert plan_gate(M(100, 64), M(64, 64, rs=128, cs=2))[0] == 2
+    assert plan_gate(M(100, 64), M(64, 64, rs=1 << 25))[0] == 2        # past 32-bit offsets
+    assert plan_gate(M(100, 0), M(64, 0))[0] == 2
+    assert plan_gate(M(4096, 2048), M(8192, 2048)) == (1, (128, 256), 1)
+    assert plan_gate(M(64, 2048), M(512, 2048))[2] > 1
 
 
 def test_linear_q8_refuses():
@@ -113,7 +136,11 @@ def test_clip_refuses():
 def test_queries():
     lib = mt.lib()
     f = lib.mt_gated_linear_workspace_f32
-    assert f(0, 8, 8) == 0 and f(-1, 8, 8) == 0 and f(1 << 31, 8, 8) == 0
+    assert f(R(M(0, 8)), R(M(8, 8))) == 0 and f(R(M(8, 8)), R(M(0, 8))) == 0
+    assert f(R(M(8, 8)), R(M(8, 9))) == 0 and f(None, R(M(8, 8))) == 0
+    # neither way contiguous: the projections go to the workspace
+    assert f(R(M(100, 64, rs=256, cs=2)), R(M(512, 64))) >= 100 * 512 * 4
+    assert f(R(M(8, 64)), R(M(512, 64))) == 0
     for f in (lib.mt_linear_q8_workspace, lib.mt_gated_linear_q8_workspace):
         assert f(R(Q(0, 8)), R(Q(8, 8))) == 0 and f(R(Q(8, 8)), R(Q(0, 8))) == 0
         assert f(R(Q(8, 8)), R(Q(8, 9))) == 0 and f(None, R(Q(8, 8))) == 0

@@ -244,7 +244,8 @@ def test_gate_infinities(dev):
 
 # ---- gated Linear ----------------------------------------------------------------
 GATE_SIZES = [(1, 1, 1), (1, 64, 16), (2, 33, 17), (4, 100, 256), (5, 31, 257), (8, 512, 1024),
-              (9, 65, 100), (16, 256, 2048), (33, 64, 130), (64, 128, 512), (100, 257, 300),
+              (3, 9, 513), (9, 65, 100), (16, 256, 2048), (17, 40, 63), (32, 100, 515), (33, 64, 130),
+              (48, 77, 64), (49, 64, 130), (64, 128, 512), (100, 257, 300),
               (130, 96, 1000), (257, 200, 64), (300, 515, 333), (509, 320, 1285)]
 
 
@@ -273,7 +274,20 @@ def test_gated_linear(dev, m, f, k):
         assert torch.equal(out, r.h), what
 
 
-@pytest.mark.parametrize("m,f,k", [(2048, 640, 100), (1024, 2048, 128), (700, 3001, 200)])
+GATE_LARGE = [(2048, 640, 100), (1024, 2048, 128), (700, 3001, 200), (2048, 2000, 250), (1024, 4096, 130),
+              (500, 2570, 700)]
+
+
+def test_gated_linear_kernels():
+    """Which sizes take which kernel, so that the tests here reach all of them."""
+    from test_ffn_capi import M, plan_gate
+    plans = [plan_gate(M(m, k), M(2 * f, k)) for m, f, k in GATE_SIZES + GATE_LARGE]
+    assert {p[0] for p in plans} == {0, 1}
+    assert {p[1] for p in plans} == {(0, 0), (64, 128), (128, 128), (128, 256)}, plans
+    assert any(p[2] > 1 for p in plans)
+
+
+@pytest.mark.parametrize("m,f,k", GATE_LARGE)
 def test_gated_linear_large_tiles(dev, m, f, k):
     g = rng(7, m, f, k)
     x, w, b = normal(g, m, k), normal(g, 2 * f, k) / np.float32(k ** 0.5), normal(g, 2 * f)
