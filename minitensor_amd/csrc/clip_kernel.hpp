@@ -21,15 +21,17 @@
 namespace mtk {
 
 constexpr int kClipTensors = 128;     // of a launch: 28 bytes each of 4 KB of arguments
-constexpr int kClipChunk = 8192;      // elements
-constexpr int kClipBlocks = 1024;     // workgroups of a launch, at most
-constexpr int kClipPartials = 1 << 20;  // of a call (so that their count stays 32-bit)
+constexpr int kClipThreads = 512, kClipQuads = 4;
+constexpr int kClipChunk = kClipThreads * kClipQuads * 4;   // elements
+constexpr int kClipBlocks = 1024;     // workgroups of a launch, at most: four on a CU
+constexpr int kClipMostParts = 4096;  // partial sums that every scaling workgroup adds up
 
 struct ClipTable {
     const float* src[kClipTensors];
     float* dst[kClipTensors];
     int64_t n[kClipTensors];
-    uint32_t first[kClipTensors];     // chunk of the launch that the tensor starts with
+    uint32_t first[kClipTensors];     // chunk of the launch that the tensor starts with (past
+                                      // the last tensor: the largest number)
     int count;
     uint32_t chunks;
 };
@@ -48,22 +50,31 @@ struct ClipNorm {
     float* norm;
     double most, eps;
 };
+// Gradients, in bytes, beyond which they and as many outputs do not stay in the 256 MB of the
+// last cache: outputs written past it leave it to the gradients (138M elements, again and
+// again: 288 us against 319; 38M: 85 and 86; the other way, 25.6 us against 27.5 for half of
+// those 38M, which stay).
+constexpr int64_t kClipStream = (int64_t)160 << 20;
 
-// The sum of x over a workgroup of 256, in every thread.
+// The sum of x over a workgroup of NT, in every thread, in a fixed order.
+template <int NT>
 __device__ __forceinline__ double clip_block_sum(double x, double* red) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
     __syncthreads();
-    const double s = (red[0] + red[1]) + (red[2] + red[3]);
+    double s = red[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) s += red[w];
     __syncthreads();
     return s;
 }
-// All partial sums together.
+// All partial sums together, the same in every workgroup.
+template <int NT>
 __device__ __forceinline__ double clip_total(const ClipNorm& c, double* red) {
     double s = 0;
-    for (int i = threadIdx.x; i < c.parts; i += 256) s += c.part[i];
-    return clip_block_sum(s, red);
+    for (int i = threadIdx.x; i < c.parts; i += NT) s += c.part[i];
+    return clip_block_sum<NT>(s, red);
 }
 // The factor; 1: nothing to scale.  (A NaN stays one; an infinite norm gives 0.)
 __device__ __forceinline__ float clip_factor(const ClipNorm& c, double total) {
@@ -71,66 +82,116 @@ __device__ __forceinline__ float clip_factor(const ClipNorm& c, double total) {
     return f >= 1.0 ? 1.f : (float)f;
 }
 
-// Calls f(tensor, first element, elements) for the workgroup's chunks.
-template <class F>
-__device__ __forceinline__ void clip_chunks(const ClipTable& t, F f) {
+// A workgroup's run of chunks, and what it takes of one at a time.
+struct ClipRun {
+    uint32_t begin, end;
+};
+__device__ __forceinline__ ClipRun clip_run(const ClipTable& t) {
     const uint32_t per = (t.chunks + gridDim.x - 1) / gridDim.x;
-    uint32_t c = blockIdx.x * per;
-    const uint32_t end = min(c + per, t.chunks);
-    if (c >= end) return;
-    int lo = 0, hi = t.count;                         // the tensor of chunk c
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (t.first[mid] <= c) lo = mid;
-        else hi = mid;
+    const uint32_t begin = min(blockIdx.x * per, t.chunks);
+    return {begin, min(begin + per, t.chunks)};
+}
+struct ClipPiece {
+    const float* src;
+    float* dst;
+    int n;                            // elements, at most kClipChunk
+};
+// (the tensor of a chunk: one look at every tensor's first chunk, a lane two of them)
+__device__ __forceinline__ ClipPiece clip_piece(const ClipTable& t, uint32_t c) {
+    static_assert(kClipTensors == 128, "two tensors a lane");
+    const int lane = threadIdx.x & 63;
+    const int k = __builtin_amdgcn_readfirstlane(__popcll(__ballot(t.first[lane] <= c)) +
+                                                 __popcll(__ballot(t.first[64 + lane] <= c)) - 1);
+    const int64_t at = (int64_t)(c - t.first[k]) * kClipChunk;
+    return {t.src[k] + at, t.dst[k] + at, (int)min(t.n[k] - at, (int64_t)kClipChunk)};
+}
+// A thread's groups of four, zeros past the end, and (thread < n % 4) one of the last elements.
+struct ClipValues {
+    rowf4 x[kClipQuads];
+    float last;
+};
+__device__ __forceinline__ void clip_load(const ClipPiece& p, ClipValues& v) {
+    v.last = 0.f;
+    if (p.n == kClipChunk) {
+#pragma unroll
+        for (int i = 0; i < kClipQuads; ++i)
+            v.x[i] = *reinterpret_cast<const rowf4_u*>(p.src + 4 * (threadIdx.x + i * kClipThreads));
+        return;
     }
-    for (; c < end; ++c) {
-        while (lo + 1 < t.count && t.first[lo + 1] <= c) ++lo;
-        const int64_t at = (int64_t)(c - t.first[lo]) * kClipChunk;
-        f(lo, at, (int)min(t.n[lo] - at, (int64_t)kClipChunk));
+    const int quads = p.n >> 2;
+#pragma unroll
+    for (int i = 0; i < kClipQuads; ++i) {
+        const int q = threadIdx.x + i * kClipThreads;
+        v.x[i] = rowf4{0.f, 0.f, 0.f, 0.f};
+        if (q < quads) v.x[i] = *reinterpret_cast<const rowf4_u*>(p.src + 4 * q);
     }
+    if ((int)threadIdx.x < (p.n & 3)) v.last = p.src[4 * quads + threadIdx.x];
 }
 
-__global__ void __launch_bounds__(256) clip_squares(ClipTable t, double* part) {
-    __shared__ double red[4];
+__global__ void __launch_bounds__(kClipThreads) clip_squares(ClipTable t, double* part) {
+    __shared__ double red[kClipThreads / 64];
     double s = 0;
-    clip_chunks(t, [&](int k, int64_t at, int n) {
-        const float* const g = t.src[k] + at;
-        const int quads = n >> 2;
-        for (int i = threadIdx.x; i < quads; i += 256) {
-            const rowf4 x = *reinterpret_cast<const rowf4_u*>(g + 4 * i);
+    const ClipRun r = clip_run(t);
+    ClipValues v, next;
+    if (r.begin < r.end) clip_load(clip_piece(t, r.begin), v);
+    for (uint32_t c = r.begin; c < r.end; ++c) {
+        if (c + 1 < r.end) clip_load(clip_piece(t, c + 1), next);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = fma((double)x[e], (double)x[e], s);
-        }
-        const int e = 4 * quads + threadIdx.x;
-        if (e < n) s = fma((double)g[e], (double)g[e], s);
-    });
-    s = clip_block_sum(s, red);
+        for (int i = 0; i < kClipQuads; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = fma((double)v.x[i][e], (double)v.x[i][e], s);
+        s = fma((double)v.last, (double)v.last, s);
+        v = next;
+    }
+    s = clip_block_sum<kClipThreads>(s, red);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
-__global__ void __launch_bounds__(256) clip_scale(ClipTable t, ClipNorm c) {
-    __shared__ double red[4];
-    const double total = clip_total(c, red);
+// From the last chunk to the first: what the squares read last is still in the cache.
+// STREAM: outputs are written past the caches.
+template <bool STREAM>
+__global__ void __launch_bounds__(kClipThreads) clip_scale(ClipTable t, ClipNorm c) {
+    __shared__ double red[kClipThreads / 64];
+    const ClipRun r = clip_run(t);
+    ClipPiece p{}, q{};
+    ClipValues v, next;
+    if (r.begin < r.end) {                            // (on its way while the sums are added up)
+        p = clip_piece(t, r.end - 1);
+        clip_load(p, v);
+    }
+    const double total = clip_total<kClipThreads>(c, red);
     if (blockIdx.x == 0 && threadIdx.x == 0) *c.norm = (float)sqrt(total);
     const float f = clip_factor(c, total);
-    clip_chunks(t, [&](int k, int64_t at, int n) {
-        const float* const g = t.src[k] + at;
-        float* const o = t.dst[k] + at;
-        if (f == 1.f && o == g) return;
-        const int quads = n >> 2;
-        for (int i = threadIdx.x; i < quads; i += 256)
-            *reinterpret_cast<rowf4_u*>(o + 4 * i) = *reinterpret_cast<const rowf4_u*>(g + 4 * i) * f;
-        const int e = 4 * quads + threadIdx.x;
-        if (e < n) o[e] = g[e] * f;
-    });
+    for (uint32_t i = r.end; i > r.begin; --i) {
+        if (i - 1 > r.begin) {
+            q = clip_piece(t, i - 2);
+            clip_load(q, next);
+        }
+        if (f != 1.f || p.dst != p.src) {
+            const int quads = p.n >> 2;
+#pragma unroll
+            for (int k = 0; k < kClipQuads; ++k) {
+                const int at = threadIdx.x + k * kClipThreads;
+                if (at >= quads) continue;
+                rowf4_u* const d = reinterpret_cast<rowf4_u*>(p.dst + 4 * at);
+                const rowf4 x = v.x[k] * f;
+                if constexpr (STREAM) __builtin_nontemporal_store(x, d);
+                else *d = x;
+            }
+            if ((int)threadIdx.x < (p.n & 3)) p.dst[4 * quads + threadIdx.x] = v.last * f;
+        }
+        p = q;
+        v = next;
+    }
 }
 
-// The norm alone.
-__global__ void __launch_bounds__(256) clip_norm(ClipNorm c) {
-    __shared__ double red[4];
-    const double total = clip_total(c, red);
-    if (threadIdx.x == 0) *c.norm = (float)sqrt(total);
+// The norm alone; or (norm nullptr) all partial sums as one, behind them.
+__global__ void __launch_bounds__(kClipThreads) clip_norm(ClipNorm c) {
+    __shared__ double red[kClipThreads / 64];
+    const double total = clip_total<kClipThreads>(c, red);
+    if (threadIdx.x != 0) return;
+    if (c.norm) *c.norm = (float)sqrt(total);
+    else c.part[c.parts] = total;
 }
 
 template <class F>
@@ -149,12 +210,12 @@ __global__ void __launch_bounds__(256) clip_squares_strided(ClipStrided t, doubl
         const double x = t.src[a];
         s = fma(x, x, s);
     });
-    s = clip_block_sum(s, red);
+    s = clip_block_sum<256>(s, red);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 __global__ void __launch_bounds__(256) clip_scale_strided(ClipStrided t, ClipNorm c) {
     __shared__ double red[4];
-    const double total = clip_total(c, red);
+    const double total = clip_total<256>(c, red);
     if (blockIdx.x == 0 && threadIdx.x == 0) *c.norm = (float)sqrt(total);
     const float f = clip_factor(c, total);
     if (f == 1.f && t.dst == t.src) return;

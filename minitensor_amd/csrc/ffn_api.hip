@@ -251,8 +251,10 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
     const mt_mat_f32* const to = out ? out : grads;
     Tensor d{};
     std::vector<const float*> at;
+    int64_t all = 0;
     for (int64_t i = 0; i < count; ++i) {
         if (!tensor_of(&grads[i], &to[i], scale, &d)) return MT_ERR_INVALID;
+        all += d.n;
         if (scale && d.n > 0) at.push_back(d.dst);
     }
     std::sort(at.begin(), at.end());                   // no output twice
@@ -266,10 +268,12 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
         ClipTable t;
         t.count = 0;
         t.chunks = 0;
+        std::fill(t.first, t.first + kClipTensors, ~0u);
         auto flush = [&] {
             if (t.count > 0) table(t, std::min<uint32_t>(t.chunks, kClipBlocks));
             t.count = 0;
             t.chunks = 0;
+            std::fill(t.first, t.first + kClipTensors, ~0u);
         };
         for (int64_t i = 0; i < count; ++i) {
             tensor_of(&grads[i], &to[i], scale, &d);
@@ -291,21 +295,28 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
     int parts = 0;
     launches(
         [&](const ClipTable& t, unsigned blocks) {
-            hipLaunchKernelGGL(clip_squares, dim3(blocks), dim3(256), 0, s, t, part + parts);
+            hipLaunchKernelGGL(clip_squares, dim3(blocks), dim3(kClipThreads), 0, s, t, part + parts);
             parts += (int)blocks;
         },
         [&](const ClipStrided& t, unsigned blocks) {
             hipLaunchKernelGGL(clip_squares_strided, dim3(blocks), dim3(256), 0, s, t, part + parts);
             parts += (int)blocks;
         });
-    const ClipNorm c{part, parts, norm, most, eps};
+    const bool past = out != nullptr && all * 4 > kClipStream;
+    ClipNorm c{part, parts, norm, most, eps};
     if (!scale || parts == 0) {
-        hipLaunchKernelGGL(clip_norm, dim3(1), dim3(256), 0, s, c);
+        hipLaunchKernelGGL(clip_norm, dim3(1), dim3(kClipThreads), 0, s, c);
         return launched();
+    }
+    if (parts > kClipMostParts) {
+        c.norm = nullptr;
+        hipLaunchKernelGGL(clip_norm, dim3(1), dim3(kClipThreads), 0, s, c);
+        c = {part + parts, 1, norm, most, eps};
     }
     launches(
         [&](const ClipTable& t, unsigned blocks) {
-            hipLaunchKernelGGL(clip_scale, dim3(blocks), dim3(256), 0, s, t, c);
+            if (past) hipLaunchKernelGGL(clip_scale<true>, dim3(blocks), dim3(kClipThreads), 0, s, t, c);
+            else hipLaunchKernelGGL(clip_scale<false>, dim3(blocks), dim3(kClipThreads), 0, s, t, c);
         },
         [&](const ClipStrided& t, unsigned blocks) {
             hipLaunchKernelGGL(clip_scale_strided, dim3(blocks), dim3(256), 0, s, t, c);
