@@ -78,6 +78,7 @@ __device__ __forceinline__ double clip_total(const ClipNorm& c, double* red) {
 }
 // The factor; 1: nothing to scale.  (A NaN stays one; an infinite norm gives 0.)
 __device__ __forceinline__ float clip_factor(const ClipNorm& c, double total) {
+    if (total == 0.0) return 1.f;
     const double f = c.most / (sqrt(total) + c.eps);
     return f >= 1.0 ? 1.f : (float)f;
 }

@@ -18,8 +18,6 @@ namespace {
 constexpr int64_t kMaxTerms = ((int64_t)1 << 17) - 128;
 // Bytes between a tile's rows: their offsets, 255 of them and a chunk, are 32-bit.
 constexpr int64_t kMaxRow = ((int64_t)1 << 24) - 256;
-constexpr int64_t kFewRows = 32;
-
 enum Kind { FEW, LONG, TILES };
 struct Q8Plan {
     Kind kind;
@@ -44,10 +42,18 @@ constexpr Q8Tile kTiles[] = {{64, 128, 2, 0.34, 0.45, 2.2},
                              {128, 256, 1, 0.88, 0, 6.5},
                              {256, 256, 1, 1.6, 0, 10}};
 
+// Whether the kernel of few rows takes a product, which reads x for every workgroup's columns
+// anew.  (Against 64x128 tiles, us: 64 rows 4096 -> 4096 12.0 and 11.8, 2048 -> 2048 6.9 and 9.3,
+// 4096 -> 8192 14.3 and 14.1 -- 33 rows 11.7 and 14.1 --, 4096 -> 16384 25.7 and 16.8, 32 rows of
+// those 14.6 and 16.8.)
+bool few_rows(int64_t M, int64_t cols, int64_t K) {
+    return K < kQ8Segment && (M <= 32 || (M <= 64 && M * cols * K <= (int64_t)1200 << 20));
+}
+
 // cols: columns of the launch (gated: whole blocks of 32 features, twice).
 Q8Plan q8_plan(int64_t M, int64_t cols, int64_t K) {
     if (K > kMaxRow) return {LONG, 0, 0, 1, 0, 0, 0, 0};
-    if (M <= kFewRows && K < kQ8Segment) return {FEW, 0, 0, 1, 0, 0, 0, 0};
+    if (few_rows(M, cols, K)) return {FEW, 0, 0, 1, 0, 0, 0, 0};
     Q8Plan best{};
     double least = 0;
     const int64_t chunks = std::max<int64_t>(1, (K + 127) / 128);
@@ -100,17 +106,34 @@ Q8Space q8_space(const Q8Plan& plan, const mt_rows_q8* X, const mt_rows_q8* W) {
     return s;
 }
 
+// Column blocks (of 16, gated ones counted twice) of a workgroup of few rows: more of them
+// read x less often, as long as there is a workgroup for every CU.  (4096 -> 16384, 1 row: one
+// block 18.0 us, two 14.5, four 13.6; gated 4096 -> 2 x 8192: two 12.0, four 14.6; 32 rows: one
+// 23.9, four 14.6; 64 rows: one 38, two 26.  Four of 64 rows do not fit.)
+int few_columns(int64_t rows, int64_t cols) {
+    const int64_t blocks = (cols + 15) / 16;
+    return blocks >= 4 * kCus && rows > 16 && rows <= 32 ? 4 : blocks >= 2 * kCus ? 2 : 1;
+}
 template <bool GATED>
 void launch_few(const Q8Params& p, bool words, hipStream_t s) {
     using std::integral_constant;
-    auto go = [&](auto mb, auto kind) {
-        constexpr int NC = GATED ? 2 : 1, F = 16;
-        const dim3 grid((unsigned)((p.N + F - 1) / F));
-        hipLaunchKernelGGL((q8_few<mb(), NC, GATED, kind()>), grid, dim3(512), 0, s, p);
+    const int columns = few_columns(p.M, GATED ? 2 * (int64_t)p.N : p.N);
+    auto go = [&](auto mb, auto nc, auto kind) {
+        constexpr int F = 16 * nc() / (GATED ? 2 : 1);
+        hipLaunchKernelGGL((q8_few<mb(), nc(), GATED, kind()>), dim3((unsigned)((p.N + F - 1) / F)),
+                           dim3(512), 0, s, p);
+    };
+    auto blocks = [&](auto mb, auto kind) {
+        if constexpr (mb() == 2)
+            if (columns == 4) return go(mb, integral_constant<int, 4>{}, kind);
+        if constexpr (!GATED)
+            if (columns == 1) return go(mb, integral_constant<int, 1>{}, kind);
+        go(mb, integral_constant<int, 2>{}, kind);
     };
     auto rows = [&](auto kind) {
-        if (p.M <= 16) go(integral_constant<int, 1>{}, kind);
-        else go(integral_constant<int, 2>{}, kind);
+        if (p.M <= 16) blocks(integral_constant<int, 1>{}, kind);
+        else if (p.M <= 32) blocks(integral_constant<int, 2>{}, kind);
+        else blocks(integral_constant<int, 4>{}, kind);
     };
     if (words) rows(integral_constant<int, Q8_WORDS>{});
     else rows(integral_constant<int, Q8_BYTES>{});

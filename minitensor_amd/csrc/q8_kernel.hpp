@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(256) q8_align_rows(Q8Align p) {
         for (int64_t i = (int64_t)blockIdx.x * 4 + (t >> 6); i < total; i += (int64_t)p.wave_blocks * 4) {
             at(i, src, dst);
             const uint32_t shift = (uint32_t)(uintptr_t)src & 3;
-            constexpr int U = 4;
+            constexpr int U = 2;
             for (int u0 = lane; u0 < whole; u0 += 64 * U) {
                 Q8Unit x[U];
 #pragma unroll

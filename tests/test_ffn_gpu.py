@@ -75,7 +75,8 @@ def rows8(g, r, k, dev, how="dense"):
 # around their blocks
 Q8_SIZES = [(1, 1, 1), (1, 64, 16), (2, 17, 33), (1, 100, 256), (3, 255, 257), (16, 1000, 2048),
             (17, 48, 63), (31, 129, 500), (32, 32, 4096), (33, 65, 127), (33, 1, 1000), (40, 200, 64),
-            (64, 128, 128), (65, 129, 129), (100, 257, 300), (128, 256, 512), (257, 511, 255),
+            (64, 128, 128), (65, 129, 129), (17, 16400, 100), (32, 8200, 65),
+            (64, 8200, 64), (70, 8200, 96), (100, 257, 300), (128, 256, 512), (257, 511, 255),
             (255, 40, 8192), (300, 1000, 1024), (513, 769, 640), (1027, 520, 2047)]
 
 
@@ -121,7 +122,7 @@ def test_linear_q8_large_tiles(dev, m, n, k):
             check(mt.gated_linear(x, wt, act="silu").h, *ref.gate("silu", gu, e), how)
 
 
-@pytest.mark.parametrize("m", [1, 20, 40])
+@pytest.mark.parametrize("m", [1, 20, 40, 70])
 @pytest.mark.parametrize("k", [131071, 131073, 300001, 600000])
 def test_linear_q8_sums_past_32_bits(dev, m, k):
     """Every product 2^14: sums beyond 2^31 from 131072 inputs on."""
@@ -137,16 +138,16 @@ def test_linear_q8_sums_past_32_bits(dev, m, k):
 def test_linear_q8_long_rows(dev):
     """Rows of 2^24 inputs and more, and rows that far apart: neither goes to the tiles as it is."""
     k = (1 << 24) + 77
-    q = torch.full((35, k), -128, dtype=torch.int8, device=dev)
+    q = torch.full((70, k), -128, dtype=torch.int8, device=dev)
     w = torch.full((3, k), 127, dtype=torch.int8, device=dev)
     q[33, -1] = 5
-    y = cpu(mt.linear_q8(mt.Q8Rows(q, torch.ones(35, device=dev)), mt.Q8Rows(w, torch.ones(3, device=dev))))
-    want = np.full((35, 3), -128.0 * 127 * k)
+    y = cpu(mt.linear_q8(mt.Q8Rows(q, torch.ones(70, device=dev)), mt.Q8Rows(w, torch.ones(3, device=dev))))
+    want = np.full((70, 3), -128.0 * 127 * k)
     want[33] += 127 * 133
     assert np.array_equal(y, want.astype(np.float32))
     g = rng(31)
-    codes, s = g.integers(-128, 128, (35, 100)).astype(np.int8), g.random(35).astype(np.float32)
-    far = q.flatten()[:35 * (1 << 24)].view(35, 1 << 24)[:, :100]
+    codes, s = g.integers(-128, 128, (70, 100)).astype(np.int8), g.random(70).astype(np.float32)
+    far = q.flatten()[:70 * (1 << 24)].view(70, 1 << 24)[:, :100]
     far.copy_(gpu(codes, dev))
     wq, ws, wt = rows8(g, 64, 100, dev)
     check(mt.linear_q8(mt.Q8Rows(far, gpu(s, dev)), wt), *ref.linear_q8(codes, s, wq, ws))
@@ -161,7 +162,7 @@ def test_linear_q8_same_for_any_tile(dev):
     _, _, w = rows8(g, 333, 1111, dev)
     b = gpu(normal(g, 333), dev)
     all_ = mt.linear_q8(x, w, b)
-    for n in (1, 5, 32, 33, 130, 400):
+    for n in (1, 5, 32, 33, 64, 65, 130, 400):
         part = mt.linear_q8(mt.Q8Rows(x.q[:n], x.scale[:n]), w, b)
         assert torch.equal(part, all_[:n]), n
 
@@ -649,7 +650,7 @@ def test_refusals(dev):
     assert all(bool((t == 1).all()) for t in (x, w, gu, dh))
     small = torch.empty(4, dtype=torch.uint8, device=dev)
     for f in (lambda: mt.clip_grad_norm([x], 0.5, ws=small),
-              lambda: mt.linear_q8(mt.quantize_q8(torch.ones(64, 4096, device=dev)),
+              lambda: mt.linear_q8(mt.quantize_q8(torch.ones(80, 4096, device=dev)),
                                    mt.quantize_q8(torch.ones(64, 4096, device=dev)), ws=small)):
         with pytest.raises(RuntimeError):
             f()
