@@ -108,7 +108,9 @@ int gate_layout(const RowView& v, int64_t K, int64_t span, bool weight) {
 // 48 rows 25 and 26, 500 -> 2 x 1000 8 and 11; but 4096 -> 2 x 8192 32 rows 67 and 62, 48 rows 95
 // and 69, 8192 -> 2 x 512 8 rows 38 and 19, and 5632 -> 2 x 2048 16 rows 32 and 35, 32 rows 42
 // and 35.)
+// (Their grids hold 4 features at least a workgroup.)
 bool few_rows(int64_t M, int64_t F, int64_t K) {
+    if (F > 4 * (kMaxTiles - 1)) return false;
     if (M <= kGemvRows) return true;
     return M <= 16 ? K <= 4 * F : M <= kFewRows && K <= F && F * K <= (int64_t)12 << 20;
 }

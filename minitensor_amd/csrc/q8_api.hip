@@ -46,8 +46,9 @@ constexpr Q8Tile kTiles[] = {{64, 128, 2, 0.34, 0.45, 2.2},
 // anew.  (Against 64x128 tiles, us: 64 rows 4096 -> 4096 12.0 and 11.8, 2048 -> 2048 6.9 and 9.3,
 // 4096 -> 8192 14.3 and 14.1 -- 33 rows 11.7 and 14.1 --, 4096 -> 16384 25.7 and 16.8, 32 rows of
 // those 14.6 and 16.8.)
+// (Its grid holds 16 columns at least a workgroup.)
 bool few_rows(int64_t M, int64_t cols, int64_t K) {
-    return K < kQ8Segment && (M <= 32 || (M <= 64 && M * cols * K <= (int64_t)1200 << 20));
+    return K < kQ8Segment && cols <= 16 * (kMaxTiles - 1) && (M <= 32 || (M <= 64 && M * cols * K <= (int64_t)1200 << 20));
 }
 
 // cols: columns of the launch (gated: whole blocks of 32 features, twice).

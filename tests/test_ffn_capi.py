@@ -54,6 +54,16 @@ def test_gate_plans():
     assert plan_gate(M(64, 2048), M(512, 2048))[2] > 1
 
 
+def test_plans_of_most_columns():
+    """A grid holds fewer than 2^23 workgroups of 512 threads, one for every 4 features (16
+    columns) of few rows at least: past them, tiles."""
+    for m in (1, 4):
+        assert plan_gate(M(m, 1), M((1 << 26) - 8, 1))[0] == 0
+        assert plan_gate(M(m, 1), M(1 << 26, 1))[0] == 1
+    assert plan_q8(1, 1, (1 << 27) - 16)[0] == (0, 0) and plan_q8(1, 1, 1 << 27)[0] != (0, 0)
+    assert plan_q8(1, 1, (1 << 26) - 32, True)[0] == (0, 0) and plan_q8(1, 1, 1 << 26, True)[0] != (0, 0)
+
+
 def test_linear_q8_refuses():
     def call(x=Q(4, 64), w=Q(8, 64), y=M(4, 8), b=None, bs=0, ws=None, n=0):
         return mt.lib().mt_linear_q8(R(x), R(w), b, bs, R(y), ws, n, None)

@@ -135,6 +135,24 @@ def test_linear_q8_sums_past_32_bits(dev, m, k):
     assert np.array_equal(y, np.broadcast_to(want.astype(np.float32), (m, 5)))
 
 
+def test_most_columns(dev):
+    """One row by more columns than a grid of few rows holds: the tiles."""
+    n = (1 << 27) + 40
+    q = torch.randint(-127, 128, (n,), dtype=torch.int8, device=dev)
+    s = torch.rand(n, device=dev)
+    x = mt.Q8Rows(torch.tensor([[-3]], dtype=torch.int8, device=dev), torch.tensor([0.5], device=dev))
+    w = mt.Q8Rows(q[:, None], s)
+    # (0.5·s and the sum are exact: one rounding)
+    want = (-3.0 * q.double() * (0.5 * s.double())).float()
+    assert torch.equal(mt.linear_q8(x, w)[0], want)
+    del want, w, q, s
+    f = (1 << 25) + 9
+    w = torch.randn(2 * f, 1, device=dev)
+    r = mt.gated_linear(torch.tensor([[2.0]], device=dev), w, act="relu", keep=True)
+    assert torch.equal(r.gu[0], 2 * w[:, 0])
+    assert torch.equal(r.h[0], (2 * w[:f, 0]).clamp(min=0) * (2 * w[f:, 0]))
+
+
 def test_linear_q8_long_rows(dev):
     """Rows of 2^24 inputs and more, and rows that far apart: neither goes to the tiles as it is."""
     k = (1 << 24) + 77
