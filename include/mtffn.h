@@ -66,8 +66,9 @@ int mt_grad_norm_f32(const mt_mat_f32* grads, int64_t count, float* norm, void* 
 /* ... and out[i] = grads[i] * c with c = min(1, max_norm / (norm + eps)) in fp64, rounded
  * to fp32 (a NaN norm gives NaN throughout; an infinite one 0, and NaN where the gradient is
  * infinite).  out NULL: in place; with c = 1 nothing is written then.  Otherwise out[i] has the
- * shape of grads[i], and may be the same view.  No output may appear twice.  norm is that
- * before the scaling. */
+ * shape of grads[i], and may be the same view; but for that no output may overlap another
+ * tensor (refused, but for views with gaps between their elements, of which only the first
+ * one is looked at).  norm is that before the scaling. */
 int mt_clip_grad_norm_f32(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count,
                           float max_norm, float eps, float* norm, void* workspace, size_t ws_bytes,
                           void* stream);

@@ -144,6 +144,36 @@ def test_clip_refuses():
     assert call([x], ws=None, alone=True) == WORKSPACE
 
 
+def test_clip_refuses_overlaps():
+    """Outputs over each other or over other tensors: what is scaled would be scaled twice, or
+    read when it is."""
+    def call(g, o=None):
+        a = (mt.MatF32 * len(g))(*g)
+        b = (mt.MatF32 * len(o))(*o) if o is not None else None
+        # (no workspace: what is not refused goes no further)
+        return mt.lib().mt_clip_grad_norm_f32(a, b, len(g), 1.0, 1e-6, 0x9000, None, 0, None)
+    at = lambda e, n=32, **k: M(1, n, base=0x10000 + 4 * e, **k)
+    fine = WORKSPACE
+    assert call([at(0), at(32), at(100)]) == fine
+    assert call([at(0), at(31)]) == INVALID
+    assert call([at(100, 8), at(0, 200)]) == INVALID                 # one within another
+    assert call([at(0, 200), at(50, 0), at(200)]) == fine
+    assert call([at(0), at(32)], [at(100), at(131)]) == INVALID
+    assert call([at(0), at(32)], [at(32), at(100)]) == INVALID       # over the next one's input
+    assert call([at(0), at(32)], [at(32), at(0)]) == INVALID
+    assert call([at(0)], [at(4)]) == INVALID
+    assert call([at(0), at(0)], [at(100), at(200)]) == fine          # one input, two outputs
+    assert call([at(0), at(0)], [at(0), at(200)]) == INVALID
+    assert call([at(0), at(32)], [at(0), at(100)]) == fine
+    # two views that lie between each other's elements; one over a dense tensor
+    odd = [M(4, 8, rs=32, cs=2, base=0x10000 + 4 * e) for e in (0, 1)]
+    assert call(odd) == fine
+    assert call([odd[0], at(0, 100)]) == INVALID
+    # a matrix over itself, transposed
+    assert call([M(8, 8, base=0x10000)], [M(8, 8, rs=1, cs=8, base=0x10000)]) == INVALID
+    assert call([M(8, 8, rs=1, cs=8, base=0x10000)], [M(8, 8, rs=1, cs=8, base=0x10000)]) == fine
+
+
 def test_queries():
     lib = mt.lib()
     f = lib.mt_gated_linear_workspace_f32
