@@ -20,8 +20,8 @@ from typing import NamedTuple, Optional, Sequence, Union
 
 import torch
 
-from . import (MatF32, _api, _check, _handle, _nbytes, _ptr, _require_gpu, _stream, lib,
-               linear_backward, mat, native)
+from . import (MT_ERR_WORKSPACE, MatF32, _api, _check, _handle, _nbytes, _ptr, _require_gpu,
+               _require_ws, _stream, lib, linear_backward, mat, native)
 from .lowbit import (Q8Plan, Q8Rows, RowsQ8, _empty, _matrix, _rows, _vector, _ws,
                      linear_backward_q8)
 
@@ -187,8 +187,16 @@ def gated_linear_backward(dh: torch.Tensor, gu: torch.Tensor, x: Union[torch.Ten
         raise ValueError("gated_linear_backward: a dx to write to without the w that gives it")
     if (need_dw and dw is None and beta_w != 0.0) or (need_db and db is None and beta_b != 0.0):
         raise ValueError("gated_linear_backward: a beta without a gradient to add to")
+    for t in (dgu, dx, dw, db):
+        if t is not None and any(e > 1 and at == 0 for e, at in zip(t.shape, t.stride())):
+            raise ValueError("gated_linear_backward: an output must not be an expanded view")
     if q8:
         _rows(x)
+    if ws is not None:
+        need = (lib().mt_linear_backward_q8_workspace_f32 if q8 else lib().mt_linear_workspace_f32)(n, k, 2 * f)
+        _require_ws(ws)
+        if _nbytes(ws) < need:
+            _check(MT_ERR_WORKSPACE, "gated_linear_backward")
     dgu = gate_backward(dh, gu, act, dgu)
     if q8:
         return linear_backward_q8(dgu, x, w, need_dw, need_db, dx, dw, db, beta_w, beta_b, ws)

@@ -674,3 +674,53 @@ def test_refusals(dev):
             f()
     torch.cuda.synchronize()
     assert bool((x == 1).all())
+
+
+def test_backward_refuses_before_it_writes(dev):
+    """What is wrong with the second product's operands shows before the projections are
+    written over."""
+    g = rng(17)
+    x, w, gu, dh = (gpu(normal(g, *s), dev) for s in ((200, 96), (400, 96), (200, 400), (200, 200)))
+    was = gu.clone()
+    row = torch.zeros(1, 96, device=dev)
+    for q in (x, mt.quantize_q8(x)):
+        small = torch.empty(16, dtype=torch.uint8, device=dev)
+        need = (mt.lib().mt_linear_workspace_f32 if q is x else mt.lib().mt_linear_backward_q8_workspace_f32)(200, 96, 400)
+        for error, f in (
+                (ValueError, lambda: mt.gated_linear_backward(dh, gu, q, w, dgu=gu, dw=row.expand(400, 96))),
+                (ValueError, lambda: mt.gated_linear_backward(dh, gu, q, w, dgu=gu, dx=row.expand(200, 96))),
+                (ValueError, lambda: mt.gated_linear_backward(dh, gu, q, w, dgu=gu, db=row[0, :1].expand(400))),
+                (ValueError, lambda: mt.gated_linear_backward(dh, gu, q, w, dgu=gu, ws=torch.empty(1 << 24))),
+                (ValueError, lambda: mt.gated_linear_backward(dh, gu, q, w, dgu=gu, ws=small[:1].expand(1 << 24)))):
+            with pytest.raises(error):
+                f()
+        if need > 16:
+            with pytest.raises(RuntimeError):
+                mt.gated_linear_backward(dh, gu, q, w, dgu=gu, ws=small)
+        assert torch.equal(gu, was)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        a, b = mt.gated_linear_backward(dh, gu, q, w, ws=ws), mt.gated_linear_backward(dh, gu, q, w)
+        assert all(torch.equal(c, d) for c, d in zip(a, b))
+
+
+def test_two_threads(dev):
+    """Two threads, a stream each, one operator of another kind in flight beside each."""
+    import threading
+    inputs = [block_inputs(dev), block_inputs(dev, 67, 130, 300)]
+    want = [block(*i) for i in inputs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for n in range(10):
+                got = block(*inputs[i])
+                s.synchronize()
+                wrong.extend((i, n, j) for j, (a, b) in enumerate(zip(got, want[i])) if not torch.equal(a, b))
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
