@@ -37,8 +37,8 @@ int run_gate(const mt_mat_f32* GU, const mt_mat_f32* dH, const mt_mat_f32* out, 
 
 // ---- gated projections in fp32 ---------------------------------------------------------
 
-// How a call goes: few rows (the vector units, the fp32 matrix units), tiles of gemm_f32_sp with the gate in their
-// epilogue, or (operands with no neighbouring elements either way, or too far apart for the
+// How a call goes: few rows (the vector units, the fp32 matrix units), tiles of gemm_f32_sp
+// with the gate in their epilogue, or (operands with no neighbouring elements either way, or too far apart for the
 // tiles' 32-bit offsets) the product to memory first.
 enum GateKind { GATE_FEW, GATE_TILES, GATE_APART };
 constexpr int64_t kGemvRows = 4, kFewRows = 48;

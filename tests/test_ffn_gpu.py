@@ -97,7 +97,8 @@ def test_linear_q8(dev, m, n, k):
 
 
 # ... and outputs large enough for the larger tiles
-Q8_LARGE = [(1000, 4000, 1100), (1900, 4000, 200), (2000, 8190, 300), (2048, 8192, 256)]
+Q8_LARGE = [(1000, 4000, 1100), (1900, 4000, 200), (2000, 8190, 300), (2048, 8192, 256),
+            (1000, 4000, 1104), (2000, 8190, 336)]
 
 
 def test_linear_q8_kernels():
@@ -120,6 +121,17 @@ def test_linear_q8_large_tiles(dev, m, n, k):
         x = mt.Q8Rows(x.q, gpu(s / 16, dev))
         if n % 2 == 0:
             check(mt.gated_linear(x, wt, act="silu").h, *ref.gate("silu", gu, e), how)
+
+
+@pytest.mark.parametrize("m,n,k", [(70, 200, 33), (100, 300, 16), (513, 769, 650), (1000, 2000, 255), (2000, 8190, 300)])
+def test_linear_q8_one_operand_in_place(dev, m, n, k):
+    """Rows that the tiles read in place beside rows that are copied first, to the inputs that
+    there are, and both copied, to whole chunks."""
+    g = rng(18, m, n, k)
+    for a, b in (("by 16", "odd"), ("offset", "by 16"), ("odd", "offset"), ("by 16", "by 16")):
+        q, s, x = rows8(g, m, k, dev, a)
+        w, ws, wt = rows8(g, n, k, dev, b)
+        check(mt.linear_q8(x, wt), *ref.linear_q8(q, s, w, ws), a + ", " + b)
 
 
 @pytest.mark.parametrize("m", [1, 20, 40, 70])
