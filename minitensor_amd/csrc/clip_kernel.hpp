@@ -5,8 +5,9 @@
 // fp32 values are exact in fp64 and their sums are held there: nothing overflows, and a
 // model's 10^9 squares lose nothing that fp32 would show.
 //
-// A launch takes a table of up to kClipTensors tensors in its arguments (no memory beside the
-// workspace is written or read for it, so that a captured launch holds its own).  Dense
+// A launch takes a table of up to kClipTensors tensors in its arguments (half as many where
+// they are scaled into others; no memory beside the workspace is written or read for it, so
+// that a captured launch holds its own).  Dense
 // tensors are cut into chunks; a workgroup takes a run of neighbouring chunks, and leaves
 // one partial sum, all of which the scaling launch's workgroups add up again in the same
 // order.
@@ -20,21 +21,21 @@
 
 namespace mtk {
 
-constexpr int kClipTensors = 128;     // of a launch: 28 bytes each of 4 KB of arguments
+constexpr int kClipTensors = 256;     // of a launch: 14 bytes each of 4 KB of arguments
 constexpr int kClipThreads = 512, kClipQuads = 4;
 constexpr int kClipChunk = kClipThreads * kClipQuads * 4;   // elements
 constexpr int kClipBlocks = 1024;     // workgroups of a launch, at most: four on a CU
 constexpr int kClipMostParts = 4096;  // partial sums that every scaling workgroup adds up
 
 struct ClipTable {
-    const float* src[kClipTensors];
-    float* dst[kClipTensors];
-    int64_t n[kClipTensors];
+    float* at[kClipTensors];          // tensors, and their outputs from `to` on (0: themselves)
     uint32_t first[kClipTensors];     // chunk of the launch that the tensor starts with (past
                                       // the last tensor: the largest number)
-    int count;
+    uint16_t last[kClipTensors];      // elements of its last chunk, less one
+    int count, to;
     uint32_t chunks;
 };
+static_assert(kClipChunk <= 1 << 16, "a chunk's elements in 16 bits");
 static_assert(sizeof(ClipTable) <= 3840, "kernel arguments");
 
 // A tensor of any strides.
@@ -97,14 +98,15 @@ struct ClipPiece {
     float* dst;
     int n;                            // elements, at most kClipChunk
 };
-// (the tensor of a chunk: one look at every tensor's first chunk, a lane two of them)
+// (the tensor of a chunk: one look at every tensor's first chunk, a lane four of them)
 __device__ __forceinline__ ClipPiece clip_piece(const ClipTable& t, uint32_t c) {
-    static_assert(kClipTensors == 128, "two tensors a lane");
-    const int lane = threadIdx.x & 63;
-    const int k = __builtin_amdgcn_readfirstlane(__popcll(__ballot(t.first[lane] <= c)) +
-                                                 __popcll(__ballot(t.first[64 + lane] <= c)) - 1);
+    int n = -1;
+#pragma unroll
+    for (int i = threadIdx.x & 63; i < kClipTensors; i += 64) n += __popcll(__ballot(t.first[i] <= c));
+    const int k = __builtin_amdgcn_readfirstlane(n);
+    const uint32_t end = k + 1 < t.count ? t.first[k + 1] : t.chunks;
     const int64_t at = (int64_t)(c - t.first[k]) * kClipChunk;
-    return {t.src[k] + at, t.dst[k] + at, (int)min(t.n[k] - at, (int64_t)kClipChunk)};
+    return {t.at[k] + at, t.at[k + t.to] + at, c + 1 == end ? t.last[k] + 1 : kClipChunk};
 }
 // A thread's groups of four, zeros past the end, and (thread < n % 4) one of the last elements.
 struct ClipValues {

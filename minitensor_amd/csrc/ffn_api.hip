@@ -296,17 +296,20 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
     double* const part = static_cast<double*>(workspace);
 
     // Launches: the dense tensors' by the table, the others' one by one.
-    auto launches = [&](auto table, auto single) {
+    auto launches = [&](bool apart, auto table, auto single) {
         ClipTable t;
-        t.count = 0;
-        t.chunks = 0;
-        std::fill(t.first, t.first + kClipTensors, ~0u);
-        auto flush = [&] {
-            if (t.count > 0) table(t, std::min<uint32_t>(t.chunks, kClipBlocks));
+        auto clear = [&] {
             t.count = 0;
             t.chunks = 0;
             std::fill(t.first, t.first + kClipTensors, ~0u);
         };
+        auto flush = [&] {
+            if (t.count > 0) table(t, std::min<uint32_t>(t.chunks, kClipBlocks));
+            clear();
+        };
+        clear();
+        t.to = apart ? kClipTensors / 2 : 0;
+        const int most = kClipTensors - t.to;
         for (int64_t i = 0; i < count; ++i) {
             tensor_of(&grads[i], &to[i], scale, &d);
             if (d.n == 0) continue;
@@ -315,10 +318,10 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
                 continue;
             }
             const int64_t chunks = (d.n + kClipChunk - 1) / kClipChunk;
-            if (t.count == kClipTensors || t.chunks + chunks > (int64_t)1 << 31) flush();
-            t.src[t.count] = d.src;
-            t.dst[t.count] = d.dst;
-            t.n[t.count] = d.n;
+            if (t.count == most || t.chunks + chunks > (int64_t)1 << 31) flush();
+            t.at[t.count] = const_cast<float*>(d.src);
+            if (apart) t.at[t.count + t.to] = d.dst;
+            t.last[t.count] = (uint16_t)((d.n - 1) % kClipChunk);
             t.first[t.count++] = t.chunks;
             t.chunks += (uint32_t)chunks;
         }
@@ -326,6 +329,7 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
     };
     int parts = 0;
     launches(
+        false,
         [&](const ClipTable& t, unsigned blocks) {
             hipLaunchKernelGGL(clip_squares, dim3(blocks), dim3(kClipThreads), 0, s, t, part + parts);
             parts += (int)blocks;
@@ -346,6 +350,7 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
         c = {part + parts, 1, norm, most, eps};
     }
     launches(
+        out != nullptr,
         [&](const ClipTable& t, unsigned blocks) {
             if (past) hipLaunchKernelGGL(clip_scale<true>, dim3(blocks), dim3(kClipThreads), 0, s, t, c);
             else hipLaunchKernelGGL(clip_scale<false>, dim3(blocks), dim3(kClipThreads), 0, s, t, c);

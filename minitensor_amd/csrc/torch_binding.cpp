@@ -624,6 +624,80 @@ py::object gate_backward(py::handle pdh, py::handle pgu, int act, py::handle pou
     return pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout);
 }
 
+// The gradient at the projections, then the Linear layer's from it; x: fp32 rows (pxscale None)
+// or 8-bit ones.  Nothing is enqueued before all checks (dgu may be gu itself).
+py::object gated_linear_backward(py::handle pdh, py::handle pgu, py::handle px, py::handle pxscale,
+                                 py::handle pw, int act, bool need_dw, bool need_db,
+                                 py::handle pdgu, py::handle pdx, py::handle pdw, py::handle pdb,
+                                 float beta_w, float beta_b, py::handle pws, py::handle stream) {
+    bool ok = true;
+    const bool q8 = !pxscale.is_none();
+    const at::Tensor gws = given_ws(pws, &ok);
+    const at::Tensor dh = arg(pdh, &ok), gu = arg(pgu, &ok), w = arg(pw, &ok);
+    const at::Tensor x = q8 ? rows_arg(px, at::kChar, 2, &ok) : arg(px, &ok);
+    at::Tensor xscale;
+    if (q8) xscale = rows_arg(pxscale, at::kFloat, 1, &ok);
+    at::Tensor dgu = arg(pdgu, &ok), dx = arg(pdx, &ok), dw = arg(pdw, &ok), db = arg(pdb, &ok);
+    if (!ok || !dh.defined() || !gu.defined() || !x.defined() || dh.dim() != 2 || x.dim() != 2 ||
+        !here(dh, gu, x, xscale, w, dgu, dx, dw, db))
+        return py::none();
+    const int64_t n = dh.size(0), f2 = 2 * dh.size(1), k = x.size(1);
+    const bool need_dx = w.defined();
+    const auto expanded = [](const at::Tensor& t) {
+        for (int64_t i = 0; t.defined() && i < t.dim(); ++i)
+            if (t.size(i) > 1 && t.stride(i) == 0) return true;
+        return false;
+    };
+    if (x.size(0) != n || (q8 && xscale.size(0) != n) || !shaped(gu, n, f2) || !shaped(dgu, n, f2) ||
+        !shaped(w, f2, k) || !shaped(dx, n, k) || !shaped(dw, f2, k) || !vec_of(db, f2) ||
+        (dx.defined() && !need_dx) || (need_dw && !dw.defined() && beta_w != 0.f) ||
+        (need_db && !db.defined() && beta_b != 0.f) || expanded(dgu) || expanded(dx) ||
+        expanded(dw) || expanded(db))
+        return py::none();
+    const size_t need = q8 ? mt_linear_backward_q8_workspace_f32(n, k, f2)
+                           : mt_linear_workspace_f32(n, k, f2);
+    if (gws.defined() && gws.nbytes() < need) return py::none();
+    void* const s = stream_of(stream);
+    {
+        const py::gil_scoped_release nogil;
+        if (!dgu.defined()) dgu = empty({n, f2}, dh);
+        if (need_dx && !dx.defined()) dx = empty({n, k}, dh);
+        if (need_dw && !dw.defined()) dw = empty({f2, k}, dh);
+        if (need_db && !db.defined()) db = empty({f2}, dh);
+        const Workspace ws(gws, dh, [&] { return need; });
+        const mt_mat_f32 mdh = mat(dh), mgu = mat(gu), mdgu = mat(dgu);
+        check(mt_gate_backward_f32(&mdh, &mgu, act, &mdgu, s), "mt_gate_backward_f32");
+        // (without a w there is no dx, and nothing reads what stands in for it)
+        mt_mat_f32 mw{ptr(dgu), 0, f2, k, 0, 0, 1, 0}, mdx{}, mdw{};
+        if (need_dx) {
+            mw = mat(w);
+            mdx = mat(dx);
+        }
+        if (need_dw) mdw = mat(dw);
+        float* const pb = need_db ? out_ptr(db) : nullptr;
+        const int64_t bs = need_db ? step(db) : 0;
+        if (q8) {
+            const mt_rows_q8 mq = rows_q8(x, xscale);
+            check(mt_linear_backward_q8_f32(&mdgu, &mq, need_dx ? &mw : nullptr,
+                                            need_dx ? &mdx : nullptr, need_dw ? &mdw : nullptr,
+                                            beta_w, pb, bs, beta_b, ws.p, ws.n, s),
+                  "mt_linear_backward_q8_f32");
+        } else {
+            const mt_mat_f32 mx = mat(x);
+            check(mt_linear_backward_f32(&mdgu, &mx, &mw, need_dx ? &mdx : nullptr,
+                                         need_dw ? &mdw : nullptr, beta_w, pb, bs, beta_b, ws.p,
+                                         ws.n, s),
+                  "mt_linear_backward_f32");
+        }
+    }
+    const auto back = [](bool need, py::handle given, const at::Tensor& t) {
+        return !need             ? py::object(py::none())
+               : given.is_none() ? tensor(t)
+                                 : py::reinterpret_borrow<py::object>(given);
+    };
+    return py::make_tuple(back(need_dx, pdx, dx), back(need_dw, pdw, dw), back(need_db, pdb, db));
+}
+
 // Lists of tensors that are each one run of elements, in the same order in both; anything
 // else is the caller's.
 py::object clip(py::handle pgrads, py::handle pout, bool scale, float most, float eps,
@@ -682,5 +756,6 @@ PYBIND11_MODULE(_native, m) {
     m.def("linear_q8", &linear_q8);
     m.def("gated_linear", &gated_linear);
     m.def("gate_backward", &gate_backward);
+    m.def("gated_linear_backward", &gated_linear_backward);
     m.def("clip", &clip);
 }

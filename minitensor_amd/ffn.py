@@ -172,8 +172,13 @@ def gated_linear_backward(dh: torch.Tensor, gu: torch.Tensor, x: Union[torch.Ten
 
     `dgu` [R, 2F]: where the gradient at the projections goes, which may be gu itself.
     dW = beta_w·dw + ∂L/∂W and db = beta_b·db + ∂L/∂b where a dw, db is passed."""
+    a, q8 = _act(act, "gated_linear_backward"), isinstance(x, Q8Rows)
+    r = native().gated_linear_backward(dh, gu, x[0] if q8 else x, x[1] if q8 else None, w, a,
+                                       bool(need_dw), bool(need_db), dgu, dx, dw, db, beta_w, beta_b,
+                                       ws, _handle(stream))
+    if r is not None:
+        return r
     # (all checks first: dgu may be written over gu)
-    q8 = isinstance(x, Q8Rows)
     _here(dh, gu, dgu, x[1] if q8 else x, w, dx, dw, db)
     rows = x[0] if q8 else x
     if dh.dim() != 2 or rows.dim() != 2 or rows.shape[0] != dh.shape[0]:
