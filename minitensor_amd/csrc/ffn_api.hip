@@ -247,35 +247,40 @@ bool tensor_of(const mt_mat_f32* g, const mt_mat_f32* o, bool written, Tensor* t
     return true;
 }
 
-// What a tensor's elements lie in, of a strided one its first element: views may lie between
+// What tensors' elements lie in, of a strided one its first element: views may lie between
 // each other's elements.
 struct Extent {
     const float *begin, *end;
-    bool written;
+    bool operator<(const Extent& o) const { return std::less<const float*>()(begin, o.begin); }
 };
-// Adds t's to `all`; false where its output is over itself in another order.
-bool add_extents(const Tensor& t, std::vector<Extent>& all) {
-    all.push_back({t.dst, t.dst + (t.dense ? t.n : 1), true});
-    if (t.src != t.dst) {
-        all.push_back({t.src, t.src + (t.dense ? t.n : 1), false});
+struct Extents {
+    std::vector<Extent> written, read;
+    // false where t's output is over itself in another order
+    bool add(const Tensor& t) {
+        const int64_t n = t.dense ? t.n : 1;
+        written.push_back({t.dst, t.dst + n});
+        if (t.src != t.dst) {
+            read.push_back({t.src, t.src + n});
+            return true;
+        }
+        for (int i = 0; i < 3 && !t.dense; ++i)
+            if (t.strided.size[i] > 1 && t.strided.src_stride[i] != t.strided.dst_stride[i]) return false;
         return true;
     }
-    for (int i = 0; i < 3 && !t.dense; ++i)
-        if (t.strided.size[i] > 1 && t.strided.src_stride[i] != t.strided.dst_stride[i]) return false;
-    return true;
-}
-// Whether something written lies over another tensor.
-bool overlapping(std::vector<Extent>& all) {
-    std::sort(all.begin(), all.end(),
-              [](const Extent& a, const Extent& b) { return std::less<const float*>()(a.begin, b.begin); });
-    const float *read = nullptr, *written = nullptr;   // ends so far
-    for (const Extent& e : all) {
-        if (e.begin < written || (e.written && e.begin < read)) return true;
-        const float*& end = e.written ? written : read;
-        end = std::max(end, e.end);
+    // whether something written lies over another tensor
+    bool overlap() {
+        for (auto* v : {&written, &read})              // (out of one buffer they are in order)
+            if (!std::is_sorted(v->begin(), v->end())) std::sort(v->begin(), v->end());
+        for (size_t i = 1; i < written.size(); ++i)
+            if (written[i].begin < written[i - 1].end) return true;
+        size_t i = 0;
+        for (const Extent& r : read) {
+            while (i < written.size() && written[i].end <= r.begin) ++i;
+            if (i < written.size() && written[i].begin < r.end) return true;
+        }
+        return false;
     }
-    return false;
-}
+};
 
 int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool scale,
              float most, float eps, float* norm, void* workspace, size_t ws_bytes, hipStream_t s) {
@@ -283,14 +288,14 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
     if (scale && (!(most >= 0.f) || !(eps >= 0.f))) return MT_ERR_INVALID;
     const mt_mat_f32* const to = out ? out : grads;
     Tensor d{};
-    std::vector<Extent> extents;
+    Extents extents;
     int64_t all = 0;
     for (int64_t i = 0; i < count; ++i) {
         if (!tensor_of(&grads[i], &to[i], scale, &d)) return MT_ERR_INVALID;
         all += d.n;
-        if (scale && d.n > 0 && !add_extents(d, extents)) return MT_ERR_INVALID;
+        if (scale && d.n > 0 && !extents.add(d)) return MT_ERR_INVALID;
     }
-    if (overlapping(extents)) return MT_ERR_INVALID;
+    if (extents.overlap()) return MT_ERR_INVALID;
     const size_t need = mt_grad_norm_workspace_f32(count);
     if (!workspace || ws_bytes < need || ((uintptr_t)workspace & 7)) return MT_ERR_WORKSPACE;
     double* const part = static_cast<double*>(workspace);

@@ -709,20 +709,25 @@ py::object clip(py::handle pgrads, py::handle pout, bool scale, float most, floa
     const Py_ssize_t n = PyList_GET_SIZE(pgrads.ptr());
     if (n == 0 || (own && PyList_GET_SIZE(pout.ptr()) != n)) return py::none();
     std::vector<mt_mat_f32> g((size_t)n), o(own ? (size_t)n : 0);
-    at::Tensor first;
-    for (Py_ssize_t i = 0; i < n; ++i) {
-        const at::Tensor t = arg(PyList_GET_ITEM(pgrads.ptr(), i), &ok);
-        if (!ok || !t.defined() || !t.is_contiguous() || !here(t)) return py::none();
+    // (hundreds of tensors: no copies of their handles, the device asked for once)
+    const auto device = c10::hip::current_device();
+    const auto run = [&](PyObject* list, Py_ssize_t i, mt_mat_f32& m) -> const at::Tensor* {
+        PyObject* const item = PyList_GET_ITEM(list, i);
+        if (!THPVariable_Check(item)) return nullptr;
+        const at::Tensor& t = THPVariable_Unpack(item);
+        if (!plain(t) || !t.is_contiguous() || t.get_device() != device) return nullptr;
         const int64_t e = t.numel();
-        g[(size_t)i] = mt_mat_f32{ptr(t), 0, 1, e, e, 1, 1, 0};
-        if (own) {
-            const at::Tensor u = arg(PyList_GET_ITEM(pout.ptr(), i), &ok);
-            if (!ok || !u.defined() || !u.is_contiguous() || !here(u) || u.sizes() != t.sizes())
-                return py::none();
-            o[(size_t)i] = mt_mat_f32{ptr(u), 0, 1, e, e, 1, 1, 0};
-        }
-        if (i == 0) first = t;
+        m = mt_mat_f32{ptr(t), 0, 1, e, e, 1, 1, 0};
+        return &t;
+    };
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const at::Tensor* const t = run(pgrads.ptr(), i, g[(size_t)i]);
+        if (!t) return py::none();
+        if (!own) continue;
+        const at::Tensor* const u = run(pout.ptr(), i, o[(size_t)i]);
+        if (!u || u->sizes() != t->sizes()) return py::none();
     }
+    const at::Tensor first = THPVariable_Unpack(PyList_GET_ITEM(pgrads.ptr(), 0));
     void* const s = stream_of(stream);
     at::Tensor norm;
     {
