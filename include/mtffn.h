@@ -56,6 +56,14 @@ int mt_gate_f32(const mt_mat_f32* GU, int act, const mt_mat_f32* H, void* stream
 int mt_gate_backward_f32(const mt_mat_f32* dH, const mt_mat_f32* GU, int act,
                          const mt_mat_f32* dGU, void* stream);
 
+/* ... and db = beta*db + the sums of dGU over the rows, the gradient of the projections' bias,
+ * from the same pass (mt_linear_backward_f32 then needs no db).  beta 0: db is not read.
+ * workspace: a multiple of 4. */
+int mt_gate_backward_bias_f32(const mt_mat_f32* dH, const mt_mat_f32* GU, int act,
+                              const mt_mat_f32* dGU, float* db, int64_t db_stride, float beta,
+                              void* workspace, size_t ws_bytes, void* stream);
+size_t mt_gate_backward_bias_workspace_f32(int64_t rows, int64_t features);
+
 /* ---- gradients of a whole model ----------------------------------------------------
  * norm = sqrt(sum of the squares of every element of every tensor), held in fp64 until it is
  * rounded to fp32.  Tensors are views of up to three axes (batch, rows, cols), each below 2^42

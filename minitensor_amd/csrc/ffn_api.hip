@@ -35,6 +35,37 @@ int run_gate(const mt_mat_f32* GU, const mt_mat_f32* dH, const mt_mat_f32* out, 
     return launched();
 }
 
+// The gradients with their sums over the rows: runs of rows, 16 at least, for eight workgroups
+// on a CU.
+int64_t bias_run(int64_t rows, int64_t strips) {
+    const int64_t runs = std::min((rows + 15) / 16, std::max<int64_t>(8 * kCus / strips, 1));
+    return ((rows + runs - 1) / runs + 3) / 4 * 4;
+}
+int64_t bias_runs(int64_t rows, int64_t strips) {
+    const int64_t run = bias_run(rows, strips);
+    return (rows + run - 1) / run;
+}
+int run_gate_bias(const mt_mat_f32* dH, const mt_mat_f32* GU, int act, const mt_mat_f32* dGU,
+                  const GateBias& b, void* workspace, size_t ws_bytes, hipStream_t s) {
+    const int64_t M = GU->rows, F = dH->cols;
+    if (F == 0) return MT_OK;
+    GateParams p{view(GU), view(dH), view(dGU), M, (int)F, act};
+    const bool units = unit(p.gu) && unit(p.dh) && unit(p.out);
+    const int64_t strips = (F + (units ? 255 : 63)) / (units ? 256 : 64);
+    if (strips >= kMaxTiles) return MT_ERR_INVALID;
+    const int64_t run = M ? bias_run(M, strips) : 4, runs = M ? bias_runs(M, strips) : 1;
+    if (run >= kMaxDim) return MT_ERR_INVALID;
+    float* const part = static_cast<float*>(workspace);
+    if (runs > 1 && (!workspace || ws_bytes < (size_t)(runs * 2 * F) * 4)) return MT_ERR_WORKSPACE;
+    const dim3 grid((unsigned)strips, (unsigned)runs);
+    if (units) hipLaunchKernelGGL(gate_rows_sums<true>, grid, dim3(256), 0, s, p, b, part, (int)run);
+    else hipLaunchKernelGGL(gate_rows_sums<false>, grid, dim3(256), 0, s, p, b, part, (int)run);
+    if (runs > 1)
+        hipLaunchKernelGGL(gate_bias_sum<>, dim3((unsigned)((2 * F + 63) / 64)), dim3(512), 0, s, part,
+                           (int)runs, 2 * F, b);
+    return launched();
+}
+
 // ---- gated projections in fp32 ---------------------------------------------------------
 
 // How a call goes: few rows (the vector units, the fp32 matrix units), tiles of gemm_f32_sp
@@ -383,6 +414,24 @@ int mt_gate_backward_f32(const mt_mat_f32* dH, const mt_mat_f32* GU, int act, co
         GU->rows != dH->rows || GU->cols != 2 * dH->cols || !same_shape(GU, dGU))
         return MT_ERR_INVALID;
     return run_gate<true>(GU, dH, dGU, dH->cols, act, stream);
+}
+
+size_t mt_gate_backward_bias_workspace_f32(int64_t rows, int64_t features) {
+    if (rows <= 0 || features <= 0 || rows >= kMaxDim || features >= kMaxDim / 2) return 0;
+    // (of rows with neighbouring elements: of others the runs are fewer)
+    const int64_t runs = bias_runs(rows, (features + 255) / 256);
+    return runs > 1 ? (size_t)(runs * 2 * features) * 4 : 0;
+}
+
+int mt_gate_backward_bias_f32(const mt_mat_f32* dH, const mt_mat_f32* GU, int act,
+                              const mt_mat_f32* dGU, float* db, int64_t db_stride, float beta,
+                              void* workspace, size_t ws_bytes, void* stream) {
+    if (!valid(dH, false) || !valid(GU, false) || !valid(dGU, true) || !valid_act(act) ||
+        GU->rows != dH->rows || GU->cols != 2 * dH->cols || !same_shape(GU, dGU) ||
+        (dH->cols > 0 && (!db || db_stride <= 0)) || ((uintptr_t)workspace & 3) != 0)
+        return MT_ERR_INVALID;
+    return run_gate_bias(dH, GU, act, dGU, {db, db_stride, beta}, workspace, ws_bytes,
+                         static_cast<hipStream_t>(stream));
 }
 
 size_t mt_gated_linear_workspace_f32(const mt_mat_f32* X, const mt_mat_f32* W) {

@@ -84,6 +84,27 @@ __device__ __forceinline__ rowf4 gate4(int act, const rowf4& g, const rowf4& u) 
     return h;
 }
 
+// Projections g, u, and the gradient dh at act(g)*u, to the gradients at them.
+__device__ __forceinline__ void gate_slopes(int act, float dh, float& g, float& u) {
+    with_act(act, [&](auto a) {
+        float d;
+        const float v = act_at<a(), true>(g, d);
+        g = dh * u * d;
+        u = dh * v;
+    });
+}
+__device__ __forceinline__ void gate_slopes(int act, const rowf4& dh, rowf4& g, rowf4& u) {
+    with_act(act, [&](auto a) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float d;
+            const float v = act_at<a(), true>(g[e], d);
+            g[e] = dh[e] * u[e] * d;
+            u[e] = dh[e] * v;
+        }
+    });
+}
+
 struct GateParams {
     RowView gu;                       // [M][2F], the gates first
     RowView dh;                       // backward
@@ -121,27 +142,83 @@ __global__ void __launch_bounds__(256) gate_rows(GateParams p) {
         } else {
             const auto dh = row_load<MODE>(p.dh, m, f, p.F);
             auto dg = g, du = u;
-            with_act(p.act, [&](auto a) {
-                if constexpr (VEC) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float d;
-                        const float v = act_at<a(), true>(g[e], d);
-                        dg[e] = dh[e] * u[e] * d;
-                        du[e] = dh[e] * v;
-                    }
-                } else {
-                    float d;
-                    const float v = act_at<a(), true>(g, d);
-                    dg = dh * u * d;
-                    du = dh * v;
-                }
-            });
+            gate_slopes(p.act, dh, dg, du);
             const RowView dup{p.out.p + (int64_t)p.F * p.out.cs, p.out.rs, p.out.cs};
             row_store<MODE>(p.out, m, f, p.F, dg);
             row_store<MODE>(dup, m, f, p.F, du);
         }
     }
+}
+
+// The gradients as gate_rows gives them, and their sums over the rows (a bias's gradient) from
+// the same pass.  A workgroup owns a strip of features -- 64 lanes of four, or one -- and a run
+// of rows, which its four waves take in turn; the runs' sums go to `part` [runs][2F], or, of one
+// run, to the bias gradient.  (8192 x 2 x 2048, with the runs' sums together: 75 us, 55 without
+// sums; strips four times as wide 71, but 509 x 2 x 2570 24 against 13.)
+struct GateBias {
+    float* db;
+    int64_t stride;
+    float beta;                       // 0: what was there is not read
+};
+__device__ __forceinline__ void bias_put(const GateBias& b, int64_t c, double sum) {
+    float* const d = b.db + c * b.stride;
+    *d = (float)(b.beta == 0.f ? sum : sum + (double)b.beta * *d);
+}
+template <bool VEC>
+__global__ void __launch_bounds__(256) gate_rows_sums(GateParams p, GateBias b, float* part, int run) {
+    constexpr int E = VEC ? 4 : 1, STRIP = 64 * E, MODE = VEC ? R_TAIL : R_STRIDED;
+    __shared__ float red[2][4][STRIP];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int f0 = blockIdx.x * STRIP, f = f0 + lane * E;
+    const int64_t first = (int64_t)blockIdx.y * run, end = min(first + run, p.M);
+    const RowView up{p.gu.p + (int64_t)p.F * p.gu.cs, p.gu.rs, p.gu.cs};
+    const RowView dup{p.out.p + (int64_t)p.F * p.out.cs, p.out.rs, p.out.cs};
+    using V = std::conditional_t<VEC, rowf4, float>;
+    V sg{}, su{};
+    if (f < p.F) {
+#pragma unroll 2
+        for (int64_t m = first + wave; m < end; m += 4) {
+            V g = row_load<MODE>(p.gu, m, f, p.F), u = row_load<MODE>(up, m, f, p.F);
+            const V dh = row_load<MODE>(p.dh, m, f, p.F);
+            gate_slopes(p.act, dh, g, u);
+            row_store<MODE>(p.out, m, f, p.F, g);
+            row_store<MODE>(dup, m, f, p.F, u);
+            sg += g;
+            su += u;
+        }
+    }
+    *reinterpret_cast<V*>(&red[0][wave][lane * E]) = sg;
+    *reinterpret_cast<V*>(&red[1][wave][lane * E]) = su;
+    __syncthreads();
+    for (int i = t; i < 2 * STRIP; i += 256) {
+        const int h = i / STRIP, c = i % STRIP;
+        if (f0 + c >= p.F) continue;
+        float s = red[h][0][c];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) s += red[h][w][c];
+        const int64_t col = (int64_t)h * p.F + f0 + c;
+        if (gridDim.y == 1) bias_put(b, col, s);
+        else part[blockIdx.y * 2 * (int64_t)p.F + col] = s;
+    }
+}
+// The runs' sums together, in fp64: 64 columns a workgroup, whose waves take the runs in turn.
+template <int W = 8>
+__global__ void __launch_bounds__(64 * W) gate_bias_sum(const float* part, int runs, int64_t cols, GateBias b) {
+    __shared__ double red[W][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    double s = 0;
+    if (c < cols) {
+#pragma unroll 8
+        for (int r = wave; r < runs; r += W) s += part[r * cols + c];
+    }
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave > 0 || c >= cols) return;
+    s = red[0][lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) s += red[w][lane];
+    bias_put(b, c, s);
 }
 
 }  // namespace mtk

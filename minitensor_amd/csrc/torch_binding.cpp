@@ -624,6 +624,13 @@ py::object gate_backward(py::handle pdh, py::handle pgu, int act, py::handle pou
     return pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout);
 }
 
+// Projections beyond which their bias's gradient comes from the pass over them, not with dW,
+// whose product has no sums where it is split and none for some layouts.  (us with dX and dW,
+// with the product, from the pass: 4096 x 1024 -> 4096 497, 403; 2048 x 512 -> 4096 195, 139;
+// 509 x 1285 -> 5140 150, 139; 600 x 1000 -> 4000 93, 94; 4096 x 2048 -> 8192 1383, 1383; of
+// fewer the pass's second launch costs more: 512 x 512 -> 2048 39, 44; 2293 x 275 -> 260 32, 41.)
+constexpr int64_t kSumsFrom = (int64_t)1 << 20;
+
 // The gradient at the projections, then the Linear layer's from it; x: fp32 rows (pxscale None)
 // or 8-bit ones.  Nothing is enqueued before all checks (dgu may be gu itself).
 py::object gated_linear_backward(py::handle pdh, py::handle pgu, py::handle px, py::handle pxscale,
@@ -654,8 +661,11 @@ py::object gated_linear_backward(py::handle pdh, py::handle pgu, py::handle px, 
         (need_db && !db.defined() && beta_b != 0.f) || expanded(dgu) || expanded(dx) ||
         expanded(dw) || expanded(db))
         return py::none();
-    const size_t need = q8 ? mt_linear_backward_q8_workspace_f32(n, k, f2)
-                           : mt_linear_workspace_f32(n, k, f2);
+    // (the one after the other)
+    const bool sums = !q8 && need_db && n * f2 > kSumsFrom;
+    const size_t need = std::max(q8 ? mt_linear_backward_q8_workspace_f32(n, k, f2)
+                                    : mt_linear_workspace_f32(n, k, f2),
+                                 sums ? mt_gate_backward_bias_workspace_f32(n, f2 / 2) : 0);
     if (gws.defined() && gws.nbytes() < need) return py::none();
     void* const s = stream_of(stream);
     {
@@ -666,7 +676,13 @@ py::object gated_linear_backward(py::handle pdh, py::handle pgu, py::handle px, 
         if (need_db && !db.defined()) db = empty({f2}, dh);
         const Workspace ws(gws, dh, [&] { return need; });
         const mt_mat_f32 mdh = mat(dh), mgu = mat(gu), mdgu = mat(dgu);
-        check(mt_gate_backward_f32(&mdh, &mgu, act, &mdgu, s), "mt_gate_backward_f32");
+        float* const pb = need_db ? out_ptr(db) : nullptr;
+        const int64_t bs = need_db ? step(db) : 0;
+        if (sums)
+            check(mt_gate_backward_bias_f32(&mdh, &mgu, act, &mdgu, pb, bs, beta_b, ws.p, ws.n, s),
+                  "mt_gate_backward_bias_f32");
+        else
+            check(mt_gate_backward_f32(&mdh, &mgu, act, &mdgu, s), "mt_gate_backward_f32");
         // (without a w there is no dx, and nothing reads what stands in for it)
         mt_mat_f32 mw{ptr(dgu), 0, f2, k, 0, 0, 1, 0}, mdx{}, mdw{};
         if (need_dx) {
@@ -674,8 +690,6 @@ py::object gated_linear_backward(py::handle pdh, py::handle pgu, py::handle px, 
             mdx = mat(dx);
         }
         if (need_dw) mdw = mat(dw);
-        float* const pb = need_db ? out_ptr(db) : nullptr;
-        const int64_t bs = need_db ? step(db) : 0;
         if (q8) {
             const mt_rows_q8 mq = rows_q8(x, xscale);
             check(mt_linear_backward_q8_f32(&mdgu, &mq, need_dx ? &mw : nullptr,
@@ -685,8 +699,8 @@ py::object gated_linear_backward(py::handle pdh, py::handle pgu, py::handle px, 
         } else {
             const mt_mat_f32 mx = mat(x);
             check(mt_linear_backward_f32(&mdgu, &mx, &mw, need_dx ? &mdx : nullptr,
-                                         need_dw ? &mdw : nullptr, beta_w, pb, bs, beta_b, ws.p,
-                                         ws.n, s),
+                                         need_dw ? &mdw : nullptr, beta_w, sums ? nullptr : pb,
+                                         sums ? 0 : bs, beta_b, ws.p, ws.n, s),
                   "mt_linear_backward_f32");
         }
     }

@@ -21,7 +21,7 @@ from typing import NamedTuple, Optional, Sequence, Union
 import torch
 
 from . import (MT_ERR_WORKSPACE, MatF32, _api, _check, _handle, _nbytes, _ptr, _require_gpu,
-               _require_ws, _stream, lib, linear_backward, mat, native)
+               _stream, lib, linear_backward, mat, native)
 from .lowbit import (Q8Plan, Q8Rows, RowsQ8, _empty, _matrix, _rows, _vector, _ws,
                      linear_backward_q8)
 
@@ -51,6 +51,8 @@ SIGS = {
     "mt_gated_linear_q8_plan": (_I, [_I64] * 3 + [_P(Q8Plan)]),
     "mt_gate_f32": (_I, [_M, _I, _M, _V]),
     "mt_gate_backward_f32": (_I, [_M, _M, _I, _M, _V]),
+    "mt_gate_backward_bias_f32": (_I, [_M, _M, _I, _M, _V, _I64, _F, _V, _S, _V]),
+    "mt_gate_backward_bias_workspace_f32": (_S, [_I64, _I64]),
     "mt_grad_norm_f32": (_I, [_M, _I64, _V, _V, _S, _V]),
     "mt_clip_grad_norm_f32": (_I, [_M, _M, _I64, _F, _F, _V, _V, _S, _V]),
     "mt_grad_norm_workspace_f32": (_S, [_I64]),
@@ -161,6 +163,11 @@ def gate_backward(dh: torch.Tensor, gu: torch.Tensor, act: str = "silu",
     return out
 
 
+# (projections beyond which their bias's gradient comes from the pass over them, as in the
+# native call)
+_SUMS_FROM = 1 << 20
+
+
 @_api
 def gated_linear_backward(dh: torch.Tensor, gu: torch.Tensor, x: Union[torch.Tensor, Q8Rows],
                           w: Optional[torch.Tensor] = None, act: str = "silu",
@@ -197,19 +204,31 @@ def gated_linear_backward(dh: torch.Tensor, gu: torch.Tensor, x: Union[torch.Ten
             raise ValueError("gated_linear_backward: an output must not be an expanded view")
     if q8:
         _rows(x)
-    if ws is not None:
+    sums = not q8 and need_db and 2 * n * f > _SUMS_FROM
+    if ws is not None or sums:
         need = (lib().mt_linear_backward_q8_workspace_f32 if q8 else lib().mt_linear_workspace_f32)(n, k, 2 * f)
-        _require_ws(ws)
+        if sums:
+            need = max(need, lib().mt_gate_backward_bias_workspace_f32(n, f))
+        ws = _ws(ws, need, dh)
         if _nbytes(ws) < need:
             _check(MT_ERR_WORKSPACE, "gated_linear_backward")
-    dgu = gate_backward(dh, gu, act, dgu)
+    if sums:
+        if db is None:
+            db = _empty((2 * f,), dh)
+        if dgu is None:
+            dgu = _empty((n, 2 * f), dh)
+        rc = lib().mt_gate_backward_bias_f32(mat(dh), mat(gu), a, mat(dgu), *_vector(db, 2 * f, "db"),
+                                             float(beta_b), _ptr(ws), _nbytes(ws), _stream(stream))
+        _check(rc, "mt_gate_backward_bias_f32")
+    else:
+        dgu = gate_backward(dh, gu, act, dgu)
     if q8:
         return linear_backward_q8(dgu, x, w, need_dw, need_db, dx, dw, db, beta_w, beta_b, ws)
     # (without a w there is no dx, and nothing reads the one that stands in for it)
     any_w = x.new_empty((1, 1)).expand(2 * f, k) if w is None else w
-    dx, dw, db = linear_backward(dgu, x, any_w, w is not None, need_dw, need_db, dx, dw, db, beta_w,
-                                 beta_b, ws)
-    return dx, dw if need_dw else None, db if need_db else None
+    dx, dw, own = linear_backward(dgu, x, any_w, w is not None, need_dw, need_db and not sums, dx,
+                                  dw, db, beta_w, beta_b, ws)
+    return dx, dw if need_dw else None, (db if sums else own) if need_db else None
 
 
 def _axes(g: torch.Tensor, o: torch.Tensor):

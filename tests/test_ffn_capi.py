@@ -116,6 +116,22 @@ def test_gate_refuses():
     assert b(R(M(4, 0)), R(M(4, 0)), 0, R(M(4, 0)), None) == OK
 
 
+def test_gate_backward_bias_refuses():
+    def b(dh=M(4, 4), gu=M(4, 8), act=0, dgu=M(4, 8), db=0x5000, stride=1, ws=None, n=0):
+        return mt.lib().mt_gate_backward_bias_f32(R(dh), R(gu), act, R(dgu), db, stride, 0.0, ws, n, None)
+    assert b(gu=M(4, 7)) == INVALID and b(gu=M(3, 8)) == INVALID and b(dgu=M(4, 9)) == INVALID
+    assert b(act=5) == INVALID and b(act=-1) == INVALID
+    assert b(dgu=M(4, 8, rs=0)) == INVALID and b(dgu=None) == INVALID
+    assert b(db=None) == INVALID and b(stride=0) == INVALID and b(stride=-1) == INVALID
+    assert b(ws=0x10002, n=64) == INVALID
+    assert b(M(4, 0), M(4, 0), 0, M(4, 0), None, 0) == OK
+    big = dict(dh=M(1000, 400), gu=M(1000, 800), dgu=M(1000, 800))
+    need = mt.lib().mt_gate_backward_bias_workspace_f32(1000, 400)
+    assert need >= 800 * 4 and b(**big) == WORKSPACE and b(**big, ws=0x10000, n=need - 4) == WORKSPACE
+    f = mt.lib().mt_gate_backward_bias_workspace_f32
+    assert f(0, 8) == 0 and f(8, 0) == 0 and f(-1, 8) == 0 and f(16, 1 << 29) == 0 and f(4, 1 << 31) == 0
+
+
 def test_clip_refuses():
     def call(g, o=None, n=None, most=1.0, eps=1e-6, norm=0x9000, ws=0x10000, size=1 << 30, alone=False):
         a = (mt.MatF32 * max(len(g), 1))(*g)

@@ -381,7 +381,8 @@ def test_gated_linear_empty(dev, q8):
 
 
 # ---- gradients --------------------------------------------------------------------
-@pytest.mark.parametrize("m,f,k", [(1, 1, 1), (3, 33, 17), (64, 128, 96), (130, 67, 257), (509, 320, 300)])
+@pytest.mark.parametrize("m,f,k", [(1, 1, 1), (3, 33, 17), (64, 128, 96), (130, 67, 257), (509, 320, 300),
+                                   (601, 899, 40)])
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
 def test_gated_linear_backward(dev, m, f, k, act):
     g = rng(10, m, f, k)
@@ -412,6 +413,64 @@ def test_gated_linear_backward(dev, m, f, k, act):
     n, dw3, n2 = mt.gated_linear_backward(D, again.gu, X, act=act, need_db=False)
     assert n is None and n2 is None
     check(dw3, d.T @ x, e.T @ np.abs(x) + sums(m) * (a.T @ np.abs(x)), "dw alone")
+
+
+@pytest.mark.parametrize("m,f", [(1, 1), (3, 33), (16, 300), (17, 256), (40, 257), (1000, 70), (2048, 1030), (5, 70001)])
+def test_gate_backward_with_sums(dev, m, f):
+    """The gradients of gate_backward, and their sums over the rows, over and beside what is there."""
+    import ctypes
+    g = rng(19, m, f)
+    R = lambda t: ctypes.byref(mt.mat(t))
+    ws = torch.empty(mt.lib().mt_gate_backward_bias_workspace_f32(m, f), dtype=torch.uint8, device=dev)
+    for how, act in zip(STRIDES, (0, 1, 2, 4)):
+        dh, gu = strided(normal(g, m, f), dev, how), strided(normal(g, m, 2 * f), dev, how)
+        want = mt.gate_backward(dh, gu, ref.ACTS[act])
+        for beta in (0.0, 0.5):
+            was = normal(g, 4 * f)
+            if beta == 0:
+                was[:] = np.nan
+            db = gpu(was, dev)[::2]
+            dgu = torch.empty(m, 2 * f, device=dev) if beta == 0 else gu
+            rc = mt.lib().mt_gate_backward_bias_f32(R(dh), R(gu), act, R(dgu), db.data_ptr(), db.stride(0), beta,
+                                                    ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+            assert rc == mt.MT_OK and torch.equal(dgu, want)
+            d = cpu(want).astype(np.float64)
+            old = beta * was[::2].astype(np.float64) if beta else 0.0
+            # fewer than m + 8 additions, a rounding each of a part of sum|d|, and the last one's
+            check(db, old + d.sum(0), ((m + 8) * np.abs(d).sum(0) + np.abs(old + d.sum(0))) * 2.0 ** -24, how)
+
+
+def test_gate_backward_sums_of_no_rows(dev):
+    import ctypes
+    R = lambda t: ctypes.byref(mt.mat(t))
+    dh, gu, db = torch.empty(0, 3, device=dev), torch.empty(0, 6, device=dev), torch.full((6,), 2.0, device=dev)
+    for beta, want in ((0.25, 0.5), (0.0, 0.0)):
+        assert mt.lib().mt_gate_backward_bias_f32(R(dh), R(gu), 0, R(gu), db.data_ptr(), 1, beta, None, 0,
+                                                  torch.cuda.current_stream().cuda_stream) == mt.MT_OK
+        assert bool((db == want).all())
+
+
+@pytest.mark.parametrize("m,f,k", [(20, 30, 40), (601, 899, 40)])
+def test_backward_by_either_way(dev, m, f, k, monkeypatch):
+    """The native call, and the Python one that takes what is not plain: the same."""
+    import minitensor_amd.ffn as ffn
+    g = rng(20, m, f, k)
+    dh, gu, x, w = (gpu(normal(g, *s), dev) for s in ((m, f), (m, 2 * f), (m, k), (2 * f, k)))
+    calls = [lambda: mt.gated_linear_backward(dh, gu, x, w),
+             lambda: mt.gated_linear_backward(dh, gu, x, need_dw=False),
+             lambda: mt.gated_linear_backward(dh, gu, x, w, need_db=False, dgu=torch.empty_like(gu)),
+             lambda: mt.gated_linear_backward(dh, gu.clone(), x, w, dw=w.clone(), beta_w=0.5,
+                                              db=torch.ones(2 * f, device=dev), beta_b=2.0),
+             lambda: mt.gated_linear_backward(dh, gu, mt.quantize_q8(x), w)]
+    want = [call() for call in calls]
+
+    class Native:
+        def __getattr__(self, name):
+            return (lambda *a: None) if name == "gated_linear_backward" else getattr(mt.native(), name)
+    monkeypatch.setattr(ffn, "native", lambda: Native())
+    for i, (call, a) in enumerate(zip(calls, want)):
+        for p, q in zip(call(), a):
+            assert (p is None and q is None) or torch.equal(p, q), i
 
 
 def test_gated_linear_backward_q8_rows(dev):
