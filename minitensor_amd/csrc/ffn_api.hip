@@ -69,8 +69,8 @@ int run_gate_bias(const mt_mat_f32* dH, const mt_mat_f32* GU, int act, const mt_
 // ---- gated projections in fp32 ---------------------------------------------------------
 
 // How a call goes: few rows (the vector units, the fp32 matrix units), tiles of gemm_f32_sp
-// with the gate in their epilogue, or (operands with no neighbouring elements either way, or too far apart for the
-// tiles' 32-bit offsets) the product to memory first.
+// with the gate in their epilogue, or (operands with no neighbouring elements either way, or
+// too far apart for the tiles' 32-bit offsets) the product to memory first.
 enum GateKind { GATE_FEW, GATE_TILES, GATE_APART };
 constexpr int64_t kGemvRows = 4, kFewRows = 48;
 
@@ -472,7 +472,8 @@ int mt_gated_linear_f32(const mt_mat_f32* X, const mt_mat_f32* W, const float* b
 
 size_t mt_grad_norm_workspace_f32(int64_t count) {
     if (count < 0 || count > kMaxTensors) return 0;
-    return ((size_t)((count + kClipTensors - 1) / kClipTensors) * kClipBlocks + (size_t)count * kStridedBlocks + 1) * 8;
+    const size_t tables = (size_t)((count + kClipTensors - 1) / kClipTensors);
+    return (tables * kClipBlocks + (size_t)count * kStridedBlocks + 1) * 8;
 }
 
 int mt_grad_norm_f32(const mt_mat_f32* grads, int64_t count, float* norm, void* workspace,

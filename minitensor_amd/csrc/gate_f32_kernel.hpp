@@ -58,7 +58,8 @@ __device__ __forceinline__ float wave_sums(const float (&v)[V], int lane) {
 
 // Few rows (M <= MR), bound by the weight's bytes.  A workgroup of eight waves owns NF
 // features; the waves take runs of 256 inputs in turn, a lane four neighbouring ones of each
-// of the 2·NF weight rows and of x, and their sums meet in LDS in wave order.
+// of the 2·NF weight rows and of x, and their sums meet in LDS in wave order.  (One row 2048 ->
+// 2 x 4096, 67 MB of weight: 9.6 us where it is in the 256 MB cache, 7 TB/s.)
 template <int MR, int NF>
 __global__ void __launch_bounds__(512) gate_gemv(GateGemv p) {
     constexpr int W = 8, V = 2 * NF * MR;
@@ -134,7 +135,9 @@ __global__ void __launch_bounds__(512) gate_gemv(GateGemv p) {
 // memory.  A workgroup of eight waves owns 16 features' gate and up rows; the waves take runs
 // of 64 inputs in turn.  Lane l of a product holds row (of x or of the weight) l % 16 and one
 // input; it loads four neighbouring ones, of 16 that the four lanes of a row hold, and takes
-// them in turn, x and weight alike.
+// them in turn, x and weight alike.  (16 rows 2048 -> 2 x 4096: 14 us, 4.8 TB/s; 34 rows
+// 1152 -> 2 x 5056: 26 us, 1.8 TB/s: each workgroup reads all of x, 10 KB an input chunk, for 32
+// columns.)
 template <int MB>
 __global__ void __launch_bounds__(512) gate_few(GateGemv p) {
     constexpr int W = 8, U = 4;                       // products of 16 inputs in flight

@@ -1,7 +1,8 @@
 // gate_kernel.hpp -- activations of a gated feed-forward block and its elementwise passes
 // (include/mtffn.h): h = act(g) * u, and its gradients.
 //
-// The passes are bound by memory: 12 and 20 bytes per element of h.  exp and erfc are the
+// The passes are bound by memory: 12 and 20 bytes per element of h (backward, 4096 x 2 x 4096:
+// 52 us, 6.4 TB/s, part of it from the 256 MB cache; 509 x 2 x 2570: 6.6 us, a launch and a load).  exp and erfc are the
 // device library's; a quotient by 1 + e, 1 <= 1 + e <= 2, is a product with v_rcp_f32 (1 ulp).
 #pragma once
 

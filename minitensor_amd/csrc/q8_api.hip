@@ -48,7 +48,8 @@ constexpr Q8Tile kTiles[] = {{64, 128, 2, 0.34, 0.45, 2.2},
 // those 14.6 and 16.8.)
 // (Its grid holds 16 columns at least a workgroup.)
 bool few_rows(int64_t M, int64_t cols, int64_t K) {
-    return K < kQ8Segment && cols <= 16 * (kMaxTiles - 1) && (M <= 32 || (M <= 64 && M * cols * K <= (int64_t)1200 << 20));
+    return K < kQ8Segment && cols <= 16 * (kMaxTiles - 1) &&
+           (M <= 32 || (M <= 64 && M * cols * K <= (int64_t)1200 << 20));
 }
 
 // cols: columns of the launch (gated: whole blocks of 32 features, twice).

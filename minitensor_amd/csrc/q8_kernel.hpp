@@ -142,7 +142,9 @@ __device__ __forceinline__ u32x4 q8_bytes(const int8_t* row, int k, int end) {
 // (rows on multiples of 16 bytes, 2^24 apart at most: q8_align_rows).  The fragments of the next
 // 32 k are read beside these ones' MFMAs, the next chunk's first ones too: a chunk's one
 // barrier stands before its last MFMAs, when all of it is in registers and the next one in
-// LDS, and its buffer is filled again from there on.  A chunk that the range of k ends in goes
+// LDS, and its buffer is filled again from there on.  (2048 x 4096 -> 8192 with 256 x 256 tiles:
+// 67 us, 2.05 POP/s, gated -> 2 x 8192 137 us, 2.0: the matrix units at the power limit, a library's
+// product 2.1.)  A chunk that the range of k ends in goes
 // first, with its bounds checked, all its units at once (1024 x 2064 -> 4096, rows
 // 2176 bytes apart: 20.8 us, 2048 of those inputs 19.1).
 template <int BM, int BN, int WM, int WN, int BK, int S, bool GATED>
@@ -456,7 +458,9 @@ __global__ void __launch_bounds__(256) q8_align_rows(Q8Align p) {
 // Few rows, bound by the weight's bytes.  A workgroup owns NC blocks of 16 columns (gated:
 // NC/2 of gates and the same features' up columns) and all of K; its waves take chunks of
 // 256 inputs in turn, straight from memory to the operands of 16x16x64 products (lane l: row
-// or column l % 16, 16 bytes from 16·(l/16) on), and their sums meet in LDS.
+// or column l % 16, 16 bytes from 16·(l/16) on), and their sums meet in LDS.  (One row 4096 ->
+// 4096: 5.0 us, a launch and one trip to memory; gated 4096 -> 2 x 8192, 67 MB: 10.8 us where the
+// weight is in the 256 MB cache, 6.2 TB/s.)
 // MB: blocks of 16 rows.  KIND: rows on multiples of 4 bytes, at any address, or (Q8_LONG)
 // at any address, any number of them and of inputs: blocks of rows in the grid, and the waves'
 // sums, 2^16 inputs' each, added up in 64 bits.  (For what the tiles do not take: rows of

@@ -624,12 +624,16 @@ py::object gate_backward(py::handle pdh, py::handle pgu, int act, py::handle pou
     return pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout);
 }
 
-// Projections beyond which their bias's gradient comes from the pass over them, not with dW,
-// whose product has no sums where it is split and none for some layouts.  (us with dX and dW,
-// with the product, from the pass: 4096 x 1024 -> 4096 497, 403; 2048 x 512 -> 4096 195, 139;
-// 509 x 1285 -> 5140 150, 139; 600 x 1000 -> 4000 93, 94; 4096 x 2048 -> 8192 1383, 1383; of
-// fewer the pass's second launch costs more: 512 x 512 -> 2048 39, 44; 2293 x 275 -> 260 32, 41.)
-constexpr int64_t kSumsFrom = (int64_t)1 << 20;
+// Whether the bias's gradient comes from the pass over the projections, not with dW, whose
+// product has no sums where it is split (fewer than 256 tiles of 256 x 128) and none for some
+// layouts.  (us with dX and dW, with the product, from the pass: 4096 x 1024 -> 4096 497, 403;
+// 2048 x 512 -> 4096 195, 139; 300 x 1285 -> 5140 113, 108; 600 x 1000 -> 4000 93, 94; but of few
+// projections the pass's second launch costs more: 512 x 512 -> 2048 39, 44; 2293 x 275 -> 260 32,
+// 41; and of many so do the sums where the product has them: 4096 x 2048 -> 8192 1409, 1424.)
+bool sums_in_pass(int64_t rows, int64_t cols, int64_t k) {
+    const int64_t n = rows * cols;
+    return n > (int64_t)1 << 20 && (n < (int64_t)1 << 24 || cols * k < (int64_t)1 << 23);
+}
 
 // The gradient at the projections, then the Linear layer's from it; x: fp32 rows (pxscale None)
 // or 8-bit ones.  Nothing is enqueued before all checks (dgu may be gu itself).
@@ -662,7 +666,7 @@ py::object gated_linear_backward(py::handle pdh, py::handle pgu, py::handle px, 
         expanded(dw) || expanded(db))
         return py::none();
     // (the one after the other)
-    const bool sums = !q8 && need_db && n * f2 > kSumsFrom;
+    const bool sums = !q8 && need_db && sums_in_pass(n, f2, k);
     const size_t need = std::max(q8 ? mt_linear_backward_q8_workspace_f32(n, k, f2)
                                     : mt_linear_workspace_f32(n, k, f2),
                                  sums ? mt_gate_backward_bias_workspace_f32(n, f2 / 2) : 0);

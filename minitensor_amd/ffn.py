@@ -163,9 +163,11 @@ def gate_backward(dh: torch.Tensor, gu: torch.Tensor, act: str = "silu",
     return out
 
 
-# (projections beyond which their bias's gradient comes from the pass over them, as in the
-# native call)
-_SUMS_FROM = 1 << 20
+def _sums_in_pass(rows: int, cols: int, k: int) -> bool:
+    """Whether the bias's gradient comes from the pass over the projections, as in the native
+    call."""
+    n = rows * cols
+    return n > 1 << 20 and (n < 1 << 24 or cols * k < 1 << 23)
 
 
 @_api
@@ -204,7 +206,7 @@ def gated_linear_backward(dh: torch.Tensor, gu: torch.Tensor, x: Union[torch.Ten
             raise ValueError("gated_linear_backward: an output must not be an expanded view")
     if q8:
         _rows(x)
-    sums = not q8 and need_db and 2 * n * f > _SUMS_FROM
+    sums = not q8 and need_db and _sums_in_pass(n, 2 * f, k)
     if ws is not None or sums:
         need = (lib().mt_linear_backward_q8_workspace_f32 if q8 else lib().mt_linear_workspace_f32)(n, k, 2 * f)
         if sums:
