@@ -154,8 +154,8 @@ __global__ void __launch_bounds__(256) gate_rows(GateParams p) {
 // The gradients as gate_rows gives them, and their sums over the rows (a bias's gradient) from
 // the same pass.  A workgroup owns a strip of features -- 64 lanes of four, or one -- and a run
 // of rows, which its four waves take in turn; the runs' sums go to `part` [runs][2F], or, of one
-// run, to the bias gradient.  (8192 x 2 x 2048, with the runs' sums together: 75 us, 55 without
-// sums; strips four times as wide 71, but 509 x 2 x 2570 24 against 13.)
+// run, to the bias gradient.  (4096 x 2 x 4096, with the runs' sums together: 68 us, 55 without
+// sums; 509 x 2 x 2570: 10.4, 5.7.  Strips four times as wide: 71, and 24.)
 struct GateBias {
     float* db;
     int64_t stride;
