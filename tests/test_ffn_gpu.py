@@ -795,3 +795,80 @@ def test_two_threads(dev):
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_views_past_32_bits(dev):
+    """More than 2^31 elements, or bytes between a product's rows: the first and last rows."""
+    m, f, k = 70000, 16000, 32
+    g = rng(21)
+    x, w = normal(g, m, k), normal(g, 2 * f, k) / np.float32(k ** 0.5)
+    X, W = gpu(x, dev), gpu(w, dev)
+    ends = [0, 1, m - 2, m - 1]
+    r = mt.gated_linear(X, W, keep=True)
+    gu, e = ref.linear(x[ends], w)
+    check(r.gu[ends], gu, e)
+    check(r.h[ends], *ref.gate("silu", gu, e))
+    dh = r.h                                                              # (any gradient does)
+    kept = r.gu[ends].clone()
+    want, err = ref.gate_backward("silu", cpu(dh[ends]), cpu(kept))
+    dx, dw, db = mt.gated_linear_backward(dh, r.gu, X, W, dgu=r.gu)
+    check(r.gu[ends], want, err)
+    # (in 64 bits on the GPU, rows at a time; bounds as in test_gated_linear_backward)
+    s, a = torch.zeros(2 * f, dtype=torch.float64, device=dev), torch.zeros(2 * f, dtype=torch.float64, device=dev)
+    for i in range(0, m, 5000):
+        d = r.gu[i:i + 5000].double()
+        s += d.sum(0)
+        a += d.abs().sum(0)
+        del d
+    check(db, cpu(s), (m + 600) * 2.0 ** -23 * cpu(a), "db")
+    out = torch.empty_like(r.gu)
+    n = mt.clip_grad_norm([r.gu], 1.0, out=[out])
+    total = math.sqrt(sum(float((r.gu[i:i + 5000].double() ** 2).sum()) for i in range(0, m, 5000)))
+    assert abs(float(n) - total) <= 2.0 ** -23 * total
+    c = min(1.0, 1.0 / (float(n) + 1e-6))
+    check(out[ends], c * cpu(r.gu[ends]).astype(np.float64), 2.0 ** -21 * c * np.abs(cpu(r.gu[ends])))
+    del r, dh, out, dx, dw, db
+    q, sc, xq = rows8(g, m, k, dev)
+    wq, ws, wt = rows8(g, 32768, k, dev)
+    y = mt.linear_q8(xq, wt)
+    check(y[ends], *ref.linear_q8(q[ends], sc[ends], wq, ws))
+
+
+@pytest.mark.parametrize("n,f,k", [(0, 5, 6), (7, 0, 6), (7, 5, 0)])
+def test_backward_of_nothing(dev, n, f, k):
+    """No rows, no features, no inputs: gradients of zeros, or of no elements."""
+    dh, gu = torch.ones(n, f, device=dev), torch.ones(n, 2 * f, device=dev)
+    x, w = torch.ones(n, k, device=dev), torch.ones(2 * f, k, device=dev)
+    for rows in (x, mt.quantize_q8(x)):
+        dx, dw, db = mt.gated_linear_backward(dh, gu, rows, w)
+        assert dx.shape == (n, k) and dw.shape == (2 * f, k) and db.shape == (2 * f,)
+        assert bool((dx == 0).all()) and bool((dw == 0).all())
+        if n == 0:
+            assert bool((db == 0).all())
+        elif f:
+            check(db, n * ref.gate_backward("silu", np.ones((1, f), np.float32), np.ones((1, 2 * f), np.float32))[0][0],
+                  np.full(2 * f, 1e-5))
+
+
+def test_graph_of_a_backward_with_sums(dev):
+    g = rng(22)
+    m, f, k = 700, 800, 64
+    x, w, dh = gpu(normal(g, m, k), dev), gpu(normal(g, 2 * f, k) / 8, dev), gpu(normal(g, m, f), dev)
+
+    def step():
+        r = mt.gated_linear(x, w, keep=True)
+        return mt.gated_linear_backward(dh, r.gu, x, w)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        dh.mul_(0.5).add_(0.25)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()
