@@ -100,14 +100,15 @@ struct ClipPiece {
     int n;                            // elements, at most kClipChunk
 };
 // (the tensor of a chunk: one look at every tensor's first chunk, a lane four of them)
+template <int CHUNK = kClipChunk>
 __device__ __forceinline__ ClipPiece clip_piece(const ClipTable& t, uint32_t c) {
     int n = -1;
 #pragma unroll
     for (int i = threadIdx.x & 63; i < kClipTensors; i += 64) n += __popcll(__ballot(t.first[i] <= c));
     const int k = __builtin_amdgcn_readfirstlane(n);
     const uint32_t end = k + 1 < t.count ? t.first[k + 1] : t.chunks;
-    const int64_t at = (int64_t)(c - t.first[k]) * kClipChunk;
-    return {t.at[k] + at, t.at[k + t.to] + at, c + 1 == end ? t.last[k] + 1 : kClipChunk};
+    const int64_t at = (int64_t)(c - t.first[k]) * CHUNK;
+    return {t.at[k] + at, t.at[k + t.to] + at, c + 1 == end ? t.last[k] + 1 : CHUNK};
 }
 // A thread's groups of four, zeros past the end, and (thread < n % 4) one of the last elements.
 struct ClipValues {
@@ -196,6 +197,58 @@ __global__ void __launch_bounds__(kClipThreads) clip_norm(ClipNorm c) {
     if (threadIdx.x != 0) return;
     if (c.norm) *c.norm = (float)sqrt(total);
     else c.part[c.parts] = total;
+}
+
+// Few elements, in one workgroup and one launch: a wave takes up to four chunks of 1024, all
+// on their way at once, and holds them until the norm is there.  (Calls, one after another:
+// 12288 elements 5.0 us, by two launches 8.8; 50432 7.3 and 9.0; 64000 in 64 tensors 8.9 and 11.7;
+// more would not stay in registers.)
+constexpr int kClipOneWaves = 16, kClipOnePieces = 4, kClipOneChunk = 1024;
+template <int = 0>
+__global__ void __launch_bounds__(64 * kClipOneWaves) clip_one(ClipTable t, ClipNorm c, int scale) {
+    __shared__ double red[kClipOneWaves];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    ClipPiece p[kClipOnePieces];
+    rowf4 x[kClipOnePieces][4];
+    float last[kClipOnePieces];
+#pragma unroll
+    for (int i = 0; i < kClipOnePieces; ++i) {
+        const uint32_t id = wave + kClipOneWaves * i;
+        p[i] = ClipPiece{nullptr, nullptr, 0};
+        if (id < t.chunks) p[i] = clip_piece<kClipOneChunk>(t, id);
+        const int quads = p[i].n >> 2;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = lane + 64 * q;
+            x[i][q] = rowf4{0.f, 0.f, 0.f, 0.f};
+            if (at < quads) x[i][q] = *reinterpret_cast<const rowf4_u*>(p[i].src + 4 * at);
+        }
+        last[i] = lane < (p[i].n & 3) ? p[i].src[4 * quads + lane] : 0.f;
+    }
+    double s = 0;
+#pragma unroll
+    for (int i = 0; i < kClipOnePieces; ++i) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = fma((double)x[i][q][e], (double)x[i][q][e], s);
+        s = fma((double)last[i], (double)last[i], s);
+    }
+    const double total = clip_block_sum<64 * kClipOneWaves>(s, red);
+    if (threadIdx.x == 0) *c.norm = (float)sqrt(total);
+    if (!scale) return;
+    const float f = clip_factor(c, total);
+#pragma unroll
+    for (int i = 0; i < kClipOnePieces; ++i) {
+        if (f == 1.f && p[i].dst == p[i].src) continue;
+        const int quads = p[i].n >> 2;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (lane + 64 * q < quads)
+                *reinterpret_cast<rowf4_u*>(p[i].dst + 4 * (lane + 64 * q)) = x[i][q] * f;
+        if (lane < (p[i].n & 3)) p[i].dst[4 * quads + lane] = last[i] * f;
+    }
 }
 
 template <class F>

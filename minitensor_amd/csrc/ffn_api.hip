@@ -321,11 +321,15 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
     const mt_mat_f32* const to = out ? out : grads;
     Tensor d{};
     Extents extents;
-    int64_t all = 0;
+    int64_t all = 0, pieces = 0;
+    bool dense = true;
     for (int64_t i = 0; i < count; ++i) {
         if (!tensor_of(&grads[i], &to[i], scale, &d)) return MT_ERR_INVALID;
         all += d.n;
-        if (scale && d.n > 0 && !extents.add(d)) return MT_ERR_INVALID;
+        if (d.n == 0) continue;
+        pieces += (d.n + kClipOneChunk - 1) / kClipOneChunk;
+        dense = dense && d.dense;
+        if (scale && !extents.add(d)) return MT_ERR_INVALID;
     }
     if (extents.overlap()) return MT_ERR_INVALID;
     const size_t need = mt_grad_norm_workspace_f32(count);
@@ -333,7 +337,7 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
     double* const part = static_cast<double*>(workspace);
 
     // Launches: the dense tensors' by the table, the others' one by one.
-    auto launches = [&](bool apart, auto table, auto single) {
+    auto launches = [&](bool apart, int chunk, auto table, auto single) {
         ClipTable t;
         auto clear = [&] {
             t.count = 0;
@@ -354,19 +358,29 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
                 single(d.strided, (unsigned)std::min<int64_t>((d.n + 255) / 256, kStridedBlocks));
                 continue;
             }
-            const int64_t chunks = (d.n + kClipChunk - 1) / kClipChunk;
+            const int64_t chunks = (d.n + chunk - 1) / chunk;
             if (t.count == most || t.chunks + chunks > (int64_t)1 << 31) flush();
             t.at[t.count] = const_cast<float*>(d.src);
             if (apart) t.at[t.count + t.to] = d.dst;
-            t.last[t.count] = (uint16_t)((d.n - 1) % kClipChunk);
+            t.last[t.count] = (uint16_t)((d.n - 1) % chunk);
             t.first[t.count++] = t.chunks;
             t.chunks += (uint32_t)chunks;
         }
         flush();
     };
+    if (dense && pieces > 0 && pieces <= kClipOneWaves * kClipOnePieces) {
+        launches(
+            out != nullptr, kClipOneChunk,
+            [&](const ClipTable& t, unsigned) {
+                hipLaunchKernelGGL(clip_one<>, dim3(1), dim3(64 * kClipOneWaves), 0, s, t,
+                                   ClipNorm{part, 0, norm, most, eps}, (int)scale);
+            },
+            [](const ClipStrided&, unsigned) {});
+        return launched();
+    }
     int parts = 0;
     launches(
-        false,
+        false, kClipChunk,
         [&](const ClipTable& t, unsigned blocks) {
             hipLaunchKernelGGL(clip_squares, dim3(blocks), dim3(kClipThreads), 0, s, t, part + parts);
             parts += (int)blocks;
@@ -387,7 +401,7 @@ int run_clip(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count, bool
         c = {part + parts, 1, norm, most, eps};
     }
     launches(
-        out != nullptr,
+        out != nullptr, kClipChunk,
         [&](const ClipTable& t, unsigned blocks) {
             if (past) hipLaunchKernelGGL(clip_scale<true>, dim3(blocks), dim3(kClipThreads), 0, s, t, c);
             else hipLaunchKernelGGL(clip_scale<false>, dim3(blocks), dim3(kClipThreads), 0, s, t, c);

@@ -606,6 +606,23 @@ py::object gated_linear(py::handle px, py::handle pxscale, py::handle pw, py::ha
                           tensor(gu));
 }
 
+py::object gate(py::handle pgu, int act, py::handle pout, py::handle stream) {
+    bool ok = true;
+    const at::Tensor gu = arg(pgu, &ok);
+    at::Tensor out = arg(pout, &ok);
+    if (!ok || !gu.defined() || gu.dim() != 2 || gu.size(1) % 2 != 0 || !here(gu, out) ||
+        !shaped(out, gu.size(0), gu.size(1) / 2))
+        return py::none();
+    void* const s = stream_of(stream);
+    {
+        const py::gil_scoped_release nogil;
+        if (!out.defined()) out = empty({gu.size(0), gu.size(1) / 2}, gu);
+        const mt_mat_f32 mg = mat(gu), mo = mat(out);
+        check(mt_gate_f32(&mg, act, &mo, s), "mt_gate_f32");
+    }
+    return pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout);
+}
+
 py::object gate_backward(py::handle pdh, py::handle pgu, int act, py::handle pout,
                          py::handle stream) {
     bool ok = true;
@@ -778,6 +795,7 @@ PYBIND11_MODULE(_native, m) {
     m.def("linear_q4", &linear_q4);
     m.def("linear_q8", &linear_q8);
     m.def("gated_linear", &gated_linear);
+    m.def("gate", &gate);
     m.def("gate_backward", &gate_backward);
     m.def("gated_linear_backward", &gated_linear_backward);
     m.def("clip", &clip);

@@ -133,6 +133,9 @@ def gate(gu: torch.Tensor, act: str = "silu", out: Optional[torch.Tensor] = None
          stream=None) -> torch.Tensor:
     """act(gu[:, :F]) * gu[:, F:] of projections [R, 2F]."""
     a = _act(act, "gate")
+    r = native().gate(gu, a, out, _handle(stream))
+    if r is not None:
+        return r
     _here(gu, out)
     if gu.dim() != 2:
         raise ValueError("gate: expected projections [R, 2F]")

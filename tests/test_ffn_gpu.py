@@ -595,6 +595,52 @@ def test_clip_magnitudes(dev):
     assert bool((z == 0).all())
 
 
+@pytest.mark.parametrize("sizes", [[1024] * 64, [1024] * 65, [65536], [65537], [1023, 1025, 1], [4099] * 12 + [3] * 4,
+                                   [4099] * 12 + [3] * 5, [1] * 64, [1] * 65])
+def test_clip_few_elements(dev, sizes):
+    """Up to 64 chunks of 1024 go to one workgroup, more to the two launches."""
+    g = rng(23, len(sizes), sizes[0])
+    data = [normal(g, n) * np.float32(g.random() + 0.5) for n in sizes]
+    exact = math.sqrt(math.fsum(float(np.sum(d.astype(np.float64) ** 2)) for d in data))
+    c = 0.5 * exact / (exact + 1e-6)
+    flat = torch.full((sum(sizes) + 6,), 9.0, device=dev)
+    ts = [t.copy_(gpu(d, dev)) for t, d in zip(flat[3:-3].split(sizes), data)]
+    outs = [torch.empty_like(t) for t in ts]
+    assert abs(float(mt.grad_norm(ts)) - exact) <= 1.01 * H * exact
+    n = mt.clip_grad_norm(ts, 0.5 * exact, out=outs)
+    assert abs(float(n) - exact) <= 1.01 * H * exact
+    for d, t, o in zip(data, ts, outs):
+        assert np.array_equal(cpu(t), d)
+        # (0.5·exact is rounded to fp32, c, and the product)
+        check(o, d.astype(np.float64) * c, 3.02 * H * np.abs(d) * c)
+    same = [torch.empty_like(t) for t in ts]
+    assert torch.equal(mt.clip_grad_norm(ts, 2 * exact, out=same), n) and all(map(torch.equal, same, ts))
+    assert torch.equal(mt.clip_grad_norm(ts, 2 * exact), n) and all(map(torch.equal, same, ts))
+    assert torch.equal(mt.clip_grad_norm(ts, 0.5 * exact), n) and all(map(torch.equal, outs, ts))
+    assert bool((flat[:3] == 9).all()) and bool((flat[-3:] == 9).all())
+
+
+def test_clip_magnitudes_of_many(dev):
+    """As test_clip_magnitudes, of more than one workgroup takes, and of strided tensors."""
+    for rest in (torch.zeros(70000, device=dev), torch.zeros(9, 8, device=dev)[:, ::2]):
+        big, small = torch.full((1000,), 1e30, device=dev), torch.full((1000,), 1e-30, device=dev)
+        for t in (big, small):
+            assert float(mt.grad_norm([t, rest])) == float(np.float32(math.sqrt(1000 * float(t[0]) ** 2)))
+        mt.clip_grad_norm([big, rest], 1.0)
+        assert abs(float(mt.grad_norm([big, rest])) - 1.0) < 1e-6
+        t = torch.tensor([1.0, float("-inf")], device=dev)
+        assert math.isinf(float(mt.clip_grad_norm([t, rest], 1.0)))
+        assert float(t[0]) == 0 and math.isnan(t[1])
+        t, o = torch.tensor([1.0, float("nan")], device=dev), torch.ones(5, device=dev)
+        assert math.isnan(float(mt.clip_grad_norm([o, rest, t], 1.0)))
+        assert all(bool(torch.isnan(a).all()) for a in (o, rest, t))
+        rest.zero_()
+        assert float(mt.clip_grad_norm([rest], 1.0)) == 0 and bool((rest == 0).all())
+        z = torch.ones(4, device=dev)
+        mt.clip_grad_norm([z, rest], 0.0)
+        assert bool((z == 0).all())
+
+
 # ---- use together -----------------------------------------------------------------
 def block(x, w, b, wd):
     """A feed-forward block's training step: (output, clipped gradients, norm, served output)."""
