@@ -73,7 +73,7 @@ int run_gate_bias(const mt_mat_f32* dH, const mt_mat_f32* GU, int act, const mt_
 // with the gate in their epilogue, or (operands with no neighbouring elements either way, or
 // too far apart for the tiles' 32-bit offsets) the product to memory first.
 enum GateKind { GATE_FEW, GATE_TILES, GATE_APART };
-constexpr int64_t kGemvRows = 4, kFewRows = 48;
+constexpr int64_t kFewRows = 48;
 
 // Times in us by workgroups on a CU, of a chunk of 16 inputs -- one workgroup on every fourth
 // CU or fewer, on every CU, each further one there -- and of a workgroup's beginning and end.
@@ -136,15 +136,24 @@ int gate_layout(const RowView& v, int64_t K, int64_t span, bool weight) {
     if (v.rs == 1 && span < ((int64_t)1 << 30)) return weight ? L_GMV : L_MV;
     return -1;
 }
+// Rows that the vector units' kernel takes: more than four where the matrix units' blocks of 16
+// features are few workgroups, each of which walks a long K.  (Against those and the tiles, us:
+// 8 rows 2048 -> 2 x 512 4.5 and 11.3, 1024 -> 2 x 1024 4.8 and 6.8, 5632 -> 2 x 2048 18.8 and 28,
+// but 512 -> 2 x 2048 6.1 and 4.8, 1285 -> 2 x 2570 13.2 and 7.6; 16 rows 4096 -> 2 x 1024 13.6 and
+// 23.4, 8192 -> 2 x 512 12.2 and 18.1, but 1024 -> 2 x 1024 8.1 and 7.6, 5632 -> 2 x 2048 30.1 and
+// 31.3.)
+int64_t gemv_rows(int64_t F, int64_t K) {
+    if (F <= 1024) return K >= 2 * F ? 16 : 8;
+    return F <= 2048 && K >= 2 * F ? 8 : 4;
+}
 // Whether the kernels of few rows take a product, whose waves walk all of K and read x for 16
 // features each.  (Against the tiles, us: 16 rows 2048 -> 2 x 4096 14 and 23, 32 rows 19 and 24,
 // 48 rows 25 and 26, 500 -> 2 x 1000 8 and 11; but 4096 -> 2 x 8192 32 rows 67 and 62, 48 rows 95
-// and 69, 8192 -> 2 x 512 8 rows 38 and 19, and 5632 -> 2 x 2048 16 rows 32 and 35, 32 rows 42
-// and 35.)
+// and 69, and 5632 -> 2 x 2048 16 rows 32 and 35, 32 rows 42 and 35.)
 // (Their grids hold 4 features at least a workgroup.)
 bool few_rows(int64_t M, int64_t F, int64_t K) {
     if (F > 4 * (kMaxTiles - 1)) return false;
-    if (M <= kGemvRows) return true;
+    if (M <= gemv_rows(F, K)) return true;
     return M <= 16 ? K <= 4 * F : M <= kFewRows && K <= F && F * K <= (int64_t)12 << 20;
 }
 GatePlan gate_plan(const mt_mat_f32* X, const mt_mat_f32* W, int* la, int* lb) {
@@ -175,7 +184,11 @@ int run_gated(const mt_mat_f32* X, const mt_mat_f32* W, const float* bias, int64
         const auto blocks = [&](int features) { return dim3((unsigned)((F + features - 1) / features)); };
         if (M == 1) hipLaunchKernelGGL((gate_gemv<1, 4>), blocks(4), dim3(512), 0, s, p);
         else if (M == 2) hipLaunchKernelGGL((gate_gemv<2, 4>), blocks(4), dim3(512), 0, s, p);
-        else if (M <= kGemvRows) hipLaunchKernelGGL((gate_gemv<4, 4>), blocks(4), dim3(512), 0, s, p);
+        else if (M <= 4) hipLaunchKernelGGL((gate_gemv<4, 4>), blocks(4), dim3(512), 0, s, p);
+        else if (M <= 8 && M <= gemv_rows(F, K))
+            hipLaunchKernelGGL((gate_gemv<8, 2>), blocks(2), dim3(512), 0, s, p);
+        else if (M <= gemv_rows(F, K))
+            hipLaunchKernelGGL((gate_gemv<16, 2>), blocks(2), dim3(512), 0, s, p);
         else if (M <= 16) hipLaunchKernelGGL(gate_few<1>, blocks(16), dim3(512), 0, s, p);
         else if (M <= 32) hipLaunchKernelGGL(gate_few<2>, blocks(16), dim3(512), 0, s, p);
         else hipLaunchKernelGGL(gate_few<3>, blocks(16), dim3(512), 0, s, p);

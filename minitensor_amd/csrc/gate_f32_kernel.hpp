@@ -1,5 +1,5 @@
 // gate_f32_kernel.hpp -- a gated block's projections in fp32 beside the tiles of gemm_f32_sp
-// (GateOut, gemm_kernel.hpp): up to four rows on the vector units, up to 48 on the fp32 matrix
+// (GateOut, gemm_kernel.hpp): up to 16 rows on the vector units, up to 48 on the fp32 matrix
 // units, and the sum of a split product.
 #pragma once
 

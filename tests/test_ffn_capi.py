@@ -41,7 +41,8 @@ def plan_gate(x, w):
 def test_gate_plans():
     assert plan_gate(M(1, 4096), M(8192, 4096))[0] == 0
     assert plan_gate(M(8, 64), M(64, 64))[0] == 0
-    assert plan_gate(M(16, 64), M(32, 64))[0] == 0 and plan_gate(M(16, 65), M(32, 65))[0] == 1
+    assert plan_gate(M(16, 64), M(32, 64))[0] == 0 and plan_gate(M(16, 65), M(32, 65))[0] == 0
+    assert plan_gate(M(9, 5000), M(2200, 5000))[0] == 1 and plan_gate(M(9, 4000), M(2200, 4000))[0] == 0
     assert plan_gate(M(48, 64), M(128, 64))[0] == 0 and plan_gate(M(48, 65), M(128, 65))[0] == 1
     assert plan_gate(M(49, 64), M(128, 64))[0] == 1
     assert plan_gate(M(8, 64, rs=1, cs=8), M(64, 64))[0] == 1          # x across its rows

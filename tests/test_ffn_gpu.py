@@ -276,7 +276,8 @@ def test_gate_infinities(dev):
 # ---- gated Linear ----------------------------------------------------------------
 GATE_SIZES = [(1, 1, 1), (1, 64, 16), (2, 33, 17), (4, 100, 256), (5, 31, 257), (8, 512, 1024),
               (3, 9, 513), (9, 65, 100), (16, 256, 2048), (17, 40, 63), (32, 100, 515), (33, 64, 130),
-              (48, 77, 64), (49, 64, 130), (64, 128, 512), (100, 257, 300),
+              (6, 40, 90), (8, 1030, 2061), (7, 1100, 70), (13, 70, 515), (16, 33, 1029), (10, 129, 200),
+              (16, 1040, 300), (48, 77, 64), (49, 64, 130), (64, 128, 512), (100, 257, 300),
               (130, 96, 1000), (257, 200, 64), (300, 515, 333), (509, 320, 1285)]
 
 
