@@ -42,8 +42,9 @@ int mt_gated_linear_q8(const mt_rows_q8* X, const mt_rows_q8* W, const float* bi
                        int64_t bias_stride, int act, const mt_mat_f32* H, const mt_mat_f32* GU,
                        void* workspace, size_t ws_bytes, void* stream);
 size_t mt_gated_linear_q8_workspace(const mt_rows_q8* X, const mt_rows_q8* W);
-/* The kernel that a call takes (as mt_linear_q8_plan); in fp32: kind 0 few rows, 1 tiles, 2 the
- * product first, then the gate (operands with no unit stride, no inputs). */
+/* The kernel that a call takes (as mt_linear_q8_plan); in fp32: kind 0 straight from
+ * memory (tile_rows 16, 32 or 48 on the matrix units, 0 on the vector units), 1 tiles, 2 the product
+ * first, then the gate (operands with no unit stride, no inputs). */
 typedef struct mt_gate_plan {
     int32_t kind, tile_rows, tile_cols, splits;
 } mt_gate_plan;

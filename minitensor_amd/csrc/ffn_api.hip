@@ -69,10 +69,11 @@ int run_gate_bias(const mt_mat_f32* dH, const mt_mat_f32* GU, int act, const mt_
 
 // ---- gated projections in fp32 ---------------------------------------------------------
 
-// How a call goes: few rows (the vector units, the fp32 matrix units), tiles of gemm_f32_sp
+// How a call goes: straight from memory (few rows on the vector units; few or small ones on the
+// fp32 matrix units), tiles of gemm_f32_sp
 // with the gate in their epilogue, or (operands with no neighbouring elements either way, or
 // too far apart for the tiles' 32-bit offsets) the product to memory first.
-enum GateKind { GATE_FEW, GATE_TILES, GATE_APART };
+enum GateKind { GATE_GEMV, GATE_FEW, GATE_TILES, GATE_APART };
 constexpr int64_t kFewRows = 48;
 
 // Times in us by workgroups on a CU, of a chunk of 16 inputs -- one workgroup on every fourth
@@ -97,12 +98,13 @@ constexpr GateTile kGateTiles[kNumGateCfg] = {
 
 struct GatePlan {
     GateKind kind;
-    int tile, tiles_m, tiles_n, splits, k_per_split;
+    int tile;                         // or (GATE_FEW) blocks of rows
+    int tiles_m, tiles_n, splits, k_per_split;
     size_t partials;                  // bytes, 0 without splits
 };
-GatePlan gate_tiles_plan(int64_t M, int64_t F, int64_t K) {
+GatePlan gate_tiles_plan(int64_t M, int64_t F, int64_t K, double* time) {
     GatePlan best{};
-    double least = 0;
+    double& least = *time;
     const int64_t cols = (F + 31) / 32 * 64, chunks = (K + 15) / 16;
     for (int i = 0; i < kNumGateCfg; ++i) {
         const GateTile& t = kGateTiles[i];
@@ -142,29 +144,53 @@ int gate_layout(const RowView& v, int64_t K, int64_t span, bool weight) {
 // but 512 -> 2 x 2048 6.1 and 4.8, 1285 -> 2 x 2570 13.2 and 7.6; 16 rows 4096 -> 2 x 1024 13.6 and
 // 23.4, 8192 -> 2 x 512 12.2 and 18.1, but 1024 -> 2 x 1024 8.1 and 7.6, 5632 -> 2 x 2048 30.1 and
 // 31.3.)
+// (Its grid holds 4 features a workgroup.)
 int64_t gemv_rows(int64_t F, int64_t K) {
+    if (F > 4 * (kMaxTiles - 1)) return 0;
     if (F <= 1024) return K >= 2 * F ? 16 : 8;
     return F <= 2048 && K >= 2 * F ? 8 : 4;
 }
-// Whether the kernels of few rows take a product, whose waves walk all of K and read x for 16
-// features each.  (Against the tiles, us: 16 rows 2048 -> 2 x 4096 14 and 23, 32 rows 19 and 24,
-// 48 rows 25 and 26, 500 -> 2 x 1000 8 and 11; but 4096 -> 2 x 8192 32 rows 67 and 62, 48 rows 95
-// and 69, and 5632 -> 2 x 2048 16 rows 32 and 35, 32 rows 42 and 35.)
-// (Their grids hold 4 features at least a workgroup.)
-bool few_rows(int64_t M, int64_t F, int64_t K) {
-    if (F > 4 * (kMaxTiles - 1)) return false;
-    if (M <= gemv_rows(F, K)) return true;
-    return M <= 16 ? K <= 4 * F : M <= kFewRows && K <= F && F * K <= (int64_t)12 << 20;
+// The fp32 matrix units' kernel (gate_few), whose waves walk all of K and read x for 16 features
+// each: us by blocks of 16 rows of a workgroup, its beginning and end and 512 inputs of each
+// round over the CUs.  (64 x 512 -> 2 x 2048: 7.9, 6.4 and 7.7 by one, two and three blocks, in
+// tiles 13.3; 64 x 64 -> 2 x 32: 2.7, 3.5, 4.3, 6.6; 512 x 1024 -> 2 x 512: 23.3, 17.1, 21.3, 19.0; 128 x
+// 2048 -> 2 x 256: 12.9, 16.5, 21.6, 14.7; 64 x 4000 -> 2 x 512: 23, 31, 40, 17.)  From up to
+// 4096 rows, 2048 features and 1024 workgroups, which it is kept to beyond 48 rows.
+struct GateFew {
+    double fixed, round;
+};
+constexpr GateFew kGateFew[] = {{2.4, 2.55}, {2.9, 3.6}, {3.6, 4.75}};
+// Blocks of rows, and the time; 0: none.
+int few_blocks(int64_t M, int64_t F, int64_t K, double* us) {
+    int best = 0;
+    for (int mb = 1; mb <= 3; ++mb) {
+        const int64_t wgs = (M + 16 * mb - 1) / (16 * mb) * ((F + 15) / 16);
+        if (wgs > (M <= kFewRows ? kMaxTiles - 1 : 4 * kCus)) continue;
+        const GateFew& c = kGateFew[mb - 1];
+        const int64_t rounds = (wgs + kCus - 1) / kCus;
+        // (280 x 576 -> 2 x 1379 in four rounds: 21.8 us)
+        const double t = c.fixed + c.round * (double)K / 512 * (double)rounds * (rounds > 2 ? 1.12 : 1.0);
+        if (best && t >= *us) continue;
+        best = mb;
+        *us = t;
+    }
+    return best;
 }
 GatePlan gate_plan(const mt_mat_f32* X, const mt_mat_f32* W, int* la, int* lb) {
     const int64_t M = X->rows, F = W->rows / 2, K = X->cols;
     const RowView x = view(X), w = view(W);
-    if (K > 0 && (x.cs == 1 || K == 1) && (w.cs == 1 || K == 1) && few_rows(M, F, K)) return {GATE_FEW};
+    const bool rows = K > 0 && (x.cs == 1 || K == 1) && (w.cs == 1 || K == 1);
+    if (rows && M <= gemv_rows(F, K)) return {GATE_GEMV};
+    double few = 0;
+    const int blocks = rows ? few_blocks(M, F, K, &few) : 0;
     // (a tile's rows; of the weight those of 128 features, and their up rows)
     *la = gate_layout(x, K, std::min<int64_t>(M, 256), false);
     *lb = gate_layout(w, K, F + std::min<int64_t>(F, 128), true);
-    if (K == 0 || *la < 0 || *lb < 0) return {GATE_APART};
-    const GatePlan p = gate_tiles_plan(M, F, K);
+    if (K == 0) return {GATE_APART};
+    double us = 0;
+    const GatePlan p = gate_tiles_plan(M, F, K, &us);
+    if (blocks && (few < us || *la < 0 || *lb < 0)) return {GATE_FEW, blocks};
+    if (*la < 0 || *lb < 0) return {GATE_APART};
     if ((int64_t)p.tiles_m * p.tiles_n * p.splits >= kMaxTiles) return {GATE_APART};
     return p;
 }
@@ -179,19 +205,21 @@ int run_gated(const mt_mat_f32* X, const mt_mat_f32* W, const float* bias, int64
     const GatePlan plan = gate_plan(X, W, &la, &lb);
     const RowView x = view(X), w = view(W), h = view(H), gu = view(GU);
     const int M = (int)X->rows, F = (int)H->cols, K = (int)X->cols;
-    if (plan.kind == GATE_FEW) {
+    if (plan.kind == GATE_GEMV || plan.kind == GATE_FEW) {
         const GateGemv p{x.p, x.rs, w.p, w.rs, bias, bias_stride, h, gu, M, F, K, act};
-        const auto blocks = [&](int features) { return dim3((unsigned)((F + features - 1) / features)); };
-        if (M == 1) hipLaunchKernelGGL((gate_gemv<1, 4>), blocks(4), dim3(512), 0, s, p);
-        else if (M == 2) hipLaunchKernelGGL((gate_gemv<2, 4>), blocks(4), dim3(512), 0, s, p);
-        else if (M <= 4) hipLaunchKernelGGL((gate_gemv<4, 4>), blocks(4), dim3(512), 0, s, p);
-        else if (M <= 8 && M <= gemv_rows(F, K))
-            hipLaunchKernelGGL((gate_gemv<8, 2>), blocks(2), dim3(512), 0, s, p);
-        else if (M <= gemv_rows(F, K))
-            hipLaunchKernelGGL((gate_gemv<16, 2>), blocks(2), dim3(512), 0, s, p);
-        else if (M <= 16) hipLaunchKernelGGL(gate_few<1>, blocks(16), dim3(512), 0, s, p);
-        else if (M <= 32) hipLaunchKernelGGL(gate_few<2>, blocks(16), dim3(512), 0, s, p);
-        else hipLaunchKernelGGL(gate_few<3>, blocks(16), dim3(512), 0, s, p);
+        auto go = [&](auto kernel, int features, int rows) {
+            const dim3 grid((unsigned)((F + features - 1) / features), (unsigned)((M + rows - 1) / rows));
+            hipLaunchKernelGGL(kernel, grid, dim3(512), 0, s, p);
+        };
+        if (plan.kind == GATE_FEW) {
+            if (plan.tile == 1) go(gate_few<1>, 16, 16);
+            else if (plan.tile == 2) go(gate_few<2>, 16, 32);
+            else go(gate_few<3>, 16, 48);
+        } else if (M == 1) go(gate_gemv<1, 4>, 4, 1);
+        else if (M == 2) go(gate_gemv<2, 4>, 4, 2);
+        else if (M <= 4) go(gate_gemv<4, 4>, 4, 4);
+        else if (M <= 8) go(gate_gemv<8, 2>, 2, 8);
+        else go(gate_gemv<16, 2>, 2, 16);
         return launched();
     }
     if (plan.kind == GATE_APART) {
@@ -477,7 +505,9 @@ int mt_gated_linear_plan_f32(const mt_mat_f32* X, const mt_mat_f32* W, mt_gate_p
         return MT_ERR_INVALID;
     int la, lb;
     const GatePlan p = gate_plan(X, W, &la, &lb);
-    *plan = {p.kind, 0, 0, p.kind == GATE_TILES ? p.splits : 1};
+    *plan = {p.kind == GATE_TILES ? 1 : p.kind == GATE_APART ? 2 : 0, 0, 0,
+             p.kind == GATE_TILES ? p.splits : 1};
+    if (p.kind == GATE_FEW) plan->tile_rows = 16 * p.tile;
     if (p.kind == GATE_TILES) {
         plan->tile_rows = kGateTiles[p.tile].bm;
         plan->tile_cols = kGateTiles[p.tile].bn;

@@ -1,6 +1,6 @@
 // gate_f32_kernel.hpp -- a gated block's projections in fp32 beside the tiles of gemm_f32_sp
-// (GateOut, gemm_kernel.hpp): up to 16 rows on the vector units, up to 48 on the fp32 matrix
-// units, and the sum of a split product.
+// (GateOut, gemm_kernel.hpp): few rows on the vector units, few rows and small products on the
+// fp32 matrix units, and the sum of a split product.
 #pragma once
 
 #include "gate_kernel.hpp"
@@ -131,27 +131,28 @@ __global__ void __launch_bounds__(512) gate_gemv(GateGemv p) {
     }
 }
 
-// Up to 16·MB rows, bound by the weight's bytes: fp32 products of 16x16x4 straight from
-// memory.  A workgroup of eight waves owns 16 features' gate and up rows; the waves take runs
+// Few or small: fp32 products of 16x16x4 straight from memory.  A workgroup of eight waves
+// owns 16·MB rows and 16 features' gate and up rows; the waves take runs
 // of 64 inputs in turn.  Lane l of a product holds row (of x or of the weight) l % 16 and one
 // input; it loads four neighbouring ones, of 16 that the four lanes of a row hold, and takes
-// them in turn, x and weight alike.  (16 rows 2048 -> 2 x 4096: 14 us, 4.8 TB/s; 34 rows
-// 1152 -> 2 x 5056: 26 us, 1.8 TB/s: each workgroup reads all of x, 10 KB an input chunk, for 32
-// columns.)
+// them in turn, x and weight alike.  (16 rows 2048 -> 2 x 4096: 13 us, 5 TB/s of weight; 64 rows
+// 64 -> 2 x 32: 2.7 us, in tiles, whose chunks come one after another, 6.6; beyond one workgroup
+// a CU bound by what the L2 gives, each row of x being read again for every 16 features: 512 rows
+// 512 -> 2 x 512 10.4 us, 104 TFLOP/s.)
 template <int MB>
 __global__ void __launch_bounds__(512) gate_few(GateGemv p) {
     constexpr int W = 8, U = 4;                       // products of 16 inputs in flight
     __shared__ float red[W][16 * MB][32];
     const int t = threadIdx.x, lane = t & 63, col = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int f0 = blockIdx.x * 16;
+    const int f0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MB;
     const float* w[2];
     const float* x[MB];
 #pragma unroll
     for (int q = 0; q < 2; ++q)                       // (past the end: the last, not stored)
         w[q] = p.w + ((int64_t)q * p.F + min(f0 + col, p.F - 1)) * p.w_n + 4 * j;
 #pragma unroll
-    for (int b = 0; b < MB; ++b) x[b] = p.x + min(16 * b + col, p.M - 1) * p.x_m + 4 * j;
+    for (int b = 0; b < MB; ++b) x[b] = p.x + min(m0 + 16 * b + col, p.M - 1) * p.x_m + 4 * j;
     typedef float acc4 __attribute__((ext_vector_type(4)));
     acc4 acc[MB][2];
 #pragma unroll
@@ -208,7 +209,8 @@ __global__ void __launch_bounds__(512) gate_few(GateGemv p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) red[wave][16 * m + 4 * j + r][16 * q + col] = acc[m][q][r];
     __syncthreads();
-    for (int i = t; i < p.M * 16; i += 512) {
+    const int rows = min(16 * MB, p.M - m0);
+    for (int i = t; i < rows * 16; i += 512) {
         const int m = i >> 4, c = i & 15, f = f0 + c;
         if (f >= p.F) continue;
         float g = 0.f, u = 0.f;
@@ -217,7 +219,7 @@ __global__ void __launch_bounds__(512) gate_few(GateGemv p) {
             g += red[v][m][c];
             u += red[v][m][16 + c];
         }
-        gate_put(p, m, f, g, u);
+        gate_put(p, m0 + m, f, g, u);
     }
 }
 

@@ -42,25 +42,29 @@ def test_gate_plans():
     assert plan_gate(M(1, 4096), M(8192, 4096))[0] == 0
     assert plan_gate(M(8, 64), M(64, 64))[0] == 0
     assert plan_gate(M(16, 64), M(32, 64))[0] == 0 and plan_gate(M(16, 65), M(32, 65))[0] == 0
-    assert plan_gate(M(9, 5000), M(2200, 5000))[0] == 1 and plan_gate(M(9, 4000), M(2200, 4000))[0] == 0
-    assert plan_gate(M(48, 64), M(128, 64))[0] == 0 and plan_gate(M(48, 65), M(128, 65))[0] == 1
-    assert plan_gate(M(49, 64), M(128, 64))[0] == 1
+    assert plan_gate(M(9, 5000), M(2200, 5000))[0] == 1 and plan_gate(M(9, 1000), M(2200, 1000))[0] == 0
+    assert plan_gate(M(48, 64), M(128, 64))[0] == 0 and plan_gate(M(48, 5000), M(128, 5000))[0] == 1
+    assert plan_gate(M(49, 64), M(128, 64)) == (0, (16, 0), 1)
+    assert plan_gate(M(512, 1024), M(1024, 1024)) == (0, (32, 0), 1)
+    assert plan_gate(M(500, 64), M(2048, 64))[0] == 0 and plan_gate(M(4096, 64), M(2048, 64))[0] == 1
     assert plan_gate(M(8, 64, rs=1, cs=8), M(64, 64))[0] == 1          # x across its rows
     assert plan_gate(M(100, 64), M(64, 64, rs=1, cs=64))[0] == 1
     assert plan_gate(M(100, 64, rs=128, cs=2), M(64, 64))[0] == 2
     assert plan_gate(M(100, 64), M(64, 64, rs=128, cs=2))[0] == 2
-    assert plan_gate(M(100, 64), M(64, 64, rs=1 << 25))[0] == 2        # past 32-bit offsets
+    assert plan_gate(M(100, 64), M(64, 64, rs=1 << 25))[0] == 0        # past 32-bit offsets
+    assert plan_gate(M(2000, 64), M(2048, 64, rs=1 << 25))[0] == 2
     assert plan_gate(M(100, 0), M(64, 0))[0] == 2
     assert plan_gate(M(4096, 2048), M(8192, 2048)) == (1, (128, 256), 1)
     assert plan_gate(M(64, 2048), M(512, 2048))[2] > 1
 
 
 def test_plans_of_most_columns():
-    """A grid holds fewer than 2^23 workgroups of 512 threads, one for every 4 features (16
+    """A grid holds fewer than 2^23 workgroups of 512 threads, one for every 4 or 16 features (16
     columns) of few rows at least: past them, tiles."""
     for m in (1, 4):
-        assert plan_gate(M(m, 1), M((1 << 26) - 8, 1))[0] == 0
-        assert plan_gate(M(m, 1), M(1 << 26, 1))[0] == 1
+        assert plan_gate(M(m, 1), M((1 << 26) - 8, 1)) == (0, (0, 0), 1)
+        assert plan_gate(M(m, 1), M(1 << 26, 1)) != (0, (0, 0), 1)
+        assert plan_gate(M(m, 1), M(1 << 28, 1))[0] == 1
     assert plan_q8(1, 1, (1 << 27) - 16)[0] == (0, 0) and plan_q8(1, 1, 1 << 27)[0] != (0, 0)
     assert plan_q8(1, 1, (1 << 26) - 32, True)[0] == (0, 0) and plan_q8(1, 1, 1 << 26, True)[0] != (0, 0)
 

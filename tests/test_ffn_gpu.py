@@ -278,7 +278,8 @@ GATE_SIZES = [(1, 1, 1), (1, 64, 16), (2, 33, 17), (4, 100, 256), (5, 31, 257), 
               (3, 9, 513), (9, 65, 100), (16, 256, 2048), (17, 40, 63), (32, 100, 515), (33, 64, 130),
               (6, 40, 90), (8, 1030, 2061), (7, 1100, 70), (13, 70, 515), (16, 33, 1029), (10, 129, 200),
               (16, 1040, 300), (48, 77, 64), (49, 64, 130), (64, 128, 512), (100, 257, 300),
-              (130, 96, 1000), (257, 200, 64), (300, 515, 333), (509, 320, 1285)]
+              (130, 96, 1000), (257, 200, 64), (300, 515, 333), (509, 320, 1285),
+              (70, 41, 4003), (131, 97, 3001), (513, 301, 1501), (600, 70, 130), (470, 470, 70), (97, 700, 1100)]
 
 
 @pytest.mark.parametrize("m,f,k", GATE_SIZES)
@@ -315,7 +316,7 @@ def test_gated_linear_kernels():
     from test_ffn_capi import M, plan_gate
     plans = [plan_gate(M(m, k), M(2 * f, k)) for m, f, k in GATE_SIZES + GATE_LARGE]
     assert {p[0] for p in plans} == {0, 1}
-    assert {p[1] for p in plans} == {(0, 0), (64, 128), (128, 128), (128, 256)}, plans
+    assert {p[1] for p in plans} == {(0, 0), (16, 0), (32, 0), (48, 0), (64, 128), (128, 128), (128, 256)}, plans
     assert any(p[2] > 1 for p in plans)
 
 
