@@ -18,16 +18,6 @@ namespace {
 constexpr int64_t kMaxTerms = ((int64_t)1 << 17) - 128;
 // Bytes between a tile's rows: their offsets, 255 of them and a chunk, are 32-bit.
 constexpr int64_t kMaxRow = ((int64_t)1 << 24) - 256;
-enum Kind { FEW, LONG, TILES };
-struct Q8Plan {
-    Kind kind;
-    int bm, bn;
-    int splits, k_per_split;
-    int64_t tiles;                    // the splits' among them
-    int64_t part_n;
-    size_t partials;                  // bytes, 0 without splits
-};
-
 // Times in us by workgroups on a CU, of a chunk of 128 inputs and of a workgroup's beginning
 // and end, from products of 64-4096 rows, 1000-16384 columns, 512 and 4096 inputs; workgroups
 // go in rounds over the CUs.  (2048 x 4096 -> 8192: 256x256 tiles 66-69 us, 128x256 73-78,
@@ -42,20 +32,57 @@ constexpr Q8Tile kTiles[] = {{64, 128, 2, 0.34, 0.45, 2.2},
                              {128, 256, 1, 0.88, 0, 6.5},
                              {256, 256, 1, 1.6, 0, 10}};
 
-// Whether the kernel of few rows takes a product, which reads x for every workgroup's columns
-// anew.  (Against 64x128 tiles, us: 64 rows 4096 -> 4096 12.0 and 11.8, 2048 -> 2048 6.9 and 9.3,
-// 4096 -> 8192 14.3 and 14.1 -- 33 rows 11.7 and 14.1 --, 4096 -> 16384 25.7 and 16.8, 32 rows of
-// those 14.6 and 16.8.)
-// (Its grid holds 16 columns at least a workgroup.)
-bool few_rows(int64_t M, int64_t cols, int64_t K) {
-    return K < kQ8Segment && cols <= 16 * (kMaxTiles - 1) &&
-           (M <= 32 || (M <= 64 && M * cols * K <= (int64_t)1200 << 20));
+// Variants of the kernel that reads both operands straight from memory (q8_few): blocks of 16
+// rows and of 16 columns (gated ones counted twice) of a workgroup, and us of a launch, of each
+// round of workgroups over the CUs, of 2048 inputs in it; 2.5 us a million outputs, which go to
+// memory one by one.  From 80-4096 rows, 64-4096 columns, 64-4096 inputs.  (256 x 2048 -> 512:
+// 5.8, 4.9, 4.9, 5.9, 8.2 and 8.0 us by these, 9.1 in tiles; 80 x 2048 -> 4096 11.2, 9.6, 10.2, 8.7,
+// 8.3, 8.2 and 9.3; 512 x 512 -> 512 4.1, 3.8, 3.9, 3.5, 4.4, 4.3 and 5.7; 1024 x 4096 -> 512 30.7,
+// 23.9, 23.9, 17.2, 14.4, 14.0 and 14.4.  Of few rows a weight that is read twice costs more: 33 x
+// 2048 -> 8192 7.6 by the fifth, 9.4 by the last; 20 x 4096 -> 4096 6.8 by the second, 9.4 by the
+// third.)
+struct Q8Few {
+    int mb, nc;
+    double fixed, round, inputs;
+};
+constexpr Q8Few kFew[] = {{1, 1, 1.8, 0.38, 1.6}, {2, 1, 2.0, 0.3, 2.45}, {1, 2, 2.0, 0.3, 2.45},
+                          {2, 2, 2.2, 0.3, 3.35}, {4, 2, 2.5, 0.3, 4.9},  {2, 4, 2.6, 0.3, 5.1}};
+// The best of them, or nullptr: beyond 64 rows up to 2048 workgroups are measured.
+const Q8Few* few_variant(int64_t M, int64_t cols, int64_t K, bool gated, double* us) {
+    const Q8Few* best = nullptr;
+    if (K >= kQ8Segment) return best;
+    for (const Q8Few& f : kFew) {
+        if (gated && f.nc == 1) continue;
+        const int64_t wgs = (M + 16 * f.mb - 1) / (16 * f.mb) * ((cols + 16 * f.nc - 1) / (16 * f.nc));
+        if (wgs > (M <= 64 ? kMaxTiles - 1 : 8 * kCus)) continue;
+        const double t = f.fixed + 2.5e-6 * (double)M * (double)cols +
+                         (double)((wgs + kCus - 1) / kCus) * (f.round + f.inputs * (double)K / 2048);
+        if (best && t >= *us) continue;
+        best = &f;
+        *us = t;
+    }
+    return best;
 }
 
+enum Kind { FEW, LONG, TILES };
+struct Q8Plan {
+    Kind kind;
+    int bm, bn;
+    int splits, k_per_split;
+    int64_t tiles;                    // the splits' among them
+    int64_t part_n;
+    size_t partials;                  // bytes, 0 without splits
+    const Q8Few* few;
+};
+
 // cols: columns of the launch (gated: whole blocks of 32 features, twice).
-Q8Plan q8_plan(int64_t M, int64_t cols, int64_t K) {
-    if (K > kMaxRow) return {LONG, 0, 0, 1, 0, 0, 0, 0};
-    if (few_rows(M, cols, K)) return {FEW, 0, 0, 1, 0, 0, 0, 0};
+Q8Plan q8_plan(int64_t M, int64_t cols, int64_t K, bool gated) {
+    if (K > kMaxRow) return {LONG, 0, 0, 1, 0, 0, 0, 0, nullptr};
+    double few_us = 0;
+    const Q8Few* const few = few_variant(M, cols, K, gated, &few_us);
+    const Q8Plan direct{FEW, 0, 0, 1, 0, 0, 0, 0, few};
+    // (no tiles take less; of 16 rows and fewer they waste three quarters and more)
+    if (few && (few_us < 4.5 || M <= 16)) return direct;
     Q8Plan best{};
     double least = 0;
     const int64_t chunks = std::max<int64_t>(1, (K + 127) / 128);
@@ -75,11 +102,13 @@ Q8Plan q8_plan(int64_t M, int64_t cols, int64_t K) {
             if (least == 0 || us < least) {
                 least = us;
                 best = {TILES, t.bm, t.bn, (int)splits, (int)(per * 128), wgs, tn * t.bn,
-                        splits > 1 ? (size_t)(splits * M) * (size_t)(tn * t.bn) * 4 : 0};
+                        splits > 1 ? (size_t)(splits * M) * (size_t)(tn * t.bn) * 4 : 0, nullptr};
             }
             if (wgs >= 4 * slots) break;
         }
     }
+    // (the tiles' times are without a launch, 2 us)
+    if (few && few_us < least + 2) return direct;
     return best;
 }
 int64_t launch_cols(int64_t n, bool gated) { return gated ? (n + 31) / 32 * 64 : n; }
@@ -113,37 +142,27 @@ Q8Space q8_space(const Q8Plan& plan, const mt_rows_q8* X, const mt_rows_q8* W) {
     return s;
 }
 
-// Column blocks (of 16, gated ones counted twice) of a workgroup of few rows: more of them
-// read x less often, as long as there is a workgroup for every CU.  (4096 -> 16384, 1 row: one
-// block 18.0 us, two 14.5, four 13.6; gated 4096 -> 2 x 8192: two 12.0, four 14.6; 32 rows: one
-// 23.9, four 14.6; 64 rows: one 38, two 26.  Four of 64 rows do not fit.)
-int few_columns(int64_t rows, int64_t cols) {
-    const int64_t blocks = (cols + 15) / 16;
-    return blocks >= 4 * kCus && rows > 16 && rows <= 32 ? 4 : blocks >= 2 * kCus ? 2 : 1;
-}
 template <bool GATED>
-void launch_few(const Q8Params& p, bool words, hipStream_t s) {
+void launch_few(const Q8Params& p, const Q8Few& f, bool words, hipStream_t s) {
     using std::integral_constant;
-    const int columns = few_columns(p.M, GATED ? 2 * (int64_t)p.N : p.N);
     auto go = [&](auto mb, auto nc, auto kind) {
         constexpr int F = 16 * nc() / (GATED ? 2 : 1);
-        hipLaunchKernelGGL((q8_few<mb(), nc(), GATED, kind()>), dim3((unsigned)((p.N + F - 1) / F)),
-                           dim3(512), 0, s, p);
+        const int64_t wgs = (((int64_t)p.N + F - 1) / F) * (((int64_t)p.M + 16 * mb() - 1) / (16 * mb()));
+        hipLaunchKernelGGL((q8_few<mb(), nc(), GATED, kind()>), dim3((unsigned)wgs), dim3(512), 0, s, p);
     };
-    auto blocks = [&](auto mb, auto kind) {
-        if constexpr (mb() == 2)
-            if (columns == 4) return go(mb, integral_constant<int, 4>{}, kind);
-        if constexpr (!GATED)
-            if (columns == 1) return go(mb, integral_constant<int, 1>{}, kind);
-        go(mb, integral_constant<int, 2>{}, kind);
+    auto blocks = [&](auto kind) {
+        constexpr integral_constant<int, 1> one{};
+        constexpr integral_constant<int, 2> two{};
+        if constexpr (!GATED) {
+            if (f.nc == 1) return f.mb == 1 ? go(one, one, kind) : go(two, one, kind);
+        }
+        if (f.nc == 4) go(two, integral_constant<int, 4>{}, kind);
+        else if (f.mb == 4) go(integral_constant<int, 4>{}, two, kind);
+        else if (f.mb == 2) go(two, two, kind);
+        else go(one, two, kind);
     };
-    auto rows = [&](auto kind) {
-        if (p.M <= 16) blocks(integral_constant<int, 1>{}, kind);
-        else if (p.M <= 32) blocks(integral_constant<int, 2>{}, kind);
-        else blocks(integral_constant<int, 4>{}, kind);
-    };
-    if (words) rows(integral_constant<int, Q8_WORDS>{});
-    else rows(integral_constant<int, Q8_BYTES>{});
+    if (words) blocks(integral_constant<int, Q8_WORDS>{});
+    else blocks(integral_constant<int, Q8_BYTES>{});
 }
 template <bool GATED>
 void launch_tiles(const Q8Params& p, const Q8Plan& plan, hipStream_t s) {
@@ -161,10 +180,10 @@ void launch_tiles(const Q8Params& p, const Q8Plan& plan, hipStream_t s) {
 template <bool GATED>
 int run_q8(Q8Params& p, const mt_rows_q8* X, const mt_rows_q8* W, void* workspace, size_t ws_bytes,
            hipStream_t s) {
-    const Q8Plan plan = q8_plan(p.M, launch_cols(p.N, GATED), p.K);
+    const Q8Plan plan = q8_plan(p.M, launch_cols(p.N, GATED), p.K, GATED);
     p.splits = 1;
     if (plan.kind == FEW) {
-        launch_few<GATED>(p, on(4, X) && on(4, W), s);
+        launch_few<GATED>(p, *plan.few, on(4, X) && on(4, W), s);
         return launched();
     }
     if (plan.kind == LONG) {
@@ -231,14 +250,15 @@ Q8Params q8_params(const mt_rows_q8* X, const mt_rows_q8* W, const float* bias, 
 size_t workspace_of(const mt_rows_q8* X, const mt_rows_q8* W, bool gated) {
     if (!valid(X) || !valid(W) || X->cols != W->cols || X->rows == 0 || W->rows < (gated ? 2 : 1))
         return 0;
-    const Q8Plan plan = q8_plan(X->rows, launch_cols(gated ? W->rows / 2 : W->rows, gated), X->cols);
+    const Q8Plan plan = q8_plan(X->rows, launch_cols(gated ? W->rows / 2 : W->rows, gated), X->cols,
+                                gated);
     return q8_space(plan, X, W).all;
 }
 int plan_of(int64_t rows, int64_t in_f, int64_t out_f, bool gated, mt_q8_plan* plan) {
     if (rows <= 0 || in_f <= 0 || out_f <= 0 || rows >= kMaxDim || in_f >= kMaxDim ||
         out_f >= (gated ? kMaxDim / 2 : kMaxDim) || !plan)
         return MT_ERR_INVALID;
-    const Q8Plan p = q8_plan(rows, launch_cols(out_f, gated), in_f);
+    const Q8Plan p = q8_plan(rows, launch_cols(out_f, gated), in_f, gated);
     *plan = {p.bm, p.bn, p.splits};
     return MT_OK;
 }

@@ -455,15 +455,15 @@ __global__ void __launch_bounds__(256) q8_align_rows(Q8Align p) {
     }
 }
 
-// Few rows, bound by the weight's bytes.  A workgroup owns NC blocks of 16 columns (gated:
+// Few rows, bound by the weight's bytes, and small products.  A workgroup owns MB blocks of 16
+// rows and NC blocks of 16 columns (gated:
 // NC/2 of gates and the same features' up columns) and all of K; its waves take chunks of
 // 256 inputs in turn, straight from memory to the operands of 16x16x64 products (lane l: row
 // or column l % 16, 16 bytes from 16·(l/16) on), and their sums meet in LDS.  (One row 4096 ->
 // 4096: 5.0 us, a launch and one trip to memory; gated 4096 -> 2 x 8192, 67 MB: 10.8 us where the
 // weight is in the 256 MB cache, 6.2 TB/s.)
-// MB: blocks of 16 rows.  KIND: rows on multiples of 4 bytes, at any address, or (Q8_LONG)
-// at any address, any number of them and of inputs: blocks of rows in the grid, and the waves'
-// sums, 2^16 inputs' each, added up in 64 bits.  (For what the tiles do not take: rows of
+// KIND: rows on multiples of 4 bytes, at any address, or (Q8_LONG) at any address and any number
+// of inputs: the waves' sums, 2^16 inputs' each, added up in 64 bits.  (For what the tiles do not take: rows of
 // 2^24 inputs and more.)
 enum { Q8_WORDS = 0, Q8_BYTES = 1, Q8_LONG = 2 };
 constexpr int kQ8Segment = 1 << 19;   // inputs of eight waves' 32-bit sums
@@ -478,9 +478,9 @@ __global__ void __launch_bounds__(512) q8_few(Q8Params p) {
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     // features of a workgroup: half its columns where they are gated
     constexpr int F = GATED ? C / 2 : C;
-    const int blocks = (p.N + F - 1) / F;
-    const int n0 = (KIND == Q8_LONG ? blockIdx.x % blocks : blockIdx.x) * F;
-    const int m0 = KIND == Q8_LONG ? blockIdx.x / blocks * (16 * MB) : 0;
+    // (blocks of rows of the same columns side by side, so that these come from memory once)
+    const int blocks = (p.M + 16 * MB - 1) / (16 * MB);
+    const int n0 = blockIdx.x / blocks * F, m0 = blockIdx.x % blocks * (16 * MB);
     const int8_t* wr[NC];
 #pragma unroll
     for (int q = 0; q < NC; ++q) {                    // (past the end: the last, not stored)

@@ -59,14 +59,14 @@ def test_gate_plans():
 
 
 def test_plans_of_most_columns():
-    """A grid holds fewer than 2^23 workgroups of 512 threads, one for every 4 or 16 features (16
+    """A grid holds fewer than 2^23 workgroups of 512 threads, one for every 4 or 16 features (64
     columns) of few rows at least: past them, tiles."""
     for m in (1, 4):
         assert plan_gate(M(m, 1), M((1 << 26) - 8, 1)) == (0, (0, 0), 1)
         assert plan_gate(M(m, 1), M(1 << 26, 1)) != (0, (0, 0), 1)
         assert plan_gate(M(m, 1), M(1 << 28, 1))[0] == 1
-    assert plan_q8(1, 1, (1 << 27) - 16)[0] == (0, 0) and plan_q8(1, 1, 1 << 27)[0] != (0, 0)
-    assert plan_q8(1, 1, (1 << 26) - 32, True)[0] == (0, 0) and plan_q8(1, 1, 1 << 26, True)[0] != (0, 0)
+    assert plan_q8(1, 1, (1 << 29) - 64)[0] == (0, 0) and plan_q8(1, 1, 1 << 29)[0] != (0, 0)
+    assert plan_q8(1, 1, (1 << 28) - 32, True)[0] == (0, 0) and plan_q8(1, 1, 1 << 28, True)[0] != (0, 0)
 
 
 def test_linear_q8_refuses():
@@ -207,10 +207,10 @@ def test_queries():
         assert f(R(Q(0, 8)), R(Q(8, 8))) == 0 and f(R(Q(8, 8)), R(Q(0, 8))) == 0
         assert f(R(Q(8, 8)), R(Q(8, 9))) == 0 and f(None, R(Q(8, 8))) == 0
         # rows that lie as the tiles take them need none, others a copy
-        assert f(R(Q(100, 64)), R(Q(96, 64))) == 0
-        assert 100 * 64 <= f(R(Q(100, 63)), R(Q(96, 63, rs=64))) < 100 * 64 + 32
-        assert 196 * 64 <= f(R(Q(100, 64, q=0x1008)), R(Q(96, 64, rs=72))) < 196 * 64 + 32
-        assert 96 * 64 <= f(R(Q(100, 64)), R(Q(96, 64, rs=1 << 24))) < 96 * 64 + 32
+        assert f(R(Q(3000, 64)), R(Q(2960, 64))) == 0
+        assert 3000 * 64 <= f(R(Q(3000, 63)), R(Q(2960, 63, rs=64))) < 3000 * 128 + 32
+        assert 5960 * 64 <= f(R(Q(3000, 64, q=0x1008)), R(Q(2960, 64, rs=72))) < 5960 * 128 + 32
+        assert 2960 * 64 <= f(R(Q(3000, 64)), R(Q(2960, 64, rs=1 << 24))) < 2960 * 128 + 32
         assert f(R(Q(64, 63)), R(Q(96, 63))) == 0
     assert lib.mt_grad_norm_workspace_f32(-1) == 0
     assert 0 < lib.mt_grad_norm_workspace_f32(1) <= lib.mt_grad_norm_workspace_f32(1000)

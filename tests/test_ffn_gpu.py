@@ -77,7 +77,8 @@ Q8_SIZES = [(1, 1, 1), (1, 64, 16), (2, 17, 33), (1, 100, 256), (3, 255, 257), (
             (17, 48, 63), (31, 129, 500), (32, 32, 4096), (33, 65, 127), (33, 1, 1000), (40, 200, 64),
             (64, 128, 128), (65, 129, 129), (17, 16400, 100), (32, 8200, 65),
             (64, 8200, 64), (70, 8200, 96), (100, 257, 300), (128, 256, 512), (257, 511, 255),
-            (255, 40, 8192), (300, 1000, 1024), (513, 769, 640), (1027, 520, 2047)]
+            (255, 40, 8192), (300, 1000, 1024), (513, 769, 640), (1027, 520, 2047), (1000, 1500, 257),
+            (2100, 1030, 333), (150, 700, 9001), (300, 520, 12001), (1100, 1500, 64), (700, 900, 5008)]
 
 
 @pytest.mark.parametrize("m,n,k", Q8_SIZES)
@@ -787,8 +788,8 @@ def test_refusals(dev):
     assert all(bool((t == 1).all()) for t in (x, w, gu, dh))
     small = torch.empty(4, dtype=torch.uint8, device=dev)
     for f in (lambda: mt.clip_grad_norm([x], 0.5, ws=small),
-              lambda: mt.linear_q8(mt.quantize_q8(torch.ones(80, 4096, device=dev)),
-                                   mt.quantize_q8(torch.ones(64, 4096, device=dev)), ws=small)):
+              lambda: mt.linear_q8(mt.quantize_q8(torch.ones(150, 9001, device=dev)),
+                                   mt.quantize_q8(torch.ones(700, 9001, device=dev)), ws=small)):
         with pytest.raises(RuntimeError):
             f()
     torch.cuda.synchronize()
