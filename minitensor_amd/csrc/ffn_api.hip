@@ -183,7 +183,7 @@ GatePlan gate_plan(const mt_mat_f32* X, const mt_mat_f32* W, int* la, int* lb) {
     if (rows && M <= gemv_rows(F, K)) return {GATE_GEMV};
     double few = 0;
     const int blocks = rows ? few_blocks(M, F, K, &few) : 0;
-    if (blocks && few < 5) return {GATE_FEW, blocks};   // (no tiles take less)
+    if (blocks && few < 5) return {GATE_FEW, blocks};   // (tiles take 6.6 at least)
     // (a tile's rows; of the weight those of 128 features, and their up rows)
     *la = gate_layout(x, K, std::min<int64_t>(M, 256), false);
     *lb = gate_layout(w, K, F + std::min<int64_t>(F, 128), true);
