@@ -69,10 +69,10 @@ int run_gate_bias(const mt_mat_f32* dH, const mt_mat_f32* GU, int act, const mt_
 
 // ---- gated projections in fp32 ---------------------------------------------------------
 
-// How a call goes: straight from memory (few rows on the vector units; few or small ones on the
-// fp32 matrix units), tiles of gemm_f32_sp
-// with the gate in their epilogue, or (operands with no neighbouring elements either way, or
-// too far apart for the tiles' 32-bit offsets) the product to memory first.
+// How a call goes: straight from memory (few rows on the vector units; few rows and small
+// products on the fp32 matrix units), tiles of gemm_f32_sp with the gate in their epilogue, or
+// (operands with no neighbouring elements either way, or too far apart for the tiles' 32-bit
+// offsets) the product to memory first.
 enum GateKind { GATE_GEMV, GATE_FEW, GATE_TILES, GATE_APART };
 constexpr int64_t kFewRows = 48;
 
@@ -168,7 +168,7 @@ int few_blocks(int64_t M, int64_t F, int64_t K, double* us) {
         if (wgs > (M <= kFewRows ? kMaxTiles - 1 : 4 * kCus)) continue;
         const GateFew& c = kGateFew[mb - 1];
         const int64_t rounds = (wgs + kCus - 1) / kCus;
-        // (280 x 576 -> 2 x 1379 in four rounds: 21.8 us)
+        // (more than two: 280 x 576 -> 2 x 1379, four rounds of the second, 21.8 us; in tiles 19.7)
         const double t = c.fixed + c.round * (double)K / 512 * (double)rounds * (rounds > 2 ? 1.12 : 1.0);
         if (best && t >= *us) continue;
         best = mb;
