@@ -173,6 +173,8 @@ def _require_gpu(*ts: torch.Tensor) -> None:
             raise ValueError("minitensor_amd kernels take GPU tensors only")
         if t.dtype != torch.float32:
             raise ValueError("minitensor_amd kernels take float32 tensors only")
+        if t.is_neg():   # (its memory holds the other sign)
+            raise ValueError("minitensor_amd kernels take no lazily negated views (resolve_neg() makes one plain)")
 
 
 def mat(t: torch.Tensor) -> MatF32:
@@ -430,7 +432,7 @@ def conv2d_backward(x: torch.Tensor, w: torch.Tensor, dy: torch.Tensor, stride: 
                                  bool(need_db), ws, dw, beta_w, _handle(stream))
     if r is not None:
         return r
-    _require_gpu(x, w, dy)
+    _require_gpu(x, w, dy, dw if need_dw else None)
     _require_ws(ws)
     x, w, dy = x.contiguous(), w.contiguous(), dy.contiguous()
     n, c, h, wd = x.shape

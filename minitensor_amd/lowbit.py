@@ -100,6 +100,8 @@ SIGS = {
 def _bytes_on_gpu(t, dtype, what: str) -> None:
     if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dtype != dtype:
         raise ValueError(f"{what} must be a GPU tensor of {dtype}")
+    if t.is_neg():
+        raise ValueError(f"{what} must not be a lazily negated view")
 
 
 def _rows(xq: Q8Rows) -> RowsQ8:

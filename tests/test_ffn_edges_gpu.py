@@ -1,0 +1,67 @@
+"""Calls of the operators of include/mtffn.h and mt_linear_q8 at the ends of what they take:
+views that no kernel reads, gradients past fp32's range, sums over very many rows, products of
+no inputs."""
+import pytest
+import torch
+
+import minitensor_amd as mt
+
+pytestmark = pytest.mark.gpu
+
+
+def negated(*shape, dev):
+    """A float32 view whose elements are kept with the other sign (its negative bit is set)."""
+    v = torch.complex(torch.ones(shape, device=dev), torch.ones(shape, device=dev)).conj().imag
+    assert v.is_neg() and v.dtype == torch.float32
+    return v
+
+
+def test_negated_views_are_refused(dev):
+    """Kernels read memory as it lies: a lazily negated view would be taken with the wrong sign."""
+    x, w, gu, dh = (torch.ones(*s, device=dev) for s in ((4, 64), (8, 64), (4, 8), (4, 4)))
+    b, vec = torch.ones(8, device=dev), torch.ones(64, device=dev)
+    img, ker, dimg = (torch.ones(*s, device=dev) for s in ((1, 2, 5, 5), (3, 2, 1, 1), (1, 3, 5, 5)))
+    xq, wq = mt.quantize_q8(x), mt.quantize_q8(w)
+    n = lambda *s: negated(*s, dev=dev)
+    q = mt.Q8Rows(xq.q, n(4))
+    h, rstd = x, torch.ones(4, device=dev)
+    calls = [
+        lambda: mt.gated_linear(n(4, 64), w), lambda: mt.gated_linear(x, n(8, 64)),
+        lambda: mt.gated_linear(x, w, n(8)), lambda: mt.gated_linear(x, w, out=n(4, 4)),
+        lambda: mt.gated_linear(q, wq), lambda: mt.gated_linear(xq, wq, n(8)),
+        lambda: mt.gate(n(4, 8)), lambda: mt.gate(gu, out=n(4, 4)),
+        lambda: mt.gate_backward(n(4, 4), gu), lambda: mt.gate_backward(dh, n(4, 8)),
+        lambda: mt.gate_backward(dh, gu, out=n(4, 8)),
+        lambda: mt.gated_linear_backward(n(4, 4), gu, x, w), lambda: mt.gated_linear_backward(dh, n(4, 8), x, w),
+        lambda: mt.gated_linear_backward(dh, gu, n(4, 64), w), lambda: mt.gated_linear_backward(dh, gu, x, n(8, 64)),
+        lambda: mt.gated_linear_backward(dh, gu, q, w), lambda: mt.gated_linear_backward(dh, gu, x, w, dgu=n(4, 8)),
+        lambda: mt.gated_linear_backward(dh, gu, x, w, dx=n(4, 64)),
+        lambda: mt.gated_linear_backward(dh, gu, x, w, dw=n(8, 64)),
+        lambda: mt.gated_linear_backward(dh, gu, x, w, db=n(8)),
+        lambda: mt.linear_q8(q, wq), lambda: mt.linear_q8(xq, mt.Q8Rows(wq.q, n(8))),
+        lambda: mt.linear_q8(xq, wq, n(8)), lambda: mt.linear_q8(xq, wq, out=n(4, 8)),
+        lambda: mt.grad_norm([x, n(3, 3)]), lambda: mt.clip_grad_norm([n(3, 3)], 1.0),
+        lambda: mt.clip_grad_norm([x], 1.0, out=[n(4, 64)]),
+        # ... and the operators beside them, which take their operands the same way
+        lambda: mt.gemm(n(4, 64), w.t()), lambda: mt.gemm(x, w.t(), out=n(4, 8)),
+        lambda: mt.linear(n(4, 64), w), lambda: mt.linear(x, w, n(8)),
+        lambda: mt.linear_backward(n(4, 8), x, w), lambda: mt.linear_backward(gu, x, w, db=n(8)),
+        lambda: mt.colsum(n(4, 8)), lambda: mt.axpby(n(4, 8), gu), lambda: mt.axpby(gu, n(4, 8)),
+        lambda: mt.conv2d(n(1, 2, 5, 5), ker), lambda: mt.conv2d(img, ker, n(3)),
+        lambda: mt.conv2d_backward(img, n(3, 2, 1, 1), dimg),
+        lambda: mt.conv2d_backward(img, ker, dimg, dw=n(3, 2, 1, 1)),
+        lambda: mt.rms_norm(n(4, 64)), lambda: mt.rms_norm(x, n(64)),
+        lambda: mt.rms_norm_backward(n(4, 64), h, vec, rstd), lambda: mt.rms_norm_backward(x, h, vec, n(4)),
+        lambda: mt.quantize_q8(n(4, 64)), lambda: mt.quantize_q4(n(8, 64)),
+        lambda: mt.dequantize_q8(q), lambda: mt.linear_backward_q8(gu, q, w),
+        lambda: mt.linear_q4(n(4, 64), mt.quantize_q4(w)), lambda: mt.linear_q4(x, mt.quantize_q4(w), n(8)),
+    ]
+    taken = []
+    for i, call in enumerate(calls):
+        try:
+            call()
+            taken.append(i)
+        except ValueError:
+            pass
+    assert not taken
+    assert all(bool((t == 1).all()) for t in (x, w, gu, dh, b, vec))
