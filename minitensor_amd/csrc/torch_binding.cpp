@@ -670,6 +670,7 @@ py::object gated_linear_backward(py::handle pdh, py::handle pgu, py::handle px, 
         !here(dh, gu, x, xscale, w, dgu, dx, dw, db))
         return py::none();
     const int64_t n = dh.size(0), f2 = 2 * dh.size(1), k = x.size(1);
+    constexpr int64_t most = ((int64_t)1 << 31) - (1 << 16);   // (include/mtffn.h)
     const bool need_dx = w.defined();
     const auto expanded = [](const at::Tensor& t) {
         for (int64_t i = 0; t.defined() && i < t.dim(); ++i)
@@ -680,7 +681,7 @@ py::object gated_linear_backward(py::handle pdh, py::handle pgu, py::handle px, 
         !shaped(w, f2, k) || !shaped(dx, n, k) || !shaped(dw, f2, k) || !vec_of(db, f2) ||
         (dx.defined() && !need_dx) || (need_dw && !dw.defined() && beta_w != 0.f) ||
         (need_db && !db.defined() && beta_b != 0.f) || expanded(dgu) || expanded(dx) ||
-        expanded(dw) || expanded(db))
+        expanded(dw) || expanded(db) || k >= most || (q8 && n > 1 && x.stride(0) < k))
         return py::none();
     // (the one after the other)
     const bool sums = !q8 && need_db && sums_in_pass(n, f2, k);

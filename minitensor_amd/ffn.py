@@ -25,6 +25,7 @@ from . import (MT_ERR_WORKSPACE, MatF32, _api, _check, _handle, _nbytes, _ptr, _
 from .lowbit import (Q8Plan, Q8Rows, RowsQ8, _empty, _matrix, _rows, _vector, _ws,
                      linear_backward_q8)
 
+MAX_EXTENT = (1 << 31) - (1 << 16)   # of a view's rows and columns
 ACTIVATIONS = ("silu", "gelu", "gelu_tanh", "relu", "sigmoid")   # mt_activation
 
 
@@ -209,6 +210,8 @@ def gated_linear_backward(dh: torch.Tensor, gu: torch.Tensor, x: Union[torch.Ten
             raise ValueError("gated_linear_backward: an output must not be an expanded view")
     if q8:
         _rows(x)
+    if k >= MAX_EXTENT:
+        raise ValueError(f"gated_linear_backward: x has {k} inputs")
     sums = not q8 and need_db and _sums_in_pass(n, 2 * f, k)
     if ws is not None or sums:
         need = (lib().mt_linear_backward_q8_workspace_f32 if q8 else lib().mt_linear_workspace_f32)(n, k, 2 * f)

@@ -110,6 +110,8 @@ def _rows(xq: Q8Rows) -> RowsQ8:
     _require_gpu(scale)
     if q.dim() != 2 or (q.shape[1] > 1 and q.stride(1) != 1):
         raise ValueError("Q8Rows.q must be [R, C] with neighbouring elements in a row")
+    if q.shape[0] > 1 and q.stride(0) < q.shape[1]:
+        raise ValueError("Q8Rows.q: rows must not lie over each other")
     if scale.shape != q.shape[:1] or (scale.numel() > 1 and scale.stride(0) != 1):
         raise ValueError("Q8Rows.scale must be [R], contiguous")
     return RowsQ8(q.data_ptr(), scale.data_ptr(), q.shape[0], q.shape[1],

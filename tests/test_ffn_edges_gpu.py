@@ -65,3 +65,18 @@ def test_negated_views_are_refused(dev):
             pass
     assert not taken
     assert all(bool((t == 1).all()) for t in (x, w, gu, dh, b, vec))
+
+
+def test_rows_over_each_other_are_refused_before_the_projections_are_written_over(dev):
+    """Rows that the second product does not take: those in 8 bits that share memory, and longer
+    ones than its extents hold."""
+    dh, gu, w = torch.ones(6, 5, device=dev), torch.full((6, 10), 2.0, device=dev), torch.ones(10, 32, device=dev)
+    one = torch.ones(6, device=dev)
+    q = torch.ones(1, 96, dtype=torch.int8, device=dev)
+    for rows in (q[:, :32].expand(6, 32), q[0].as_strided((6, 32), (8, 1))):
+        with pytest.raises(ValueError):
+            mt.gated_linear_backward(dh, gu, mt.Q8Rows(rows, one), w, dgu=gu)
+        assert bool((gu == 2).all())
+    with pytest.raises(ValueError):
+        mt.gated_linear_backward(dh, gu, one[:, None].expand(6, 1 << 31), need_dw=False, dgu=gu)
+    assert bool((gu == 2).all())
