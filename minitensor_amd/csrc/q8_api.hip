@@ -118,7 +118,10 @@ bool on(int bytes, const mt_rows_q8* r) {
     return r->cols == 0 || (((uintptr_t)r->q % bytes) == 0 && (r->rows <= 1 || r->row_stride % bytes == 0));
 }
 // Whether the tiles take the rows as they lie.
-bool in_place(const mt_rows_q8* r) { return on(16, r) && (r->rows <= 1 || r->row_stride <= kMaxRow); }
+// (of no inputs nothing is read)
+bool in_place(const mt_rows_q8* r) {
+    return r->cols == 0 || (on(16, r) && (r->rows <= 1 || r->row_stride <= kMaxRow));
+}
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
 // The workspace: the splits' sums, then rows of x and of the weight that do not lie as the

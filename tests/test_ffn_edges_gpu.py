@@ -80,3 +80,16 @@ def test_rows_over_each_other_are_refused_before_the_projections_are_written_ove
     with pytest.raises(ValueError):
         mt.gated_linear_backward(dh, gu, one[:, None].expand(6, 1 << 31), need_dw=False, dgu=gu)
     assert bool((gu == 2).all())
+
+
+@pytest.mark.parametrize("m,n", [(300, 4096), (3, 40), (70, 200)])
+def test_no_inputs_far_apart(dev, m, n):
+    """Rows of no inputs, whatever lies between them: the bias."""
+    x = torch.empty(1, dtype=torch.int8, device=dev).as_strided((m, 0), (1 << 24, 1))
+    x = mt.Q8Rows(x, torch.ones(m, device=dev))
+    b = torch.arange(2.0 * n, device=dev) - n / 2
+    w = lambda r: mt.Q8Rows(torch.empty(r, 0, dtype=torch.int8, device=dev), torch.ones(r, device=dev))
+    assert torch.equal(mt.linear_q8(x, w(n), b[:n]), b[:n].expand(m, n))
+    r = mt.gated_linear(x, w(2 * n), b, act="relu", keep=True)
+    assert torch.equal(r.gu, b.expand(m, 2 * n))
+    assert torch.equal(r.h, (b[:n].clamp_min(0) * b[n:]).expand(m, n))
