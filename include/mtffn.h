@@ -72,12 +72,13 @@ size_t mt_gate_backward_bias_workspace_f32(int64_t rows, int64_t features);
  * workspace: a multiple of 8. */
 int mt_grad_norm_f32(const mt_mat_f32* grads, int64_t count, float* norm, void* workspace,
                      size_t ws_bytes, void* stream);
-/* ... and out[i] = grads[i] * c with c = min(1, max_norm / (norm + eps)) in fp64, rounded
- * to fp32 (a NaN norm gives NaN throughout; an infinite one 0, and NaN where the gradient is
- * infinite).  out NULL: in place; with c = 1 nothing is written then.  Otherwise out[i] has the
- * shape of grads[i], and may be the same view; but for that no output may overlap another
- * tensor (refused, but for views with gaps between their elements, of which only the first
- * one is looked at).  norm is that before the scaling. */
+/* ... and out[i] = grads[i] * c with c = min(1, max_norm / (norm + eps)), all in fp64 but for
+ * the arguments, the product rounded to fp32 once (a NaN among the gradients gives NaN
+ * throughout; an infinity 0, and NaN where the gradient is infinite).  out NULL: in place; with
+ * c = 1 nothing is written then.  Otherwise out[i] has the shape of grads[i], and may be the
+ * same view; but for that no output may overlap another tensor (refused, but for views with
+ * gaps between their elements, of which only the first one is looked at).  norm is that before
+ * the scaling. */
 int mt_clip_grad_norm_f32(const mt_mat_f32* grads, const mt_mat_f32* out, int64_t count,
                           float max_norm, float eps, float* norm, void* workspace, size_t ws_bytes,
                           void* stream);

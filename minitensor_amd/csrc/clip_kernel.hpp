@@ -78,11 +78,23 @@ __device__ __forceinline__ double clip_total(const ClipNorm& c, double* red) {
     for (int i = threadIdx.x; i < c.parts; i += NT) s += c.part[i];
     return clip_block_sum<NT>(s, red);
 }
-// The factor; 1: nothing to scale.  (A NaN stays one; an infinite norm gives 0.)
-__device__ __forceinline__ float clip_factor(const ClipNorm& c, double total) {
-    if (total == 0.0) return 1.f;
+// The factor; 1: nothing to scale.  (A NaN stays one; an infinite norm gives 0.)  It is held in
+// fp64: gradients of 1e38 have one below fp32's normal range, where few digits of it are left,
+// and a product that is well above it.
+__device__ __forceinline__ double clip_factor(const ClipNorm& c, double total) {
+    if (total == 0.0) return 1.0;
     const double f = c.most / (sqrt(total) + c.eps);
-    return f >= 1.0 ? 1.f : (float)f;
+    return f >= 1.0 ? 1.0 : f;
+}
+__device__ __forceinline__ float clip_scaled(float x, double f) {
+    asm("" : "+v"(x));                // (not its fp64 form of the squares, kept in two registers)
+    return (float)((double)x * f);
+}
+__device__ __forceinline__ rowf4 clip_scaled(const rowf4& x, double f) {
+    rowf4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = clip_scaled(x[e], f);
+    return y;
 }
 
 // A workgroup's run of chunks, and what it takes of one at a time.
@@ -166,24 +178,24 @@ __global__ void __launch_bounds__(kClipThreads) clip_scale(ClipTable t, ClipNorm
     }
     const double total = clip_total<kClipThreads>(c, red);
     if (blockIdx.x == 0 && threadIdx.x == 0) *c.norm = (float)sqrt(total);
-    const float f = clip_factor(c, total);
+    const double f = clip_factor(c, total);
     for (uint32_t i = r.end; i > r.begin; --i) {
         if (i - 1 > r.begin) {
             q = clip_piece(t, i - 2);
             clip_load(q, next);
         }
-        if (f != 1.f || p.dst != p.src) {
+        if (f != 1.0 || p.dst != p.src) {
             const int quads = p.n >> 2;
 #pragma unroll
             for (int k = 0; k < kClipQuads; ++k) {
                 const int at = threadIdx.x + k * kClipThreads;
                 if (at >= quads) continue;
                 rowf4_u* const d = reinterpret_cast<rowf4_u*>(p.dst + 4 * at);
-                const rowf4 x = v.x[k] * f;
+                const rowf4 x = clip_scaled(v.x[k], f);
                 if constexpr (STREAM) __builtin_nontemporal_store(x, d);
                 else *d = x;
             }
-            if ((int)threadIdx.x < (p.n & 3)) p.dst[4 * quads + threadIdx.x] = v.last * f;
+            if ((int)threadIdx.x < (p.n & 3)) p.dst[4 * quads + threadIdx.x] = clip_scaled(v.last, f);
         }
         p = q;
         v = next;
@@ -238,16 +250,16 @@ __global__ void __launch_bounds__(64 * kClipOneWaves) clip_one(ClipTable t, Clip
     const double total = clip_block_sum<64 * kClipOneWaves>(s, red);
     if (threadIdx.x == 0) *c.norm = (float)sqrt(total);
     if (!scale) return;
-    const float f = clip_factor(c, total);
+    const double f = clip_factor(c, total);
 #pragma unroll
     for (int i = 0; i < kClipOnePieces; ++i) {
-        if (f == 1.f && p[i].dst == p[i].src) continue;
+        if (f == 1.0 && p[i].dst == p[i].src) continue;
         const int quads = p[i].n >> 2;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             if (lane + 64 * q < quads)
-                *reinterpret_cast<rowf4_u*>(p[i].dst + 4 * (lane + 64 * q)) = x[i][q] * f;
-        if (lane < (p[i].n & 3)) p[i].dst[4 * quads + lane] = last[i] * f;
+                *reinterpret_cast<rowf4_u*>(p[i].dst + 4 * (lane + 64 * q)) = clip_scaled(x[i][q], f);
+        if (lane < (p[i].n & 3)) p[i].dst[4 * quads + lane] = clip_scaled(last[i], f);
     }
 }
 
@@ -274,9 +286,9 @@ __global__ void __launch_bounds__(256) clip_scale_strided(ClipStrided t, ClipNor
     __shared__ double red[4];
     const double total = clip_total<256>(c, red);
     if (blockIdx.x == 0 && threadIdx.x == 0) *c.norm = (float)sqrt(total);
-    const float f = clip_factor(c, total);
-    if (f == 1.f && t.dst == t.src) return;
-    clip_elements(t, [&](int64_t a, int64_t b) { t.dst[b] = t.src[a] * f; });
+    const double f = clip_factor(c, total);
+    if (f == 1.0 && t.dst == t.src) return;
+    clip_elements(t, [&](int64_t a, int64_t b) { t.dst[b] = clip_scaled(t.src[a], f); });
 }
 
 }  // namespace mtk

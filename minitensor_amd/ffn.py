@@ -287,7 +287,8 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float,
                    out: Optional[Sequence[torch.Tensor]] = None, eps: float = 1e-6, ws=None,
                    stream=None) -> torch.Tensor:
     """Scales all tensors by min(1, max_norm/(norm + eps)), in place or into the tensors `out`,
-    and returns the norm that they had, a float32 scalar on their device."""
+    and returns the norm that they had, a float32 scalar on their device.  max_norm and eps are
+    taken in float32; each product is rounded once."""
     return _clip(grads, max_norm, out, eps, ws, stream, "clip_grad_norm")
 
 

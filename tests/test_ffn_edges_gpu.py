@@ -1,12 +1,16 @@
 """Calls of the operators of include/mtffn.h and mt_linear_q8 at the ends of what they take:
 views that no kernel reads, gradients past fp32's range, sums over very many rows, products of
 no inputs."""
+import numpy as np
 import pytest
 import torch
 
+import ffn_reference as ref
 import minitensor_amd as mt
 
 pytestmark = pytest.mark.gpu
+
+H = ref.H
 
 
 def negated(*shape, dev):
@@ -93,3 +97,23 @@ def test_no_inputs_far_apart(dev, m, n):
     r = mt.gated_linear(x, w(2 * n), b, act="relu", keep=True)
     assert torch.equal(r.gu, b.expand(m, 2 * n))
     assert torch.equal(r.h, (b[:n].clamp_min(0) * b[n:]).expand(m, n))
+
+
+@pytest.mark.parametrize("kind", ["few", "many", "strided"])
+@pytest.mark.parametrize("value,most", [(3e38, 1.0), (3e38, 1e-3), (1e36, 1e-5), (1e8, 1e-30), (1e-38, 1e-44)])
+def test_clip_factors_below_the_normal_range(dev, kind, value, most):
+    """A factor below 2^-126 times gradients that lift the product above it again: one rounding
+    of the product, not of the factor."""
+    n = {"few": 1000, "many": 100000, "strided": 5000}[kind]
+    t = torch.full((n // 10, 20), value, device=dev)
+    t = t[:, ::2] if kind == "strided" else t[:, :10].contiguous()
+    v, m = float(t[0, 0]), float(np.float32(most))
+    norm = v * (t.numel() ** 0.5)
+    want = v * min(1.0, m / (norm + float(np.float32(0.0))))
+    # the product once, of a factor that is right to a few roundings in 64 bits
+    bound = 1.01 * H * want + 2.0 ** -149
+    out = torch.empty(t.shape, device=dev)
+    mt.clip_grad_norm([t], most, out=[out], eps=0.0)
+    assert abs(out.double() - want).max().item() <= bound
+    mt.clip_grad_norm([t], most, eps=0.0)
+    assert torch.equal(t, out)
