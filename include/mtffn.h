@@ -59,6 +59,8 @@ int mt_gate_backward_f32(const mt_mat_f32* dH, const mt_mat_f32* GU, int act,
 
 /* ... and db = beta*db + the sums of dGU over the rows, the gradient of the projections' bias,
  * from the same pass (mt_linear_backward_f32 then needs no db).  beta 0: db is not read.
+ * Eight rows at a time are added up in fp32 and the rest in fp64, so that db is off by no more
+ * for many rows than for few.
  * workspace: a multiple of 4. */
 int mt_gate_backward_bias_f32(const mt_mat_f32* dH, const mt_mat_f32* GU, int act,
                               const mt_mat_f32* dGU, float* db, int64_t db_stride, float beta,

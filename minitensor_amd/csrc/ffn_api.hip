@@ -36,8 +36,8 @@ int run_gate(const mt_mat_f32* GU, const mt_mat_f32* dH, const mt_mat_f32* out, 
 }
 
 // The gradients with their sums over the rows: runs of rows, 8 at least (two a wave, loaded
-// together), for eight workgroups on a CU.  (509 x 2 x 2570: 10.4 us; 16 at least 14.0, 4 9.5, but
-// 1024 x 2 x 2048 10.9, 10.9 and 12.7.)
+// together), for eight workgroups on a CU.  (With sums in fp32, 509 x 2 x 2570: 10.4 us; 16 at
+// least 14.0, 4 9.5, but 1024 x 2 x 2048 10.9, 10.9 and 12.7.)
 int64_t bias_run(int64_t rows, int64_t strips) {
     const int64_t runs = std::min((rows + 7) / 8, std::max<int64_t>(8 * kCus / strips, 1));
     return ((rows + runs - 1) / runs + 3) / 4 * 4;

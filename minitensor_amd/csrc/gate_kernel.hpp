@@ -154,8 +154,10 @@ __global__ void __launch_bounds__(256) gate_rows(GateParams p) {
 // The gradients as gate_rows gives them, and their sums over the rows (a bias's gradient) from
 // the same pass.  A workgroup owns a strip of features -- 64 lanes of four, or one -- and a run
 // of rows, which its four waves take in turn; the runs' sums go to `part` [runs][2F], or, of one
-// run, to the bias gradient.  (4096 x 2 x 4096, with the runs' sums together: 68 us, 55 without
-// sums; 509 x 2 x 2570: 10.4, 5.7.  Strips four times as wide: 71, and 24.)
+// run, to the bias gradient.  A wave adds up eight rows in fp32 and those sums in fp64, for a run
+// has as many rows as it takes (in fp32 throughout 3e-6 of a sum of 70000 rows of one sign was
+// lost).  (4096 x 2 x 4096, with the runs' sums together: 67 us, 55 without sums; 509 x 2 x 2570:
+// 10.7, 5.7.  Every row in fp64: 69 and 10.8.  Strips four times as wide: 71, and 24.)
 struct GateBias {
     float* db;
     int64_t stride;
@@ -175,31 +177,49 @@ __global__ void __launch_bounds__(256) gate_rows_sums(GateParams p, GateBias b, 
     const RowView up{p.gu.p + (int64_t)p.F * p.gu.cs, p.gu.rs, p.gu.cs};
     const RowView dup{p.out.p + (int64_t)p.F * p.out.cs, p.out.rs, p.out.cs};
     using V = std::conditional_t<VEC, rowf4, float>;
-    V sg{}, su{};
-    if (f < p.F) {
+    double sg[E] = {}, su[E] = {};
+    auto add = [](double (&s)[E], const V& x) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += (double)x[e];
+        } else {
+            s[0] += (double)x;
+        }
+    };
+    for (int64_t b0 = first; b0 < end && f < p.F; b0 += 32) {
+        const int64_t b1 = min(b0 + 32, end);
+        V pg{}, pu{};
 #pragma unroll 2
-        for (int64_t m = first + wave; m < end; m += 4) {
+        for (int64_t m = b0 + wave; m < b1; m += 4) {
             V g = row_load<MODE>(p.gu, m, f, p.F), u = row_load<MODE>(up, m, f, p.F);
             const V dh = row_load<MODE>(p.dh, m, f, p.F);
             gate_slopes(p.act, dh, g, u);
             row_store<MODE>(p.out, m, f, p.F, g);
             row_store<MODE>(dup, m, f, p.F, u);
-            sg += g;
-            su += u;
+            pg += g;
+            pu += u;
         }
+        add(sg, pg);
+        add(su, pu);
     }
-    *reinterpret_cast<V*>(&red[0][wave][lane * E]) = sg;
-    *reinterpret_cast<V*>(&red[1][wave][lane * E]) = su;
+    auto put = [&](float* d, const double (&x)[E]) {
+        V v;
+        if constexpr (VEC) v = rowf4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+        else v = (float)x[0];
+        *reinterpret_cast<V*>(d) = v;
+    };
+    put(&red[0][wave][lane * E], sg);
+    put(&red[1][wave][lane * E], su);
     __syncthreads();
     for (int i = t; i < 2 * STRIP; i += 256) {
         const int h = i / STRIP, c = i % STRIP;
         if (f0 + c >= p.F) continue;
-        float s = red[h][0][c];
+        double s = red[h][0][c];
 #pragma unroll
         for (int w = 1; w < 4; ++w) s += red[h][w][c];
         const int64_t col = (int64_t)h * p.F + f0 + c;
         if (gridDim.y == 1) bias_put(b, col, s);
-        else part[blockIdx.y * 2 * (int64_t)p.F + col] = s;
+        else part[blockIdx.y * 2 * (int64_t)p.F + col] = (float)s;
     }
 }
 // The runs' sums together, in fp64: 64 columns a workgroup, whose waves take the runs in turn.

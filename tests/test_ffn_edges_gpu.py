@@ -1,6 +1,8 @@
 """Calls of the operators of include/mtffn.h and mt_linear_q8 at the ends of what they take:
 views that no kernel reads, gradients past fp32's range, sums over very many rows, products of
 no inputs."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -117,3 +119,32 @@ def test_clip_factors_below_the_normal_range(dev, kind, value, most):
     assert abs(out.double() - want).max().item() <= bound
     mt.clip_grad_norm([t], most, eps=0.0)
     assert torch.equal(t, out)
+
+
+@pytest.mark.parametrize("dense", [True, False])
+def test_bias_gradient_of_very_many_rows(dev, dense):
+    """Sums of values of one sign, whose rounding errors add up: the bound does not grow with
+    the number of rows."""
+    m, f = (1 << 18, 4096) if dense else (70000, 2048)
+    d = float(np.float32(1.1))
+    if dense:
+        gu, dh = torch.full((m, 2 * f), 1.0, device=dev), torch.full((m, f), d, device=dev)
+    else:
+        gu = torch.full((m, 4 * f), 1.0, device=dev)[:, ::2]
+        dh = torch.full((m, 2 * f), d, device=dev)[:, ::2]
+    # relu at 1: both gradients are dh, exactly.  Of one sign, an addition's rounding is at most half
+    # a step of the sum so far: seven of them in eight rows, then one each for the sums of a wave,
+    # of a run and of all
+    want, bound = m * d, 10.1 * H * m * d
+    if dense:
+        x, w = torch.zeros(m, 8, device=dev), torch.zeros(2 * f, 8, device=dev)
+        _, _, db = mt.gated_linear_backward(dh, gu, x, w, act="relu", need_dw=False, dgu=gu)
+        assert abs(db.double() - want).max().item() <= bound
+        gu.fill_(1.0)
+    db = torch.empty(2 * f, device=dev)
+    ws = torch.empty(mt.lib().mt_gate_backward_bias_workspace_f32(m, f), dtype=torch.uint8, device=dev)
+    R = lambda t: ctypes.byref(mt.mat(t))
+    assert mt.lib().mt_gate_backward_bias_f32(R(dh), R(gu), ref.ACTS.index("relu"), R(gu), db.data_ptr(), 1, 0.0,
+                                              ws.data_ptr(), ws.numel(),
+                                              torch.cuda.current_stream().cuda_stream) == mt.MT_OK
+    assert abs(db.double() - want).max().item() <= bound
