@@ -289,6 +289,8 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float,
     """Scales all tensors by min(1, max_norm/(norm + eps)), in place or into the tensors `out`,
     and returns the norm that they had, a float32 scalar on their device.  max_norm and eps are
     taken in float32; each product is rounded once."""
+    if max_norm is None:
+        raise ValueError("clip_grad_norm: no largest norm (grad_norm only measures)")
     return _clip(grads, max_norm, out, eps, ws, stream, "clip_grad_norm")
 
 
@@ -299,8 +301,8 @@ def _clip(grads, most, out, eps, ws, stream, what):
     outs = grads if out is None else list(out)
     if len(outs) != len(grads):
         raise ValueError(f"{what}: as many outputs as tensors")
-    r = native().clip(grads, None if out is None else outs, most is not None, most or 0.0, eps, ws,
-                      _handle(stream))
+    r = native().clip(grads, None if out is None else outs, most is not None,
+                      0.0 if most is None else most, eps, ws, _handle(stream))
     if r is not None:
         return r
     g, o, n = _tensors(grads, outs, what)

@@ -148,3 +148,12 @@ def test_bias_gradient_of_very_many_rows(dev, dense):
                                               ws.data_ptr(), ws.numel(),
                                               torch.cuda.current_stream().cuda_stream) == mt.MT_OK
     assert abs(db.double() - want).max().item() <= bound
+
+
+def test_clip_grad_norm_needs_a_largest_norm(dev):
+    x = torch.ones(4, 8, device=dev)
+    with pytest.raises(ValueError):
+        mt.clip_grad_norm([x], None)
+    assert bool((x == 1).all())
+    mt.clip_grad_norm([x], 0)
+    assert bool((x == 0).all())

@@ -25,3 +25,9 @@ def test_a_negated_view_is_refused():
     lowbit._bytes_on_gpu(view(torch.ones(3, dtype=torch.int8)), torch.int8, "q")
     with pytest.raises(ValueError, match="negated"):
         lowbit._bytes_on_gpu(view(torch._neg_view(torch.ones(3, dtype=torch.int8))), torch.int8, "q")
+
+
+def test_clipping_without_a_largest_norm_is_refused():
+    """(It used to measure the norm and scale nothing.)"""
+    with pytest.raises(ValueError, match="largest norm"):
+        mt.clip_grad_norm([torch.ones(3)], None)
