@@ -47,6 +47,8 @@ size_t mt_gated_linear_q8_workspace(const mt_rows_q8* X, const mt_rows_q8* W);
  * first, then the gate (operands with no unit stride, no inputs). */
 typedef struct mt_gate_plan {
     int32_t kind, tile_rows, tile_cols, splits;
+    int32_t vector_rows;    /* on the vector units: rows that the kernel is made for, 1, 2, 4, 8
+                               or 16; 0: another kernel */
 } mt_gate_plan;
 int mt_gated_linear_plan_f32(const mt_mat_f32* X, const mt_mat_f32* W, mt_gate_plan* plan);
 int mt_gated_linear_q8_plan(int64_t rows, int64_t in_features, int64_t features, mt_q8_plan* plan);

@@ -139,6 +139,8 @@ typedef struct mt_lowbit_plan {
 typedef struct mt_q8_plan {
     int32_t tile_rows, tile_cols;
     int32_t splits;
+    int32_t row_blocks, column_blocks;   /* without tiles: of 16 rows and of 16 columns (gated:
+                                            half of them gates), a workgroup; 0 with tiles */
 } mt_q8_plan;
 int mt_linear_q4_plan(int64_t rows, int64_t in_features, int64_t out_features, int group,
                       int x_in_8_bits, mt_lowbit_plan* plan);

@@ -150,6 +150,8 @@ int64_t gemv_rows(int64_t F, int64_t K) {
     if (F <= 1024) return K >= 2 * F ? 16 : 8;
     return F <= 2048 && K >= 2 * F ? 8 : 4;
 }
+// Rows that a kernel of the vector units is made for.
+int gemv_made_for(int64_t M) { return M <= 2 ? (int)M : M <= 4 ? 4 : M <= 8 ? 8 : 16; }
 // The fp32 matrix units' kernel (gate_few), whose waves walk all of K and read x for 16 features
 // each: us by blocks of 16 rows of a workgroup, its beginning and end and 512 inputs of each
 // round over the CUs.  (64 x 512 -> 2 x 2048: 7.9, 6.4 and 7.7 by one, two and three blocks, in
@@ -216,11 +218,15 @@ int run_gated(const mt_mat_f32* X, const mt_mat_f32* W, const float* bias, int64
             if (plan.tile == 1) go(gate_few<1>, 16, 16);
             else if (plan.tile == 2) go(gate_few<2>, 16, 32);
             else go(gate_few<3>, 16, 48);
-        } else if (M == 1) go(gate_gemv<1, 4>, 4, 1);
-        else if (M == 2) go(gate_gemv<2, 4>, 4, 2);
-        else if (M <= 4) go(gate_gemv<4, 4>, 4, 4);
-        else if (M <= 8) go(gate_gemv<8, 2>, 2, 8);
-        else go(gate_gemv<16, 2>, 2, 16);
+        } else {
+            switch (gemv_made_for(M)) {
+                case 1: go(gate_gemv<1, 4>, 4, 1); break;
+                case 2: go(gate_gemv<2, 4>, 4, 2); break;
+                case 4: go(gate_gemv<4, 4>, 4, 4); break;
+                case 8: go(gate_gemv<8, 2>, 2, 8); break;
+                default: go(gate_gemv<16, 2>, 2, 16);
+            }
+        }
         return launched();
     }
     if (plan.kind == GATE_APART) {
@@ -507,7 +513,7 @@ int mt_gated_linear_plan_f32(const mt_mat_f32* X, const mt_mat_f32* W, mt_gate_p
     int la, lb;
     const GatePlan p = gate_plan(X, W, &la, &lb);
     *plan = {p.kind == GATE_TILES ? 1 : p.kind == GATE_APART ? 2 : 0, 0, 0,
-             p.kind == GATE_TILES ? p.splits : 1};
+             p.kind == GATE_TILES ? p.splits : 1, p.kind == GATE_GEMV ? gemv_made_for(X->rows) : 0};
     if (p.kind == GATE_FEW) plan->tile_rows = 16 * p.tile;
     if (p.kind == GATE_TILES) {
         plan->tile_rows = kGateTiles[p.tile].bm;

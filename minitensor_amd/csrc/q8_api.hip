@@ -262,7 +262,14 @@ int plan_of(int64_t rows, int64_t in_f, int64_t out_f, bool gated, mt_q8_plan* p
         out_f >= (gated ? kMaxDim / 2 : kMaxDim) || !plan)
         return MT_ERR_INVALID;
     const Q8Plan p = q8_plan(rows, launch_cols(out_f, gated), in_f, gated);
-    *plan = {p.bm, p.bn, p.splits};
+    *plan = {p.bm, p.bn, p.splits, 0, 0};
+    if (p.kind == FEW) {
+        plan->row_blocks = p.few->mb;
+        plan->column_blocks = p.few->nc;
+    } else if (p.kind == LONG) {
+        plan->row_blocks = 1;
+        plan->column_blocks = gated ? 2 : 1;
+    }
     return MT_OK;
 }
 

@@ -37,7 +37,8 @@ class GatedLinear(NamedTuple):
 
 class GatePlan(ctypes.Structure):
     _fields_ = [("kind", ctypes.c_int32), ("tile_rows", ctypes.c_int32),
-                ("tile_cols", ctypes.c_int32), ("splits", ctypes.c_int32)]
+                ("tile_cols", ctypes.c_int32), ("splits", ctypes.c_int32),
+                ("vector_rows", ctypes.c_int32)]
 
 
 _P, _V, _I64, _F, _S = (ctypes.POINTER, ctypes.c_void_p, ctypes.c_int64, ctypes.c_float,

@@ -69,7 +69,8 @@ class LowbitPlan(ctypes.Structure):
 
 class Q8Plan(ctypes.Structure):
     _fields_ = [("tile_rows", ctypes.c_int32), ("tile_cols", ctypes.c_int32),
-                ("splits", ctypes.c_int32)]
+                ("splits", ctypes.c_int32), ("row_blocks", ctypes.c_int32),
+                ("column_blocks", ctypes.c_int32)]
 
 
 _P, _V, _I64, _F = ctypes.POINTER, ctypes.c_void_p, ctypes.c_int64, ctypes.c_float
