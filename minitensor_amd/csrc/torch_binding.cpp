@@ -641,12 +641,13 @@ py::object gate_backward(py::handle pdh, py::handle pgu, int act, py::handle pou
     return pout.is_none() ? tensor(out) : py::reinterpret_borrow<py::object>(pout);
 }
 
-// Whether the bias's gradient comes from the pass over the projections, not with dW, whose
-// product has no sums where it is split (fewer than 256 tiles of 256 x 128) and none for some
-// layouts.  (us with dX and dW, with the product, from the pass: 4096 x 1024 -> 4096 497, 403;
-// 2048 x 512 -> 4096 195, 139; 300 x 1285 -> 5140 113, 108; 600 x 1000 -> 4000 93, 94; but of few
-// projections the pass's second launch costs more: 512 x 512 -> 2048 39, 44; 2293 x 275 -> 260 32,
-// 41; and of many so do the sums where the product has them: 4096 x 2048 -> 8192 1409, 1424.)
+// Whether the bias's gradient comes from the pass over the projections (here and in the Python
+// form of the call), not with dW, whose product has no sums where it is split (fewer than 256
+// tiles of 256 x 128) and none for some layouts.  (us with dX and dW, with the product, from the
+// pass: 4096 x 1024 -> 4096 497, 403; 2048 x 512 -> 4096 195, 139; 300 x 1285 -> 5140 113, 108;
+// 600 x 1000 -> 4000 93, 94; but of few projections the pass's second launch costs more: 512 x 512
+// -> 2048 39, 44; 2293 x 275 -> 260 32, 41; and of many so do the sums where the product has them:
+// 4096 x 2048 -> 8192 1409, 1424.)
 bool sums_in_pass(int64_t rows, int64_t cols, int64_t k) {
     const int64_t n = rows * cols;
     return n > (int64_t)1 << 20 && (n < (int64_t)1 << 24 || cols * k < (int64_t)1 << 23);
@@ -799,5 +800,6 @@ PYBIND11_MODULE(_native, m) {
     m.def("gate", &gate);
     m.def("gate_backward", &gate_backward);
     m.def("gated_linear_backward", &gated_linear_backward);
+    m.def("sums_in_pass", &sums_in_pass);
     m.def("clip", &clip);
 }

@@ -168,13 +168,6 @@ def gate_backward(dh: torch.Tensor, gu: torch.Tensor, act: str = "silu",
     return out
 
 
-def _sums_in_pass(rows: int, cols: int, k: int) -> bool:
-    """Whether the bias's gradient comes from the pass over the projections, as in the native
-    call."""
-    n = rows * cols
-    return n > 1 << 20 and (n < 1 << 24 or cols * k < 1 << 23)
-
-
 @_api
 def gated_linear_backward(dh: torch.Tensor, gu: torch.Tensor, x: Union[torch.Tensor, Q8Rows],
                           w: Optional[torch.Tensor] = None, act: str = "silu",
@@ -213,7 +206,7 @@ def gated_linear_backward(dh: torch.Tensor, gu: torch.Tensor, x: Union[torch.Ten
         _rows(x)
     if k >= MAX_EXTENT:
         raise ValueError(f"gated_linear_backward: x has {k} inputs")
-    sums = not q8 and need_db and _sums_in_pass(n, 2 * f, k)
+    sums = not q8 and need_db and native().sums_in_pass(n, 2 * f, k)
     if ws is not None or sums:
         need = (lib().mt_linear_backward_q8_workspace_f32 if q8 else lib().mt_linear_workspace_f32)(n, k, 2 * f)
         if sums:
