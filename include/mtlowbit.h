@@ -118,8 +118,9 @@ size_t mt_linear_q4_workspace(int64_t rows, int64_t in_features, int64_t out_fea
 /* ---- Linear over 8-bit weights -------------------------------------------------
  * Y = X·Wᵀ + bias, both operands in 8 bits: W's rows are the output channels, a scale
  * each (mt_quantize_q8_f32 of the weight gives them):
- *   y[m][n] = (sum_k X.q[m][k]·W.q[n][k]) * (X.scale[m]·W.scale[n]) + bias[n].
- * The sum is exact, whatever its length, and rounded to fp32 once.  Rows may lie at any
+ *   y[m][n] = (sum_k X.q[m][k]·W.q[n][k]) * X.scale[m] * W.scale[n] + bias[n].
+ * The sum is exact, whatever its length, and rounded to fp32 once; so is its product with one
+ * scale, and y.  No finite scales overflow where y does not.  Rows may lie at any
  * address; of many rows of X (mt_linear_q8_plan: tiles), an operand whose rows do not start on
  * multiples of 16 bytes is first copied to the workspace. */
 int mt_linear_q8(const mt_rows_q8* X, const mt_rows_q8* W, const float* bias, int64_t bias_stride,

@@ -5,7 +5,10 @@
 //
 // S is exact while a sum has fewer than 2^17 terms (|q|, |wq| <= 128), which k_per_split
 // sees to; the splits' sums are added up in 64 bits.  So the result does not depend on the
-// tile or the splits: one rounding to fp32, and one for each factor.
+// tile or the splits: one rounding to fp32, and one for each factor.  The scales are not
+// multiplied by each other, whose product may leave fp32's range where y does not: the sum, zero
+// or at least one, takes the row's scale first, or, where that is so large that it might
+// overflow, the column's.
 //
 // Gated: a tile of BN columns has BN/2 features, in blocks of 32 gate columns and the same
 // features' 32 up columns, so that a wave's two neighbouring blocks meet in its epilogue.
@@ -48,15 +51,19 @@ __device__ __forceinline__ int64_t q8_channel(const Q8Params& p, int c) {
     return (c & 32) ? (int64_t)p.N + f : f;
 }
 
-// A sum to y, the same wherever it is taken: the scales' product, then one rounding.
+// A sum to y, the same wherever it is taken.  LARGE: the row's scale may be (a sum is below 2^38).
+__device__ __forceinline__ bool q8_large(float s) { return __builtin_fabsf(s) > 0x1p64f; }
+template <bool LARGE = true>
 __device__ __forceinline__ float q8_value(float sum, float s, float ws, float bias) {
-    return __builtin_fmaf(sum, s * ws, bias);
+    const bool l = LARGE && q8_large(s);
+    return __builtin_fmaf(sum * (l ? ws : s), l ? s : ws, bias);
 }
+template <bool LARGE = true>
 __device__ __forceinline__ rowf4 q8_value(const rowf4& sum, float s, const rowf4& ws,
                                           const rowf4& bias) {
     rowf4 v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = q8_value(sum[e], s, ws[e], bias[e]);
+    for (int e = 0; e < 4; ++e) v[e] = q8_value<LARGE>(sum[e], s, ws[e], bias[e]);
     return v;
 }
 // The scales and biases of four neighbouring columns n.., and of their up columns.
@@ -75,14 +82,14 @@ struct Q8Cols {
     }
 };
 // Four sums of row m, of scale s, to y; gated: a of the gates, b of the up columns.
-template <bool GATED>
+template <bool GATED, bool LARGE = true>
 __device__ __forceinline__ void q8_finish4(const Q8Params& p, int m, int n, float s,
                                            const Q8Cols<GATED>& c, const rowf4& a, const rowf4& b) {
-    const rowf4 g = q8_value(a, s, c.s[0], c.b[0]);
+    const rowf4 g = q8_value<LARGE>(a, s, c.s[0], c.b[0]);
     if constexpr (!GATED) {
         put4(p.y, m, n, p.N, g);
     } else {
-        const rowf4 u = q8_value(b, s, c.s[1], c.b[1]);
+        const rowf4 u = q8_value<LARGE>(b, s, c.s[1], c.b[1]);
         if (p.gu.p) {
             put4(p.gu, m, n, p.N, g);
             put4(p.gu, m, (int64_t)p.N + n, 2 * (int64_t)p.N, u);
@@ -310,9 +317,11 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) q8_gemm(Q8Params p) 
     __syncthreads();
     i32x4* const stage = reinterpret_cast<i32x4*>(smem) + wave * 32 * 16;
     float* const scales = reinterpret_cast<float*>(smem + NW * 32 * 64 * 4);
+    bool large = false;                                // among the wave's rows
     if (!part) {
         for (int r = t; r < BM; r += NT) scales[r] = p.xs[min(m0 + r, p.M - 1)];
         __syncthreads();
+        if constexpr (!GATED) large = __ballot(q8_large(scales[ra + lane % WM])) != 0;
     }
     constexpr int GROUPS = GATED ? 8 : 16, STEP = 64 / GROUPS, PASS = 32 / STEP;
     const int g = lane % GROUPS, r0 = lane / GROUPS;
@@ -346,6 +355,14 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) q8_gemm(Q8Params p) 
                 for (int k = 0; k < 8; ++k)
                     if (m1 + (lane >> 4) + 4 * k < p.M)
                         *reinterpret_cast<i32x4_w*>(d + 4 * k * p.part_n) = a[k];
+            } else if (!GATED && __builtin_expect(large, 0)) {   // (rolled up, and out of the way)
+#pragma unroll 1
+                for (int r = r0; r < 32; r += STEP) {
+                    const int m = m1 + r;
+                    if (m >= p.M || n >= p.N) continue;
+                    const rowf4 x = __builtin_convertvector(stage[r * 16 + (g ^ (r & 15))], rowf4);
+                    q8_finish4<GATED>(p, m, n, scales[ra + 32 * i + r], cols4, x, x);
+                }
             } else {
                 i32x4 a[PASS], b[GATED ? PASS : 1];
                 float s[PASS];
@@ -368,9 +385,9 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) q8_gemm(Q8Params p) 
                         q8_finish4<GATED>(p, m, n, s[k], cols4, x, __builtin_convertvector(b[k], rowf4));
                     } else if (vec) {
                         *reinterpret_cast<rowf4_u*>(d + STEP * k * p.y.rs) =
-                            q8_value(x, s[k], cols4.s[0], cols4.b[0]);
+                            q8_value<false>(x, s[k], cols4.s[0], cols4.b[0]);
                     } else {
-                        q8_finish4<GATED>(p, m, n, s[k], cols4, x, x);
+                        q8_finish4<GATED, false>(p, m, n, s[k], cols4, x, x);
                     }
                 }
             }

@@ -157,3 +157,31 @@ def test_clip_grad_norm_needs_a_largest_norm(dev):
     assert bool((x == 1).all())
     mt.clip_grad_norm([x], 0)
     assert bool((x == 0).all())
+
+
+def scales_of_all_sizes(n, dev, turn):
+    """n finite scales from 1e-40 to 1e37, in turn."""
+    s = torch.tensor([1e-40, 2.0 ** -126, 1e-30, 1e-12, 0.75, 1e12, 1e18, 2e19, 1e30, 1e37], device=dev)
+    return s[(torch.arange(n, device=dev) * turn) % 10] * (1 + torch.arange(n, device=dev) % 7 / 8)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 40, 100), (40, 200, 64), (17, 16400, 100), (70, 8200, 96), (17, 18, 9743),
+                                   (1000, 4000, 1104), (1900, 4000, 200), (2000, 4096, 336)])
+def test_8_bit_products_of_any_finite_scales(dev, m, n, k):
+    """Scales whose product leaves fp32's range where y does not: no digits lost, and zero where
+    the sum is zero."""
+    g = torch.Generator(device=dev).manual_seed(m)
+    codes = lambda r: torch.randint(-128, 128, (r, k), dtype=torch.int8, device=dev, generator=g)
+    x, w = mt.Q8Rows(codes(m), scales_of_all_sizes(m, dev, 1)), mt.Q8Rows(codes(n), scales_of_all_sizes(n, dev, 3))
+    x.q[1], w.q[n - 2] = 0, 0
+    assert bool(x.scale.isfinite().all()) and bool(w.scale.isfinite().all())
+    want = torch.mm(x.q.double(), w.q.double().t().contiguous()) * torch.outer(x.scale.double(), w.scale.double())
+    for y in (mt.linear_q8(x, w), mt.gated_linear(x, w, act="relu", keep=True).gu,
+              mt.linear_q8(mt.Q8Rows(x.q[:2], x.scale[:2]), w)):
+        t = want[:y.shape[0]]
+        over = t.abs() >= 2.0 ** 128 - 2.0 ** 103
+        assert bool((y[over] == torch.where(t > 0, float("inf"), float("-inf")).float()[over]).all())
+        # the sum to fp32, the product with one scale, and with the other (of small y half a step)
+        off = (y.double() - t).abs() - (3.01 * H * t.abs() + 2.0 ** -149)
+        assert off[~over].max().item() <= 0
+        assert bool((y[1] == 0).all()) and bool((y[:, n - 2] == 0).all())
