@@ -54,7 +54,8 @@ int mt_gated_linear_plan_f32(const mt_mat_f32* X, const mt_mat_f32* W, mt_gate_p
 int mt_gated_linear_q8_plan(int64_t rows, int64_t in_features, int64_t features, mt_q8_plan* plan);
 
 /* H = act(GU[:, :F]) * GU[:, F:] of projections that are there already, and the gradient
- * at them:  dG = dH * U * act'(G),  dU = dH * act(G).  dGU may be the same view as GU. */
+ * at them:  dG = dH * U * act'(G),  dU = dH * act(G).  dGU may be the same view as GU.  Of finite
+ * operands dG overflows only where the whole product does. */
 int mt_gate_f32(const mt_mat_f32* GU, int act, const mt_mat_f32* H, void* stream);
 int mt_gate_backward_f32(const mt_mat_f32* dH, const mt_mat_f32* GU, int act,
                          const mt_mat_f32* dGU, void* stream);

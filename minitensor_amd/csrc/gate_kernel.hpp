@@ -85,12 +85,23 @@ __device__ __forceinline__ rowf4 gate4(int act, const rowf4& g, const rowf4& u) 
     return h;
 }
 
+// dh·u·d of a slope d, |d| < 1.2.  Where dh·u overflows the larger of them meets d first: the
+// whole may fit, or be zero (a relu's), and does not get lost on the way either.
+__device__ __forceinline__ float gate_slope(float dh, float u, float d) {
+    const float t = dh * u;
+    if (__builtin_expect(__builtin_isinf(t), 0)) {
+        const bool up = __builtin_fabsf(u) >= __builtin_fabsf(dh);
+        return (up ? u : dh) * d * (up ? dh : u);
+    }
+    return t * d;
+}
+
 // Projections g, u, and the gradient dh at act(g)*u, to the gradients at them.
 __device__ __forceinline__ void gate_slopes(int act, float dh, float& g, float& u) {
     with_act(act, [&](auto a) {
         float d;
         const float v = act_at<a(), true>(g, d);
-        g = dh * u * d;
+        g = gate_slope(dh, u, d);
         u = dh * v;
     });
 }
@@ -100,7 +111,7 @@ __device__ __forceinline__ void gate_slopes(int act, const rowf4& dh, rowf4& g, 
         for (int e = 0; e < 4; ++e) {
             float d;
             const float v = act_at<a(), true>(g[e], d);
-            g[e] = dh[e] * u[e] * d;
+            g[e] = gate_slope(dh[e], u[e], d);
             u[e] = dh[e] * v;
         }
     });

@@ -185,3 +185,21 @@ def test_8_bit_products_of_any_finite_scales(dev, m, n, k):
         off = (y.double() - t).abs() - (3.01 * H * t.abs() + 2.0 ** -149)
         assert off[~over].max().item() <= 0
         assert bool((y[1] == 0).all()) and bool((y[:, n - 2] == 0).all())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu", "sigmoid"])
+def test_gradients_whose_factors_overflow_in_part(dev, act):
+    """dH·U·act'(G) where dH·U is past fp32's range and the whole is not."""
+    g = [-1.0, -3.0, -9.0, -12.0, -20.0, -40.0, -60.0, -80.0, 0.0, -1e4, -3e38]
+    pairs = [(1e25, 1e25), (-3e20, 2e19), (2e38, -7.0), (3.0, 2e38), (1e12, 3e38), (3e38, 3e38), (1e-3, 1e-3)]
+    gates = np.array(g * len(pairs), np.float32)
+    dh, up = (np.repeat(np.array([p[i] for p in pairs], np.float32), len(g)) for i in (0, 1))
+    gu = np.concatenate([gates, up])[None]
+    want, bound = ref.gate_backward(act, dh[None], gu)
+    fits = np.abs(want) < 2.0 ** 128 - 2.0 ** 103
+    t, d = torch.from_numpy(gu).to(dev), torch.from_numpy(dh[None]).to(dev)
+    got = mt.gate_backward(d, t, act).cpu().numpy().astype(np.float64)
+    assert (np.abs(got - want)[fits] <= bound[fits]).all()
+    assert (got[~fits] == np.copysign(np.inf, want[~fits])).all()
+    strided = torch.stack([t, t], 2)[:, :, 0]
+    assert np.array_equal(mt.gate_backward(d, strided, act).cpu().numpy().astype(np.float64), got)
