@@ -53,9 +53,10 @@ struct ClipNorm {
     double most, eps;
 };
 // Gradients, in bytes, beyond which they and as many outputs do not stay in the 256 MB of the
-// last cache: outputs written past it leave it to the gradients (138M elements, again and
-// again: 288 us against 319; 38M: 85 and 86; the other way, 25.6 us against 27.5 for half of
-// those 38M, which stay).
+// last cache: outputs are written past it then, and leave it to the gradients (138M elements,
+// again and again: 288 us against 319).  Smaller ones stay there for whoever reads them next, not
+// for the call's own sake, which written past the cache would take less (the same tensors again,
+// three sets in turn; us: 38M elements 73 and 97, past it 67 and 82; 19M 35 and 45, 33 and 35).
 constexpr int64_t kClipStream = (int64_t)160 << 20;
 
 // The sum of x over a workgroup of NT, in every thread, in a fixed order.

@@ -37,7 +37,7 @@ __device__ __forceinline__ void gate_put(const GateGemv& p, int m, int f, float 
 }
 
 // The sum over a wave of each of v[0..V): after it lane l holds that of v[l / (64/V)].  Half
-// of the values change lanes in each step while there are two or more: V + 6 - log2 V
+// of the values change lanes in each step while there are two or more: V + 5 - log2 V
 // exchanges in place of 6 V.
 template <int V, int O = 32>
 __device__ __forceinline__ float wave_sums(const float (&v)[V], int lane) {
@@ -136,9 +136,10 @@ __global__ void __launch_bounds__(512) gate_gemv(GateGemv p) {
 // of 64 inputs in turn.  Lane l of a product holds row (of x or of the weight) l % 16 and one
 // input; it loads four neighbouring ones, of 16 that the four lanes of a row hold, and takes
 // them in turn, x and weight alike.  (16 rows 2048 -> 2 x 4096: 13 us, 5 TB/s of weight; 64 rows
-// 64 -> 2 x 32: 2.7 us, in tiles, whose chunks come one after another, 6.6; beyond one workgroup
-// a CU bound by what the L2 gives, each row of x being read again for every 16 features: 512 rows
-// 512 -> 2 x 512 10.4 us, 104 TFLOP/s.)
+// 64 -> 2 x 32: 2.7 us, in tiles, whose chunks come one after another, 6.6; 512 rows 512 -> 2 x
+// 512 10.9 us, 49 of the fp32 units' 157 TFLOP/s: each row of x is read again for every 16
+// features and each feature for every 32 rows, 67 MB of operands in 512 workgroups, two a CU in
+// turn, for 3 MB of them.)
 template <int MB>
 __global__ void __launch_bounds__(512) gate_few(GateGemv p) {
     constexpr int W = 8, U = 4;                       // products of 16 inputs in flight

@@ -40,7 +40,9 @@ constexpr Q8Tile kTiles[] = {{64, 128, 2, 0.34, 0.45, 2.2},
 // 8.3, 8.2 and 9.3; 512 x 512 -> 512 4.1, 3.8, 3.9, 3.5, 4.4, 4.3 and 5.7; 1024 x 4096 -> 512 30.7,
 // 23.9, 23.9, 17.2, 14.4, 14.0 and 14.4.  Of few rows a weight that is read twice costs more: 33 x
 // 2048 -> 8192 7.6 by the fifth, 9.4 by the last; 20 x 4096 -> 4096 6.8 by the second, 9.4 by the
-// third.)
+// third.  Of rows on multiples of four bytes: at odd addresses a launch takes longer, one row
+// 4095 -> 4096 7.6 us for 5.0, 256 x 2047 -> 512 6.8 for 5.2, and so does a copy before the tiles,
+// neither of which is priced.)
 struct Q8Few {
     int mb, nc;
     double fixed, round, inputs;
@@ -81,7 +83,9 @@ Q8Plan q8_plan(int64_t M, int64_t cols, int64_t K, bool gated) {
     double few_us = 0;
     const Q8Few* const few = few_variant(M, cols, K, gated, &few_us);
     const Q8Plan direct{FEW, 0, 0, 1, 0, 0, 0, 0, few};
-    // (no tiles take less; of 16 rows and fewer they waste three quarters and more)
+    // (No tiles take less; of 16 rows and fewer they waste three quarters and more.  But their
+    // splits are not to be had so, and of a long K into few columns a few workgroups walk all of
+    // it: 16 x 65536 -> 16 56 us, where 17 rows go in 32 splits of tiles and take 13.)
     if (few && (few_us < 4.5 || M <= 16)) return direct;
     Q8Plan best{};
     double least = 0;
