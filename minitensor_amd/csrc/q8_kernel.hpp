@@ -383,11 +383,10 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64) q8_gemm(Q8Params p) 
                     const rowf4 x = __builtin_convertvector(a[k], rowf4);
                     if constexpr (GATED) {
                         q8_finish4<GATED>(p, m, n, s[k], cols4, x, __builtin_convertvector(b[k], rowf4));
-                    } else if (vec) {
-                        *reinterpret_cast<rowf4_u*>(d + STEP * k * p.y.rs) =
-                            q8_value<false>(x, s[k], cols4.s[0], cols4.b[0]);
                     } else {
-                        q8_finish4<GATED, false>(p, m, n, s[k], cols4, x, x);
+                        const rowf4 y = q8_value<false>(x, s[k], cols4.s[0], cols4.b[0]);
+                        if (vec) *reinterpret_cast<rowf4_u*>(d + STEP * k * p.y.rs) = y;
+                        else put4(p.y, m, n, p.N, y);
                     }
                 }
             }
